@@ -56,7 +56,7 @@ JX_API int jx_device_count(int *count);
 JX_API int jx_set_device(int device);
 JX_API int jx_get_device(int *device);
 /* Device-side error word (bit 0: NaN met by an arg-reduction, bit 1: a bounded
- * wait timed out).  Reads and clears it, together with the fixed error word of
+ * wait timed out, bit 2: packed offsets outside their tensor).  Reads and clears it, together with the fixed error word of
  * jx_gemm_f32_noalloc's launches (ORed in); synchronises the device. */
 JX_API int jx_device_status(unsigned int *flags);
 
@@ -471,6 +471,81 @@ JX_API int jx_col_sum_f32(const float *dy, float *db, int64_t rows, int64_t cols
 JX_API int jx_adam_step_f32(float *const *params, const float *const *grads, float *const *m, float *const *v,
                      const int64_t *sizes, int count, float lr, float beta1, float beta2, float eps,
                      int64_t step, jx_stream_t stream);
+
+/* ---- transformer operators: layer norm, attention, gradient clipping -------
+ * Pointers and row strides are checked against the sizes; sizes of zero are
+ * no-ops.  No output may overlap an input unless stated. */
+/* nn::layer_norm (src/nn.rs:712-725) over the last axis of x [rows, cols],
+ * with the affine step: y = (x - mean) * rstd * gamma + beta, rstd =
+ * 1 / sqrt(var + epsilon), biased variance.  ldx / ldy: row strides in elements
+ * (>= cols).  gamma or beta NULL leaves that factor or term out.  mean_out /
+ * rstd_out [rows] (may be NULL) keep the statistics for the backward pass.
+ * y may be x (with ldy == ldx). */
+JX_API int jx_layernorm_f32(const float *x, const float *gamma, const float *beta, float *y, float *mean_out,
+                            float *rstd_out, int64_t rows, int64_t cols, int64_t ldx, int64_t ldy, float epsilon,
+                            jx_stream_t stream);
+/* Its gradient (no reference counterpart: layer_norm is untraced there).  With
+ * xhat = (x - mean) * rstd and g = dy * gamma:
+ *   dx = (g - mean(g) - xhat * mean(g * xhat)) * rstd,
+ *   dgamma = sum over rows of dy * xhat, dbeta = sum over rows of dy.
+ * mean and rstd are the forward pass's; gamma may be NULL (ones); any of dx,
+ * dgamma and dbeta may be NULL.  The sums over rows have a fixed order: the same
+ * inputs give the same bits.  rows == 0 zero-fills dgamma and dbeta.  dx may
+ * be dy (with lddx == lddy). */
+JX_API int jx_layernorm_bwd_f32(const float *dy, const float *x, const float *gamma, const float *mean,
+                                const float *rstd, float *dx, float *dgamma, float *dbeta, int64_t rows, int64_t cols,
+                                int64_t lddy, int64_t ldx, int64_t lddx, jx_stream_t stream);
+/* nn::scaled_dot_product_attention / multi_head_attention (src/nn.rs:1460,1556:
+ * loops over one sequence) for sequences packed one behind the other, with
+ * grouped heads.  q, o [total_q, heads, head_dim]; k, v [total_k, kv_heads,
+ * head_dim]; a row's heads are contiguous and ldq / ldk / ldv / ldo are the row
+ * strides in elements, so that q, k and v may be slices of one projection's
+ * output.  heads is a multiple of kv_heads; query head h reads key head
+ * h / (heads / kv_heads).  1 <= head_dim <= 128.  cu_q, cu_k [batch + 1]:
+ * sequence b has query rows cu_q[b] .. cu_q[b+1]-1 and key rows cu_k[b] ..
+ * cu_k[b+1]-1 (device int32, not decreasing, within total_q / total_k: an
+ * offset outside is taken as the nearest one inside and sets JX_DEVERR_RANGE,
+ * bit 2 of the device error word).  Rows of no sequence are left as they were.
+ *   x[i,j] = scale * q[i] . k[j],  o[i] = sum_j softmax_j(x[i,j]) v[j],
+ *   lse[i] = log(sum_j exp(x[i,j])).
+ * causal != 0 aligns the sequence's ends: row i of lq sees the keys j <= i +
+ * lk - lq, so that lq = 1 is a decoding step behind lk - 1 cached keys.  A row
+ * that sees no key gets o = 0 and lse = -inf.  A key that a row does not see has
+ * no effect on it, whatever its values.  lse [heads, total_q] may be NULL.
+ * max_q / max_k: the longest sequences, a hint for the choice of kernel; any
+ * value >= 0 gives right results.  The products run on the tensor cores with
+ * each f32 operand split in two f16 parts under a power-of-two scale (22 bits),
+ * f32 sums; a batch of at most 16 query rows per key head runs in plain f32,
+ * split along the keys. */
+JX_API int jx_attention_f32(const float *q, const float *k, const float *v, float *o, float *lse,
+                            const int32_t *cu_q, const int32_t *cu_k, int64_t batch, int64_t total_q, int64_t total_k,
+                            int64_t max_q, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                            int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int causal,
+                            jx_stream_t stream);
+/* Its gradients: dq, dk and dv from dout [total_q, heads, head_dim], with o and
+ * lse of the forward pass.  dout has o's row stride, dq / dk / dv those of q / k
+ * / v.  With p = exp(x - lse): dv = p^T dout, ds = p * (dout v^T -
+ * rowsum(dout * o)), dq = scale * ds k, dk = scale * ds^T q, dk and dv summed
+ * over the query heads that share a key head.  Every sum has a fixed order:
+ * the same inputs give the same bits. */
+JX_API int jx_attention_bwd_f32(const float *q, const float *k, const float *v, const float *o, const float *lse,
+                                const float *dout, float *dq, float *dk, float *dv, const int32_t *cu_q,
+                                const int32_t *cu_k, int64_t batch, int64_t total_q, int64_t total_k, int64_t max_q,
+                                int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t ldq,
+                                int64_t ldk, int64_t ldv, int64_t ldo, float scale, int causal, jx_stream_t stream);
+/* Global norm over `count` tensors (no reference counterpart; the step before
+ * jx_adam_step_f32): norm_out[0] (device scalar) = sqrt(sum of all squares),
+ * summed in f64 in a fixed order.  grads and sizes are host arrays, grads' entries
+ * device pointers. */
+JX_API int jx_grad_norm_f32(const float *const *grads, const int64_t *sizes, int count, float *norm_out,
+                            jx_stream_t stream);
+/* Clipping by the global norm: outs[i] = grads[i] * min(1, max_norm / (norm +
+ * 1e-6)); norm_out (may be NULL) receives the norm before clipping.  outs[i]
+ * may be grads[i] (then nothing is written when no clipping is needed) but
+ * must not overlap it or another tensor otherwise.  A NaN norm makes every
+ * output NaN; an infinite one scales by 0. */
+JX_API int jx_clip_grads_f32(const float *const *grads, float *const *outs, const int64_t *sizes, int count,
+                             float max_norm, float *norm_out, jx_stream_t stream);
 
 /* ---- Dense-stack trainer (examples/mlp_training.rs:94-145 trains with finite
  *      differences + SGD; here: analytic backward, optim::adam_update

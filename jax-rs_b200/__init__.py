@@ -30,7 +30,7 @@ UN = {"neg": 0, "abs": 1, "sin": 2, "cos": 3, "tanh": 4, "exp": 5, "log": 6, "sq
       "floor": 25, "round": 26, "trunc": 27, "expm1": 28, "log1p": 29, "cbrt": 30, "log2": 31}
 RED = {"sum": 0, "max": 1, "min": 2, "prod": 3}
 OP_CONST, OP_STORE, OP_UNARY, OP_BINARY, OP_SELECT_GT = 1, 2, 16, 48, 64
-DEVERR_NAN, DEVERR_TIMEOUT = 1, 2
+DEVERR_NAN, DEVERR_TIMEOUT, DEVERR_RANGE = 1, 2, 4
 
 
 class JaxRsError(RuntimeError):
@@ -137,6 +137,12 @@ _SIGS = {
     "jx_col_sum_f32": [vp, vp, i64, i64, vp],
     "jx_adam_step_f32": [C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(vp), C.POINTER(i64), ci,
                          cf, cf, cf, cf, i64, vp],
+    "jx_layernorm_f32": [vp] * 6 + [i64] * 4 + [cf, vp],
+    "jx_layernorm_bwd_f32": [vp] * 8 + [i64] * 5 + [vp],
+    "jx_attention_f32": [vp] * 7 + [i64] * 12 + [cf, ci, vp],
+    "jx_attention_bwd_f32": [vp] * 11 + [i64] * 12 + [cf, ci, vp],
+    "jx_grad_norm_f32": [C.POINTER(vp), C.POINTER(i64), ci, vp, vp],
+    "jx_clip_grads_f32": [C.POINTER(vp), C.POINTER(vp), C.POINTER(i64), ci, cf, vp, vp],
     "jx_mlp_create": [C.POINTER(i64), ci, C.POINTER(ci), i64, ci, C.POINTER(vp)],
     "jx_mlp_param_count": [vp, C.POINTER(i64)],
     "jx_mlp_param_offsets": [vp, C.POINTER(i64), C.POINTER(i64)],
@@ -318,6 +324,60 @@ def fft_c2c(x, y, n, batch, inverse=False, stream=None):
 
 def fft2_c2c(x, y, h, w, batch, inverse=False, stream=None):
     call("jx_fft2_c2c_f32", x, y, h, w, batch, int(inverse), stream)
+
+
+def layernorm(x, gamma, beta, y, rows, cols, eps=1e-5, mean_out=None, rstd_out=None, ldx=None, ldy=None,
+              stream=None):
+    """Layer norm of x [rows, cols] over its last axis; row strides default to cols."""
+    call("jx_layernorm_f32", x, gamma, beta, y, mean_out, rstd_out, rows, cols, ldx if ldx is not None else cols,
+         ldy if ldy is not None else cols, eps, stream)
+
+
+def layernorm_bwd(dy, x, gamma, mean, rstd, dx, dgamma, dbeta, rows, cols, lddy=None, ldx=None, lddx=None,
+                  stream=None):
+    """Gradients of layernorm from the statistics that it kept; dx, dgamma or dbeta may be None."""
+    call("jx_layernorm_bwd_f32", dy, x, gamma, mean, rstd, dx, dgamma, dbeta, rows, cols,
+         lddy if lddy is not None else cols, ldx if ldx is not None else cols, lddx if lddx is not None else cols,
+         stream)
+
+
+def _attention_sizes(batch, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, ldq, ldk, ldv, ldo, scale,
+                     causal):
+    ldq = ldq if ldq is not None else heads * head_dim
+    ldk = ldk if ldk is not None else kv_heads * head_dim
+    ldv = ldv if ldv is not None else kv_heads * head_dim
+    ldo = ldo if ldo is not None else heads * head_dim
+    scale = scale if scale is not None else head_dim ** -0.5
+    return (batch, total_q, total_k, max_q if max_q is not None else total_q, max_k if max_k is not None else total_k,
+            heads, kv_heads, head_dim, ldq, ldk, ldv, ldo, scale, int(causal))
+
+
+def attention(q, k, v, o, lse, cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, head_dim, max_q=None,
+              max_k=None, ldq=None, ldk=None, ldv=None, ldo=None, scale=None, causal=True, stream=None):
+    """Attention over packed sequences with grouped heads; lse [heads, total_q] may be None.
+    Row strides default to dense rows, scale to 1 / sqrt(head_dim)."""
+    call("jx_attention_f32", q, k, v, o, lse, cu_q, cu_k,
+         *_attention_sizes(batch, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, ldq, ldk, ldv, ldo,
+                           scale, causal), stream)
+
+
+def attention_bwd(q, k, v, o, lse, dout, dq, dk, dv, cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, head_dim,
+                  max_q=None, max_k=None, ldq=None, ldk=None, ldv=None, ldo=None, scale=None, causal=True,
+                  stream=None):
+    """Gradients of attention; dout has o's row stride, dq, dk and dv those of q, k and v."""
+    call("jx_attention_bwd_f32", q, k, v, o, lse, dout, dq, dk, dv, cu_q, cu_k,
+         *_attention_sizes(batch, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, ldq, ldk, ldv, ldo,
+                           scale, causal), stream)
+
+
+def grad_norm(grads, sizes, count, norm_out, stream=None):
+    """Global norm over `count` tensors; grads and sizes are ctypes arrays (c_void_p, c_int64)."""
+    call("jx_grad_norm_f32", grads, sizes, count, norm_out, stream)
+
+
+def clip_grads(grads, outs, sizes, count, max_norm, norm_out=None, stream=None):
+    """outs[i] = grads[i] * min(1, max_norm / (norm + 1e-6)); outs may be grads."""
+    call("jx_clip_grads_f32", grads, outs, sizes, count, max_norm, norm_out, stream)
 
 
 class MLP:

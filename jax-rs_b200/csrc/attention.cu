@@ -1,0 +1,167 @@
+// attention.cu -- scaled dot-product attention over packed sequences with
+// grouped heads, forward and backward.
+//
+//   nn::scaled_dot_product_attention / multi_head_attention src/nn.rs:1460,1556
+//   (CPU loops over one sequence, untraced)
+//
+//   forward   x = scale q k^T, o = softmax(x) v, lse = log(sum exp(x))
+//   backward  p = exp(x - lse), dv = p^T do, ds = p (do v^T - rowsum(do o)),
+//             dq = scale ds k, dk = scale ds^T q
+#include <algorithm>
+
+#include "attn_common.cuh"
+
+namespace {
+
+using namespace jxa;
+
+constexpr int ROW_WARPS = 8;
+
+// One warp per (query row, head).
+__global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_fwd_kernel(const __grid_constant__ Shape s,
+                                                                      const float* __restrict__ q,
+                                                                      const float* __restrict__ k,
+                                                                      const float* __restrict__ v, float* o,
+                                                                      float* lse) {
+  const long long w = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+  const long long t = w / s.heads;
+  const int h = (int)(w - t * s.heads);
+  if (t >= s.total_q) return;
+  const int b = seq_of_row(s.cu_q, s.batch, t);
+  if (b < 0) return;
+  const Seq sq = seq_bounds(s, b);
+  if (t < sq.q0 || t >= sq.q0 + sq.lq) return;
+  const int hk = h / s.group;
+  row_fwd(q + t * s.ldq + (long long)h * s.dim, k + sq.k0 * s.ldk + (long long)hk * s.dim,
+          v + sq.k0 * s.ldv + (long long)hk * s.dim, o + t * s.ldo + (long long)h * s.dim,
+          lse ? lse + (long long)h * s.total_q + t : nullptr, sq.visible((int)(t - sq.q0), s.causal), s.dim, s.ldk,
+          s.ldv, s.scale);
+}
+
+__global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dq_kernel(const __grid_constant__ Shape s,
+                                                                     const float* __restrict__ q,
+                                                                     const float* __restrict__ k,
+                                                                     const float* __restrict__ v,
+                                                                     const float* __restrict__ o,
+                                                                     const float* __restrict__ lse,
+                                                                     const float* __restrict__ dout, float* dq) {
+  const long long w = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+  const long long t = w / s.heads;
+  const int h = (int)(w - t * s.heads);
+  if (t >= s.total_q) return;
+  const int b = seq_of_row(s.cu_q, s.batch, t);
+  if (b < 0) return;
+  const Seq sq = seq_bounds(s, b);
+  if (t < sq.q0 || t >= sq.q0 + sq.lq) return;
+  const long long hk = h / s.group, hd = (long long)h * s.dim;
+  row_dq(q + t * s.ldq + hd, k + sq.k0 * s.ldk + hk * s.dim, v + sq.k0 * s.ldv + hk * s.dim, o + t * s.ldo + hd,
+         dout + t * s.ldo + hd, lse[(long long)h * s.total_q + t], dq + t * s.ldq + hd,
+         sq.visible((int)(t - sq.q0), s.causal), s.dim, s.ldk, s.ldv, s.scale);
+}
+
+// One warp per (key row, key head).
+__global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dkv_kernel(const __grid_constant__ Shape s,
+                                                                      const float* __restrict__ q,
+                                                                      const float* __restrict__ k,
+                                                                      const float* __restrict__ v,
+                                                                      const float* __restrict__ o,
+                                                                      const float* __restrict__ lse,
+                                                                      const float* __restrict__ dout, float* dk,
+                                                                      float* dv) {
+  const long long w = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+  const long long t = w / s.kv_heads;
+  const int hk = (int)(w - t * s.kv_heads);
+  if (t >= s.total_k) return;
+  const int b = seq_of_row(s.cu_k, s.batch, t);
+  if (b < 0) return;
+  const Seq sq = seq_bounds(s, b);
+  if (t < sq.k0 || t >= sq.k0 + sq.lk) return;
+  const long long hd = (long long)hk * s.dim, h0 = (long long)hk * s.group;
+  row_dkv(q + sq.q0 * s.ldq + h0 * s.dim, o + sq.q0 * s.ldo + h0 * s.dim, dout + sq.q0 * s.ldo + h0 * s.dim,
+          lse + h0 * s.total_q + sq.q0, k + t * s.ldk + hd, v + t * s.ldv + hd, dk + t * s.ldk + hd,
+          dv + t * s.ldv + hd, sq.first_row((int)(t - sq.k0), s.causal), sq.lq, s.group, s.dim, s.ldq, s.ldo,
+          s.total_q, s.scale);
+}
+
+int check_shape(const char* what, Shape& s, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q,
+                int64_t total_k, int64_t max_q, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int causal) {
+  JX_REQUIRE(batch >= 0 && batch < (1 << 24), "%s: batch must be in [0, 2^24)", what);
+  JX_REQUIRE(total_q >= 0 && total_q < (1LL << 31) && total_k >= 0 && total_k < (1LL << 31),
+             "%s: total_q and total_k must be in [0, 2^31)", what);
+  JX_REQUIRE(max_q >= 0 && max_k >= 0, "%s: max_q and max_k must not be negative", what);
+  JX_REQUIRE(heads >= 1 && kv_heads >= 1 && heads <= 65535 && heads % kv_heads == 0,
+             "%s: heads must be a multiple of kv_heads (and at most 65535)", what);
+  JX_REQUIRE(head_dim >= 1 && head_dim <= MAX_DIM, "%s: head_dim must be in [1, %d]", what, MAX_DIM);
+  JX_REQUIRE(ldq >= heads * head_dim && ldo >= heads * head_dim && ldk >= kv_heads * head_dim &&
+                 ldv >= kv_heads * head_dim,
+             "%s: row stride smaller than the row", what);
+  JX_REQUIRE(isfinite(scale), "%s: scale must be finite", what);
+  s.cu_q = cu_q;
+  s.cu_k = cu_k;
+  s.batch = (int)batch;
+  s.heads = (int)heads;
+  s.kv_heads = (int)kv_heads;
+  s.group = (int)(heads / kv_heads);
+  s.dim = (int)head_dim;
+  s.total_q = total_q;
+  s.total_k = total_k;
+  s.ldq = ldq;
+  s.ldk = ldk;
+  s.ldv = ldv;
+  s.ldo = ldo;
+  s.scale = scale;
+  s.causal = causal != 0;
+  return JX_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int jx_attention_f32(const float* q, const float* k, const float* v, float* o, float* lse, const int32_t* cu_q,
+                     const int32_t* cu_k, int64_t batch, int64_t total_q, int64_t total_k, int64_t max_q,
+                     int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t ldq, int64_t ldk,
+                     int64_t ldv, int64_t ldo, float scale, int causal, jx_stream_t stream) {
+  JX_TRACE("jx_attention_f32");
+  Shape s;
+  if (int rc = check_shape("attention", s, cu_q, cu_k, batch, total_q, total_k, max_q, max_k, heads, kv_heads,
+                           head_dim, ldq, ldk, ldv, ldo, scale, causal))
+    return rc;
+  if (batch == 0 || total_q == 0) return JX_OK;
+  JX_REQUIRE(q && o && cu_q && cu_k && (total_k == 0 || (k && v)), "attention: NULL pointer");
+  cudaStream_t st = jx::as_stream(stream);
+  s.err = jx::device_error_word();
+  const long long blocks = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
+  JX_REQUIRE(blocks < (1LL << 31), "attention: too many rows");
+  attn_rows_fwd_kernel<<<(unsigned)blocks, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse);
+  JX_LAUNCH_CHECK("attn_rows_fwd_kernel");
+  return JX_OK;
+}
+
+int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
+                         const float* dout, float* dq, float* dk, float* dv, const int32_t* cu_q, const int32_t* cu_k,
+                         int64_t batch, int64_t total_q, int64_t total_k, int64_t max_q, int64_t max_k, int64_t heads,
+                         int64_t kv_heads, int64_t head_dim, int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo,
+                         float scale, int causal, jx_stream_t stream) {
+  JX_TRACE("jx_attention_bwd_f32");
+  Shape s;
+  if (int rc = check_shape("attention_bwd", s, cu_q, cu_k, batch, total_q, total_k, max_q, max_k, heads, kv_heads,
+                           head_dim, ldq, ldk, ldv, ldo, scale, causal))
+    return rc;
+  if (batch == 0 || (total_q == 0 && total_k == 0)) return JX_OK;
+  JX_REQUIRE(cu_q && cu_k, "attention_bwd: NULL pointer");
+  JX_REQUIRE(total_q == 0 || (q && o && lse && dout && dq), "attention_bwd: NULL pointer");
+  JX_REQUIRE(total_k == 0 || (k && v && dk && dv), "attention_bwd: NULL pointer");
+  cudaStream_t st = jx::as_stream(stream);
+  s.err = jx::device_error_word();
+  const long long bq = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
+  const long long bk = (total_k * kv_heads + ROW_WARPS - 1) / ROW_WARPS;
+  JX_REQUIRE(bq < (1LL << 31) && bk < (1LL << 31), "attention_bwd: too many rows");
+  if (bq) attn_rows_dq_kernel<<<(unsigned)bq, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse, dout, dq);
+  if (bk) attn_rows_dkv_kernel<<<(unsigned)bk, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse, dout, dk, dv);
+  JX_LAUNCH_CHECK("attention_bwd kernels");
+  return JX_OK;
+}
+
+}  // extern "C"

@@ -82,6 +82,7 @@ int tensor_map_f32_3d(CUtensorMap_st* map, const void* base, const uint64_t* dim
 // Device error codes recorded in the device error word (bit flags).
 #define JX_DEVERR_NAN 0x1u
 #define JX_DEVERR_TIMEOUT 0x2u
+#define JX_DEVERR_RANGE 0x4u
 
 // ---------------------------------------------------------------------------
 // Device-side PTX helpers (sm_100a)
