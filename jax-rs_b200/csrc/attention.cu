@@ -9,7 +9,7 @@
 //             dq = scale ds k, dk = scale ds^T q
 #include <algorithm>
 
-#include "attn_common.cuh"
+#include "attn_tc.cuh"
 
 namespace {
 
@@ -132,6 +132,7 @@ int jx_attention_f32(const float* q, const float* k, const float* v, float* o, f
   JX_REQUIRE(q && o && cu_q && cu_k && (total_k == 0 || (k && v)), "attention: NULL pointer");
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
+  if (total_k > 0 && max_q * s.group > 16) return attention_fwd_tiles(s, q, k, v, o, lse, st);
   const long long blocks = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
   JX_REQUIRE(blocks < (1LL << 31), "attention: too many rows");
   attn_rows_fwd_kernel<<<(unsigned)blocks, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse);

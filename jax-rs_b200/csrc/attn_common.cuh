@@ -95,7 +95,7 @@ __device__ __forceinline__ void row_store(float* p, const float (&r)[ROW_E], flo
 }
 
 // o[0 .. dim) and the log-sum-exp of one query row over nk keys.
-__device__ __noinline__ void row_fwd(const float* q, const float* k, const float* v, float* o, float* lse, int nk,
+static __device__ __noinline__ void row_fwd(const float* q, const float* k, const float* v, float* o, float* lse, int nk,
                                      int dim, long long ldk, long long ldv, float scale) {
   const int lane = threadIdx.x & 31, g = lane >> 3, l = lane & 7;
   float qr[ROW_E], acc[ROW_E];
@@ -133,7 +133,7 @@ __device__ __noinline__ void row_fwd(const float* q, const float* k, const float
 }
 
 // dq of one query row over nk keys.
-__device__ __noinline__ void row_dq(const float* q, const float* k, const float* v, const float* o, const float* dout,
+static __device__ __noinline__ void row_dq(const float* q, const float* k, const float* v, const float* o, const float* dout,
                                     float lse, float* dq, int nk, int dim, long long ldk, long long ldv,
                                     float scale) {
   const int lane = threadIdx.x & 31, g = lane >> 3, l = lane & 7;
@@ -163,7 +163,7 @@ __device__ __noinline__ void row_dq(const float* q, const float* k, const float*
 // dk and dv of one key row: query rows i0 .. lq-1 of the `group` heads that
 // share it.  q, o and dout point at the sequence's first row of the group's
 // first head, lse at that head's entry of the same row.
-__device__ __noinline__ void row_dkv(const float* q, const float* o, const float* dout, const float* lse,
+static __device__ __noinline__ void row_dkv(const float* q, const float* o, const float* dout, const float* lse,
                                      const float* k, const float* v, float* dk, float* dv, int i0, int lq, int group,
                                      int dim, long long ldq, long long ldo, long long total_q, float scale) {
   const int lane = threadIdx.x & 31, g = lane >> 3, l = lane & 7;

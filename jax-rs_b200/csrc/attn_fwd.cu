@@ -1,0 +1,491 @@
+// attn_fwd.cu -- attention's forward pass on the tensor cores, and the split of
+// its streamed operands into f16 tiles (attn_tc.cuh).
+//
+// One CTA per (128 query rows, head).  Q's parts lie in tensor memory; K and V
+// tiles of 128 keys stream through shared memory.  Per key tile j:
+//   S = Q K^T          24 MMAs of 128 x 128 x 16 (3 parts x 8 steps) for dim 128
+//   P = exp2(S f - m)  eight warps, two threads per row, 64 columns each; P's
+//                      parts go back over S's columns
+//   part = P V         24 MMAs, A from tensor memory
+//   O = O alpha + part in registers, 64 columns per thread
+// The MMA warp issues S(j+1) before part(j), so the softmax of tile j+1 has the
+// time of part(j) and S(j+2): 3072 cycles of MMA at dim 128 against about 1500 of
+// ALU work.  Tensor memory: S twice 128 columns, Q 128, part 128.
+#include <algorithm>
+#include <atomic>
+
+#include "attn_tc.cuh"
+
+namespace {
+
+using namespace jxa;
+using jxg::wait_bounded;
+
+// ---- splitting -----------------------------------------------------------------
+// One block per (tile, head, tensor): 16 threads per row, 8 columns each (4 for DP = 64).
+template <int DP>
+__global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant__ Shape s, int over_q,
+                                                         const __grid_constant__ TileSources src, int heads) {
+  constexpr int CW = DP / 16;  // columns per thread
+  __shared__ uint32_t sm_top[8], sm_low[8];
+  const TileSource& t = src.t[blockIdx.z];
+  const int id = blockIdx.x, h = blockIdx.y;
+  int j;
+  const int b = seq_of_tile(over_q ? s.cu_q : s.cu_k, s.batch, id, &j);
+  const Seq sq = seq_bounds(s, b);
+  const int len = over_q ? sq.lq : sq.lk;
+  if (j < 0 || (long long)j * TILE >= len) return;
+  const long long row0 = (over_q ? sq.q0 : sq.k0) + (long long)j * TILE;
+  const int rows = min(TILE, len - j * TILE);
+  const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int col = c * CW;
+  const float* base = t.x + row0 * t.ld + (long long)h * s.dim + col;
+  const bool vec = (s.dim & 3) == 0 && (t.ld & 3) == 0 && (reinterpret_cast<uintptr_t>(t.x) & 15) == 0;
+  float x[8][CW];
+  uint32_t top = 0, low = 0x7fffffffu;  // the tile's largest row maximum, and the smallest one that is not zero
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
+#pragma unroll
+    for (int e = 0; e < CW; e += 4) {
+      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < rows) {
+        const float* p = base + (long long)r * t.ld + e;
+        if (vec && col + e + 4 <= s.dim) {
+          f = *reinterpret_cast<const float4*>(p);
+        } else {
+          if (col + e < s.dim) f.x = p[0];
+          if (col + e + 1 < s.dim) f.y = p[1];
+          if (col + e + 2 < s.dim) f.z = p[2];
+          if (col + e + 3 < s.dim) f.w = p[3];
+        }
+      }
+      x[i][e] = f.x;
+      x[i][e + 1] = f.y;
+      x[i][e + 2] = f.z;
+      x[i][e + 3] = f.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < CW; ++e) m = max(m, __float_as_uint(x[i][e]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    top = max(top, m);
+    if (m) low = min(low, m);
+  }
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
+  low = min(low, __shfl_xor_sync(0xffffffffu, low, 16));
+  if ((threadIdx.x & 31) == 0) {
+    sm_top[threadIdx.x >> 5] = top;
+    sm_low[threadIdx.x >> 5] = low;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    top = max(top, sm_top[w]);
+    low = min(low, sm_low[w]);
+  }
+  const int e_top = (int)(top >> 23), e_low = (int)(low >> 23);
+  const long long slot = (long long)id * heads + h;
+  if (threadIdx.x == 0) {
+    t.inverse[slot] = inverse_of(e_top);
+    t.bad[slot] = e_top == 255 || (top && e_top - max(e_low, 15) > WIDE_BITS);
+  }
+  const float factor = scale_of(min(e_top, 254));
+  uint8_t* out = t.tiles + slot * tile_bytes(DP);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
+    uint32_t hi[CW / 2], lo[CW / 2];
+#pragma unroll
+    for (int e = 0; e < CW / 2; ++e) split_half(x[i][2 * e] * factor, x[i][2 * e + 1] * factor, hi[e], lo[e]);
+    const int at = col * 2;  // byte of the row
+    uint8_t* p = out + (at >> 7) * PANEL + r * 128 + ((((at & 127) >> 4) ^ (r & 7)) << 4) + (at & 15);
+    if constexpr (CW == 8) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(p + tile_part(DP)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    } else {
+      *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(p + tile_part(DP)) = make_uint2(lo[0], lo[1]);
+    }
+  }
+}
+
+// ---- forward -------------------------------------------------------------------
+constexpr int FW_THREADS = 384;  // warp 0 copies, warp 1 MMA, warps 4..11 softmax
+constexpr int FW_FIRST = 4;
+constexpr int FW_LAUNCH_REGS = 168;
+constexpr int FW_LOW_REGS = 56;
+constexpr int FW_HIGH_REGS = 216;
+static_assert(128 * FW_LOW_REGS + 256 * FW_HIGH_REGS <= FW_THREADS * FW_LAUNCH_REGS,
+              "register split exceeds the launch allocation");
+constexpr uint32_t T_Q = 256, T_O = 384;  // columns of tensor memory; S0 at 0, S1 at 128
+constexpr float P_SHIFT = 14.0f;          // P is scaled by 2^14 for its f16 parts
+
+__host__ __device__ constexpr int fw_stages(int DP) { return DP == 128 ? 3 : 6; }
+__host__ __device__ constexpr size_t fw_smem(int DP) {
+  return (size_t)fw_stages(DP) * tile_bytes(DP) + 1024 /*align*/ + 2 * 128 * 4 /*exchange*/ + 256 /*barriers*/;
+}
+
+struct FwdTiles {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* inv_k;
+  const float* inv_v;
+  const int* bad_k;
+  const int* bad_v;
+  int q_tiles;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(FW_THREADS, 1)
+    attn_fwd_kernel(const __grid_constant__ Shape s, const __grid_constant__ FwdTiles ft, const float* __restrict__ q,
+                    const float* __restrict__ k, const float* __restrict__ v, float* o, float* lse) {
+  constexpr int STAGES = fw_stages(DP), STAGE = tile_bytes(DP), PART = tile_part(DP);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = jxd::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  float* xch = reinterpret_cast<float*>(smem + STAGES * STAGE);  // [2][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(xch + 2 * 128);   // [STAGES]
+  uint64_t* empty = full + STAGES;                               // [STAGES]
+  uint64_t* sfull = empty + STAGES;                              // [2]
+  uint64_t* pfull = sfull + 2;                                   // [2]
+  uint64_t* ofull = pfull + 2;
+  uint64_t* ofree = ofull + 1;
+  uint64_t* qfull = ofree + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(qfull + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the last tiles of a sequence, which see the most keys, start first
+  const int id = ft.q_tiles - 1 - (int)(blockIdx.x / (unsigned)s.heads), h = (int)(blockIdx.x % (unsigned)s.heads);
+  int jt;
+  const int b = seq_of_tile(s.cu_q, s.batch, id, &jt);
+  const Seq sq = seq_bounds(s, b);
+  if (jt < 0 || (long long)jt * TILE >= sq.lq) return;
+  const int i0 = jt * TILE, rows = min(TILE, sq.lq - i0);
+  const int hk = h / s.group;
+  const int nk = sq.visible(i0 + rows - 1, s.causal);  // keys that the tile's last row sees
+  const int nb = (nk + TILE - 1) / TILE;
+  const long long slot0 = (long long)first_tile(sq.k0, b) * s.kv_heads + hk;
+
+  // Q's rows, and whether the tile has to be computed row by row
+  const int quarter = warp & 3, half = (warp - FW_FIRST) >> 2;
+  const int row = quarter * 32 + lane;
+  const bool soft = warp >= FW_FIRST;
+  float x[DP / 2];
+  uint32_t top = 0;
+  if (soft) {
+    const bool vec = (s.dim & 3) == 0 && (s.ldq & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+    top = row_half_load<DP>(
+        x, row < rows ? q + (sq.q0 + i0 + row) * s.ldq + (long long)h * s.dim : nullptr, s.dim, half, vec);
+    reinterpret_cast<uint32_t*>(xch)[half * 128 + row] = top;
+  }
+  bool bad = top >= 0x7f800000u;
+  for (int j = threadIdx.x; j < nb; j += FW_THREADS)
+    bad = bad || ft.bad_k[slot0 + (long long)j * s.kv_heads] || ft.bad_v[slot0 + (long long)j * s.kv_heads];
+  if (__syncthreads_or(bad)) {
+    for (int r = warp; r < rows; r += FW_THREADS / 32) {
+      const long long t = sq.q0 + i0 + r;
+      row_fwd(q + t * s.ldq + (long long)h * s.dim, k + sq.k0 * s.ldk + (long long)hk * s.dim,
+              v + sq.k0 * s.ldv + (long long)hk * s.dim, o + t * s.ldo + (long long)h * s.dim,
+              lse ? lse + (long long)h * s.total_q + t : nullptr, sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv,
+              s.scale);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      jxd::mbar_init(&full[i], 1);
+      jxd::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      jxd::mbar_init(&sfull[i], 1);
+      jxd::mbar_init(&pfull[i], 8);
+    }
+    jxd::mbar_init(ofull, 1);
+    jxd::mbar_init(ofree, 8);
+    jxd::mbar_init(qfull, 8);
+    *abort_flag = 0;
+    jxd::fence_mbar_init();
+  }
+  if (warp == 1) {
+    jxd::tmem_alloc(tmem_slot, 512);
+    jxd::tmem_relinquish();
+  }
+  jxd::tc_fence_before();
+  __syncthreads();
+  jxd::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (!soft) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FW_LOW_REGS));
+    if (warp == 0 && jxd::elect_one()) {
+      // ---- copies, in the order of use: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1)
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      for (int u = 0; u < 2 * nb; ++u) {
+        const bool is_v = u == 2 * nb - 1 || (u >= 2 && (u & 1) == 0);
+        const int j = u == 0 ? 0 : u == 2 * nb - 1 ? nb - 1 : is_v ? u / 2 - 1 : (u + 1) / 2;
+        if (*abort_flag || !wait_bounded(&empty[stage], phase ^ 1u, s.err)) { *abort_flag = 1; break; }
+        jxd::mbar_arrive_expect_tx(&full[stage], STAGE);
+        bulk_load(jxd::smem_u32(smem + stage * STAGE),
+                  (is_v ? ft.v : ft.k) + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE, &full[stage]);
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      }
+      // every copy has landed before the CTA may end
+      for (int u = max(0, issued - STAGES); u < issued; ++u)
+        wait_bounded(&full[u % STAGES], (uint32_t)(u / STAGES) & 1u, s.err);
+    }
+    if (warp == 1 && nb > 0 && jxd::elect_one()) {
+      // ---- MMA
+      constexpr uint32_t id_s = idesc_f16(128, false), id_o = idesc_f16(DP, true);
+      const uint32_t sbase = jxd::smem_u32(smem);
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = wait_bounded(qfull, 0, s.err);
+      auto scores = [&](int j) {
+        if (!ok || !(ok = !*abort_flag && wait_bounded(&full[stage], phase, s.err))) return;
+        jxd::tc_fence_after();
+        const uint32_t kt = sbase + stage * STAGE, d = tmem + (j & 1) * 128u;
+        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
+          mma_f16_ts(d, tmem + T_Q + a + ks * 8, jxd::smem_desc_k_sw128(kt + part + (ks >> 2) * PANEL + (ks & 3) * 32),
+                     id_s, acc);
+        };
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          step(ks, DP / 2, 0, ks > 0);  // lo.hi
+          step(ks, 0, PART, 1);         // hi.lo
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
+        jxd::mma_commit(&sfull[j & 1]);
+        jxd::mma_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      };
+      scores(0);
+      for (int j = 0; j < nb && ok; ++j) {
+        if (j + 1 < nb) scores(j + 1);
+        if (!ok || !(ok = !*abort_flag && wait_bounded(&full[stage], phase, s.err) &&
+                          wait_bounded(&pfull[j & 1], (uint32_t)(j >> 1) & 1u, s.err) &&
+                          wait_bounded(ofree, (uint32_t)(j + 1) & 1u, s.err)))
+          break;
+        jxd::tc_fence_after();
+        const uint32_t vt = sbase + stage * STAGE, p = tmem + (j & 1) * 128u, d = tmem + T_O;
+        // P's keys 0..63: hi at column 0, lo at 32; keys 64..127: hi at 64, lo at 96
+        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
+          mma_f16_ts(d, p + a + (ks >> 2) * 64 + (ks & 3) * 8, smem_desc_mn_sw128(vt + part + ks * 2048, PANEL), id_o,
+                     acc);
+        };
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          step(ks, 32, 0, ks > 0);
+          step(ks, 0, PART, 1);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) step(ks, 0, 0, 1);
+        jxd::mma_commit(ofull);
+        jxd::mma_commit(&empty[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FW_HIGH_REGS));
+    // ---- softmax and output
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int e_row = (int)(max(top, reinterpret_cast<uint32_t*>(xch)[(half ^ 1) * 128 + row]) >> 23);
+    row_half_store<DP>(x, s.scale < 0.0f ? -scale_of(e_row) : scale_of(e_row), tmem + lanes + T_Q, half);
+    tmem_st_wait();
+    jxd::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) jxd::mbar_arrive(qfull);
+    const float f_row = inverse_of(e_row) * (fabsf(s.scale) * LOG2E);
+    const int vis = row < rows ? sq.visible(i0 + row, s.causal) : 0;
+    const int vis_all = sq.visible(i0, s.causal);  // keys that every row of the tile sees
+
+    float acc[DP / 2];
+#pragma unroll
+    for (int c = 0; c < DP / 2; ++c) acc[c] = 0.0f;
+    float m = -INFINITY, sum = 0.0f, alpha_prev = 0.0f, inv_v_prev = 0.0f;
+    bool ok = true;
+
+    auto add_part = [&](int j, float alpha, float inv_v) {
+      ok = ok && jxg::warp_wait_bounded(ofull, (uint32_t)j & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < DP / 2; c += 32) {
+        uint32_t r[32];
+        jxd::tmem_ld32(tmem + lanes + T_O + half * (DP / 2) + c, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 part = make_float2(__uint_as_float(r[i]) * inv_v, __uint_as_float(r[i + 1]) * inv_v);
+          const float2 v2 = fma2(make_float2(acc[c + i], acc[c + i + 1]), make_float2(alpha, alpha), part);
+          acc[c + i] = v2.x;
+          acc[c + i + 1] = v2.y;
+        }
+      }
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(ofree);
+    };
+
+    for (int j = 0; j < nb; ++j) {
+      const float inv_k = ft.inv_k[slot0 + (long long)j * s.kv_heads];
+      const float inv_v = ft.inv_v[slot0 + (long long)j * s.kv_heads];
+      const float f = fmaxf(f_row * inv_k, 1.17549435e-38f);  // above zero, so that a masked score stays -inf
+      ok = ok && jxg::warp_wait_bounded(&sfull[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+      const uint32_t s_addr = tmem + lanes + (j & 1) * 128u + half * 64u;
+      float sc[64];
+      {
+        uint32_t r[32];
+        jxd::tmem_ld32(s_addr, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sc[i] = __uint_as_float(r[i]);
+        jxd::tmem_ld32(s_addr + 32, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sc[32 + i] = __uint_as_float(r[i]);
+      }
+      const int key0 = j * TILE + half * 64;
+      if (j * TILE + TILE > vis_all) {  // some row does not see all of the tile's keys
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (key0 + i >= vis) sc[i] = -INFINITY;
+      }
+      float mx = sc[0];
+#pragma unroll
+      for (int i = 1; i < 64; ++i) mx = fmaxf(mx, sc[i]);
+      // the row's other half
+      xch[half * 128 + row] = mx;
+      pair_sync(1 + quarter);
+      mx = fmaxf(mx, xch[(half ^ 1) * 128 + row]);
+      pair_sync(1 + quarter);
+      const float m_new = mx == -INFINITY ? m : fmaxf(m, mx * f);
+      const float base = m_new == -INFINITY ? 0.0f : m_new;
+      const float alpha = exp2_fast(m - base);
+      m = m_new;
+      const float2 f2 = make_float2(f, f), b2 = make_float2(P_SHIFT - base, P_SHIFT - base);
+      float2 add = make_float2(0.0f, 0.0f);
+      uint32_t hi[32], lo[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float2 z = fma2(make_float2(sc[2 * i], sc[2 * i + 1]), f2, b2);
+        const float2 p = make_float2(exp2_fast(z.x), exp2_fast(z.y));
+        add.x += p.x;
+        add.y += p.y;
+        split_half(p.x, p.y, hi[i], lo[i]);
+      }
+      sum = sum * alpha + (add.x + add.y);
+      tmem_st32(s_addr, hi);
+      tmem_st32(s_addr + 32, lo);
+      tmem_st_wait();
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(&pfull[j & 1]);
+      if (j > 0) add_part(j - 1, alpha_prev, inv_v_prev);
+      alpha_prev = alpha;
+      inv_v_prev = inv_v;
+    }
+    if (nb > 0) add_part(nb - 1, alpha_prev, inv_v_prev);
+
+    xch[half * 128 + row] = sum;
+    pair_sync(1 + quarter);
+    sum += xch[(half ^ 1) * 128 + row];
+    if (row < rows) {
+      const long long t = sq.q0 + i0 + row;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      float* out = o + t * s.ldo + (long long)h * s.dim + half * (DP / 2);
+      const int n = s.dim - half * (DP / 2);
+      if ((s.dim & 3) == 0 && (s.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+        for (int c = 0; c < DP / 2; c += 4)
+          if (c < n)
+            *reinterpret_cast<float4*>(out + c) =
+                make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
+      } else {
+#pragma unroll
+        for (int c = 0; c < DP / 2; ++c)
+          if (c < n) out[c] = acc[c] * inv;
+      }
+      if (lse && half == 0)
+        lse[(long long)h * s.total_q + t] = sum == 0.0f ? -INFINITY : (m + (log2f(sum) - P_SHIFT)) * LN2;
+    }
+  }
+  jxd::tc_fence_before();
+  __syncthreads();
+  jxd::tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    jxd::tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+namespace jxa {
+
+int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st) {
+  const long long tiles = tile_count(over_q ? s.total_q : s.total_k, s.batch);
+  const dim3 grid((unsigned)tiles, (unsigned)heads, (unsigned)count);
+  if (DP == 128) split_tiles_kernel<128><<<grid, 256, 0, st>>>(s, over_q, src, heads);
+  else split_tiles_kernel<64><<<grid, 256, 0, st>>>(s, over_q, src, heads);
+  JX_LAUNCH_CHECK("split_tiles_kernel");
+  return JX_OK;
+}
+
+// Per device and variant, once: the shared-memory limit and the registers the kernel was built with.
+int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs) {
+  static std::atomic<int> done[64][8];
+  int dev = 0;
+  JX_CUDA(cudaGetDevice(&dev));
+  std::atomic<int>& d = done[dev & 63][variant];
+  if (d.load(std::memory_order_acquire)) return JX_OK;
+  cudaFuncAttributes fa;
+  JX_CUDA(cudaFuncGetAttributes(&fa, kernel));
+  if (fa.numRegs != launch_regs)  // setmaxnreg.inc would wait for registers that never come
+    return jx::fail(JX_EUNSUPPORTED, "attention kernel built with %d registers per thread, expected %d", fa.numRegs,
+                    launch_regs);
+  JX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  d.store(1, std::memory_order_release);
+  return JX_OK;
+}
+
+int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
+                        cudaStream_t st) {
+  const int DP = s.dim <= 64 ? 64 : 128;
+  const long long kt = tile_count(s.total_k, s.batch), qt = tile_count(s.total_q, s.batch);
+  JX_REQUIRE(qt * s.heads < (1LL << 31) && kt < (1LL << 31), "attention: too many rows");
+  const size_t slots = (size_t)kt * s.kv_heads, bytes = slots * tile_bytes(DP);
+  void* p = nullptr;
+  if (int rc = jx::scratch_get(2 * bytes + 4 * slots * sizeof(float), &p, st)) return rc;
+  uint8_t* base = static_cast<uint8_t*>(p);
+  float* inv = reinterpret_cast<float*>(base + 2 * bytes);
+  int* bad = reinterpret_cast<int*>(inv + 2 * slots);
+  TileSources src = {{{k, s.ldk, base, inv, bad}, {v, s.ldv, base + bytes, inv + slots, bad + slots}}};
+  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, (int)qt};
+  int rc = split_tiles(s, false, src, 2, s.kv_heads, DP, st);
+  if (!rc) {
+    const unsigned grid = (unsigned)(qt * s.heads);
+    if (DP == 128) {
+      if (!(rc = prepare_kernel((const void*)attn_fwd_kernel<128>, 0, fw_smem(128), FW_LAUNCH_REGS)))
+        attn_fwd_kernel<128><<<grid, FW_THREADS, fw_smem(128), st>>>(s, ft, q, k, v, o, lse);
+    } else {
+      if (!(rc = prepare_kernel((const void*)attn_fwd_kernel<64>, 1, fw_smem(64), FW_LAUNCH_REGS)))
+        attn_fwd_kernel<64><<<grid, FW_THREADS, fw_smem(64), st>>>(s, ft, q, k, v, o, lse);
+    }
+    const cudaError_t e = cudaGetLastError();
+    if (!rc && e != cudaSuccess) rc = jx::check_cuda(e, "attn_fwd_kernel");
+  }
+  jx::scratch_release(p, st);
+  return rc;
+}
+
+}  // namespace jxa

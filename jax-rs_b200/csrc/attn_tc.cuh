@@ -1,0 +1,216 @@
+// attn_tc.cuh -- the tensor-core attention kernels' shared pieces: operand
+// tiles split into two f16 parts, their layout in scratch and shared memory,
+// and the tcgen05 wrappers for operands in tensor memory.
+//
+// Numbers.  An f32 operand x is held as hi + lo, hi = f16(x s), lo = f16(x s -
+// hi), with s a power of two that brings the largest magnitude of its scaling
+// group (a row of the operand that stays, a tile of 128 rows of the one that
+// streams) into [2^14, 2^15).  hi + lo keeps 22 bits of every value within 2^-17
+// of the largest and an absolute 2^-39 of the largest below that.  A product is
+// lo.hi + hi.lo + hi.hi, three f16 products with f32 sums: twice the rate of
+// the same with tf32 parts, whose 22 bits are the same.  A tile that holds a
+// non-finite value, or rows whose largest values differ by more than 2^20, is
+// marked; the tiles of output that need it are computed row by row in plain f32.
+//
+// Sums.  The tensor core truncates as it accumulates, so a sum in tensor memory
+// spans at most 128 terms, small parts first; spans are added in f32 registers.
+//
+// Layout.  Tile (id, head): 128 rows of DP = 64 or 128 columns (zero behind the
+// head's dim), [hi][lo], each part as panels of 64 columns: row r of a panel is
+// 128 bytes, its 16-byte chunk c at r * 128 + ((c ^ (r & 7)) * 16), the 128-byte
+// swizzle.  The same bytes serve as a K-major operand (rows x columns summed
+// over columns) and as an MN-major one (summed over rows).
+//
+// Tiles of a packed sequence.  Sequence b's tile j has id (start / 128) + b + j:
+// ids of different sequences never meet, whatever the lengths, and
+// total / 128 + batch of them are enough, so neither a table nor the lengths on
+// the host are needed.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "attn_common.cuh"
+#include "tc_gemm.cuh"
+
+namespace jxa {
+
+constexpr int TILE = 128;
+constexpr int PANEL = TILE * 128;  // bytes of 128 rows x 64 f16 columns
+constexpr int WIDE_BITS = 20;
+
+__host__ __device__ constexpr int tile_part(int DP) { return DP / 64 * PANEL; }      // one part of a tile
+__host__ __device__ constexpr int tile_bytes(int DP) { return 2 * tile_part(DP); }   // hi and lo
+
+inline long long tile_count(long long total, int batch) { return total / TILE + batch; }
+
+// Sequence and index within it of tile `id`; the index may lie behind the sequence's end.
+__device__ __forceinline__ int seq_of_tile(const int32_t* cu, int batch, int id, int* j) {
+  int lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((cu[mid] >> 7) + mid <= id) lo = mid;
+    else hi = mid;
+  }
+  *j = id - ((cu[lo] >> 7) + lo);
+  return lo;
+}
+__device__ __forceinline__ int first_tile(long long start, int b) { return (int)(start >> 7) + b; }
+
+// Power of two that brings a magnitude with biased exponent e into [2^14, 2^15), and its inverse.
+__device__ __forceinline__ float scale_of(int e) { return __uint_as_float((uint32_t)(268 - max(e, 15)) << 23); }
+__device__ __forceinline__ float inverse_of(int e) { return __uint_as_float((uint32_t)(max(e, 15) - 14) << 23); }
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b) {  // a in the low half
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  return r;
+}
+// hi and lo parts of two scaled values.
+__device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half(a, b);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_half(a - h.x, b - h.y);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+
+// ---- tcgen05 ------------------------------------------------------------------
+// D f32, A and B f16; N columns, M = 128 rows; B_MN: B is MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16(int N, bool B_MN) {
+  return (1u << 4) | (B_MN ? (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D[tmem] (+)= A[smem] * B[smem]
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// MN-major f16 operand with 128-byte swizzle: groups of eight k-rows 1024 B apart
+// (SBO), panels of 64 columns `panel` bytes apart (LBO).
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t panel) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((panel >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)((1024u >> 4) & 0x3FFFu) << 32;
+  d |= (uint64_t)1u << 46;
+  d |= (uint64_t)2u << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Untiled bulk copy, global -> shared, both 16-byte aligned.
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst),
+      "l"(src), "r"(bytes), "r"(jxd::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// ---- the operand that stays: rows of a [rows, heads, dim] tensor into tensor memory ----
+// Two warps share 32 rows (TMEM lanes); this thread's row is `src` (NULL: zeros)
+// and its columns are half * DP/2 ..+DP/2.  Returns the largest magnitude's bits.
+template <int DP>
+__device__ __forceinline__ uint32_t row_half_load(float (&x)[DP / 2], const float* src, int dim, int half, bool vec) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < DP / 2; c += 4) {
+    const int col = half * (DP / 2) + c;
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (src) {
+      if (vec && col + 4 <= dim) {
+        f = *reinterpret_cast<const float4*>(src + col);
+      } else {
+        if (col < dim) f.x = src[col];
+        if (col + 1 < dim) f.y = src[col + 1];
+        if (col + 2 < dim) f.z = src[col + 2];
+        if (col + 3 < dim) f.w = src[col + 3];
+      }
+    }
+    x[c] = f.x;
+    x[c + 1] = f.y;
+    x[c + 2] = f.z;
+    x[c + 3] = f.w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[c + i]) & 0x7fffffffu);
+  }
+  return top;
+}
+// Stores the scaled halves' parts: hi at column `col` of tensor memory, lo DP/2 columns behind it.
+template <int DP>
+__device__ __forceinline__ void row_half_store(const float (&x)[DP / 2], float factor, uint32_t taddr, int half) {
+  constexpr int N = DP / 4;  // packed columns of this half: 32 or 16
+  uint32_t hi[N], lo[N];
+#pragma unroll
+  for (int c = 0; c < N; ++c) split_half(x[2 * c] * factor, x[2 * c + 1] * factor, hi[c], lo[c]);
+  if constexpr (N == 32) {
+    tmem_st32(taddr + half * N, hi);
+    tmem_st32(taddr + DP / 2 + half * N, lo);
+  } else {
+    tmem_st16(taddr + half * N, hi);
+    tmem_st16(taddr + DP / 2 + half * N, lo);
+  }
+}
+
+// Streams that are split into tiles, for one launch of split_tiles_kernel.
+struct TileSource {
+  const float* x;
+  long long ld;
+  uint8_t* tiles;
+  float* inverse;  // of the tile's scale, [id][head]
+  int* bad;        // the tile is marked, [id][head]
+};
+struct TileSources {
+  TileSource t[2];
+};
+
+// Implemented in attn_fwd.cu: splits 1 or 2 tensors of `heads` heads over the same packed sequences.
+int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st);
+int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs);
+int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
+                        cudaStream_t st);
+
+}  // namespace jxa
