@@ -156,6 +156,8 @@ int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const f
   JX_REQUIRE(total_k == 0 || (k && v && dk && dv), "attention_bwd: NULL pointer");
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
+  if (total_q > 0 && total_k > 0 && max_q * s.group > 16)
+    return attention_bwd_tiles(s, q, k, v, o, lse, dout, dq, dk, dv, st);
   const long long bq = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
   const long long bk = (total_k * kv_heads + ROW_WARPS - 1) / ROW_WARPS;
   JX_REQUIRE(bq < (1LL << 31) && bk < (1LL << 31), "attention_bwd: too many rows");

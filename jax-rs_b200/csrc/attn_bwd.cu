@@ -1,0 +1,792 @@
+// attn_bwd.cu -- attention's gradients on the tensor cores (operands and sums as
+// in attn_tc.cuh).
+//
+// Two kernels, each with its sums in registers, so that every sum has a fixed
+// order and nothing is added atomically; the price is that the scores and
+// dout v^T are computed in both (seven products a tile instead of five).
+//
+// dq: one CTA per (128 query rows, head), streaming K and V tiles.
+//   S = Q K^T, dP = dO V^T        Q and dO in tensor memory
+//   dS = P (dP - delta)           P = exp2(S f - lse2)
+//   dQ += dS K                    dS in tensor memory, over S's columns
+// dk, dv: one CTA per (128 keys, key head, part of the query rows), streaming
+// blocks of 64 rows of Q and dO of every head of the group.
+//   S^T = K Q^T, dP^T = V dO^T    K and V in tensor memory
+//   dV += P^T dO, dK += dS^T Q    P^T over S^T's columns, dS^T over dP^T's
+// An operand computed here needs its scale before its largest value is known:
+// |dP - delta| <= |dout row| |v row| + |delta| (norms), times the largest P of the
+// row, bounds dS; it overestimates by a few bits of the 39 there are.
+#include <algorithm>
+
+#include "attn_tc.cuh"
+
+namespace {
+
+using namespace jxa;
+using jxg::wait_bounded;
+
+constexpr int BW_THREADS = 384;  // warp 0 copies, warp 1 MMA, warps 4..11 the rest
+constexpr int BW_FIRST = 4;
+constexpr int BW_LAUNCH_REGS = 168;
+constexpr int BW_LOW_REGS = 56;
+constexpr int BW_HIGH_REGS = 216;
+static_assert(128 * BW_LOW_REGS + 256 * BW_HIGH_REGS <= BW_THREADS * BW_LAUNCH_REGS,
+              "register split exceeds the launch allocation");
+
+struct BwdTiles {
+  const uint8_t *q, *k, *v, *d;  // tiles; d is dout
+  const float *inv_q, *inv_k, *inv_v, *inv_d;
+  const int *bad_q, *bad_k, *bad_v, *bad_d;
+  const float *norm_v, *norm_d, *lse2, *delta, *delta_top;
+  int q_tiles, k_tiles, parts;
+  float *part_k, *part_v;  // [parts][total_k * kv_heads * dim], used where parts > 1
+};
+
+// 1 / f of a power of two.
+__device__ __forceinline__ float inverse_pow2(float f) { return __uint_as_float((254u << 23) - __float_as_uint(f)); }
+
+// Scale for a computed operand of magnitude <= bound, at most 2^100.
+__device__ __forceinline__ float bound_scale(float bound) {
+  const int e = (int)(__float_as_uint(bound) >> 23);
+  return __uint_as_float((uint32_t)(268 - min(max(e, 41), 254)) << 23);
+}
+
+// The largest of a row's two halves; `xch` is [2][128].
+__device__ __forceinline__ float row_max(float v, float* xch, int half, int row, int id) {
+  xch[half * 128 + row] = v;
+  pair_sync(id);
+  v = fmaxf(v, xch[(half ^ 1) * 128 + row]);
+  pair_sync(id);
+  return v;
+}
+
+// A row's half into tensor memory; returns its scale's exponent and, with `norm`, the row's norm.
+template <int DP>
+__device__ __forceinline__ int stay_row(const float* src, int dim, int half, int row, bool vec, bool negate,
+                                        uint32_t taddr, float* xch, int id, float* norm) {
+  float x[DP / 2];
+  const float t = __uint_as_float(row_half_load<DP>(x, src, dim, half, vec));
+  const int e = (int)(__float_as_uint(row_max(t, xch, half, row, id)) >> 23);
+  const float f = scale_of(e);
+  if (norm) {
+    float n = 0.0f;
+#pragma unroll
+    for (int c = 0; c < DP / 2; ++c) n = fmaf(x[c] * f, x[c] * f, n);
+    xch[half * 128 + row] = n;
+    pair_sync(id);
+    *norm = sqrtf(n + xch[(half ^ 1) * 128 + row]) * inverse_of(e);
+    pair_sync(id);
+  }
+  row_half_store<DP>(x, negate ? -f : f, taddr, half);
+  return e;
+}
+
+// acc += part * factor for this thread's DP/2 columns of a tensor-memory sum.
+template <int DP>
+__device__ __forceinline__ void drain(float (&acc)[DP / 2], uint32_t taddr, float factor) {
+  const float2 f2 = make_float2(factor, factor);
+#pragma unroll
+  for (int c = 0; c < DP / 2; c += 16) {
+    uint32_t r[16];
+    jxd::tmem_ld16(taddr + c, r);
+    jxd::tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      const float2 v = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2,
+                            make_float2(acc[c + i], acc[c + i + 1]));
+      acc[c + i] = v.x;
+      acc[c + i + 1] = v.y;
+    }
+  }
+}
+
+// One row's half of a result.
+template <int DP>
+__device__ __forceinline__ void store_half(float* out, const float (&acc)[DP / 2], float factor, int n, bool vec) {
+  if (vec) {
+#pragma unroll
+    for (int c = 0; c < DP / 2; c += 4)
+      if (c < n)
+        *reinterpret_cast<float4*>(out + c) =
+            make_float4(acc[c] * factor, acc[c + 1] * factor, acc[c + 2] * factor, acc[c + 3] * factor);
+  } else {
+#pragma unroll
+    for (int c = 0; c < DP / 2; ++c)
+      if (c < n) out[c] = acc[c] * factor;
+  }
+}
+
+__device__ __forceinline__ bool aligned16(const void* p, int dim, long long ld) {
+  return (dim & 3) == 0 && (ld & 3) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// ---- dq ------------------------------------------------------------------------
+constexpr uint32_t DQ_Q = 0, DQ_D = 128, DQ_X = 256, DQ_Y = 384;
+__host__ __device__ constexpr int dq_k_stages(int) { return 2; }
+__host__ __device__ constexpr int dq_v_stages(int DP) { return DP == 128 ? 1 : 2; }
+__host__ __device__ constexpr size_t dq_smem(int DP) {
+  return (size_t)(dq_k_stages(DP) + dq_v_stages(DP)) * tile_bytes(DP) + 1024 + 2 * 128 * 4 + 256;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(BW_THREADS, 1)
+    attn_dq_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
+                   const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
+                   const float* __restrict__ lse, const float* __restrict__ dout, float* dq) {
+  constexpr int KS = dq_k_stages(DP), VS = dq_v_stages(DP), STAGE = tile_bytes(DP), PART = tile_part(DP);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = jxd::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  float* xch = reinterpret_cast<float*>(smem + (KS + VS) * STAGE);
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(xch + 2 * 128);
+  uint64_t* kempty = kfull + KS;
+  uint64_t* vfull = kempty + KS;
+  uint64_t* vempty = vfull + VS;
+  uint64_t* stayfull = vempty + VS;
+  uint64_t* sfull = stayfull + 1;
+  uint64_t* dpfull = sfull + 1;
+  uint64_t* dsfull = dpfull + 1;
+  uint64_t* dqfull = dsfull + 1;
+  uint64_t* yfree = dqfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(yfree + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int id = bt.q_tiles - 1 - (int)(blockIdx.x / (unsigned)s.heads), h = (int)(blockIdx.x % (unsigned)s.heads);
+  int jt;
+  const int b = seq_of_tile(s.cu_q, s.batch, id, &jt);
+  const Seq sq = seq_bounds(s, b);
+  if (jt < 0 || (long long)jt * TILE >= sq.lq) return;
+  const int i0 = jt * TILE, rows = min(TILE, sq.lq - i0);
+  const int hk = h / s.group;
+  const int nb = (sq.visible(i0 + rows - 1, s.causal) + TILE - 1) / TILE;
+  const long long slot0 = (long long)first_tile(sq.k0, b) * s.kv_heads + hk;
+  const long long qslot = ((long long)first_tile(sq.q0, b) + jt) * s.heads + h;
+
+  bool bad = threadIdx.x == 0 && (bt.bad_q[qslot] || bt.bad_d[qslot]);
+  for (int j = threadIdx.x; j < nb; j += BW_THREADS)
+    bad = bad || bt.bad_k[slot0 + (long long)j * s.kv_heads] || bt.bad_v[slot0 + (long long)j * s.kv_heads];
+  if (__syncthreads_or(bad)) {
+    for (int r = warp; r < rows; r += BW_THREADS / 32) {
+      const long long t = sq.q0 + i0 + r, hd = (long long)h * s.dim;
+      row_dq(q + t * s.ldq + hd, k + sq.k0 * s.ldk + (long long)hk * s.dim, v + sq.k0 * s.ldv + (long long)hk * s.dim,
+             o + t * s.ldo + hd, dout + t * s.ldo + hd, lse[(long long)h * s.total_q + t], dq + t * s.ldq + hd,
+             sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv, s.scale);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KS; ++i) {
+      jxd::mbar_init(&kfull[i], 1);
+      jxd::mbar_init(&kempty[i], 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      jxd::mbar_init(&vfull[i], 1);
+      jxd::mbar_init(&vempty[i], 1);
+    }
+    jxd::mbar_init(stayfull, 8);
+    jxd::mbar_init(sfull, 1);
+    jxd::mbar_init(dpfull, 1);
+    jxd::mbar_init(dsfull, 8);
+    jxd::mbar_init(dqfull, 1);
+    jxd::mbar_init(yfree, 8);
+    *abort_flag = 0;
+    jxd::fence_mbar_init();
+  }
+  if (warp == 1) {
+    jxd::tmem_alloc(tmem_slot, 512);
+    jxd::tmem_relinquish();
+  }
+  jxd::tc_fence_before();
+  __syncthreads();
+  jxd::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < BW_FIRST) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
+    if (warp == 0 && jxd::elect_one()) {
+      int j = 0, nv = 0;
+      for (; j < nb; ++j) {
+        const long long at = (slot0 + (long long)j * s.kv_heads) * STAGE;
+        const int ks = j % KS, vs = j % VS;
+        if (*abort_flag || !wait_bounded(&kempty[ks], (uint32_t)(j / KS + 1) & 1u, s.err)) break;
+        jxd::mbar_arrive_expect_tx(&kfull[ks], STAGE);
+        bulk_load(jxd::smem_u32(smem + ks * STAGE), bt.k + at, STAGE, &kfull[ks]);
+        if (*abort_flag || !wait_bounded(&vempty[vs], (uint32_t)(j / VS + 1) & 1u, s.err)) { ++j; break; }
+        jxd::mbar_arrive_expect_tx(&vfull[vs], STAGE);
+        bulk_load(jxd::smem_u32(smem + (KS + vs) * STAGE), bt.v + at, STAGE, &vfull[vs]);
+        ++nv;
+      }
+      if (nv < nb) *abort_flag = 1;
+      // every copy has landed before the CTA may end
+      for (int u = max(0, j - KS); u < j; ++u) wait_bounded(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
+      for (int u = max(0, nv - VS); u < nv; ++u) wait_bounded(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err);
+    }
+    if (warp == 1 && nb > 0 && jxd::elect_one()) {
+      constexpr uint32_t id_s = idesc_f16(128, false), id_o = idesc_f16(DP, true);
+      const uint32_t sbase = jxd::smem_u32(smem);
+      bool ok = wait_bounded(stayfull, 0, s.err);
+      // 128 x 128 scores of a row operand in tensor memory and a streamed tile
+      auto scores = [&](uint32_t d, uint32_t a0, uint32_t tile) {
+        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
+          mma_f16_ts(d, a0 + a + ks * 8, jxd::smem_desc_k_sw128(tile + part + (ks >> 2) * PANEL + (ks & 3) * 32), id_s,
+                     acc);
+        };
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          step(ks, DP / 2, 0, ks > 0);
+          step(ks, 0, PART, 1);
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
+      };
+      for (int j = 0; ok && j < nb; ++j) {
+        const uint32_t kt = sbase + (j % KS) * STAGE, vt = sbase + (KS + j % VS) * STAGE;
+        if (!(ok = !*abort_flag && wait_bounded(&kfull[j % KS], (uint32_t)(j / KS) & 1u, s.err))) break;
+        jxd::tc_fence_after();
+        scores(tmem + DQ_X, tmem + DQ_Q, kt);
+        jxd::mma_commit(sfull);
+        if (!(ok = !*abort_flag && wait_bounded(&vfull[j % VS], (uint32_t)(j / VS) & 1u, s.err) &&
+                   wait_bounded(yfree, (uint32_t)(j + 1) & 1u, s.err)))
+          break;
+        jxd::tc_fence_after();
+        scores(tmem + DQ_Y, tmem + DQ_D, vt);
+        jxd::mma_commit(dpfull);
+        jxd::mma_commit(&vempty[j % VS]);
+        if (!(ok = !*abort_flag && wait_bounded(dsfull, (uint32_t)j & 1u, s.err))) break;
+        jxd::tc_fence_after();
+        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
+          mma_f16_ts(tmem + DQ_Y, tmem + DQ_X + a + (ks >> 2) * 64 + (ks & 3) * 8,
+                     smem_desc_mn_sw128(kt + part + ks * 2048, PANEL), id_o, acc);
+        };
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          step(ks, 32, 0, ks > 0);
+          step(ks, 0, PART, 1);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) step(ks, 0, 0, 1);
+        jxd::mma_commit(dqfull);
+        jxd::mma_commit(&kempty[j % KS]);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_HIGH_REGS));
+    const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane, bar = 1 + quarter;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const long long t = sq.q0 + i0 + row, hd = (long long)h * s.dim;
+    float norm_d;
+    const int e_q = stay_row<DP>(row < rows ? q + t * s.ldq + hd : nullptr, s.dim, half, row,
+                                 aligned16(q, s.dim, s.ldq), s.scale < 0.0f, tmem + lanes + DQ_Q, xch, bar, nullptr);
+    const int e_d = stay_row<DP>(row < rows ? dout + t * s.ldo + hd : nullptr, s.dim, half, row,
+                                 aligned16(dout, s.dim, s.ldo), false, tmem + lanes + DQ_D, xch, bar, &norm_d);
+    tmem_st_wait();
+    jxd::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) jxd::mbar_arrive(stayfull);
+    const float f_row = inverse_of(e_q) * (fabsf(s.scale) * LOG2E), inv_d = inverse_of(e_d);
+    const float lse2 = bt.lse2[qslot * TILE + row], delta = bt.delta[qslot * TILE + row];
+    const int vis = row < rows ? sq.visible(i0 + row, s.causal) : 0;
+    const int vis_all = sq.visible(i0, s.causal);
+
+    float acc[DP / 2];
+#pragma unroll
+    for (int c = 0; c < DP / 2; ++c) acc[c] = 0.0f;
+    float g_prev = 0.0f;
+    bool ok = true;
+    auto add_part = [&](int j) {
+      ok = ok && jxg::warp_wait_bounded(dqfull, (uint32_t)j & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+      drain<DP>(acc, tmem + lanes + DQ_Y + half * (DP / 2), g_prev);
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(yfree);
+    };
+    for (int j = 0; j < nb; ++j) {
+      const long long slot = slot0 + (long long)j * s.kv_heads;
+      const float inv_k = bt.inv_k[slot], inv_v = bt.inv_v[slot], norm_v = bt.norm_v[slot];
+      if (j > 0) add_part(j - 1);
+      ok = ok && jxg::warp_wait_bounded(sfull, (uint32_t)j & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+      const float f = f_row * inv_k;
+      const float2 f2 = make_float2(f, f), l2 = make_float2(-lse2, -lse2);
+      const int key0 = j * TILE + half * 64;
+      const bool edge = j * TILE + TILE > vis_all;
+      float p[64];
+      float most = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t r[32];
+        jxd::tmem_ld32(tmem + lanes + DQ_X + half * 64 + c, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float2 z = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2, l2);
+          p[c + i] = exp2_fast(z.x);
+          p[c + i + 1] = exp2_fast(z.y);
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+          if (key0 + i >= vis) p[i] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 64; ++i) most = fmaxf(most, p[i]);
+      most = row_max(most, xch, half, row, bar);
+      const float fd = inv_d * inv_v;
+      const float sc = bound_scale(most * (norm_d * norm_v + fabsf(delta)));
+      const float pf = sc * fd, dl = -delta * inverse_pow2(fd);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) p[i] *= pf;
+      ok = ok && jxg::warp_wait_bounded(dpfull, (uint32_t)j & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+      uint32_t hi[32], lo[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t r[32];
+        jxd::tmem_ld32(tmem + lanes + DQ_Y + half * 64 + c, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float a = p[c + i] * (__uint_as_float(r[i]) + dl), e = p[c + i + 1] * (__uint_as_float(r[i + 1]) + dl);
+          split_half(a, e, hi[(c + i) / 2], lo[(c + i) / 2]);
+        }
+      }
+      tmem_st32(tmem + lanes + DQ_X + half * 64, hi);
+      tmem_st32(tmem + lanes + DQ_X + half * 64 + 32, lo);
+      tmem_st_wait();
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(dsfull);
+      g_prev = inv_k * inverse_pow2(sc) * 6.103515625e-05f;  // P's 2^14
+    }
+    if (nb > 0) add_part(nb - 1);
+    if (row < rows)
+      store_half<DP>(dq + t * s.ldq + hd + half * (DP / 2), acc, s.scale, s.dim - half * (DP / 2),
+                     aligned16(dq, s.dim, s.ldq));
+  }
+  jxd::tc_fence_before();
+  __syncthreads();
+  jxd::tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    jxd::tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- dk, dv --------------------------------------------------------------------
+constexpr int BLK = 64;  // query rows per step
+constexpr uint32_t KV_K = 0, KV_V = 128, KV_X = 256, KV_Y = 320, KV_Z = 384;
+constexpr int HPANEL = BLK * 128;  // bytes of a panel of a half tile
+constexpr int KV_STAGES = 3;       // of Q and of dout each
+__host__ __device__ constexpr int kv_stage(int DP) { return tile_bytes(DP) / 2; }
+__host__ __device__ constexpr size_t kv_smem(int DP) {
+  return (size_t)2 * KV_STAGES * kv_stage(DP) + 1024 + KV_STAGES * 512 /*lse2, delta*/ + 2 * 128 * 4 + 256;
+}
+
+template <int DP>
+__global__ void __launch_bounds__(BW_THREADS, 1)
+    attn_dkv_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
+                    const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
+                    const float* __restrict__ lse, const float* __restrict__ dout, float* dk, float* dv) {
+  constexpr int ST = KV_STAGES, STAGE = kv_stage(DP), PART = STAGE / 2;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = jxd::smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  float* stats = reinterpret_cast<float*>(smem + 2 * ST * STAGE);  // [ST][lse2 64, delta 64]
+  float* xch = stats + ST * 128;
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(xch + 2 * 128);
+  uint64_t* qempty = qfull + ST;
+  uint64_t* dfull = qempty + ST;
+  uint64_t* dempty = dfull + ST;
+  uint64_t* stayfull = dempty + ST;
+  uint64_t* sfull = stayfull + 1;
+  uint64_t* pfull = sfull + 1;
+  uint64_t* dpfull = pfull + 1;
+  uint64_t* dsfull = dpfull + 1;
+  uint64_t* zfull = dsfull + 1;
+  uint64_t* zfree = zfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(zfree + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the first keys of a sequence, which the most rows see, start first
+  unsigned w = blockIdx.x;
+  const int part = (int)(w % (unsigned)bt.parts);
+  w /= (unsigned)bt.parts;
+  const int hk = (int)(w % (unsigned)s.kv_heads), id = (int)(w / (unsigned)s.kv_heads);
+  int jt;
+  const int b = seq_of_tile(s.cu_k, s.batch, id, &jt);
+  const Seq sq = seq_bounds(s, b);
+  if (jt < 0 || (long long)jt * TILE >= sq.lk) return;
+  const int j0 = jt * TILE, rows = min(TILE, sq.lk - j0);
+  const int blk0 = sq.first_row(j0, s.causal) / BLK;
+  const int nblk = max(0, (sq.lq + BLK - 1) / BLK - blk0);
+  const long long steps = (long long)s.group * nblk;
+  const int it0 = (int)(steps * part / bt.parts), it1 = (int)(steps * (part + 1) / bt.parts);
+  const long long qslot0 = (long long)first_tile(sq.q0, b) * s.heads + (long long)hk * s.group;
+  const long long kslot = ((long long)first_tile(sq.k0, b) + jt) * s.kv_heads + hk;
+  const int h0 = hk * s.group;
+  const long long kd = (long long)hk * s.dim;
+  // where this part's sums go
+  float* out_k = bt.parts > 1 ? bt.part_k + (long long)part * s.total_k * s.kv_heads * s.dim : dk;
+  float* out_v = bt.parts > 1 ? bt.part_v + (long long)part * s.total_k * s.kv_heads * s.dim : dv;
+  const long long ld_k = bt.parts > 1 ? (long long)s.kv_heads * s.dim : s.ldk;
+  const long long ld_v = bt.parts > 1 ? (long long)s.kv_heads * s.dim : s.ldv;
+
+  bool bad = threadIdx.x == 0 && (bt.bad_k[kslot] || bt.bad_v[kslot]);
+  {
+    const int t0 = blk0 / 2, nt = nblk > 0 ? (sq.lq + TILE - 1) / TILE - t0 : 0;
+    for (long long e = threadIdx.x; e < (long long)nt * s.group; e += BW_THREADS) {
+      const long long slot = qslot0 + (t0 + e / s.group) * s.heads + e % s.group;
+      bad = bad || bt.bad_q[slot] || bt.bad_d[slot];
+    }
+  }
+  if (__syncthreads_or(bad)) {
+    // the first part computes every row whole, the others add zeros
+    for (int r = warp; r < rows; r += BW_THREADS / 32) {
+      const long long t = sq.k0 + j0 + r;
+      row_dkv(q + sq.q0 * s.ldq + (long long)h0 * s.dim, o + sq.q0 * s.ldo + (long long)h0 * s.dim,
+              dout + sq.q0 * s.ldo + (long long)h0 * s.dim, lse + (long long)h0 * s.total_q + sq.q0,
+              k + t * s.ldk + kd, v + t * s.ldv + kd, out_k + t * ld_k + kd, out_v + t * ld_v + kd,
+              part == 0 ? sq.first_row(j0 + r, s.causal) : sq.lq, sq.lq, s.group, s.dim, s.ldq, s.ldo, s.total_q,
+              s.scale);
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      jxd::mbar_init(&qfull[i], 1);
+      jxd::mbar_init(&qempty[i], 1);
+      jxd::mbar_init(&dfull[i], 1);
+      jxd::mbar_init(&dempty[i], 1);
+    }
+    jxd::mbar_init(stayfull, 8);
+    jxd::mbar_init(sfull, 1);
+    jxd::mbar_init(pfull, 8);
+    jxd::mbar_init(dpfull, 1);
+    jxd::mbar_init(dsfull, 8);
+    jxd::mbar_init(zfull, 1);
+    jxd::mbar_init(zfree, 8);
+    *abort_flag = 0;
+    jxd::fence_mbar_init();
+  }
+  if (warp == 1) {
+    jxd::tmem_alloc(tmem_slot, 512);
+    jxd::tmem_relinquish();
+  }
+  jxd::tc_fence_before();
+  __syncthreads();
+  jxd::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int n = it1 - it0;
+
+  if (warp < BW_FIRST) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
+    if (warp == 0 && jxd::elect_one()) {
+      // half a tile: each part's panels, 64 rows of them
+      auto load = [&](uint8_t* dst, const uint8_t* tile, int hb, uint64_t* bar) {
+#pragma unroll
+        for (int e = 0; e < 2 * (DP / 64); ++e)
+          bulk_load(jxd::smem_u32(dst + e * HPANEL), tile + (long long)e * PANEL + hb * HPANEL, HPANEL, bar);
+      };
+      int u = 0, nd = 0;
+      for (; u < n; ++u) {
+        const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
+        const long long slot = qslot0 + (long long)(blk >> 1) * s.heads + g;
+        if (*abort_flag || !wait_bounded(&qempty[st], (uint32_t)(u / ST + 1) & 1u, s.err)) break;
+        jxd::mbar_arrive_expect_tx(&qfull[st], STAGE + 512);
+        load(smem + st * STAGE, bt.q + slot * tile_bytes(DP), blk & 1, &qfull[st]);
+        bulk_load(jxd::smem_u32(stats + st * 128), bt.lse2 + slot * TILE + (blk & 1) * BLK, 256, &qfull[st]);
+        bulk_load(jxd::smem_u32(stats + st * 128 + 64), bt.delta + slot * TILE + (blk & 1) * BLK, 256, &qfull[st]);
+        if (*abort_flag || !wait_bounded(&dempty[st], (uint32_t)(u / ST + 1) & 1u, s.err)) { ++u; break; }
+        jxd::mbar_arrive_expect_tx(&dfull[st], STAGE);
+        load(smem + (ST + st) * STAGE, bt.d + slot * tile_bytes(DP), blk & 1, &dfull[st]);
+        ++nd;
+      }
+      if (nd < n) *abort_flag = 1;
+      for (int e = max(0, u - ST); e < u; ++e) wait_bounded(&qfull[e % ST], (uint32_t)(e / ST) & 1u, s.err);
+      for (int e = max(0, nd - ST); e < nd; ++e) wait_bounded(&dfull[e % ST], (uint32_t)(e / ST) & 1u, s.err);
+    }
+    if (warp == 1 && n > 0 && jxd::elect_one()) {
+      constexpr uint32_t id_s = idesc_f16(BLK, false), id_o = idesc_f16(DP, true);
+      const uint32_t sbase = jxd::smem_u32(smem);
+      bool ok = wait_bounded(stayfull, 0, s.err);
+      auto ready = [&](uint64_t* bar, int u) {
+        return !*abort_flag && wait_bounded(bar, (uint32_t)u & 1u, s.err);
+      };
+      // 128 x 64 scores
+      auto scores = [&](uint32_t d, uint32_t a0, uint32_t tile) {
+        auto step = [&](int ks, uint32_t a, uint32_t p, uint32_t acc) {
+          mma_f16_ts(d, a0 + a + ks * 8, jxd::smem_desc_k_sw128(tile + p + (ks >> 2) * HPANEL + (ks & 3) * 32), id_s,
+                     acc);
+        };
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          step(ks, DP / 2, 0, ks > 0);
+          step(ks, 0, PART, 1);
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
+      };
+      // 128 x DP sums over the block's 64 rows; rows 0..31: hi at column 0, lo at 16, rows 32..63: 32 and 48
+      auto sums = [&](uint32_t a0, uint32_t tile) {
+        auto step = [&](int ks, uint32_t a, uint32_t p, uint32_t acc) {
+          mma_f16_ts(tmem + KV_Z, a0 + a + (ks >> 1) * 32 + (ks & 1) * 8,
+                     smem_desc_mn_sw128(tile + p + ks * 2048, HPANEL), id_o, acc);
+        };
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          step(ks, 16, 0, ks > 0);
+          step(ks, 0, PART, 1);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) step(ks, 0, 0, 1);
+      };
+      auto q_scores = [&](int u) {
+        if (!ok || !(ok = ready(&qfull[u % ST], u / ST))) return;
+        jxd::tc_fence_after();
+        scores(tmem + KV_X, tmem + KV_K, sbase + (u % ST) * STAGE);
+        jxd::mma_commit(sfull);
+      };
+      auto d_scores = [&](int u) {
+        if (!ok || !(ok = ready(&dfull[u % ST], u / ST))) return;
+        jxd::tc_fence_after();
+        scores(tmem + KV_Y, tmem + KV_V, sbase + (ST + u % ST) * STAGE);
+        jxd::mma_commit(dpfull);
+      };
+      q_scores(0);
+      d_scores(0);
+      for (int u = 0; ok && u < n; ++u) {
+        if (!(ok = ready(pfull, u) && ready(zfree, 2 * u + 1))) break;
+        jxd::tc_fence_after();
+        sums(tmem + KV_X, sbase + (ST + u % ST) * STAGE);
+        jxd::mma_commit(zfull);
+        jxd::mma_commit(&dempty[u % ST]);
+        if (u + 1 < n) q_scores(u + 1);
+        if (!ok || !(ok = ready(dsfull, u) && ready(zfree, 2 * u))) break;
+        jxd::tc_fence_after();
+        sums(tmem + KV_Y, sbase + (u % ST) * STAGE);
+        jxd::mma_commit(zfull);
+        jxd::mma_commit(&qempty[u % ST]);
+        if (u + 1 < n) d_scores(u + 1);
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_HIGH_REGS));
+    const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane, bar = 1 + quarter;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const long long t = sq.k0 + j0 + row;
+    float norm_v;
+    const int e_k = stay_row<DP>(row < rows ? k + t * s.ldk + kd : nullptr, s.dim, half, row,
+                                 aligned16(k, s.dim, s.ldk), s.scale < 0.0f, tmem + lanes + KV_K, xch, bar, nullptr);
+    const int e_v = stay_row<DP>(row < rows ? v + t * s.ldv + kd : nullptr, s.dim, half, row,
+                                 aligned16(v, s.dim, s.ldv), false, tmem + lanes + KV_V, xch, bar, &norm_v);
+    tmem_st_wait();
+    jxd::tc_fence_before();
+    __syncwarp();
+    if (lane == 0) jxd::mbar_arrive(stayfull);
+    const float f_row = inverse_of(e_k) * (fabsf(s.scale) * LOG2E), inv_v = inverse_of(e_v);
+    const int first = row < rows ? sq.first_row(j0 + row, s.causal) : 0x7fffffff;  // first query row that sees this key
+    const int first_all = sq.first_row(j0 + rows - 1, s.causal);
+
+    float ak[DP / 2], av[DP / 2];
+#pragma unroll
+    for (int c = 0; c < DP / 2; ++c) ak[c] = av[c] = 0.0f;
+    float g_prev = 0.0f;
+    bool ok = true;
+    auto ready = [&](uint64_t* b8, int u) {
+      ok = ok && jxg::warp_wait_bounded(b8, (uint32_t)u & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+    };
+    auto done = [&](uint64_t* b8) {
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(b8);
+    };
+    for (int u = 0; u < n; ++u) {
+      const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
+      const long long slot = qslot0 + (long long)(blk >> 1) * s.heads + g;
+      const float inv_q = bt.inv_q[slot], inv_d = bt.inv_d[slot], norm_d = bt.norm_d[slot], top_d = bt.delta_top[slot];
+      const float* lse2 = stats + st * 128 + half * 32;
+      const float* delta = lse2 + 64;
+      ready(&qfull[st], u / ST);  // landed before the scores were issued: its statistics are visible here too
+      ready(sfull, u);
+      const float f = f_row * inv_q;
+      float p[32];
+      float most = 0.0f;
+      {
+        uint32_t r[32];
+        jxd::tmem_ld32(tmem + lanes + KV_X + half * 32, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(lse2 + i);
+          p[i] = exp2_fast(fmaf(__uint_as_float(r[i]), f, -l.x));
+          p[i + 1] = exp2_fast(fmaf(__uint_as_float(r[i + 1]), f, -l.y));
+          p[i + 2] = exp2_fast(fmaf(__uint_as_float(r[i + 2]), f, -l.z));
+          p[i + 3] = exp2_fast(fmaf(__uint_as_float(r[i + 3]), f, -l.w));
+        }
+      }
+      if (blk * BLK < first_all || rows < TILE) {
+        const int i0 = blk * BLK + half * 32;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i0 + i < first) p[i] = 0.0f;
+      }
+      {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) split_half(p[2 * i], p[2 * i + 1], hi[i], lo[i]);
+        tmem_st16(tmem + lanes + KV_X + half * 32, hi);
+        tmem_st16(tmem + lanes + KV_X + half * 32 + 16, lo);
+        tmem_st_wait();
+        done(pfull);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) most = fmaxf(most, p[i]);
+      most = row_max(most, xch, half, row, bar);
+      if (u > 0) {
+        ready(zfull, 2 * u - 1);
+        drain<DP>(ak, tmem + lanes + KV_Z + half * (DP / 2), g_prev);
+        done(zfree);
+      }
+      const float fd = inv_v * inv_d;
+      const float sc = bound_scale(most * (norm_v * norm_d + top_d));
+      const float pf = sc * fd, nf = -inverse_pow2(fd);
+      ready(dpfull, u);
+      {
+        uint32_t r[32], hi[16], lo[16];
+        jxd::tmem_ld32(tmem + lanes + KV_Y + half * 32, r);
+        jxd::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 d = *reinterpret_cast<const float4*>(delta + i);
+          const float a0 = (p[i] * pf) * fmaf(d.x, nf, __uint_as_float(r[i]));
+          const float a1 = (p[i + 1] * pf) * fmaf(d.y, nf, __uint_as_float(r[i + 1]));
+          const float a2 = (p[i + 2] * pf) * fmaf(d.z, nf, __uint_as_float(r[i + 2]));
+          const float a3 = (p[i + 3] * pf) * fmaf(d.w, nf, __uint_as_float(r[i + 3]));
+          split_half(a0, a1, hi[i / 2], lo[i / 2]);
+          split_half(a2, a3, hi[i / 2 + 1], lo[i / 2 + 1]);
+        }
+        tmem_st16(tmem + lanes + KV_Y + half * 32, hi);
+        tmem_st16(tmem + lanes + KV_Y + half * 32 + 16, lo);
+        tmem_st_wait();
+        done(dsfull);
+      }
+      ready(zfull, 2 * u);
+      drain<DP>(av, tmem + lanes + KV_Z + half * (DP / 2), inv_d * 6.103515625e-05f);  // P's 2^14
+      done(zfree);
+      g_prev = inv_q * inverse_pow2(sc) * 6.103515625e-05f;
+    }
+    if (n > 0) {
+      ready(zfull, 2 * n - 1);
+      drain<DP>(ak, tmem + lanes + KV_Z + half * (DP / 2), g_prev);
+    }
+    if (row < rows) {
+      const int left = s.dim - half * (DP / 2);
+      store_half<DP>(out_k + t * ld_k + kd + half * (DP / 2), ak, s.scale, left, aligned16(out_k, s.dim, ld_k));
+      store_half<DP>(out_v + t * ld_v + kd + half * (DP / 2), av, 1.0f, left, aligned16(out_v, s.dim, ld_v));
+    }
+  }
+  jxd::tc_fence_before();
+  __syncthreads();
+  jxd::tc_fence_after();
+  if (warp == 1) {
+    __syncwarp();
+    jxd::tmem_dealloc(tmem, 512);
+  }
+}
+
+// The parts' sums in order, one block per (key tile, key head).
+__global__ void __launch_bounds__(256) attn_dkv_join_kernel(const __grid_constant__ Shape s,
+                                                           const __grid_constant__ BwdTiles bt, float* dk, float* dv) {
+  int jt;
+  const int b = seq_of_tile(s.cu_k, s.batch, blockIdx.x, &jt);
+  const Seq sq = seq_bounds(s, b);
+  if (jt < 0 || (long long)jt * TILE >= sq.lk) return;
+  const int rows = min(TILE, sq.lk - jt * TILE);
+  const long long t0 = sq.k0 + (long long)jt * TILE, hd = (long long)blockIdx.y * s.dim;
+  const long long ld = (long long)s.kv_heads * s.dim, all = s.total_k * ld;
+  for (int e = threadIdx.x; e < rows * s.dim; e += 256) {
+    const int r = e / s.dim, c = e - r * s.dim;
+    const long long at = (t0 + r) * ld + hd + c;
+    float a = 0.0f, d = 0.0f;
+    for (int p = 0; p < bt.parts; ++p) {
+      a += bt.part_k[p * all + at];
+      d += bt.part_v[p * all + at];
+    }
+    dk[(t0 + r) * s.ldk + hd + c] = a;
+    dv[(t0 + r) * s.ldv + hd + c] = d;
+  }
+}
+
+template <int DP>
+int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, const float* v, const float* o,
+           const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st) {
+  if (int rc = prepare_kernel((const void*)attn_dq_kernel<DP>, DP == 128 ? 2 : 3, dq_smem(DP), BW_LAUNCH_REGS))
+    return rc;
+  if (int rc = prepare_kernel((const void*)attn_dkv_kernel<DP>, DP == 128 ? 4 : 5, kv_smem(DP), BW_LAUNCH_REGS))
+    return rc;
+  attn_dq_kernel<DP><<<(unsigned)((long long)bt.q_tiles * s.heads), BW_THREADS, dq_smem(DP), st>>>(
+      s, bt, q, k, v, o, lse, dout, dq);
+  attn_dkv_kernel<DP><<<(unsigned)((long long)bt.k_tiles * s.kv_heads * bt.parts), BW_THREADS, kv_smem(DP), st>>>(
+      s, bt, q, k, v, o, lse, dout, dk, dv);
+  if (bt.parts > 1) attn_dkv_join_kernel<<<dim3(bt.k_tiles, s.kv_heads), 256, 0, st>>>(s, bt, dk, dv);
+  JX_LAUNCH_CHECK("attention_bwd kernels");
+  return JX_OK;
+}
+
+}  // namespace
+
+namespace jxa {
+
+int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
+                        const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st) {
+  const int DP = s.dim <= 64 ? 64 : 128;
+  const long long kt = tile_count(s.total_k, s.batch), qt = tile_count(s.total_q, s.batch);
+  // key tiles are few where heads are shared: enough parts of the query rows for four CTAs per SM
+  const long long ctas = kt * s.kv_heads;
+  const int parts = (int)std::max<long long>(1, std::min<long long>(8, 4LL * jx::num_sms() / std::max(1LL, ctas)));
+  JX_REQUIRE(qt * s.heads < (1LL << 31) && kt * s.kv_heads * parts < (1LL << 31), "attention_bwd: too many rows");
+  const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
+  const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
+  // tiles first, then arrays whose pieces the copies read 16-byte aligned, then the rest
+  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (5 * ks + 6 * qs) * 4 + 2 * part_floats * 4;
+  void* p = nullptr;
+  if (int rc = jx::scratch_get(bytes + 64, &p, st)) return rc;
+  uint8_t* at = static_cast<uint8_t*>(p);
+  auto take = [&](size_t n) {
+    uint8_t* r = at;
+    at += n;
+    return r;
+  };
+  uint8_t *tk = take(ks * tb), *tv = take(ks * tb), *tq = take(qs * tb), *td = take(qs * tb);
+  float* lse2 = (float*)take(qs * TILE * 4);
+  float* delta = (float*)take(qs * TILE * 4);
+  float* part_k = (float*)take(part_floats * 4);
+  float* part_v = (float*)take(part_floats * 4);
+  float *inv_k = (float*)take(ks * 4), *inv_v = (float*)take(ks * 4), *norm_v = (float*)take(ks * 4);
+  float *inv_q = (float*)take(qs * 4), *inv_d = (float*)take(qs * 4), *norm_d = (float*)take(qs * 4);
+  float* delta_top = (float*)take(qs * 4);
+  int *bad_k = (int*)take(ks * 4), *bad_v = (int*)take(ks * 4), *bad_q = (int*)take(qs * 4), *bad_d = (int*)take(qs * 4);
+  TileSources kv = {}, qd = {};
+  kv.t[0] = {k, s.ldk, tk, inv_k, bad_k};
+  kv.t[1] = {v, s.ldv, tv, inv_v, bad_v, norm_v};
+  qd.t[0] = {q, s.ldq, tq, inv_q, bad_q};
+  qd.t[1] = {dout, s.ldo, td, inv_d, bad_d, norm_d, o, lse, lse2, delta, delta_top};
+  const BwdTiles bt = {tq,     tk,     tv,    td,    inv_q, inv_k,     inv_v,   inv_d,   bad_q, bad_k,  bad_v,
+                       bad_d,  norm_v, norm_d, lse2, delta, delta_top, (int)qt, (int)kt, parts, part_k, part_v};
+  int rc = split_tiles(s, false, kv, 2, s.kv_heads, DP, st);
+  if (!rc) rc = split_tiles(s, true, qd, 2, s.heads, DP, st);
+  if (!rc)
+    rc = DP == 128 ? launch<128>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st)
+                   : launch<64>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st);
+  jx::scratch_release(p, st);
+  return rc;
+}
+
+}  // namespace jxa

@@ -92,9 +92,59 @@ __global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant_
   const long long slot = (long long)id * heads + h;
   if (threadIdx.x == 0) {
     t.inverse[slot] = inverse_of(e_top);
-    t.bad[slot] = e_top == 255 || (top && e_top - max(e_low, 15) > WIDE_BITS);
+    t.bad[slot] = unscaled(top) || (top && e_top - e_low > WIDE_BITS);
   }
-  const float factor = scale_of(min(e_top, 254));
+  const float factor = scale_of(e_top);
+  if (t.norm) {
+    float most = 0.0f, most_delta = 0.0f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 16 * i;
+      float n = 0.0f, d = 0.0f;
+#pragma unroll
+      for (int e = 0; e < CW; ++e) {
+        n += (x[i][e] * factor) * (x[i][e] * factor);
+        if (t.o && r < rows && col + e < s.dim)
+          d = fmaf(x[i][e], t.o[(row0 + r) * s.ldo + (long long)h * s.dim + col + e], d);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        n += __shfl_xor_sync(0xffffffffu, n, o);
+        d += __shfl_xor_sync(0xffffffffu, d, o);
+      }
+      most = fmaxf(most, n);
+      if (t.o && c == 0) {
+        const float z = r < rows ? t.lse[(long long)h * s.total_q + row0 + r] : -INFINITY;
+        odd = odd || !isfinite(d) || isnan(z) || z == INFINITY;
+        t.lse2[slot * TILE + r] = z == -INFINITY ? INFINITY : z * LOG2E - P_SHIFT;
+        t.delta[slot * TILE + r] = d;
+        most_delta = fmaxf(most_delta, fabsf(d));
+      }
+    }
+    odd = __syncthreads_or(odd);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+      most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+    }
+    if ((threadIdx.x & 31) == 0) {
+      sm_top[threadIdx.x >> 5] = __float_as_uint(most);
+      sm_low[threadIdx.x >> 5] = __float_as_uint(most_delta);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) {
+        most = fmaxf(most, __uint_as_float(sm_top[w]));
+        most_delta = fmaxf(most_delta, __uint_as_float(sm_low[w]));
+      }
+      t.norm[slot] = sqrtf(most) * inverse_of(e_top);
+      if (t.o) {
+        t.delta_top[slot] = most_delta;
+        if (odd) t.bad[slot] = 1;
+      }
+    }
+  }
   uint8_t* out = t.tiles + slot * tile_bytes(DP);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -123,7 +173,6 @@ constexpr int FW_HIGH_REGS = 216;
 static_assert(128 * FW_LOW_REGS + 256 * FW_HIGH_REGS <= FW_THREADS * FW_LAUNCH_REGS,
               "register split exceeds the launch allocation");
 constexpr uint32_t T_Q = 256, T_O = 384;  // columns of tensor memory; S0 at 0, S1 at 128
-constexpr float P_SHIFT = 14.0f;          // P is scaled by 2^14 for its f16 parts
 
 __host__ __device__ constexpr int fw_stages(int DP) { return DP == 128 ? 3 : 6; }
 __host__ __device__ constexpr size_t fw_smem(int DP) {
@@ -184,7 +233,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         x, row < rows ? q + (sq.q0 + i0 + row) * s.ldq + (long long)h * s.dim : nullptr, s.dim, half, vec);
     reinterpret_cast<uint32_t*>(xch)[half * 128 + row] = top;
   }
-  bool bad = top >= 0x7f800000u;
+  __syncthreads();
+  if (soft) top = max(top, reinterpret_cast<uint32_t*>(xch)[(half ^ 1) * 128 + row]);
+  bool bad = unscaled(top);
   for (int j = threadIdx.x; j < nb; j += FW_THREADS)
     bad = bad || ft.bad_k[slot0 + (long long)j * s.kv_heads] || ft.bad_v[slot0 + (long long)j * s.kv_heads];
   if (__syncthreads_or(bad)) {
@@ -298,7 +349,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FW_HIGH_REGS));
     // ---- softmax and output
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const int e_row = (int)(max(top, reinterpret_cast<uint32_t*>(xch)[(half ^ 1) * 128 + row]) >> 23);
+    const int e_row = (int)(top >> 23);
     row_half_store<DP>(x, s.scale < 0.0f ? -scale_of(e_row) : scale_of(e_row), tmem + lanes + T_Q, half);
     tmem_st_wait();
     jxd::tc_fence_before();
@@ -469,7 +520,9 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
   uint8_t* base = static_cast<uint8_t*>(p);
   float* inv = reinterpret_cast<float*>(base + 2 * bytes);
   int* bad = reinterpret_cast<int*>(inv + 2 * slots);
-  TileSources src = {{{k, s.ldk, base, inv, bad}, {v, s.ldv, base + bytes, inv + slots, bad + slots}}};
+  TileSources src = {};
+  src.t[0] = {k, s.ldk, base, inv, bad};
+  src.t[1] = {v, s.ldv, base + bytes, inv + slots, bad + slots};
   FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, (int)qt};
   int rc = split_tiles(s, false, src, 2, s.kv_heads, DP, st);
   if (!rc) {

@@ -37,6 +37,7 @@ namespace jxa {
 constexpr int TILE = 128;
 constexpr int PANEL = TILE * 128;  // bytes of 128 rows x 64 f16 columns
 constexpr int WIDE_BITS = 20;
+constexpr float P_SHIFT = 14.0f;  // softmax weights are scaled by 2^14 for their f16 parts
 
 __host__ __device__ constexpr int tile_part(int DP) { return DP / 64 * PANEL; }      // one part of a tile
 __host__ __device__ constexpr int tile_bytes(int DP) { return 2 * tile_part(DP); }   // hi and lo
@@ -57,8 +58,18 @@ __device__ __forceinline__ int seq_of_tile(const int32_t* cu, int batch, int id,
 __device__ __forceinline__ int first_tile(long long start, int b) { return (int)(start >> 7) + b; }
 
 // Power of two that brings a magnitude with biased exponent e into [2^14, 2^15), and its inverse.
-__device__ __forceinline__ float scale_of(int e) { return __uint_as_float((uint32_t)(268 - max(e, 15)) << 23); }
-__device__ __forceinline__ float inverse_of(int e) { return __uint_as_float((uint32_t)(max(e, 15) - 14) << 23); }
+// e below LEAST_E (zeros among them) takes LEAST_E's scale.
+constexpr int LEAST_E = 79;
+__device__ __forceinline__ float scale_of(int e) {
+  return __uint_as_float((uint32_t)(268 - min(max(e, LEAST_E), 254)) << 23);
+}
+__device__ __forceinline__ float inverse_of(int e) {
+  return __uint_as_float((uint32_t)(min(max(e, LEAST_E), 254) - 14) << 23);
+}
+// Magnitude bits that the scales do not serve: not finite, or tiny but not zero.
+__device__ __forceinline__ bool unscaled(uint32_t top) {
+  return top >= 0x7f800000u || (top != 0 && (int)(top >> 23) < LEAST_E - 17);
+}
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b) {  // a in the low half
   uint32_t r;
@@ -202,6 +213,15 @@ struct TileSource {
   uint8_t* tiles;
   float* inverse;  // of the tile's scale, [id][head]
   int* bad;        // the tile is marked, [id][head]
+  float* norm;     // largest Euclidean norm of the tile's rows, [id][head]; may be NULL
+  // for dout alone (NULL otherwise): o and lse; the rows' lse in base 2 less
+  // P_SHIFT (+inf for rows without keys or behind the end) and rowsum(dout o), [id][head][TILE]; the
+  // largest magnitude of the latter, [id][head]
+  const float* o;
+  const float* lse;
+  float* lse2;
+  float* delta;
+  float* delta_top;
 };
 struct TileSources {
   TileSource t[2];
@@ -212,5 +232,7 @@ int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, 
 int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs);
 int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
                         cudaStream_t st);
+int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
+                        const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st);
 
 }  // namespace jxa
