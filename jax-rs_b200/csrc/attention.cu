@@ -18,26 +18,6 @@ using namespace jxa;
 constexpr int ROW_WARPS = 8;
 
 // One warp per (query row, head).
-__global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_fwd_kernel(const __grid_constant__ Shape s,
-                                                                      const float* __restrict__ q,
-                                                                      const float* __restrict__ k,
-                                                                      const float* __restrict__ v, float* o,
-                                                                      float* lse) {
-  const long long w = (long long)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
-  const long long t = w / s.heads;
-  const int h = (int)(w - t * s.heads);
-  if (t >= s.total_q) return;
-  const int b = seq_of_row(s.cu_q, s.batch, t);
-  if (b < 0) return;
-  const Seq sq = seq_bounds(s, b);
-  if (t < sq.q0 || t >= sq.q0 + sq.lq) return;
-  const int hk = h / s.group;
-  row_fwd(q + t * s.ldq + (long long)h * s.dim, k + sq.k0 * s.ldk + (long long)hk * s.dim,
-          v + sq.k0 * s.ldv + (long long)hk * s.dim, o + t * s.ldo + (long long)h * s.dim,
-          lse ? lse + (long long)h * s.total_q + t : nullptr, sq.visible((int)(t - sq.q0), s.causal), s.dim, s.ldk,
-          s.ldv, s.scale);
-}
-
 __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dq_kernel(const __grid_constant__ Shape s,
                                                                      const float* __restrict__ q,
                                                                      const float* __restrict__ k,
@@ -132,12 +112,9 @@ int jx_attention_f32(const float* q, const float* k, const float* v, float* o, f
   JX_REQUIRE(q && o && cu_q && cu_k && (total_k == 0 || (k && v)), "attention: NULL pointer");
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
+  JX_REQUIRE(total_q * heads < (1LL << 31), "attention: too many rows");
   if (total_k > 0 && max_q * s.group > 16) return attention_fwd_tiles(s, q, k, v, o, lse, st);
-  const long long blocks = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
-  JX_REQUIRE(blocks < (1LL << 31), "attention: too many rows");
-  attn_rows_fwd_kernel<<<(unsigned)blocks, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse);
-  JX_LAUNCH_CHECK("attn_rows_fwd_kernel");
-  return JX_OK;
+  return attention_decode(s, q, k, v, o, lse, max_q * s.group, max_k, st);
 }
 
 int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
