@@ -30,7 +30,6 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dq_kernel(const __gr
   const int h = (int)(w - t * s.heads);
   if (t >= s.total_q) return;
   const int b = seq_of_row(s.cu_q, s.batch, t);
-  if (b < 0) return;
   const Seq sq = seq_bounds(s, b);
   if (t < sq.q0 || t >= sq.q0 + sq.lq) return;
   const long long hk = h / s.group, hd = (long long)h * s.dim;
@@ -53,7 +52,6 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dkv_kernel(const __g
   const int hk = (int)(w - t * s.kv_heads);
   if (t >= s.total_k) return;
   const int b = seq_of_row(s.cu_k, s.batch, t);
-  if (b < 0) return;
   const Seq sq = seq_bounds(s, b);
   if (t < sq.k0 || t >= sq.k0 + sq.lk) return;
   const long long hd = (long long)hk * s.dim, h0 = (long long)hk * s.group;
@@ -114,7 +112,7 @@ int jx_attention_f32(const float* q, const float* k, const float* v, float* o, f
   s.err = jx::device_error_word();
   JX_REQUIRE(total_q * heads < (1LL << 31), "attention: too many rows");
   if (total_k > 0 && max_q * s.group > 16) return attention_fwd_tiles(s, q, k, v, o, lse, st);
-  return attention_decode(s, q, k, v, o, lse, max_q * s.group, max_k, st);
+  return attention_decode(s, q, k, v, o, lse, max_q * s.group, st);
 }
 
 int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,

@@ -52,16 +52,26 @@ __device__ __forceinline__ Seq seq_bounds(const Shape& s, int b) {
   return r;
 }
 
-// The last sequence b with cu[b] <= t, or -1: the one that row t belongs to, if
-// t < cu[b + 1].
-__device__ __forceinline__ int seq_of_row(const int32_t* cu, int batch, long long t) {
-  int lo = -1, hi = batch;
+// The last b in [0, batch) with at(b) <= x for a function that does not decrease
+// (0 if there is none), found by a whole warp: 32 places are tried at a time, so
+// that up to 32 sequences cost one load's latency.
+template <class At>
+__device__ __forceinline__ int last_at_most(int batch, long long x, At at) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = batch;
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t) lo = mid;
-    else hi = mid;
+    const int step = (hi - lo + 32) / 33;
+    const long long mid = lo + (long long)(lane + 1) * step;
+    const bool in = mid < hi && at((int)mid) <= x;
+    const int c = __popc(__ballot_sync(0xffffffffu, in));
+    lo += c * step;
+    hi = min(hi, lo + step);
   }
   return lo;
+}
+// The sequence that row t belongs to, if t lies within its bounds.  Warp-uniform t.
+__device__ __forceinline__ int seq_of_row(const int32_t* cu, int batch, long long t) {
+  return last_at_most(batch, t, [&](int b) { return (long long)cu[b]; });
 }
 
 // ---- one row by one warp, in plain f32 ------------------------------------------

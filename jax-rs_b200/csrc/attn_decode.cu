@@ -1,51 +1,117 @@
 // attn_decode.cu -- attention's forward pass for few query rows per key head (a
 // decoding step), in plain f32.
 //
-// Bound by reading K and V once from HBM.  A warp's lanes form groups, LPK lanes
-// to a key, each lane with DP / LPK of its columns, so that a load instruction
-// reads whole rows; a group keeps a running maximum, sum and output of its own
-// for the R query rows that the CTA serves (query rows times heads of the
-// group, so that K and V are read once for all of them), and nothing is
-// exchanged before the end but the LPK-lane sums of the scores.  The keys are
-// cut in chunks over CTAs; attn_join_kernel joins the chunks' results.
+// Bound by reading K and V once from HBM.  The keys of all sequences and key heads
+// are one line of positions, (sequence, key head, key) in order, cut in equal
+// ranges; a ring of shared-memory stages, eight keys each, streams a range with
+// TMA, and one to eight warps read it, four query rows each (rows of
+// the sequence times heads of the group), so that K and V are read once for all
+// rows.  In a warp eight lanes share a key, 16 columns each for dim 128, and the
+// four groups of lanes keep a running maximum, sum and output of their own:
+// nothing is exchanged per key but the eight-lane sums of the scores.  A range's
+// piece of a head goes to scratch unless it is the whole head, and
+// attn_join_kernel joins the pieces.
+//
+// One token behind eight histories, 14.7k keys of 8 heads of 128 (118 MB): 33 us for
+// both kernels, 3.6 TB/s, against 18 us of reading at the copy rate.  The
+// kernel itself takes 25 us; the rest is the join, which waits for the slowest
+// ring.  Copying row by row (one bulk copy of 512 B each) took 37 us, the rate of
+// copy instructions being the bound.
+//
+// 192 KB of stages per SM keep about 128 KB of loads in flight, three times what
+// HBM's latency needs at full rate.
 #include <algorithm>
+#include <atomic>
 
-#include "attn_common.cuh"
+#include "attn_tc.cuh"
 
 namespace {
 
 using namespace jxa;
+using jxg::wait_bounded;
 
-constexpr int DC_WARPS = 4;
-constexpr int DC_U = 2;  // keys that a group loads at a time
+constexpr int DC_WARPS = 8;
+constexpr int DC_KEYS = 8;  // keys per stage
+constexpr int DC_LPK = 8;   // lanes per key
+constexpr int DC_GROUPS = 32 / DC_LPK;
+constexpr int DC_RING = 192 * 1024;
 
-// Rows of a sequence are numbered i * group + head: chunk id of R rows, as seq_of_tile numbers tiles.
-__device__ __forceinline__ int seq_of_chunk(const int32_t* cu, int batch, int group, int R, long long id,
-                                            long long* j) {
-  int lo = 0, hi = batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((long long)cu[mid] * group / R + mid <= id) lo = mid;
-    else hi = mid;
+__host__ __device__ constexpr int dc_stage(int DP) { return DC_KEYS * 2 * DP * 4; }
+__host__ __device__ constexpr int dc_stages(int DP) { return DC_RING / dc_stage(DP); }  // of all rings
+__host__ __device__ constexpr size_t dc_smem(int DP) { return DC_RING + 2 * 8 * dc_stages(DP) + 128; }
+
+// A place in the line of positions.  A head takes lk + VOID of them: starting and
+// storing a head costs a ring about as much as VOID keys, so that short heads
+// weigh what they cost.
+constexpr int VOID = 32;
+struct Cursor {
+  long long pos;  // line_start(k0, b) + hk * (lk + VOID) + key
+  int b, hk, key;
+  Seq sq;
+  bool on;
+
+  // To the first key at or behind `pos`, in a sequence from b on.
+  __device__ __forceinline__ void settle(const Shape& s, long long end) {
+    for (on = false; b < s.batch; ++b) {
+      sq = seq_bounds(s, b);
+      if (sq.lq == 0 || sq.lk == 0) continue;
+      const long long base = (sq.k0 + (long long)b * VOID) * s.kv_heads, in = max(0LL, pos - base);
+      const int len = sq.lk + VOID;
+      if (in >= (long long)s.kv_heads * len) continue;
+      hk = (int)(in / len);
+      key = (int)(in - (long long)hk * len);
+      if (key >= sq.lk) {
+        key = 0;
+        if (++hk == s.kv_heads) continue;
+      }
+      pos = base + (long long)hk * len + key;
+      on = pos < end;
+      return;
+    }
   }
-  *j = id - ((long long)cu[lo] * group / R + lo);
-  return lo;
+  __device__ __forceinline__ int keys(long long end) const {  // of the next stage
+    return (int)min((long long)min(DC_KEYS, sq.lk - key), end - pos);
+  }
+  __device__ __forceinline__ void step(const Shape& s, int n, long long end) {
+    pos += n;
+    key += n;
+    on = pos < end;
+    if (key == sq.lk) {
+      key = 0;
+      pos += VOID;
+      on = pos < end;
+      if (++hk == s.kv_heads && on) {
+        ++b;
+        settle(s, end);
+      }
+    }
+  }
+};
+__device__ __forceinline__ int seq_of_position(const Shape& s, long long pos) {
+  return last_at_most(s.batch, pos, [&](int i) { return (s.cu_k[i] + (long long)i * VOID) * s.kv_heads; });
 }
 
-__device__ __forceinline__ float exp2_of(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// Lane l's columns of a row: vectors of four, LPK vectors apart.
-template <int E, int LPK, bool VEC>
-__device__ __forceinline__ void load_cols(float (&x)[E], const float* p, int l, int dim) {
+// Lane l's columns of a row of shared memory: vectors of four, DC_LPK vectors apart.
+template <int E>
+__device__ __forceinline__ void load_cols(float (&x)[E], const float* p, int l) {
 #pragma unroll
   for (int c = 0; c < E / 4; ++c) {
-    const int col = (c * LPK + l) * 4;
+    const float4 f = *reinterpret_cast<const float4*>(p + (c * DC_LPK + l) * 4);
+    x[4 * c] = f.x;
+    x[4 * c + 1] = f.y;
+    x[4 * c + 2] = f.z;
+    x[4 * c + 3] = f.w;
+  }
+}
+
+// The same columns of a row of `dim` values in global memory, zeros behind them.
+template <int E>
+__device__ __forceinline__ void load_row(float (&x)[E], const float* p, int l, int dim, bool vec) {
+#pragma unroll
+  for (int c = 0; c < E / 4; ++c) {
+    const int col = (c * DC_LPK + l) * 4;
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (VEC) {
+    if (vec) {
       if (col < dim) f = *reinterpret_cast<const float4*>(p + col);
     } else {
       if (col < dim) f.x = p[col];
@@ -60,207 +126,393 @@ __device__ __forceinline__ void load_cols(float (&x)[E], const float* p, int l, 
   }
 }
 
-// grid: (row chunks, key heads, splits).  Split z takes the key chunks z, z +
-// gridDim.z, ...; with one split the results go straight to o and lse.
-template <int R, int LPK, int DP, bool VEC>
-__global__ void __launch_bounds__(32 * DC_WARPS)
-    attn_decode_kernel(const __grid_constant__ Shape s, const float* __restrict__ q, const float* __restrict__ k,
-                       const float* __restrict__ v, float* o, float* lse, float* __restrict__ part, int chunk) {
-  constexpr int E = DP / LPK, G = 32 / LPK;  // columns per lane, groups per warp
-  __shared__ float sm_acc[DC_WARPS][R][DP];
-  __shared__ float sm_m[DC_WARPS][R], sm_sum[DC_WARPS][R];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / LPK, l = lane % LPK;
-  long long jc;
-  const int b = seq_of_chunk(s.cu_q, s.batch, s.group, R, blockIdx.x, &jc);
-  const Seq sq = seq_bounds(s, b);
-  const long long all_rows = (long long)sq.lq * s.group, row0 = jc * R;
-  if (jc < 0 || row0 >= all_rows) return;
-  const int rows = (int)min((long long)R, all_rows - row0), hk = blockIdx.y;
-  if (blockIdx.z > 0 && (long long)blockIdx.z * chunk >= sq.lk) return;
-
-  float qr[R][E], acc[R][E], m[R], sum[R];
-  int vis[R];
-  int vis_least = sq.lk;
+// Sums of x over the warp's four groups; lane (g, l) is left with four columns
+// of it: those of vector g (DP = 128), or of vector g / 2 (DP = 64, held twice).
+template <int E>
+__device__ __forceinline__ float4 sum_groups(const float (&x)[E], int g) {
+  const bool up = g & 2, odd = g & 1;
+  float y[E / 2];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int i = (int)((row0 + r) / s.group), h = hk * s.group + (int)((row0 + r) % s.group);
-    const bool on = r < rows;
-    if (on) {
-      load_cols<E, LPK, VEC>(qr[r], q + (sq.q0 + i) * s.ldq + (long long)h * s.dim, l, s.dim);
-    }
-    vis[r] = on ? sq.visible(i, s.causal) : 0;
-    if (on) vis_least = min(vis_least, vis[r]);
-    m[r] = -INFINITY;
-    sum[r] = 0.0f;
+  for (int e = 0; e < E / 2; ++e) {
+    const float mine = up ? x[E / 2 + e] : x[e], other = up ? x[e] : x[E / 2 + e];
+    y[e] = mine + __shfl_xor_sync(0xffffffffu, other, 16);
+  }
+  float z[4];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      qr[r][e] = on ? qr[r][e] * (s.scale * LOG2E) : 0.0f;
-      acc[r][e] = 0.0f;
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (E == 16) {
+      const float mine = odd ? y[4 + e] : y[e], other = odd ? y[e] : y[4 + e];
+      z[e] = mine + __shfl_xor_sync(0xffffffffu, other, 8);
+    } else {
+      z[e] = y[e] + __shfl_xor_sync(0xffffffffu, y[e], 8);
     }
   }
-  const float* kb = k + sq.k0 * s.ldk + (long long)hk * s.dim;
-  const float* vb = v + sq.k0 * s.ldv + (long long)hk * s.dim;
-  const int vis_most = sq.visible((int)((row0 + rows - 1) / s.group), s.causal);
-  for (long long c0 = (long long)blockIdx.z * chunk; c0 < vis_most; c0 += (long long)gridDim.z * chunk) {
-    const int end = (int)min(c0 + chunk, (long long)vis_most);
-    for (int j0 = (int)c0 + warp * G * DC_U; j0 < end; j0 += DC_WARPS * G * DC_U) {
-      // the warp's G * DC_U consecutive keys: u-th load takes keys j0 + u * G + g
-      float kr[DC_U][E], vr[DC_U][E];
-#pragma unroll
-      for (int u = 0; u < DC_U; ++u) {
-        const int j = min(j0 + u * G + g, end - 1);
-        load_cols<E, LPK, VEC>(kr[u], kb + (long long)j * s.ldk, l, s.dim);
+  return make_float4(z[0], z[1], z[2], z[3]);
+}
+
+// Ring w of `rings` takes the positions w * per .. +per.  warps_per_ring = WR in
+// {1, 2, 4, 8}; warp i of a ring has the rows i * R .. +R of a sequence.
+template <int R, int DP, bool VEC>
+__global__ void __launch_bounds__(32 * DC_WARPS, 1)
+    attn_decode_kernel(const __grid_constant__ Shape s, const __grid_constant__ CUtensorMap map_k,
+                       const __grid_constant__ CUtensorMap map_v, const float* __restrict__ q, const float* __restrict__ k,
+                       const float* __restrict__ v, float* o, float* lse, float* __restrict__ part, long long per,
+                       int WR) {
+  constexpr int E = DP / DC_LPK, STEPS = DC_KEYS / DC_GROUPS, STAGE = dc_stage(DP);
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / DC_LPK, l = lane % DC_LPK;
+  const int ring = warp / WR, wr = warp % WR, nst = dc_stages(DP) / DC_WARPS * WR;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + DC_RING) + ring * nst;
+  uint64_t* empty = full + dc_stages(DP);
+  float* stages = reinterpret_cast<float*>(smem + (size_t)ring * nst * STAGE);
+  if (wr == 0 && lane == 0) {
+    for (int i = 0; i < nst; ++i) {
+      jxd::mbar_init(&full[i], VEC ? 1 : 32);
+      jxd::mbar_init(&empty[i], WR);
+    }
+    jxd::fence_mbar_init();
+  }
+  if (VEC) {
+    if (threadIdx.x == 0) {
+      jxd::tma_prefetch_desc(&map_k);
+      jxd::tma_prefetch_desc(&map_v);
+    }
+  } else {  // columns behind the head's dim stay zero
+    for (int i = threadIdx.x; i < DC_RING / 16; i += 32 * DC_WARPS)
+      reinterpret_cast<float4*>(smem)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  jxd::fence_proxy_async_smem();
+  __syncthreads();
+
+  const long long w = (long long)ring * gridDim.x + blockIdx.x;  // few rings' worth of work spreads over all SMs
+  const long long begin = w * per, end = min(begin + per, (s.total_k + (long long)s.batch * VOID) * s.kv_heads);
+  const bool vec_q = !(s.dim & 3) && !(s.ldq & 3) && !(reinterpret_cast<uintptr_t>(q) & 15);
+  const bool vec_o = !(s.dim & 3) && !(s.ldo & 3) && !(reinterpret_cast<uintptr_t>(o) & 15);
+  Cursor c;
+  c.pos = begin;
+  c.b = seq_of_position(s, begin);
+  c.settle(s, end);
+  Cursor pc = c;  // the copies' place, up to nst stages ahead
+  int in_st = 0, out_st = 0, issued = 0;
+  uint32_t in_ph = 0, out_ph = 0;
+  bool ok = true;
+  auto produce = [&]() {  // the ring's first warp: the next stage's rows
+    if (!pc.on || !ok) return;
+    const int st = in_st, n = pc.keys(end);
+    ok = __all_sync(0xffffffffu, wait_bounded(&empty[st], in_ph ^ 1u, s.err));
+    if (!ok) return;
+    const long long t = pc.sq.k0 + pc.key;
+    float* dst = stages + (size_t)st * (STAGE / 4);
+    if constexpr (VEC) {
+      // eight rows each, whatever n is: the rest is other sequences' or zeros, and masked
+      if (lane == 0) {
+        jxd::mbar_arrive_expect_tx(&full[st], (uint32_t)STAGE);
+        jxd::tma_load_3d(dst, &map_k, &full[st], 0, (int)t, pc.hk);
+        jxd::tma_load_3d(dst + DC_KEYS * DP, &map_v, &full[st], 0, (int)t, pc.hk);
       }
-#pragma unroll
-      for (int u = 0; u < DC_U; ++u) {
-        const int j = min(j0 + u * G + g, end - 1);
-        load_cols<E, LPK, VEC>(vr[u], vb + (long long)j * s.ldv, l, s.dim);
-      }
-      const bool whole = j0 + DC_U * G <= min(end, vis_least);  // every row sees all of these keys
+    } else {
+      const long long hd = (long long)pc.hk * s.dim;
+      for (int r = 0; r < n; ++r)
+        for (int col = lane; col < s.dim; col += 32) {
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(jxd::smem_u32(dst + r * DP + col)),
+                       "l"(k + (t + r) * s.ldk + hd + col)
+                       : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(jxd::smem_u32(dst + (8 + r) * DP + col)),
+                       "l"(v + (t + r) * s.ldv + hd + col)
+                       : "memory");
+        }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(jxd::smem_u32(&full[st])) : "memory");
+    }
+    ++issued;
+    if (++in_st == nst) {
+      in_st = 0;
+      in_ph ^= 1u;
+    }
+    pc.step(s, n, end);
+  };
+  if (wr == 0)
+    for (int i = 0; i < nst; ++i) produce();
+
+  while (c.on && ok) {
+    // one piece of a (sequence, key head)
+    const int b = c.b, hk = c.hk, first_key = c.key;
+    const Seq sq = c.sq;
+    const int all_rows = (int)min((long long)sq.lq * s.group, (long long)R * WR), row0 = wr * R;
+    float qr[R][E], acc[R][E], m[R], sum[R];
+    int vis[R], vis_least = sq.lk;
+    {
+      int i = row0 / s.group, hg = row0 - i * s.group;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        float x[DC_U];
-#pragma unroll
-        for (int u = 0; u < DC_U; ++u) {
-          float d = 0.0f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) d = fmaf(qr[r][e], kr[u][e], d);
-#pragma unroll
-          for (int w = LPK / 2; w > 0; w >>= 1) d += __shfl_xor_sync(0xffffffffu, d, w);
-          x[u] = d;
+        const bool on = row0 + r < all_rows;
+        load_row<E>(qr[r], q + (sq.q0 + i) * s.ldq + (long long)(hk * s.group + hg) * s.dim, l, on ? s.dim : 0, vec_q);
+        vis[r] = on ? sq.visible(i, s.causal) : 0;
+        if (on) vis_least = min(vis_least, vis[r]);
+        if (++hg == s.group) {
+          hg = 0;
+          ++i;
         }
-        bool on[DC_U];
+      }
 #pragma unroll
-        for (int u = 0; u < DC_U; ++u) {
-          const int j = j0 + u * G + g;
-          on[u] = whole || (j < end && j < vis[r]);
-          if (!on[u]) x[u] = -INFINITY;
+      for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          qr[r][e] *= s.scale * LOG2E;
+          acc[r][e] = 0.0f;
         }
-        float top = m[r];
+      }
+    }
+    while (c.on && c.b == b && c.hk == hk) {
+      const int n = c.keys(end), st = out_st, j0 = c.key;
+      ok = ok && __all_sync(0xffffffffu, wait_bounded(&full[st], out_ph, s.err));
+      if (!ok) break;
+      const float* base = stages + (size_t)st * (STAGE / 4);
+      float x[R][STEPS];
 #pragma unroll
-        for (int u = 0; u < DC_U; ++u) top = fmaxf(top, x[u]);
-        if (__any_sync(0xffffffffu, top > m[r])) {
-          const float f = exp2_of(m[r] - (top == -INFINITY ? 0.0f : top));
+      for (int u = 0; u < STEPS; ++u) {
+        float kr[E];
+        load_cols<E>(kr, base + (u * DC_GROUPS + g) * DP, l);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float2 d = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int e = 0; e < E; e += 2)
+            d = fma2(make_float2(qr[r][e], qr[r][e + 1]), make_float2(kr[e], kr[e + 1]), d);
+          x[r][u] = d.x + d.y;
+        }
+      }
+#pragma unroll
+      for (int t = DC_LPK / 2; t > 0; t >>= 1)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int u = 0; u < STEPS; ++u) x[r][u] += __shfl_xor_sync(0xffffffffu, x[r][u], t);
+      const bool whole = j0 + DC_KEYS <= vis_least && n == DC_KEYS;  // every row sees all of the stage's keys
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int u = 0; u < STEPS; ++u)
+            if (u * DC_GROUPS + g >= n || j0 + u * DC_GROUPS + g >= vis[r]) x[r][u] = -INFINITY;
+      }
+      bool grows = false;
+      float top[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        top[r] = m[r];
+#pragma unroll
+        for (int u = 0; u < STEPS; ++u) top[r] = fmaxf(top[r], x[r][u]);
+        grows = grows || top[r] > m[r];
+      }
+      if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float f = exp2_fast(m[r] - (top[r] == -INFINITY ? 0.0f : top[r]));
           sum[r] *= f;
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[r][e] *= f;
-          m[r] = top;
+          m[r] = top[r];
         }
-        const float base = top == -INFINITY ? 0.0f : top;
+      }
 #pragma unroll
-        for (int u = 0; u < DC_U; ++u) {
-          const float p = exp2_of(x[u] - base);
-          sum[r] += p;
-          if (whole) {
+      for (int r = 0; r < R; ++r) {
+        const float z = top[r] == -INFINITY ? 0.0f : top[r];
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[r][e] = fmaf(p, vr[u][e], acc[r][e]);
-          } else if (on[u]) {  // an unseen key's value may be anything
+        for (int u = 0; u < STEPS; ++u) {
+          x[r][u] = exp2_fast(x[r][u] - z);
+          sum[r] += x[r][u];
+        }
+      }
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[r][e] = fmaf(p, vr[u][e], acc[r][e]);
+      for (int u = 0; u < STEPS; ++u) {
+        float vr[E];
+        load_cols<E>(vr, base + (DC_KEYS + u * DC_GROUPS + g) * DP, l);
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+              const float2 a = fma2(make_float2(x[r][u], x[r][u]), make_float2(vr[e], vr[e + 1]),
+                                    make_float2(acc[r][e], acc[r][e + 1]));
+              acc[r][e] = a.x;
+              acc[r][e + 1] = a.y;
+            }
+        } else {  // an unseen key's value, or what an earlier stage left, may be anything
+          const int j = j0 + u * DC_GROUPS + g;
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            if (u * DC_GROUPS + g < n && j < vis[r]) {
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[r][e] = fmaf(x[r][u], vr[e], acc[r][e]);
+            }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(&empty[st]);
+      if (++out_st == nst) {
+        out_st = 0;
+        out_ph ^= 1u;
+      }
+      c.step(s, n, end);
+      if (wr == 0) produce();
+    }
+    if (!ok) break;
+    // join the warp's groups, store
+    // the head's first position
+    const long long seg = (sq.k0 + (long long)b * VOID) * s.kv_heads + (long long)hk * (sq.lk + VOID);
+    const bool last = seg >= begin && seg + sq.lk <= end;
+    int i = row0 / s.group, hg = row0 - i * s.group;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float t = m[r];
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+      const float f = exp2_fast(m[r] - (t == -INFINITY ? 0.0f : t));
+      float a = sum[r] * f;
+      a += __shfl_xor_sync(0xffffffffu, a, 8);
+      a += __shfl_xor_sync(0xffffffffu, a, 16);
+      const float inv = !last ? f : a == 0.0f ? 0.0f : f / a;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[r][e] *= inv;
+      const float4 y = sum_groups<E>(acc[r], g);
+      if (row0 + r < all_rows) {
+        const long long tok = sq.q0 + i;
+        const int h = hk * s.group + hg, col = ((E == 16 ? g : g >> 1) * DC_LPK + l) * 4;
+        float* out = last ? o + tok * s.ldo + (long long)h * s.dim
+                          : part + ((w * 2 + (first_key == 0)) * (R * WR) + row0 + r) * (DP + 4);
+        if (E == 16 || !(g & 1)) {
+          if (!last || vec_o) {
+            if (col < s.dim) *reinterpret_cast<float4*>(out + col) = y;
+          } else {
+            if (col < s.dim) out[col] = y.x;
+            if (col + 1 < s.dim) out[col + 1] = y.y;
+            if (col + 2 < s.dim) out[col + 2] = y.z;
+            if (col + 3 < s.dim) out[col + 3] = y.w;
+          }
+        }
+        if (lane == 0) {
+          if (!last) {
+            out[DP] = t;
+            out[DP + 1] = a;
+          } else if (lse) {
+            lse[(long long)h * s.total_q + tok] = a == 0.0f ? -INFINITY : (t + log2f(a)) * LN2;
           }
         }
       }
-    }
-  }
-  // the warp's groups, then the warps
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float top = m[r];
-#pragma unroll
-    for (int w = LPK; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    const float f = exp2_of(m[r] - (top == -INFINITY ? 0.0f : top));
-    float t = sum[r] * f;
-#pragma unroll
-    for (int w = LPK; w < 32; w <<= 1) t += __shfl_xor_sync(0xffffffffu, t, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      float a = acc[r][e] * f;
-#pragma unroll
-      for (int w = LPK; w < 32; w <<= 1) a += __shfl_xor_sync(0xffffffffu, a, w);
-      if (g == 0) sm_acc[warp][r][((e / 4) * LPK + l) * 4 + (e & 3)] = a;
-    }
-    if (lane == 0) {
-      sm_m[warp][r] = top;
-      sm_sum[warp][r] = t;
-    }
-  }
-  __syncthreads();
-  const bool last = gridDim.z == 1;
-  for (int r = warp; r < rows; r += DC_WARPS) {
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < DC_WARPS; ++w) top = fmaxf(top, sm_m[w][r]);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float t = 0.0f, f[DC_WARPS];
-#pragma unroll
-    for (int w = 0; w < DC_WARPS; ++w) {
-      f[w] = exp2_of(sm_m[w][r] - base);
-      t += sm_sum[w][r] * f[w];
-    }
-    const int i = (int)((row0 + r) / s.group), h = hk * s.group + (int)((row0 + r) % s.group);
-    const long long tok = sq.q0 + i;
-    float* out = last ? o + tok * s.ldo + (long long)h * s.dim
-                      : part + ((tok * s.heads + h) * gridDim.z + blockIdx.z) * (MAX_DIM + 2);
-    const float inv = !last ? 1.0f : t == 0.0f ? 0.0f : 1.0f / t;
-    for (int c = lane; c < s.dim; c += 32) {
-      float a = 0.0f;
-#pragma unroll
-      for (int w = 0; w < DC_WARPS; ++w) a += sm_acc[w][r][c] * f[w];
-      out[c] = a * inv;
-    }
-    if (lane == 0) {
-      if (!last) {
-        out[MAX_DIM] = top;
-        out[MAX_DIM + 1] = t;
-      } else if (lse) {
-        lse[(long long)h * s.total_q + tok] = t == 0.0f ? -INFINITY : (top + log2f(t)) * LN2;
+      if (++hg == s.group) {
+        hg = 0;
+        ++i;
       }
     }
   }
+  // not before: the join's blocks would wait where rings still stream (37.0 us against 33.2 at the start of the kernel)
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (!ok && wr == 0)  // every copy has landed before the CTA may end
+    for (int u = max(0, issued - nst); u < issued; ++u) wait_bounded(&full[u % nst], (uint32_t)(u / nst) & 1u, s.err);
 }
 
-// One warp per (query row, head): the splits' results in order.
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ Shape s, const float* __restrict__ part,
-                                                       float* o, float* lse, int splits, int chunk) {
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  const long long tok = w / s.heads;
-  const int h = (int)(w - tok * s.heads);
-  if (tok >= s.total_q) return;
+// One block per (query row, head): the pieces in order; rows without keys; rows
+// behind the ones that the rings took (where the caller's hint was too small).
+constexpr int JN_WARPS = 4;
+constexpr int JN_AHEAD = 8;
+__global__ void __launch_bounds__(32 * JN_WARPS)
+    attn_join_kernel(const __grid_constant__ Shape s, const float* __restrict__ q, const float* __restrict__ k,
+                     const float* __restrict__ v, const float* part, float* o, float* lse, long long per,
+                     int ring_rows, int DP) {
+  __shared__ float red[2 * JN_WARPS];
+  __shared__ float4 acc[JN_WARPS][32];
+  const long long tok = blockIdx.x / (unsigned)s.heads;
+  const int h = (int)(blockIdx.x % (unsigned)s.heads), hk = h / s.group;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = seq_of_row(s.cu_q, s.batch, tok);
-  if (b < 0) return;
   const Seq sq = seq_bounds(s, b);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the rings' results are complete and visible behind it
   if (tok < sq.q0 || tok >= sq.q0 + sq.lq) return;
-  const int n = max(1, (int)min((long long)splits, ((long long)sq.lk + chunk - 1) / chunk));
-  const float* p = part + (tok * s.heads + h) * splits * (MAX_DIM + 2);
-  float top = -INFINITY;
-  for (int z = lane; z < n; z += 32) top = fmaxf(top, p[(long long)z * (MAX_DIM + 2) + MAX_DIM]);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  const float base = top == -INFINITY ? 0.0f : top;
-  float a[4] = {0.f, 0.f, 0.f, 0.f}, t = 0.0f;
-#pragma unroll 4
-  for (int z = 0; z < n; ++z) {
-    const float* e = p + (long long)z * (MAX_DIM + 2);
-    const float f = exp2_of(e[MAX_DIM] - base);
-    t += e[MAX_DIM + 1] * f;
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (lane + 32 * c < s.dim) a[c] += e[lane + 32 * c] * f;
+  const int i = (int)(tok - sq.q0);
+  const long long row = (long long)i * s.group + h % s.group;
+  float* out = o + tok * s.ldo + (long long)h * s.dim;
+  if (row >= ring_rows || sq.lk == 0) {
+    if (warp == 0)
+      row_fwd(q + tok * s.ldq + (long long)h * s.dim, k + sq.k0 * s.ldk + (long long)hk * s.dim,
+              v + sq.k0 * s.ldv + (long long)hk * s.dim, out, lse ? lse + (long long)h * s.total_q + tok : nullptr,
+              sq.visible(i, s.causal), s.dim, s.ldk, s.ldv, s.scale);
+    return;
   }
-  const float inv = t == 0.0f ? 0.0f : 1.0f / t;
+  const long long seg = (sq.k0 + (long long)b * VOID) * s.kv_heads + (long long)hk * (sq.lk + VOID);
+  const long long w0 = seg / per;
+  const int n = (int)((seg + sq.lk - 1) / per - w0) + 1;
+  if (n == 1) return;
+  // piece z lies in ring w0 + z's slot 1 if it starts the head, else in slot 0
+  auto piece = [&](int z) { return part + (((w0 + z) * 2 + (z == 0)) * ring_rows + row) * (DP + 4); };
+  // each warp takes every JN_WARPS-th piece, a lane four columns; the first ones are loaded before the maximum is known
+  const bool in = lane * 4 < DP;
+  float4 x[JN_AHEAD];
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < s.dim) o[tok * s.ldo + (long long)h * s.dim + lane + 32 * c] = a[c] * inv;
-  if (lane == 0 && lse) lse[(long long)h * s.total_q + tok] = t == 0.0f ? -INFINITY : (top + log2f(t)) * LN2;
+  for (int e = 0; e < JN_AHEAD; ++e) {
+    const int z = warp + JN_WARPS * e;
+    x[e] = in && z < n ? reinterpret_cast<const float4*>(piece(z))[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  float top = -INFINITY;
+  for (int z = threadIdx.x; z < n; z += 32 * JN_WARPS) top = fmaxf(top, piece(z)[DP]);
+#pragma unroll
+  for (int e = 16; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, e));
+  if (lane == 0) red[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < JN_WARPS; ++e) top = fmaxf(top, red[e]);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float t = 0.0f;
+  for (int z0 = warp; z0 < n; z0 += JN_WARPS * JN_AHEAD) {
+    float f[JN_AHEAD];
+#pragma unroll
+    for (int e = 0; e < JN_AHEAD; ++e) {
+      const int z = z0 + JN_WARPS * e;
+      f[e] = z < n ? exp2_fast(piece(z)[DP] - base) : 0.0f;
+      t += z < n ? piece(z)[DP + 1] * f[e] : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < JN_AHEAD; ++e) {
+      a.x = fmaf(x[e].x, f[e], a.x);
+      a.y = fmaf(x[e].y, f[e], a.y);
+      a.z = fmaf(x[e].z, f[e], a.z);
+      a.w = fmaf(x[e].w, f[e], a.w);
+      const int z = z0 + JN_WARPS * (JN_AHEAD + e);
+      x[e] = in && z < n ? reinterpret_cast<const float4*>(piece(z))[lane] : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
+  acc[warp][lane] = a;
+  if (lane == 0) red[JN_WARPS + warp] = t;
+  __syncthreads();
+  if (warp == 0) {
+    t = 0.0f;
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int e = 0; e < JN_WARPS; ++e) {
+      t += red[JN_WARPS + e];
+      a.x += acc[e][lane].x;
+      a.y += acc[e][lane].y;
+      a.z += acc[e][lane].z;
+      a.w += acc[e][lane].w;
+    }
+    const float inv = t == 0.0f ? 0.0f : 1.0f / t;
+    const int c = lane * 4;
+    if (c < s.dim) out[c] = a.x * inv;
+    if (c + 1 < s.dim) out[c + 1] = a.y * inv;
+    if (c + 2 < s.dim) out[c + 2] = a.z * inv;
+    if (c + 3 < s.dim) out[c + 3] = a.w * inv;
+    if (lane == 0 && lse) lse[(long long)h * s.total_q + tok] = t == 0.0f ? -INFINITY : (top + log2f(t)) * LN2;
+  }
 }
 
-using DecodeKernel = void (*)(Shape, const float*, const float*, const float*, float*, float*, float*, int);
+using DecodeKernel = void (*)(Shape, CUtensorMap, CUtensorMap, const float*, const float*, const float*, float*, float*, float*, long long, int);
 
-template <int R, int L128, int L64>
+template <int R>
 DecodeKernel kernel_of(int DP, bool vec) {
-  if (DP == 128) return vec ? attn_decode_kernel<R, L128, 128, true> : attn_decode_kernel<R, L128, 128, false>;
-  return vec ? attn_decode_kernel<R, L64, 64, true> : attn_decode_kernel<R, L64, 64, false>;
+  if (DP == 128) return vec ? attn_decode_kernel<R, 128, true> : attn_decode_kernel<R, 128, false>;
+  return vec ? attn_decode_kernel<R, 64, true> : attn_decode_kernel<R, 64, false>;
 }
 
 }  // namespace
@@ -269,32 +521,47 @@ namespace jxa {
 
 // rows: query rows per key head of the longest sequence, a hint.
 int attention_decode(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
-                     long long rows, long long max_k, cudaStream_t st) {
+                     long long rows, cudaStream_t st) {
   const int DP = s.dim <= 64 ? 64 : 128;
   auto a16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  const bool vec = !(s.dim & 3) && !(s.ldq & 3) && !(s.ldk & 3) && !(s.ldv & 3) && a16(q) && a16(k) && a16(v);
-  const int R = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-  const DecodeKernel kernel = R == 1   ? kernel_of<1, 8, 8>(DP, vec)
-                              : R == 2 ? kernel_of<2, 8, 8>(DP, vec)
-                              : R == 4 ? kernel_of<4, 8, 8>(DP, vec)
-                              : R == 8 ? kernel_of<8, 16, 16>(DP, vec)
-                                       : kernel_of<16, 32, 16>(DP, vec);
-  const long long chunks = s.total_q * s.group / R + s.batch;
-  JX_REQUIRE(chunks < (1LL << 31), "attention: too many rows");
-  // keys per CTA: four CTAs per SM over all sequences, 64 keys at least
-  const long long even = s.total_k * s.kv_heads / (4LL * jx::num_sms());
-  const int chunk = (int)std::min<long long>(1 << 20, std::max<long long>(64, (even + 63) / 64 * 64));
-  const int splits = (int)std::max<long long>(1, std::min<long long>(128, (max_k + chunk - 1) / chunk));
+  const bool vec = s.total_k > 0 && !(s.dim & 3) && !(s.ldk & 3) && !(s.ldv & 3) && a16(k) && a16(v) &&
+                   s.ldk < (1LL << 37) && s.ldv < (1LL << 37);  // what a tensor map takes
+  const int R = rows <= 1 ? 1 : rows <= 2 ? 2 : 4;
+  const int WR = rows <= 4 ? 1 : rows <= 8 ? 2 : rows <= 16 ? 4 : 8;
+  const DecodeKernel kernel = R == 1 ? kernel_of<1>(DP, vec) : R == 2 ? kernel_of<2>(DP, vec) : kernel_of<4>(DP, vec);
+  if (int rc = prepare_kernel((const void*)kernel, 8 + (R >> 1) * 4 + (DP == 128) * 2 + vec, dc_smem(DP), 0)) return rc;
+  CUtensorMap map_k = {}, map_v = {};
+  if (vec) {
+    const uint64_t dims[3] = {(uint64_t)s.dim, (uint64_t)s.total_k, (uint64_t)s.kv_heads};
+    const uint64_t in_k[2] = {(uint64_t)s.ldk * 4, (uint64_t)s.dim * 4}, in_v[2] = {(uint64_t)s.ldv * 4, in_k[1]};
+    const uint32_t box[2] = {(uint32_t)DP, DC_KEYS};
+    if (int rc = jx::tensor_map_f32_3d(&map_k, k, dims, in_k, box)) return rc;
+    if (int rc = jx::tensor_map_f32_3d(&map_v, v, dims, in_v, box)) return rc;
+  }
+  // positions per ring: an equal share, 32 at least
+  const int max_rings = jx::num_sms() * (DC_WARPS / WR);
+  const long long all = (s.total_k + (long long)s.batch * VOID) * s.kv_heads;
+  const long long per = std::max<long long>(32, ((all + max_rings - 1) / max_rings + 7) / 8 * 8);
+  const int rings = (int)((all + per - 1) / per);
+  const int grid = std::min(jx::num_sms(), rings);
   void* part = nullptr;
-  if (splits > 1)
-    if (int rc = jx::scratch_get(sizeof(float) * (size_t)s.total_q * s.heads * splits * (MAX_DIM + 2), &part, st))
-      return rc;
-  kernel<<<dim3((unsigned)chunks, (unsigned)s.kv_heads, (unsigned)splits), 32 * DC_WARPS, 0, st>>>(
-      s, q, k, v, o, lse, static_cast<float*>(part), chunk);
-  if (splits > 1)
-    attn_join_kernel<<<(unsigned)((s.total_q * s.heads + 3) / 4), 128, 0, st>>>(s, static_cast<float*>(part), o, lse,
-                                                                              splits, chunk);
-  const cudaError_t e = cudaGetLastError();
+  if (int rc = jx::scratch_get(sizeof(float) * (size_t)grid * (DC_WARPS / WR) * 2 * R * WR * (DP + 4), &part, st))
+    return rc;
+  if (rings > 0)
+    kernel<<<grid, 32 * DC_WARPS, dc_smem(DP), st>>>(s, map_k, map_v, q, k, v, o, lse, static_cast<float*>(part), per, WR);
+  // the join's blocks may start while the last rings finish; they wait for them before they read
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(s.total_q * s.heads));
+  cfg.blockDim = dim3(32 * JN_WARPS);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = cudaLaunchKernelEx(&cfg, attn_join_kernel, s, q, k, v, static_cast<const float*>(part), o, lse, per, R * WR, DP);
   jx::scratch_release(part, st);
   return e == cudaSuccess ? JX_OK : jx::check_cuda(e, "attn_decode_kernel");
 }

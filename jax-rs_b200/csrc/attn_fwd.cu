@@ -492,18 +492,21 @@ int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, 
   return JX_OK;
 }
 
-// Per device and variant, once: the shared-memory limit and the registers the kernel was built with.
+// Per device and variant, once: the shared-memory limit, and (launch_regs not 0) a
+// check of the registers that the kernel was built with.
 int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs) {
-  static std::atomic<int> done[64][8];
+  static std::atomic<int> done[64][32];
   int dev = 0;
   JX_CUDA(cudaGetDevice(&dev));
   std::atomic<int>& d = done[dev & 63][variant];
   if (d.load(std::memory_order_acquire)) return JX_OK;
-  cudaFuncAttributes fa;
-  JX_CUDA(cudaFuncGetAttributes(&fa, kernel));
-  if (fa.numRegs != launch_regs)  // setmaxnreg.inc would wait for registers that never come
-    return jx::fail(JX_EUNSUPPORTED, "attention kernel built with %d registers per thread, expected %d", fa.numRegs,
-                    launch_regs);
+  if (launch_regs) {
+    cudaFuncAttributes fa;
+    JX_CUDA(cudaFuncGetAttributes(&fa, kernel));
+    if (fa.numRegs != launch_regs)  // setmaxnreg.inc would wait for registers that never come
+      return jx::fail(JX_EUNSUPPORTED, "attention kernel built with %d registers per thread, expected %d", fa.numRegs,
+                      launch_regs);
+  }
   JX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   d.store(1, std::memory_order_release);
   return JX_OK;

@@ -44,16 +44,11 @@ __host__ __device__ constexpr int tile_bytes(int DP) { return 2 * tile_part(DP);
 
 inline long long tile_count(long long total, int batch) { return total / TILE + batch; }
 
-// Sequence and index within it of tile `id`; the index may lie behind the sequence's end.
+// Sequence and index within it of tile `id` (warp-uniform); the index may lie behind the sequence's end.
 __device__ __forceinline__ int seq_of_tile(const int32_t* cu, int batch, int id, int* j) {
-  int lo = 0, hi = batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((cu[mid] >> 7) + mid <= id) lo = mid;
-    else hi = mid;
-  }
-  *j = id - ((cu[lo] >> 7) + lo);
-  return lo;
+  const int b = last_at_most(batch, id, [&](int i) { return (long long)((cu[i] >> 7) + i); });
+  *j = id - ((cu[b] >> 7) + b);
+  return b;
 }
 __device__ __forceinline__ int first_tile(long long start, int b) { return (int)(start >> 7) + b; }
 
@@ -224,7 +219,7 @@ int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs
 int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
                         cudaStream_t st);
 int attention_decode(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
-                     long long rows, long long max_k, cudaStream_t st);
+                     long long rows, cudaStream_t st);
 int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
                         const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st);
 
