@@ -8,6 +8,13 @@
 //   backward  xhat = (x - mean) * rstd, g = dy * gamma,
 //             dx = (g - mean(g) - xhat * mean(g * xhat)) * rstd,
 //             dgamma = sum over rows of dy * xhat, dbeta = sum over rows of dy
+//
+// Bound by HBM: 8 bytes an element forward, 12 backward.  A row is read once
+// and held in registers, by a warp (narrow rows) or by a block; the variance is
+// of the centred values, so a mean far from zero costs no digits.  Backward, a
+// block keeps its columns' sums over all of its rows in registers and loads the
+// next row while it reduces the present one; the blocks' sums are added in
+// order by a second kernel.
 #include <math.h>
 
 #include <algorithm>
@@ -19,75 +26,269 @@ namespace {
 
 using jxn::warp_sum;
 
-constexpr int LN_THREADS = 256;
-
-// Sum over the block; every thread gets it.  sm has one slot per warp and is
-// free again at the caller's next block_sum with the other buffer.
-__device__ __forceinline__ float block_sum(float v, float* sm) {
+// Sum over the T threads that share a row (a warp, or the whole block: one slot
+// of sm per warp).
+template <int T>
+__device__ __forceinline__ float row_sum(float v, float* sm) {
   v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.0f;
+  if constexpr (T > 32) {
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sm[threadIdx.x & (T / 32 - 1)];
 #pragma unroll
-  for (int w = 0; w < LN_THREADS / 32; ++w) t += sm[w];
-  return t;
+    for (int o = T / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  }
+  return v;
 }
 
-// One block per row, the row read three times (from L1 or L2 after the first).
-__global__ void ln_fwd_kernel(const float* __restrict__ x, const float* __restrict__ gamma,
-                              const float* __restrict__ beta, float* y, float* __restrict__ mean_out,
-                              float* __restrict__ rstd_out, long long rows, int cols, long long ldx, long long ldy,
-                              float eps) {
-  __shared__ float sm[2][LN_THREADS / 32];
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float* in = x + r * ldx;
-    float* out = y + r * ldy;
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += LN_THREADS) s += in[c];
-    const float mean = block_sum(s, sm[0]) / (float)cols;
-    float q = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += LN_THREADS) {
-      const float d = in[c] - mean;
-      q += d * d;
+// This thread's N vectors of V columns of a row: vector i starts at column
+// (i * T + t) * V; zeros behind the end.
+template <int T, int V, int N>
+__device__ __forceinline__ void load_row(float (&x)[N * V], const float* p, int t, int cols) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = (i * T + t) * V;
+    if constexpr (V == 4) {
+      const float4 f = c < cols ? *reinterpret_cast<const float4*>(p + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      x[4 * i] = f.x;
+      x[4 * i + 1] = f.y;
+      x[4 * i + 2] = f.z;
+      x[4 * i + 3] = f.w;
+    } else {
+      x[i] = c < cols ? p[c] : 0.0f;
     }
-    const float rstd = 1.0f / sqrtf(block_sum(q, sm[1]) / (float)cols + eps);
-    for (int c = threadIdx.x; c < cols; c += LN_THREADS) {
-      float v = (in[c] - mean) * rstd;
-      if (gamma) v *= gamma[c];
-      if (beta) v += beta[c];
-      out[c] = v;
+  }
+}
+template <int T, int V, int N>
+__device__ __forceinline__ void store_row(float* p, const float (&x)[N * V], int t, int cols) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = (i * T + t) * V;
+    if (c < cols) {
+      if constexpr (V == 4)
+        *reinterpret_cast<float4*>(p + c) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      else
+        p[c] = x[i];
     }
-    if (threadIdx.x == 0) {
-      if (mean_out) mean_out[r] = mean;
-      if (rstd_out) rstd_out[r] = rstd;
-    }
-    __syncthreads();
+  }
+}
+template <int T, int V, int N>
+__device__ __forceinline__ void fill_row(float (&x)[N * V], const float* p, int t, int cols, float value) {
+  if (p) {
+    load_row<T, V, N>(x, p, t, cols);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N * V; ++i) x[i] = value;
   }
 }
 
-__global__ void ln_dx_kernel(const float* dy, const float* __restrict__ x, const float* __restrict__ gamma,
-                             const float* __restrict__ mean, const float* __restrict__ rstd, float* dx,
-                             long long rows, int cols, long long lddy, long long ldx, long long lddx) {
-  __shared__ float sm[2][LN_THREADS / 32];
-  for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-    const float m = mean[r], rs = rstd[r];
+constexpr int block_of(int T) { return T == 32 ? 256 : T; }
+
+// T threads per row.
+template <int T, int V, int N>
+__global__ void __launch_bounds__(block_of(T))
+    ln_fwd_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta, float* y,
+                  float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, long long ldx,
+                  long long ldy, float eps) {
+  __shared__ float sm[2][32];
+  const int t = threadIdx.x % T;
+  const long long r = (long long)blockIdx.x * (block_of(T) / T) + threadIdx.x / T;
+  if (r >= rows) return;  // whole warps; a block with T > 32 has one row
+  float v[N * V], g[N * V], b[N * V];
+  load_row<T, V, N>(v, x + r * ldx, t, cols);
+  fill_row<T, V, N>(g, gamma, t, cols, 1.0f);
+  fill_row<T, V, N>(b, beta, t, cols, 0.0f);
+  const float inv = 1.0f / (float)cols;
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N * V; ++i) s += v[i];
+  const float mean = row_sum<T>(s, sm[0]) * inv;
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool in = (i * T + t) * V < cols;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      v[i * V + e] -= mean;
+      if (in) q = fmaf(v[i * V + e], v[i * V + e], q);
+    }
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<T>(q, sm[1]) * inv + eps);
+#pragma unroll
+  for (int i = 0; i < N * V; ++i) v[i] = fmaf(v[i] * rstd, g[i], b[i]);
+  store_row<T, V, N>(y + r * ldy, v, t, cols);
+  if (t == 0) {
+    if (mean_out) mean_out[r] = mean;
+    if (rstd_out) rstd_out[r] = rstd;
+  }
+}
+
+// Rows too wide for a block's registers: read three times, from L2 after the first.
+constexpr int WIDE = 1024;
+__global__ void __launch_bounds__(WIDE)
+    ln_fwd_wide_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta, float* y,
+                       float* __restrict__ mean_out, float* __restrict__ rstd_out, int cols, long long ldx,
+                       long long ldy, float eps) {
+  __shared__ float sm[2][32];
+  const long long r = blockIdx.x;
+  const float* in = x + r * ldx;
+  float* out = y + r * ldy;
+  float s = 0.0f;
+  for (int c = threadIdx.x; c < cols; c += WIDE) s += in[c];
+  const float mean = row_sum<WIDE>(s, sm[0]) / (float)cols;
+  float q = 0.0f;
+  for (int c = threadIdx.x; c < cols; c += WIDE) {
+    const float d = in[c] - mean;
+    q = fmaf(d, d, q);
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<WIDE>(q, sm[1]) / (float)cols + eps);
+  for (int c = threadIdx.x; c < cols; c += WIDE)
+    out[c] = fmaf((in[c] - mean) * rstd, gamma ? gamma[c] : 1.0f, beta ? beta[c] : 0.0f);
+  if (threadIdx.x == 0) {
+    if (mean_out) mean_out[r] = mean;
+    if (rstd_out) rstd_out[r] = rstd;
+  }
+}
+
+// dx (may be NULL) of the rows blockIdx.x * RPB + .., step gridDim.x * RPB, and the
+// block's column sums into part[blockIdx.x][2][cols] (may be NULL).  AHEAD: the
+// next row is loaded before the present one is reduced.
+template <int T, int V, int N, bool AHEAD>
+__global__ void __launch_bounds__(block_of(T))
+    ln_bwd_kernel(const float* dy, const float* __restrict__ x, const float* __restrict__ gamma,
+                  const float* __restrict__ mean, const float* __restrict__ rstd, float* dx, float* __restrict__ part,
+                  long long rows, int cols, long long lddy, long long ldx, long long lddx) {
+  constexpr int RPB = block_of(T) / T;  // rows per block at a time
+  __shared__ float sm[2][2][32];
+  __shared__ float join[T == 32 ? 7 * 2 * 32 * N * V : 1];
+  const int t = threadIdx.x % T, sub = threadIdx.x / T;
+  const long long step = (long long)gridDim.x * RPB;
+  const float inv = 1.0f / (float)cols;
+  float g[N * V], dg[N * V], db[N * V], xv[N * V], dv[N * V];
+  fill_row<T, V, N>(g, gamma, t, cols, 1.0f);
+#pragma unroll
+  for (int i = 0; i < N * V; ++i) dg[i] = db[i] = 0.0f;
+  long long r = (long long)blockIdx.x * RPB + sub;
+  float m = 0.0f, rs = 0.0f;
+  if (AHEAD && r < rows) {
+    load_row<T, V, N>(dv, dy + r * lddy, t, cols);
+    load_row<T, V, N>(xv, x + r * ldx, t, cols);
+    m = mean[r];
+    rs = rstd[r];
+  }
+  for (int buf = 0; r < rows; r += step, buf ^= 1) {
+    float xn[N * V], dn[N * V], mn = 0.0f, rn = 0.0f;
+    if (AHEAD) {
+      const long long r1 = r + step;
+      if (r1 < rows) {
+        load_row<T, V, N>(dn, dy + r1 * lddy, t, cols);
+        load_row<T, V, N>(xn, x + r1 * ldx, t, cols);
+        mn = mean[r1];
+        rn = rstd[r1];
+      }
+    } else {
+      load_row<T, V, N>(dv, dy + r * lddy, t, cols);
+      load_row<T, V, N>(xv, x + r * ldx, t, cols);
+      m = mean[r];
+      rs = rstd[r];
+    }
     float s1 = 0.0f, s2 = 0.0f;
-    for (int c = threadIdx.x; c < cols; c += LN_THREADS) {
-      const float g = dy[r * lddy + c] * (gamma ? gamma[c] : 1.0f);
-      s1 += g;
-      s2 += g * ((x[r * ldx + c] - m) * rs);
+#pragma unroll
+    for (int i = 0; i < N * V; ++i) {  // behind the end dy is zero
+      xv[i] = (xv[i] - m) * rs;
+      dg[i] = fmaf(dv[i], xv[i], dg[i]);
+      db[i] += dv[i];
+      dv[i] *= g[i];
+      s1 += dv[i];
+      s2 = fmaf(dv[i], xv[i], s2);
     }
-    const float c1 = block_sum(s1, sm[0]) / (float)cols;
-    const float c2 = block_sum(s2, sm[1]) / (float)cols;
-    for (int c = threadIdx.x; c < cols; c += LN_THREADS) {
-      const float g = dy[r * lddy + c] * (gamma ? gamma[c] : 1.0f);
-      dx[r * lddx + c] = (g - c1 - (x[r * ldx + c] - m) * rs * c2) * rs;
+    if (dx) {
+      s1 = warp_sum(s1);
+      s2 = warp_sum(s2);
+      if constexpr (T > 32) {
+        if ((threadIdx.x & 31) == 0) {
+          sm[buf][0][threadIdx.x >> 5] = s1;
+          sm[buf][1][threadIdx.x >> 5] = s2;
+        }
+        __syncthreads();  // one per row: the other buffer is read before the next one's
+        s1 = sm[buf][0][threadIdx.x & (T / 32 - 1)];
+        s2 = sm[buf][1][threadIdx.x & (T / 32 - 1)];
+#pragma unroll
+        for (int o = T / 64; o > 0; o >>= 1) {
+          s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+          s2 += __shfl_xor_sync(0xffffffffu, s2, o);
+        }
+      }
+      const float c1 = s1 * inv, c2 = s2 * inv;
+      float out[N * V];
+#pragma unroll
+      for (int i = 0; i < N * V; ++i) out[i] = (dv[i] - c1 - xv[i] * c2) * rs;
+      store_row<T, V, N>(dx + r * lddx, out, t, cols);
+    }
+    if (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < N * V; ++i) {
+        xv[i] = xn[i];
+        dv[i] = dn[i];
+      }
+      m = mn;
+      rs = rn;
+    }
+  }
+  if (!part) return;
+  if constexpr (T == 32) {  // the block's warps have the same columns
+    constexpr int W = 2 * 32 * N * V;
+    if (sub > 0) {
+#pragma unroll
+      for (int i = 0; i < N * V; ++i) {
+        join[(sub - 1) * W + i * 32 + t] = dg[i];
+        join[(sub - 1) * W + (N * V + i) * 32 + t] = db[i];
+      }
     }
     __syncthreads();
+    if (sub > 0) return;
+    for (int w = 0; w < 7; ++w) {
+#pragma unroll
+      for (int i = 0; i < N * V; ++i) {
+        dg[i] += join[w * W + i * 32 + t];
+        db[i] += join[w * W + (N * V + i) * 32 + t];
+      }
+    }
+  }
+  float* out = part + (long long)blockIdx.x * 2 * cols;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int c = (i * T + t) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (c + e < cols) {
+        out[c + e] = dg[i * V + e];
+        out[cols + c + e] = db[i * V + e];
+      }
   }
 }
 
-// Column sums over chunks of rows, then over the chunks in order.
+// Rows too wide for registers: dx with the row read twice, and column sums over chunks of rows.
+__global__ void __launch_bounds__(WIDE)
+    ln_dx_wide_kernel(const float* dy, const float* __restrict__ x, const float* __restrict__ gamma,
+                      const float* __restrict__ mean, const float* __restrict__ rstd, float* dx, int cols,
+                      long long lddy, long long ldx, long long lddx) {
+  __shared__ float sm[2][32];
+  const long long r = blockIdx.x;
+  const float m = mean[r], rs = rstd[r];
+  float s1 = 0.0f, s2 = 0.0f;
+  for (int c = threadIdx.x; c < cols; c += WIDE) {
+    const float g = dy[r * lddy + c] * (gamma ? gamma[c] : 1.0f);
+    s1 += g;
+    s2 = fmaf(g, (x[r * ldx + c] - m) * rs, s2);
+  }
+  const float c1 = row_sum<WIDE>(s1, sm[0]) / (float)cols;
+  const float c2 = row_sum<WIDE>(s2, sm[1]) / (float)cols;
+  for (int c = threadIdx.x; c < cols; c += WIDE) {
+    const float g = dy[r * lddy + c] * (gamma ? gamma[c] : 1.0f);
+    dx[r * lddx + c] = (g - c1 - (x[r * ldx + c] - m) * rs * c2) * rs;
+  }
+}
 __global__ void ln_col_partial_kernel(const float* __restrict__ dy, const float* __restrict__ x,
                                       const float* __restrict__ mean, const float* __restrict__ rstd,
                                       float* __restrict__ part, long long rows, int cols, long long lddy,
@@ -96,22 +297,119 @@ __global__ void ln_col_partial_kernel(const float* __restrict__ dy, const float*
   if (c >= cols) return;
   const long long r0 = (long long)blockIdx.y * chunk, r1 = min(r0 + chunk, rows);
   float a = 0.0f, b = 0.0f;
+#pragma unroll 4
   for (long long r = r0; r < r1; ++r) {
     const float d = dy[r * lddy + c];
-    a += d * ((x[r * ldx + c] - mean[r]) * rstd[r]);
+    a = fmaf(d, (x[r * ldx + c] - mean[r]) * rstd[r], a);
     b += d;
   }
   part[(long long)blockIdx.y * 2 * cols + c] = a;
   part[(long long)blockIdx.y * 2 * cols + cols + c] = b;
 }
-__global__ void ln_col_final_kernel(const float* __restrict__ part, float* __restrict__ dgamma,
-                                    float* __restrict__ dbeta, int chunks, int cols) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= 2 * cols) return;
-  float acc = 0.0f;
-  for (int k = 0; k < chunks; ++k) acc += part[(long long)k * 2 * cols + c];
-  float* out = c < cols ? dgamma : dbeta;
-  if (out) out[c < cols ? c : c - cols] = acc;
+
+// dgamma and dbeta from part[parts][2 * cols]: 32 columns a block, 32 warps that
+// take every 32nd part, then the warps in order.
+__global__ void __launch_bounds__(1024) ln_join_kernel(const float* part, float* __restrict__ dgamma,
+                                                      float* __restrict__ dbeta, int parts, int cols) {
+  __shared__ float sm[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const long long c = (long long)blockIdx.x * 32 + lane;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the parts are complete behind it
+  float a = 0.0f;
+  if (c < 2LL * cols) {
+#pragma unroll 8
+    for (int p = w; p < parts; p += 32) a += part[(long long)p * 2 * cols + c];
+  }
+  sm[w][lane] = a;
+  __syncthreads();
+  // warp w adds column w's 32 sums
+  a = warp_sum(sm[lane][w]);
+  const long long cc = (long long)blockIdx.x * 32 + w;
+  if (lane == 0 && cc < 2LL * cols) {
+    float* out = cc < cols ? dgamma : dbeta;
+    if (out) out[cc < cols ? cc : cc - cols] = a;
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct FwdArgs {
+  const float *x, *gamma, *beta;
+  float *y, *mean, *rstd;
+  long long rows;
+  int cols;
+  long long ldx, ldy;
+  float eps;
+};
+template <int T, int V, int N>
+void fwd(const FwdArgs& a, cudaStream_t st) {
+  constexpr int RPB = block_of(T) / T;
+  ln_fwd_kernel<T, V, N><<<(unsigned)((a.rows + RPB - 1) / RPB), block_of(T), 0, st>>>(
+      a.x, a.gamma, a.beta, a.y, a.mean, a.rstd, a.rows, a.cols, a.ldx, a.ldy, a.eps);
+}
+
+struct BwdArgs {
+  const float *dy, *x, *gamma, *mean, *rstd;
+  float *dx, *dgamma, *dbeta;
+  long long rows;
+  int cols;
+  long long lddy, ldx, lddx;
+};
+
+int join(const BwdArgs& a, const float* part, int parts, cudaStream_t st) {
+  // its blocks may start while the last rows are summed; they wait before they read
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((2LL * a.cols + 31) / 32));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  JX_CUDA(cudaLaunchKernelEx(&cfg, ln_join_kernel, part, a.dgamma, a.dbeta, parts, a.cols));
+  return JX_OK;
+}
+
+// per_sm: blocks per SM that the grid is made for.
+template <int T, int V, int N, bool AHEAD>
+int bwd(const BwdArgs& a, int per_sm, cudaStream_t st) {
+  constexpr int RPB = block_of(T) / T;
+  const int grid = (int)std::min<long long>((a.rows + RPB - 1) / RPB, (long long)jx::num_sms() * per_sm);
+  const bool sums = a.dgamma || a.dbeta;
+  void* part = nullptr;
+  if (sums)
+    if (int rc = jx::scratch_get(sizeof(float) * 2 * (size_t)grid * a.cols, &part, st)) return rc;
+  ln_bwd_kernel<T, V, N, AHEAD><<<grid, block_of(T), 0, st>>>(a.dy, a.x, a.gamma, a.mean, a.rstd, a.dx,
+                                                              static_cast<float*>(part), a.rows, a.cols, a.lddy, a.ldx,
+                                                              a.lddx);
+  const cudaError_t e = cudaGetLastError();
+  int rc = e == cudaSuccess ? JX_OK : jx::check_cuda(e, "ln_bwd_kernel");
+  if (!rc && sums) rc = join(a, static_cast<const float*>(part), grid, st);
+  jx::scratch_release(part, st);
+  return rc;
+}
+
+int bwd_wide(const BwdArgs& a, cudaStream_t st) {
+  if (a.dgamma || a.dbeta) {  // before dx, which may be dy
+    const long long chunk = std::max<long long>(16, (a.rows + 255) / 256);
+    const int chunks = (int)((a.rows + chunk - 1) / chunk);
+    void* part = nullptr;
+    if (int rc = jx::scratch_get(sizeof(float) * 2 * (size_t)chunks * a.cols, &part, st)) return rc;
+    ln_col_partial_kernel<<<dim3((unsigned)((a.cols + 127) / 128), chunks), 128, 0, st>>>(
+        a.dy, a.x, a.mean, a.rstd, static_cast<float*>(part), a.rows, a.cols, a.lddy, a.ldx, chunk);
+    const cudaError_t e = cudaGetLastError();
+    int rc = e == cudaSuccess ? JX_OK : jx::check_cuda(e, "ln_col_partial_kernel");
+    if (!rc) rc = join(a, static_cast<const float*>(part), chunks, st);
+    jx::scratch_release(part, st);
+    if (rc) return rc;
+  }
+  if (a.dx) {
+    ln_dx_wide_kernel<<<(unsigned)a.rows, WIDE, 0, st>>>(a.dy, a.x, a.gamma, a.mean, a.rstd, a.dx, a.cols, a.lddy,
+                                                         a.ldx, a.lddx);
+    JX_LAUNCH_CHECK("ln_dx_wide_kernel");
+  }
+  return JX_OK;
 }
 
 }  // namespace
@@ -121,15 +419,39 @@ extern "C" {
 int jx_layernorm_f32(const float* x, const float* gamma, const float* beta, float* y, float* mean_out, float* rstd_out,
                      int64_t rows, int64_t cols, int64_t ldx, int64_t ldy, float epsilon, jx_stream_t stream) {
   JX_TRACE("jx_layernorm_f32");
-  JX_REQUIRE(rows >= 0 && cols >= 1 && cols < (1LL << 31) - 8192, "layernorm: bad size");
+  JX_REQUIRE(rows >= 0 && rows < (1LL << 31) && cols >= 1 && cols < (1LL << 30), "layernorm: bad size");
   JX_REQUIRE(ldx >= cols && ldy >= cols, "layernorm: row stride smaller than the row");
   JX_REQUIRE(epsilon >= 0.0f, "layernorm: epsilon must not be negative");
   if (rows == 0) return JX_OK;
   JX_REQUIRE(x && y, "layernorm: NULL pointer");
   JX_REQUIRE(y != x || ldy == ldx, "layernorm: in place needs equal row strides");
-  const int grid = (int)std::min<long long>(rows, (long long)jx::num_sms() * 8);
-  ln_fwd_kernel<<<grid, LN_THREADS, 0, jx::as_stream(stream)>>>(x, gamma, beta, y, mean_out, rstd_out, rows, (int)cols,
-                                                                ldx, ldy, epsilon);
+  cudaStream_t st = jx::as_stream(stream);
+  const FwdArgs a = {x, gamma, beta, y, mean_out, rstd_out, rows, (int)cols, ldx, ldy, epsilon};
+  const bool vec = !(cols & 3) && !(ldx & 3) && !(ldy & 3) && aligned16(x) && aligned16(y) && aligned16(gamma) &&
+                   aligned16(beta);
+  // few rows: as many threads to a row as it has vectors, so that one load each covers it
+  const bool few = rows < jx::num_sms();
+  if (vec) {
+    if (cols <= 128) fwd<32, 4, 1>(a, st);
+    else if (cols <= 256) fwd<32, 4, 2>(a, st);
+    else if (cols <= 512) few ? fwd<128, 4, 1>(a, st) : fwd<32, 4, 4>(a, st);
+    else if (cols <= 1024) few ? fwd<256, 4, 1>(a, st) : fwd<128, 4, 2>(a, st);
+    else if (cols <= 2048) few ? fwd<512, 4, 1>(a, st) : fwd<128, 4, 4>(a, st);
+    else if (cols <= 4096) few ? fwd<1024, 4, 1>(a, st) : fwd<256, 4, 4>(a, st);
+    else if (cols <= 8192) few ? fwd<1024, 4, 2>(a, st) : fwd<512, 4, 4>(a, st);
+    else if (cols <= 16384) fwd<1024, 4, 4>(a, st);
+  } else {
+    if (cols <= 128) fwd<32, 1, 4>(a, st);
+    else if (cols <= 512) fwd<32, 1, 16>(a, st);
+    else if (cols <= 1024) fwd<128, 1, 8>(a, st);
+    else if (cols <= 2048) fwd<256, 1, 8>(a, st);
+    else if (cols <= 4096) fwd<512, 1, 8>(a, st);
+    else if (cols <= 8192) fwd<512, 1, 16>(a, st);
+    else if (cols <= 16384) fwd<1024, 1, 16>(a, st);
+  }
+  if (cols > 16384)
+    ln_fwd_wide_kernel<<<(unsigned)rows, WIDE, 0, st>>>(x, gamma, beta, y, mean_out, rstd_out, (int)cols, ldx, ldy,
+                                                        epsilon);
   JX_LAUNCH_CHECK("ln_fwd_kernel");
   return JX_OK;
 }
@@ -138,7 +460,7 @@ int jx_layernorm_bwd_f32(const float* dy, const float* x, const float* gamma, co
                          float* dx, float* dgamma, float* dbeta, int64_t rows, int64_t cols, int64_t lddy, int64_t ldx,
                          int64_t lddx, jx_stream_t stream) {
   JX_TRACE("jx_layernorm_bwd_f32");
-  JX_REQUIRE(rows >= 0 && cols >= 1 && cols < (1LL << 30), "layernorm_bwd: bad size");
+  JX_REQUIRE(rows >= 0 && rows < (1LL << 31) && cols >= 1 && cols < (1LL << 30), "layernorm_bwd: bad size");
   JX_REQUIRE(lddy >= cols && ldx >= cols && (!dx || lddx >= cols), "layernorm_bwd: row stride smaller than the row");
   cudaStream_t st = jx::as_stream(stream);
   if (rows == 0) {
@@ -149,25 +471,28 @@ int jx_layernorm_bwd_f32(const float* dy, const float* x, const float* gamma, co
   JX_REQUIRE(dy && x && mean && rstd, "layernorm_bwd: NULL pointer");
   JX_REQUIRE(dx != x, "layernorm_bwd: dx must not be x");
   JX_REQUIRE(dx != dy || lddx == lddy, "layernorm_bwd: in place needs equal row strides");
-  if (dgamma || dbeta) {
-    const long long chunk = std::max<long long>(64, (rows + 255) / 256);
-    const int chunks = (int)((rows + chunk - 1) / chunk);
-    void* part = nullptr;
-    if (int rc = jx::scratch_get(sizeof(float) * 2 * (size_t)chunks * cols, &part, st)) return rc;
-    float* pp = static_cast<float*>(part);
-    ln_col_partial_kernel<<<dim3((unsigned)((cols + 127) / 128), chunks), 128, 0, st>>>(
-        dy, x, mean, rstd, pp, rows, (int)cols, lddy, ldx, chunk);
-    ln_col_final_kernel<<<(unsigned)((2 * cols + 127) / 128), 128, 0, st>>>(pp, dgamma, dbeta, chunks, (int)cols);
-    const cudaError_t e = cudaGetLastError();
-    jx::scratch_release(part, st);
-    if (e != cudaSuccess) return jx::check_cuda(e, "layernorm_bwd column kernels");
+  if (!dx && !dgamma && !dbeta) return JX_OK;
+  const BwdArgs a = {dy, x, gamma, mean, rstd, dx, dgamma, dbeta, rows, (int)cols, lddy, ldx, lddx};
+  const bool vec = !(cols & 3) && !(lddy & 3) && !(ldx & 3) && (!dx || !(lddx & 3)) && aligned16(dy) && aligned16(x) &&
+                   aligned16(dx) && aligned16(gamma);
+  if (vec) {
+    if (cols <= 128) return bwd<32, 4, 1, true>(a, 4, st);
+    if (cols <= 256) return bwd<32, 4, 2, true>(a, 2, st);
+    if (cols <= 512) return bwd<128, 4, 1, true>(a, 8, st);
+    if (cols <= 1024) return bwd<128, 4, 2, true>(a, 4, st);
+    if (cols <= 2048) return bwd<256, 4, 2, true>(a, 2, st);
+    if (cols <= 4096) return bwd<512, 4, 2, true>(a, 1, st);
+    if (cols <= 8192) return bwd<1024, 4, 2, false>(a, 1, st);
+  } else {
+    if (cols <= 128) return bwd<32, 1, 4, true>(a, 4, st);
+    if (cols <= 256) return bwd<32, 1, 8, true>(a, 2, st);
+    if (cols <= 512) return bwd<128, 1, 4, true>(a, 8, st);
+    if (cols <= 1024) return bwd<128, 1, 8, true>(a, 4, st);
+    if (cols <= 2048) return bwd<256, 1, 8, true>(a, 2, st);
+    if (cols <= 4096) return bwd<512, 1, 8, true>(a, 1, st);
+    if (cols <= 8192) return bwd<1024, 1, 8, false>(a, 1, st);
   }
-  if (dx) {
-    const int grid = (int)std::min<long long>(rows, (long long)jx::num_sms() * 8);
-    ln_dx_kernel<<<grid, LN_THREADS, 0, st>>>(dy, x, gamma, mean, rstd, dx, rows, (int)cols, lddy, ldx, lddx);
-    JX_LAUNCH_CHECK("ln_dx_kernel");
-  }
-  return JX_OK;
+  return bwd_wide(a, st);
 }
 
 }  // extern "C"
