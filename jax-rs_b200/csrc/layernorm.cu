@@ -86,7 +86,7 @@ constexpr int block_of(int T) { return T == 32 ? 256 : T; }
 
 // T threads per row.
 template <int T, int V, int N>
-__global__ void __launch_bounds__(block_of(T))
+__global__ void __launch_bounds__(block_of(T), T == 512 && N * V >= 16 ? 2 : 1)
     ln_fwd_kernel(const float* x, const float* __restrict__ gamma, const float* __restrict__ beta, float* y,
                   float* __restrict__ mean_out, float* __restrict__ rstd_out, long long rows, int cols, long long ldx,
                   long long ldy, float eps) {
@@ -94,10 +94,8 @@ __global__ void __launch_bounds__(block_of(T))
   const int t = threadIdx.x % T;
   const long long r = (long long)blockIdx.x * (block_of(T) / T) + threadIdx.x / T;
   if (r >= rows) return;  // whole warps; a block with T > 32 has one row
-  float v[N * V], g[N * V], b[N * V];
+  float v[N * V];
   load_row<T, V, N>(v, x + r * ldx, t, cols);
-  fill_row<T, V, N>(g, gamma, t, cols, 1.0f);
-  fill_row<T, V, N>(b, beta, t, cols, 0.0f);
   const float inv = 1.0f / (float)cols;
   float s = 0.0f;
 #pragma unroll
@@ -115,8 +113,15 @@ __global__ void __launch_bounds__(block_of(T))
   }
   const float rstd = 1.0f / sqrtf(row_sum<T>(q, sm[1]) * inv + eps);
 #pragma unroll
-  for (int i = 0; i < N * V; ++i) v[i] = fmaf(v[i] * rstd, g[i], b[i]);
-  store_row<T, V, N>(y + r * ldy, v, t, cols);
+  for (int i = 0; i < N; ++i) {  // gamma and beta come from L1; loaded earlier they cost the registers of other rows
+    const int c = (i * T + t) * V;
+    float g[V], b[V], out[V];
+    fill_row<1, V, 1>(g, gamma ? gamma + c : nullptr, 0, cols - c, 1.0f);
+    fill_row<1, V, 1>(b, beta ? beta + c : nullptr, 0, cols - c, 0.0f);
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = fmaf(v[i * V + e] * rstd, g[e], b[e]);
+    store_row<1, V, 1>(y + r * ldy + c, out, 0, cols - c);
+  }
   if (t == 0) {
     if (mean_out) mean_out[r] = mean;
     if (rstd_out) rstd_out[r] = rstd;
@@ -153,8 +158,8 @@ __global__ void __launch_bounds__(WIDE)
 // dx (may be NULL) of the rows blockIdx.x * RPB + .., step gridDim.x * RPB, and the
 // block's column sums into part[blockIdx.x][2][cols] (may be NULL).  AHEAD: the
 // next row is loaded before the present one is reduced.
-template <int T, int V, int N, bool AHEAD>
-__global__ void __launch_bounds__(block_of(T))
+template <int T, int V, int N, bool AHEAD, int PER_SM>
+__global__ void __launch_bounds__(block_of(T), PER_SM)
     ln_bwd_kernel(const float* dy, const float* __restrict__ x, const float* __restrict__ gamma,
                   const float* __restrict__ mean, const float* __restrict__ rstd, float* dx, float* __restrict__ part,
                   long long rows, int cols, long long lddy, long long ldx, long long lddx) {
@@ -236,6 +241,7 @@ __global__ void __launch_bounds__(block_of(T))
     }
   }
   if (!part) return;
+  asm volatile("griddepcontrol.launch_dependents;");
   if constexpr (T == 32) {  // the block's warps have the same columns
     constexpr int W = 2 * 32 * N * V;
     if (sub > 0) {
@@ -371,18 +377,18 @@ int join(const BwdArgs& a, const float* part, int parts, cudaStream_t st) {
   return JX_OK;
 }
 
-// per_sm: blocks per SM that the grid is made for.
-template <int T, int V, int N, bool AHEAD>
-int bwd(const BwdArgs& a, int per_sm, cudaStream_t st) {
+// PER_SM: blocks per SM that the grid is made for.
+template <int T, int V, int N, bool AHEAD, int PER_SM>
+int bwd(const BwdArgs& a, cudaStream_t st) {
   constexpr int RPB = block_of(T) / T;
-  const int grid = (int)std::min<long long>((a.rows + RPB - 1) / RPB, (long long)jx::num_sms() * per_sm);
+  const int grid = (int)std::min<long long>((a.rows + RPB - 1) / RPB, (long long)jx::num_sms() * PER_SM);
   const bool sums = a.dgamma || a.dbeta;
   void* part = nullptr;
   if (sums)
     if (int rc = jx::scratch_get(sizeof(float) * 2 * (size_t)grid * a.cols, &part, st)) return rc;
-  ln_bwd_kernel<T, V, N, AHEAD><<<grid, block_of(T), 0, st>>>(a.dy, a.x, a.gamma, a.mean, a.rstd, a.dx,
-                                                              static_cast<float*>(part), a.rows, a.cols, a.lddy, a.ldx,
-                                                              a.lddx);
+  ln_bwd_kernel<T, V, N, AHEAD, PER_SM><<<grid, block_of(T), 0, st>>>(a.dy, a.x, a.gamma, a.mean, a.rstd, a.dx,
+                                                                      static_cast<float*>(part), a.rows, a.cols,
+                                                                      a.lddy, a.ldx, a.lddx);
   const cudaError_t e = cudaGetLastError();
   int rc = e == cudaSuccess ? JX_OK : jx::check_cuda(e, "ln_bwd_kernel");
   if (!rc && sums) rc = join(a, static_cast<const float*>(part), grid, st);
@@ -435,19 +441,22 @@ int jx_layernorm_f32(const float* x, const float* gamma, const float* beta, floa
     if (cols <= 128) fwd<32, 4, 1>(a, st);
     else if (cols <= 256) fwd<32, 4, 2>(a, st);
     else if (cols <= 512) few ? fwd<128, 4, 1>(a, st) : fwd<32, 4, 4>(a, st);
-    else if (cols <= 1024) few ? fwd<256, 4, 1>(a, st) : fwd<128, 4, 2>(a, st);
+    else if (cols <= 1024) few ? fwd<256, 4, 1>(a, st) : fwd<64, 4, 4>(a, st);
     else if (cols <= 2048) few ? fwd<512, 4, 1>(a, st) : fwd<128, 4, 4>(a, st);
     else if (cols <= 4096) few ? fwd<1024, 4, 1>(a, st) : fwd<256, 4, 4>(a, st);
     else if (cols <= 8192) few ? fwd<1024, 4, 2>(a, st) : fwd<512, 4, 4>(a, st);
-    else if (cols <= 16384) fwd<1024, 4, 4>(a, st);
+    else if (cols <= 16384) fwd<512, 4, 8>(a, st);
   } else {
     if (cols <= 128) fwd<32, 1, 4>(a, st);
-    else if (cols <= 512) fwd<32, 1, 16>(a, st);
+    else if (cols <= 256) fwd<32, 1, 8>(a, st);
+    else if (cols <= 512) fwd<64, 1, 8>(a, st);
+    else if (cols <= 640) fwd<128, 1, 5>(a, st);
     else if (cols <= 1024) fwd<128, 1, 8>(a, st);
+    else if (cols <= 1280) fwd<256, 1, 5>(a, st);
     else if (cols <= 2048) fwd<256, 1, 8>(a, st);
-    else if (cols <= 4096) fwd<512, 1, 8>(a, st);
+    else if (cols <= 4096) fwd<256, 1, 16>(a, st);
     else if (cols <= 8192) fwd<512, 1, 16>(a, st);
-    else if (cols <= 16384) fwd<1024, 1, 16>(a, st);
+    else if (cols <= 16384) fwd<512, 1, 32>(a, st);
   }
   if (cols > 16384)
     ln_fwd_wide_kernel<<<(unsigned)rows, WIDE, 0, st>>>(x, gamma, beta, y, mean_out, rstd_out, (int)cols, ldx, ldy,
@@ -476,21 +485,23 @@ int jx_layernorm_bwd_f32(const float* dy, const float* x, const float* gamma, co
   const bool vec = !(cols & 3) && !(lddy & 3) && !(ldx & 3) && (!dx || !(lddx & 3)) && aligned16(dy) && aligned16(x) &&
                    aligned16(dx) && aligned16(gamma);
   if (vec) {
-    if (cols <= 128) return bwd<32, 4, 1, true>(a, 4, st);
-    if (cols <= 256) return bwd<32, 4, 2, true>(a, 2, st);
-    if (cols <= 512) return bwd<128, 4, 1, true>(a, 8, st);
-    if (cols <= 1024) return bwd<128, 4, 2, true>(a, 4, st);
-    if (cols <= 2048) return bwd<256, 4, 2, true>(a, 2, st);
-    if (cols <= 4096) return bwd<512, 4, 2, true>(a, 1, st);
-    if (cols <= 8192) return bwd<1024, 4, 2, false>(a, 1, st);
+    if (cols <= 128) return bwd<32, 4, 1, true, 3>(a, st);
+    if (cols <= 256) return bwd<32, 4, 2, true, 2>(a, st);
+    if (cols <= 512) return bwd<64, 4, 2, true, 12>(a, st);
+    if (cols <= 1024) return bwd<128, 4, 2, true, 6>(a, st);
+    if (cols <= 2048) return bwd<256, 4, 2, true, 3>(a, st);
+    if (cols <= 4096) return bwd<256, 4, 4, true, 2>(a, st);
+    if (cols <= 8192) return bwd<512, 4, 4, true, 1>(a, st);
   } else {
-    if (cols <= 128) return bwd<32, 1, 4, true>(a, 4, st);
-    if (cols <= 256) return bwd<32, 1, 8, true>(a, 2, st);
-    if (cols <= 512) return bwd<128, 1, 4, true>(a, 8, st);
-    if (cols <= 1024) return bwd<128, 1, 8, true>(a, 4, st);
-    if (cols <= 2048) return bwd<256, 1, 8, true>(a, 2, st);
-    if (cols <= 4096) return bwd<512, 1, 8, true>(a, 1, st);
-    if (cols <= 8192) return bwd<1024, 1, 8, false>(a, 1, st);
+    if (cols <= 128) return bwd<32, 1, 4, true, 3>(a, st);
+    if (cols <= 256) return bwd<32, 1, 8, true, 2>(a, st);
+    if (cols <= 512) return bwd<64, 1, 8, true, 12>(a, st);
+    if (cols <= 640) return bwd<128, 1, 5, true, 8>(a, st);
+    if (cols <= 1024) return bwd<128, 1, 8, true, 6>(a, st);
+    if (cols <= 1280) return bwd<256, 1, 5, true, 4>(a, st);
+    if (cols <= 2048) return bwd<256, 1, 8, true, 3>(a, st);
+    if (cols <= 4096) return bwd<256, 1, 16, true, 2>(a, st);
+    if (cols <= 8192) return bwd<512, 1, 16, true, 1>(a, st);
   }
   return bwd_wide(a, st);
 }
