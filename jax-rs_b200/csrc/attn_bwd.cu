@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     float g_prev = 0.0f;
     bool ok = true;
     auto add_part = [&](int j) {
-      ok = ok && jxg::warp_wait_bounded(dqfull, (uint32_t)j & 1u, abort_flag, s.err);
+      ok = ok && warp_wait(dqfull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
       drain<DP>(acc, tmem + lanes + DQ_Y + half * (DP / 2), g_prev);
       jxd::tc_fence_before();
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const long long slot = slot0 + (long long)j * s.kv_heads;
       const float inv_k = bt.inv_k[slot], inv_v = bt.inv_v[slot], norm_v = bt.norm_v[slot];
       if (j > 0) add_part(j - 1);
-      ok = ok && jxg::warp_wait_bounded(sfull, (uint32_t)j & 1u, abort_flag, s.err);
+      ok = ok && warp_wait(sfull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
       const float f = f_row * inv_k;
       const float2 f2 = make_float2(f, f), l2 = make_float2(-lse2, -lse2);
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const float pf = sc * fd, dl = -delta * inverse_pow2(fd);
 #pragma unroll
       for (int i = 0; i < 64; ++i) p[i] *= pf;
-      ok = ok && jxg::warp_wait_bounded(dpfull, (uint32_t)j & 1u, abort_flag, s.err);
+      ok = ok && warp_wait(dpfull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
       uint32_t hi[32], lo[32];
 #pragma unroll
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     float g_prev = 0.0f;
     bool ok = true;
     auto ready = [&](uint64_t* b8, int u) {
-      ok = ok && jxg::warp_wait_bounded(b8, (uint32_t)u & 1u, abort_flag, s.err);
+      ok = ok && warp_wait(b8, (uint32_t)u & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
     };
     auto done = [&](uint64_t* b8) {
@@ -701,26 +701,43 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   }
 }
 
-// The parts' sums in order, one block per (key tile, key head).
+// The parts' sums in order, 16 key rows of one key head per block.
+constexpr int JOIN_ROWS = 16;
+template <bool VEC>
 __global__ void __launch_bounds__(256) attn_dkv_join_kernel(const __grid_constant__ Shape s,
                                                            const __grid_constant__ BwdTiles bt, float* dk, float* dv) {
   int jt;
-  const int b = seq_of_tile(s.cu_k, s.batch, blockIdx.x, &jt);
+  const int b = seq_of_tile(s.cu_k, s.batch, blockIdx.x / (TILE / JOIN_ROWS), &jt);
   const Seq sq = seq_bounds(s, b);
-  if (jt < 0 || (long long)jt * TILE >= sq.lk) return;
-  const int rows = min(TILE, sq.lk - jt * TILE);
-  const long long t0 = sq.k0 + (long long)jt * TILE, hd = (long long)blockIdx.y * s.dim;
+  const long long j0 = (long long)jt * TILE + blockIdx.x % (TILE / JOIN_ROWS) * JOIN_ROWS;
+  if (jt < 0 || j0 >= sq.lk) return;
+  const int rows = (int)min((long long)JOIN_ROWS, sq.lk - j0);
+  const long long t0 = sq.k0 + j0, hd = (long long)blockIdx.y * s.dim;
   const long long ld = (long long)s.kv_heads * s.dim, all = s.total_k * ld;
-  for (int e = threadIdx.x; e < rows * s.dim; e += 256) {
-    const int r = e / s.dim, c = e - r * s.dim;
-    const long long at = (t0 + r) * ld + hd + c;
-    float a = 0.0f, d = 0.0f;
-    for (int p = 0; p < bt.parts; ++p) {
-      a += bt.part_k[p * all + at];
-      d += bt.part_v[p * all + at];
+  constexpr int V = VEC ? 4 : 1;
+  const int cols = s.dim / V, half = rows * cols;  // the rows of dk, then those of dv
+  for (int e = threadIdx.x; e < 2 * half; e += 256) {
+    const bool is_v = e >= half;
+    const int f = is_v ? e - half : e, r = f / cols, c = (f - r * cols) * V;
+    const float* p = (is_v ? bt.part_v : bt.part_k) + (t0 + r) * ld + hd + c;
+    float* out = (is_v ? dv + (t0 + r) * s.ldv : dk + (t0 + r) * s.ldk) + hd + c;
+    if constexpr (VEC) {
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+      for (int i = 0; i < bt.parts; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(p + i * all);
+        a.x += x.x;
+        a.y += x.y;
+        a.z += x.z;
+        a.w += x.w;
+      }
+      *reinterpret_cast<float4*>(out) = a;
+    } else {
+      float a = 0.0f;
+#pragma unroll 4
+      for (int i = 0; i < bt.parts; ++i) a += p[i * all];
+      *out = a;
     }
-    dk[(t0 + r) * s.ldk + hd + c] = a;
-    dv[(t0 + r) * s.ldv + hd + c] = d;
   }
 }
 
@@ -735,7 +752,13 @@ int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, c
       s, bt, q, k, v, o, lse, dout, dq);
   attn_dkv_kernel<DP><<<(unsigned)((long long)bt.k_tiles * s.kv_heads * bt.parts), BW_THREADS, kv_smem(DP), st>>>(
       s, bt, q, k, v, o, lse, dout, dk, dv);
-  if (bt.parts > 1) attn_dkv_join_kernel<<<dim3(bt.k_tiles, s.kv_heads), 256, 0, st>>>(s, bt, dk, dv);
+  if (bt.parts > 1) {
+    const dim3 grid((unsigned)(bt.k_tiles * (TILE / JOIN_ROWS)), (unsigned)s.kv_heads);
+    const bool vec = !(s.dim & 3) && !(s.ldk & 3) && !(s.ldv & 3) &&
+                     !((reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15);
+    if (vec) attn_dkv_join_kernel<true><<<grid, 256, 0, st>>>(s, bt, dk, dv);
+    else attn_dkv_join_kernel<false><<<grid, 256, 0, st>>>(s, bt, dk, dv);
+  }
   JX_LAUNCH_CHECK("attention_bwd kernels");
   return JX_OK;
 }
@@ -751,7 +774,8 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   // key tiles are few where heads are shared: enough parts of the query rows for four CTAs per SM
   const long long ctas = kt * s.kv_heads;
   const int parts = (int)std::max<long long>(1, std::min<long long>(8, 4LL * jx::num_sms() / std::max(1LL, ctas)));
-  JX_REQUIRE(qt * s.heads < (1LL << 31) && kt * s.kv_heads * parts < (1LL << 31), "attention_bwd: too many rows");
+  JX_REQUIRE(qt * s.heads < (1LL << 31) && kt * s.kv_heads * parts < (1LL << 31) && kt < (1LL << 27),
+             "attention_bwd: too many rows");
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
   const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
   // tiles first, then arrays whose pieces the copies read 16-byte aligned, then the rest

@@ -40,6 +40,13 @@ __host__ __device__ constexpr int dc_stage(int DP) { return DC_KEYS * 2 * DP * 4
 __host__ __device__ constexpr int dc_stages(int DP) { return DC_RING / dc_stage(DP); }  // of all rings
 __host__ __device__ constexpr size_t dc_smem(int DP) { return DC_RING + 2 * 8 * dc_stages(DP) + 128; }
 
+// One lane polls for its warp.
+__device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsigned int* err) {
+  int got = 1;
+  if ((threadIdx.x & 31) == 0) got = wait_bounded(bar, parity, err) ? 1 : 0;
+  return __shfl_sync(0xffffffffu, got, 0) != 0;
+}
+
 // A place in the line of positions.  A head takes lk + VOID of them: starting and
 // storing a head costs a ring about as much as VOID keys, so that short heads
 // weigh what they cost.
@@ -199,7 +206,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
   auto produce = [&]() {  // the ring's first warp: the next stage's rows
     if (!pc.on || !ok) return;
     const int st = in_st, n = pc.keys(end);
-    ok = __all_sync(0xffffffffu, wait_bounded(&empty[st], in_ph ^ 1u, s.err));
+    ok = ring_wait(&empty[st], in_ph ^ 1u, s.err);
     if (!ok) return;
     const long long t = pc.sq.k0 + pc.key;
     float* dst = stages + (size_t)st * (STAGE / 4);
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
     }
     while (c.on && c.b == b && c.hk == hk) {
       const int n = c.keys(end), st = out_st, j0 = c.key;
-      ok = ok && __all_sync(0xffffffffu, wait_bounded(&full[st], out_ph, s.err));
+      ok = ok && ring_wait(&full[st], out_ph, s.err);
       if (!ok) break;
       const float* base = stages + (size_t)st * (STAGE / 4);
       float x[R][STEPS];

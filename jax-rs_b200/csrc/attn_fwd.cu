@@ -174,9 +174,11 @@ static_assert(128 * FW_LOW_REGS + 256 * FW_HIGH_REGS <= FW_THREADS * FW_LAUNCH_R
               "register split exceeds the launch allocation");
 constexpr uint32_t T_Q = 256, T_O = 384;  // columns of tensor memory; S0 at 0, S1 at 128
 
-__host__ __device__ constexpr int fw_stages(int DP) { return DP == 128 ? 3 : 6; }
+// A stage is one part of a tile: the lo part is used, and its stage free again,
+// before the hi part is.
+__host__ __device__ constexpr int fw_stages(int DP) { return DP == 128 ? 6 : 12; }
 __host__ __device__ constexpr size_t fw_smem(int DP) {
-  return (size_t)fw_stages(DP) * tile_bytes(DP) + 1024 /*align*/ + 2 * 128 * 4 /*exchange*/ + 256 /*barriers*/;
+  return (size_t)fw_stages(DP) * tile_part(DP) + 1024 /*align*/ + 2 * 128 * 4 /*exchange*/ + 512 /*barriers*/;
 }
 
 struct FwdTiles {
@@ -193,7 +195,7 @@ template <int DP>
 __global__ void __launch_bounds__(FW_THREADS, 1)
     attn_fwd_kernel(const __grid_constant__ Shape s, const __grid_constant__ FwdTiles ft, const float* __restrict__ q,
                     const float* __restrict__ k, const float* __restrict__ v, float* o, float* lse) {
-  constexpr int STAGES = fw_stages(DP), STAGE = tile_bytes(DP), PART = tile_part(DP);
+  constexpr int STAGES = fw_stages(DP), STAGE = tile_part(DP), PART = tile_part(DP);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
@@ -278,13 +280,15 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       // ---- copies, in the order of use: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
-      for (int u = 0; u < 2 * nb; ++u) {
-        const bool is_v = u == 2 * nb - 1 || (u >= 2 && (u & 1) == 0);
-        const int j = u == 0 ? 0 : u == 2 * nb - 1 ? nb - 1 : is_v ? u / 2 - 1 : (u + 1) / 2;
-        if (*abort_flag || !wait_bounded(&empty[stage], phase ^ 1u, s.err)) { *abort_flag = 1; break; }
+      for (int u = 0; u < 4 * nb && !*abort_flag; ++u) {
+        const int w = u >> 1;  // tile in this order; its lo part, then hi
+        const bool is_v = w == 2 * nb - 1 || (w >= 2 && (w & 1) == 0);
+        const int j = w == 0 ? 0 : w == 2 * nb - 1 ? nb - 1 : is_v ? w / 2 - 1 : (w + 1) / 2;
+        if (!wait_bounded(&empty[stage], phase ^ 1u, s.err)) { *abort_flag = 1; break; }
         jxd::mbar_arrive_expect_tx(&full[stage], STAGE);
         bulk_load(jxd::smem_u32(smem + stage * STAGE),
-                  (is_v ? ft.v : ft.k) + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE, &full[stage]);
+                  (is_v ? ft.v : ft.k) + (slot0 + (long long)j * s.kv_heads) * tile_bytes(DP) + (u & 1 ? 0 : PART), STAGE,
+                  &full[stage]);
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
@@ -299,49 +303,60 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = wait_bounded(qfull, 0, s.err);
-      auto scores = [&](int j) {
-        if (!ok || !(ok = !*abort_flag && wait_bounded(&full[stage], phase, s.err))) return;
+      // the next stage's shared-memory address once its copy has landed
+      auto next = [&]() {
+        ok = ok && !*abort_flag && wait_bounded(&full[stage], phase, s.err);
         jxd::tc_fence_after();
-        const uint32_t kt = sbase + stage * STAGE, d = tmem + (j & 1) * 128u;
-        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
-          mma_f16_ts(d, tmem + T_Q + a + ks * 8, jxd::smem_desc_k_sw128(kt + part + (ks >> 2) * PANEL + (ks & 3) * 32),
-                     id_s, acc);
-        };
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          step(ks, DP / 2, 0, ks > 0);  // lo.hi
-          step(ks, 0, PART, 1);         // hi.lo
-        }
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
-        jxd::mma_commit(&sfull[j & 1]);
+        return sbase + stage * STAGE;
+      };
+      auto release = [&]() {
         jxd::mma_commit(&empty[stage]);
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      };
+      auto scores = [&](int j) {
+        const uint32_t d = tmem + (j & 1) * 128u;
+        auto step = [&](uint32_t kt, int ks, uint32_t a, uint32_t acc) {
+          mma_f16_ts(d, tmem + T_Q + a + ks * 8, jxd::smem_desc_k_sw128(kt + (ks >> 2) * PANEL + (ks & 3) * 32), id_s,
+                     acc);
+        };
+        uint32_t kt = next();
+        if (!ok) return;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) step(kt, ks, 0, ks > 0);  // hi.lo
+        release();
+        kt = next();
+        if (!ok) return;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) step(kt, ks, DP / 2, 1);  // lo.hi
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) step(kt, ks, 0, 1);
+        jxd::mma_commit(&sfull[j & 1]);
+        release();
       };
       scores(0);
       for (int j = 0; j < nb && ok; ++j) {
         if (j + 1 < nb) scores(j + 1);
-        if (!ok || !(ok = !*abort_flag && wait_bounded(&full[stage], phase, s.err) &&
-                          wait_bounded(&pfull[j & 1], (uint32_t)(j >> 1) & 1u, s.err) &&
+        if (!ok || !(ok = !*abort_flag && wait_bounded(&pfull[j & 1], (uint32_t)(j >> 1) & 1u, s.err) &&
                           wait_bounded(ofree, (uint32_t)(j + 1) & 1u, s.err)))
           break;
-        jxd::tc_fence_after();
-        const uint32_t vt = sbase + stage * STAGE, p = tmem + (j & 1) * 128u, d = tmem + T_O;
+        const uint32_t p = tmem + (j & 1) * 128u, d = tmem + T_O;
         // P's keys 0..63: hi at column 0, lo at 32; keys 64..127: hi at 64, lo at 96
-        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
-          mma_f16_ts(d, p + a + (ks >> 2) * 64 + (ks & 3) * 8, smem_desc_mn_sw128(vt + part + ks * 2048, PANEL), id_o,
-                     acc);
+        auto step = [&](uint32_t vt, int ks, uint32_t a, uint32_t acc) {
+          mma_f16_ts(d, p + a + (ks >> 2) * 64 + (ks & 3) * 8, smem_desc_mn_sw128(vt + ks * 2048, PANEL), id_o, acc);
         };
+        uint32_t vt = next();
+        if (!ok) break;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          step(ks, 32, 0, ks > 0);
-          step(ks, 0, PART, 1);
-        }
+        for (int ks = 0; ks < 8; ++ks) step(vt, ks, 0, ks > 0);
+        release();
+        vt = next();
+        if (!ok) break;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) step(ks, 0, 0, 1);
+        for (int ks = 0; ks < 8; ++ks) step(vt, ks, 32, 1);
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) step(vt, ks, 0, 1);
         jxd::mma_commit(ofull);
-        jxd::mma_commit(&empty[stage]);
-        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        release();
       }
       if (!ok) *abort_flag = 1;
     }
@@ -366,7 +381,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     bool ok = true;
 
     auto add_part = [&](int j, float alpha, float inv_v) {
-      ok = ok && jxg::warp_wait_bounded(ofull, (uint32_t)j & 1u, abort_flag, s.err);
+      ok = ok && warp_wait(ofull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
 #pragma unroll
       for (int c = 0; c < DP / 2; c += 32) {
@@ -390,7 +405,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       const float inv_k = ft.inv_k[slot0 + (long long)j * s.kv_heads];
       const float inv_v = ft.inv_v[slot0 + (long long)j * s.kv_heads];
       const float f = fmaxf(f_row * inv_k, 1.17549435e-38f);  // above zero, so that a masked score stays -inf
-      ok = ok && jxg::warp_wait_bounded(&sfull[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag, s.err);
+      ok = ok && warp_wait(&sfull[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
       const uint32_t s_addr = tmem + lanes + (j & 1) * 128u + half * 64u;
       float sc[64];

@@ -145,6 +145,39 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
       "l"(src), "r"(bytes), "r"(jxd::smem_u32(bar))
       : "memory");
 }
+// jxg::wait_bounded that polls without suspending the thread: the steps that wait
+// here are a few hundred cycles apart.
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(jxd::smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool spin_bounded(uint64_t* bar, uint32_t parity, unsigned int* err) {
+  if (poll(bar, parity)) return true;
+  const uint64_t t0 = jxg::global_ns();
+  while (true) {
+    for (int i = 0; i < 1024; ++i)
+      if (poll(bar, parity)) return true;
+    if (jxg::global_ns() - t0 > 4000000000ull) {
+      atomicOr(err, JX_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+// One lane polls for its warp.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
+  int got = 1;
+  if ((threadIdx.x & 31) == 0) got = spin_bounded(bar, parity, err) ? 1 : 0;
+  got = __shfl_sync(0xffffffffu, got, 0);
+  if (!got) *abort_flag = 1;
+  return got != 0;
+}
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // ---- the operand that stays: rows of a [rows, heads, dim] tensor into tensor memory ----
