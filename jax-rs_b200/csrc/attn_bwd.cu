@@ -14,8 +14,9 @@
 //   S^T = K Q^T, dP^T = V dO^T    K and V in tensor memory
 //   dV += P^T dO, dK += dS^T Q    P^T over S^T's columns, dS^T over dP^T's
 // An operand computed here needs its scale before its largest value is known:
-// |dP - delta| <= |dout row| |v row| + |delta| (norms), times the largest P of the
-// row, bounds dS; it overestimates by a few bits of the 39 there are.
+// P <= 1 and |dP - delta| <= |dout row| |v row| + |delta| (norms) bound dS; it
+// overestimates by some bits of the 39 there are (a row of 2^14 keys with equal
+// weights keeps 21 bits of each dS).
 #include <algorithm>
 
 #include "attn_tc.cuh"
@@ -121,8 +122,17 @@ __device__ __forceinline__ bool aligned16(const void* p, int dim, long long ld) 
 }
 
 // ---- dq ------------------------------------------------------------------------
-constexpr uint32_t DQ_Q = 0, DQ_D = 128, DQ_X = 256, DQ_Y = 384;
-__host__ __device__ constexpr int dq_k_stages(int) { return 2; }
+// Tensor memory: Q, dO, X (scores), Y (dP) and the sum's part D.  At DP = 128 the
+// first four fill it: dS goes over X and D over Y, and S(j+1) has to wait for
+// dS(j) K.  At DP = 64 D has its own columns: dS goes over Y, and S(j+1) runs
+// while dS(j) is computed.
+template <int DP>
+struct DqLayout {
+  static constexpr bool AHEAD = DP == 64;
+  static constexpr uint32_t Q = 0, DO = AHEAD ? 64 : 128, X = AHEAD ? 128 : 256, Y = AHEAD ? 256 : 384;
+  static constexpr uint32_t DS = AHEAD ? Y : X, D = AHEAD ? 384 : Y;
+};
+__host__ __device__ constexpr int dq_k_stages(int DP) { return DP == 128 ? 2 : 3; }
 __host__ __device__ constexpr int dq_v_stages(int DP) { return DP == 128 ? 1 : 2; }
 __host__ __device__ constexpr size_t dq_smem(int DP) {
   return (size_t)(dq_k_stages(DP) + dq_v_stages(DP)) * tile_bytes(DP) + 1024 + 2 * 128 * 4 + 256;
@@ -133,6 +143,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_dq_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
                    const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
                    const float* __restrict__ lse, const float* __restrict__ dout, float* dq) {
+  using L = DqLayout<DP>;
   constexpr int KS = dq_k_stages(DP), VS = dq_v_stages(DP), STAGE = tile_bytes(DP), PART = tile_part(DP);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
@@ -147,8 +158,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   uint64_t* dpfull = sfull + 1;
   uint64_t* dsfull = dpfull + 1;
   uint64_t* dqfull = dsfull + 1;
-  uint64_t* yfree = dqfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(yfree + 1);
+  uint64_t* dfree = dqfull + 1;  // D is drained
+  uint64_t* xfree = dfree + 1;   // X is read
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xfree + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -189,7 +201,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     jxd::mbar_init(dpfull, 1);
     jxd::mbar_init(dsfull, 8);
     jxd::mbar_init(dqfull, 1);
-    jxd::mbar_init(yfree, 8);
+    jxd::mbar_init(dfree, 8);
+    jxd::mbar_init(xfree, 8);
     *abort_flag = 0;
     jxd::fence_mbar_init();
   }
@@ -240,34 +253,42 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
       };
-      for (int j = 0; ok && j < nb; ++j) {
-        const uint32_t kt = sbase + (j % KS) * STAGE, vt = sbase + (KS + j % VS) * STAGE;
-        if (!(ok = !*abort_flag && wait_bounded(&kfull[j % KS], (uint32_t)(j / KS) & 1u, s.err))) break;
+      auto ready = [&](uint64_t* bar, int n) {
+        ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)n & 1u, s.err);
         jxd::tc_fence_after();
-        scores(tmem + DQ_X, tmem + DQ_Q, kt);
+        return ok;
+      };
+      auto q_scores = [&](int j) {
+        if (!ready(&kfull[j % KS], j / KS)) return;
+        if (L::AHEAD && j > 0 && !ready(xfree, j - 1)) return;
+        scores(tmem + L::X, tmem + L::Q, sbase + (j % KS) * STAGE);
         jxd::mma_commit(sfull);
-        if (!(ok = !*abort_flag && wait_bounded(&vfull[j % VS], (uint32_t)(j / VS) & 1u, s.err) &&
-                   wait_bounded(yfree, (uint32_t)(j + 1) & 1u, s.err)))
-          break;
-        jxd::tc_fence_after();
-        scores(tmem + DQ_Y, tmem + DQ_D, vt);
+      };
+      q_scores(0);
+      for (int j = 0; ok && j < nb; ++j) {
+        if (!ready(&vfull[j % VS], j / VS)) break;
+        if (!L::AHEAD && !ready(dfree, j + 1)) break;  // D is Y
+        scores(tmem + L::Y, tmem + L::DO, sbase + (KS + j % VS) * STAGE);
         jxd::mma_commit(dpfull);
         jxd::mma_commit(&vempty[j % VS]);
-        if (!(ok = !*abort_flag && wait_bounded(dsfull, (uint32_t)j & 1u, s.err))) break;
-        jxd::tc_fence_after();
+        if (L::AHEAD && j + 1 < nb) q_scores(j + 1);
+        if (!ready(dsfull, j)) break;
+        if (L::AHEAD && !ready(dfree, j + 1)) break;
+        const uint32_t kt = sbase + (j % KS) * STAGE;
         auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
-          mma_f16_ts(tmem + DQ_Y, tmem + DQ_X + a + (ks >> 2) * 64 + (ks & 3) * 8,
+          mma_f16_ts(tmem + L::D, tmem + L::DS + a + (ks >> 1) * 32 + (ks & 1) * 8,
                      smem_desc_mn_sw128(kt + part + ks * 2048, PANEL), id_o, acc);
         };
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          step(ks, 32, 0, ks > 0);
+          step(ks, 16, 0, ks > 0);
           step(ks, 0, PART, 1);
         }
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) step(ks, 0, 0, 1);
         jxd::mma_commit(dqfull);
         jxd::mma_commit(&kempty[j % KS]);
+        if (!L::AHEAD && j + 1 < nb) q_scores(j + 1);
       }
       if (!ok) *abort_flag = 1;
     }
@@ -278,9 +299,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const long long t = sq.q0 + i0 + row, hd = (long long)h * s.dim;
     float norm_d;
     const int e_q = stay_row<DP>(row < rows ? q + t * s.ldq + hd : nullptr, s.dim, half, row,
-                                 aligned16(q, s.dim, s.ldq), s.scale < 0.0f, tmem + lanes + DQ_Q, xch, bar, nullptr);
+                                 aligned16(q, s.dim, s.ldq), s.scale < 0.0f, tmem + lanes + L::Q, xch, bar, nullptr);
     const int e_d = stay_row<DP>(row < rows ? dout + t * s.ldo + hd : nullptr, s.dim, half, row,
-                                 aligned16(dout, s.dim, s.ldo), false, tmem + lanes + DQ_D, xch, bar, &norm_d);
+                                 aligned16(dout, s.dim, s.ldo), false, tmem + lanes + L::DO, xch, bar, &norm_d);
     tmem_st_wait();
     jxd::tc_fence_before();
     __syncwarp();
@@ -295,71 +316,71 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     for (int c = 0; c < DP / 2; ++c) acc[c] = 0.0f;
     float g_prev = 0.0f;
     bool ok = true;
+    auto done = [&](uint64_t* b8) {
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(b8);
+    };
     auto add_part = [&](int j) {
       ok = ok && warp_wait(dqfull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
-      drain<DP>(acc, tmem + lanes + DQ_Y + half * (DP / 2), g_prev);
-      jxd::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) jxd::mbar_arrive(yfree);
+      drain<DP>(acc, tmem + lanes + L::D + half * (DP / 2), g_prev);
+      done(dfree);
     };
     for (int j = 0; j < nb; ++j) {
       const long long slot = slot0 + (long long)j * s.kv_heads;
       const float inv_k = bt.inv_k[slot], inv_v = bt.inv_v[slot], norm_v = bt.norm_v[slot];
-      if (j > 0) add_part(j - 1);
+      if (!L::AHEAD && j > 0) add_part(j - 1);
       ok = ok && warp_wait(sfull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
       const float f = f_row * inv_k;
       const float2 f2 = make_float2(f, f), l2 = make_float2(-lse2, -lse2);
-      const int key0 = j * TILE + half * 64;
-      const bool edge = j * TILE + TILE > vis_all;
-      float p[64];
-      float most = 0.0f;
+      float2 p[32];
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t r[32];
-        jxd::tmem_ld32(tmem + lanes + DQ_X + half * 64 + c, r);
+        jxd::tmem_ld32(tmem + lanes + L::X + half * 64 + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           const float2 z = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2, l2);
-          p[c + i] = exp2_fast(z.x);
-          p[c + i + 1] = exp2_fast(z.y);
+          p[(c + i) / 2] = make_float2(exp2_fast(z.x), exp2_fast(z.y));
         }
       }
-      if (edge) {
+      if (L::AHEAD) done(xfree);
+      if (j * TILE + TILE > vis_all) {  // some row does not see all of the tile's keys
+        const int key0 = j * TILE + half * 64;
 #pragma unroll
-        for (int i = 0; i < 64; ++i)
-          if (key0 + i >= vis) p[i] = 0.0f;
+        for (int i = 0; i < 32; ++i) {
+          if (key0 + 2 * i >= vis) p[i].x = 0.0f;
+          if (key0 + 2 * i + 1 >= vis) p[i].y = 0.0f;
+        }
       }
-#pragma unroll
-      for (int i = 0; i < 64; ++i) most = fmaxf(most, p[i]);
-      most = row_max(most, xch, half, row, bar);
-      const float fd = inv_d * inv_v;
-      const float sc = bound_scale(most * (norm_d * norm_v + fabsf(delta)));
+      // P is at most 2^14
+      const float fd = inv_d * inv_v, sc = bound_scale(16384.0f * (norm_d * norm_v + fabsf(delta)));
       const float pf = sc * fd, dl = -delta * inverse_pow2(fd);
+      const float2 pf2 = make_float2(pf, pf), one2 = make_float2(1.0f, 1.0f), dl2 = make_float2(dl, dl);
 #pragma unroll
-      for (int i = 0; i < 64; ++i) p[i] *= pf;
+      for (int i = 0; i < 32; ++i) p[i] = mul2(p[i], pf2);
+      if (L::AHEAD && j > 0) add_part(j - 1);
       ok = ok && warp_wait(dpfull, (uint32_t)j & 1u, abort_flag, s.err);
       jxd::tc_fence_after();
-      uint32_t hi[32], lo[32];
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
-        uint32_t r[32];
-        jxd::tmem_ld32(tmem + lanes + DQ_Y + half * 64 + c, r);
+        uint32_t r[32], hi[16], lo[16];
+        jxd::tmem_ld32(tmem + lanes + L::Y + half * 64 + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float a = p[c + i] * (__uint_as_float(r[i]) + dl), e = p[c + i + 1] * (__uint_as_float(r[i + 1]) + dl);
-          split_half(a, e, hi[(c + i) / 2], lo[(c + i) / 2]);
+        for (int i = 0; i < 16; ++i) {
+          const float2 e = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), one2, dl2);
+          const float2 ds = mul2(p[c / 2 + i], e);
+          split_half(ds.x, ds.y, hi[i], lo[i]);
         }
+        tmem_st16(tmem + lanes + L::DS + half * 64 + c, hi);
+        tmem_st16(tmem + lanes + L::DS + half * 64 + c + 16, lo);
       }
-      tmem_st32(tmem + lanes + DQ_X + half * 64, hi);
-      tmem_st32(tmem + lanes + DQ_X + half * 64 + 32, lo);
       tmem_st_wait();
-      jxd::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) jxd::mbar_arrive(dsfull);
+      done(dsfull);
       g_prev = inv_k * inverse_pow2(sc) * 6.103515625e-05f;  // P's 2^14
     }
     if (nb > 0) add_part(nb - 1);
@@ -377,13 +398,22 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 }
 
 // ---- dk, dv --------------------------------------------------------------------
-constexpr int BLK = 64;  // query rows per step
-constexpr uint32_t KV_K = 0, KV_V = 128, KV_X = 256, KV_Y = 320, KV_Z = 384;
-constexpr int HPANEL = BLK * 128;  // bytes of a panel of a half tile
-constexpr int KV_STAGES = 3;       // of Q and of dout each
-__host__ __device__ constexpr int kv_stage(int DP) { return tile_bytes(DP) / 2; }
+// Query rows per step: 128 at DP = 64, where the parts of dV and dK have columns of
+// their own (Z and W); 64 at DP = 128, where they share Z.  (An MMA of 64 columns
+// takes 45 cycles where half of one of 128 would be 32.)
+template <int DP>
+struct KvLayout {
+  static constexpr bool APART = DP == 64;
+  static constexpr int BLK = APART ? 128 : 64;
+  static constexpr uint32_t K = 0, V = APART ? 64 : 128, X = APART ? 128 : 256, Y = APART ? 256 : 320, Z = 384,
+                            W = APART ? 448 : 384;
+  static constexpr int PANEL_BYTES = BLK * 128;             // of a block
+  static constexpr int STAGE = DP / 64 * 2 * PANEL_BYTES;   // one block of Q or of dout: 32 KB
+};
+constexpr int KV_STAGES = 3;  // of Q and of dout each
 __host__ __device__ constexpr size_t kv_smem(int DP) {
-  return (size_t)2 * KV_STAGES * kv_stage(DP) + 1024 + KV_STAGES * 512 /*lse2, delta*/ + 2 * 128 * 4 + 256;
+  return (size_t)2 * KV_STAGES * (DP == 64 ? KvLayout<64>::STAGE : KvLayout<128>::STAGE) + 1024 +
+         KV_STAGES * 1024 /*lse2, delta*/ + 2 * 128 * 4 + 256;
 }
 
 template <int DP>
@@ -391,12 +421,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_dkv_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
                     const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
                     const float* __restrict__ lse, const float* __restrict__ dout, float* dk, float* dv) {
-  constexpr int ST = KV_STAGES, STAGE = kv_stage(DP), PART = STAGE / 2;
+  using L = KvLayout<DP>;
+  constexpr int ST = KV_STAGES, BLK = L::BLK, STAGE = L::STAGE, PART = STAGE / 2, HPANEL = L::PANEL_BYTES;
+  constexpr int PER_TILE = TILE / BLK;  // blocks of a tile
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  float* stats = reinterpret_cast<float*>(smem + 2 * ST * STAGE);  // [ST][lse2 64, delta 64]
-  float* xch = stats + ST * 128;
+  float* stats = reinterpret_cast<float*>(smem + 2 * ST * STAGE);  // [ST][lse2 BLK, delta BLK]
+  float* xch = stats + ST * 2 * BLK;
   uint64_t* qfull = reinterpret_cast<uint64_t*>(xch + 2 * 128);
   uint64_t* qempty = qfull + ST;
   uint64_t* dfull = qempty + ST;
@@ -407,8 +439,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   uint64_t* dpfull = pfull + 1;
   uint64_t* dsfull = dpfull + 1;
   uint64_t* zfull = dsfull + 1;
-  uint64_t* zfree = zfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(zfree + 1);
+  uint64_t* zfree = zfull + 1;  // dV's part
+  uint64_t* wfull = zfree + 1;  // dK's
+  uint64_t* wfree = wfull + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(wfree + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -438,7 +472,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 
   bool bad = threadIdx.x == 0 && (bt.bad_k[kslot] || bt.bad_v[kslot]);
   {
-    const int t0 = blk0 / 2, nt = nblk > 0 ? (sq.lq + TILE - 1) / TILE - t0 : 0;
+    const int t0 = blk0 / PER_TILE, nt = nblk > 0 ? (sq.lq + TILE - 1) / TILE - t0 : 0;
     for (long long e = threadIdx.x; e < (long long)nt * s.group; e += BW_THREADS) {
       const long long slot = qslot0 + (t0 + e / s.group) * s.heads + e % s.group;
       bad = bad || bt.bad_q[slot] || bt.bad_d[slot];
@@ -470,6 +504,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     jxd::mbar_init(dsfull, 8);
     jxd::mbar_init(zfull, 1);
     jxd::mbar_init(zfree, 8);
+    jxd::mbar_init(wfull, 1);
+    jxd::mbar_init(wfree, 8);
     *abort_flag = 0;
     jxd::fence_mbar_init();
   }
@@ -486,7 +522,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   if (warp < BW_FIRST) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
     if (warp == 0 && jxd::elect_one()) {
-      // half a tile: each part's panels, 64 rows of them
+      // a block: its rows of each part's panels
       auto load = [&](uint8_t* dst, const uint8_t* tile, int hb, uint64_t* bar) {
 #pragma unroll
         for (int e = 0; e < 2 * (DP / 64); ++e)
@@ -495,15 +531,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       int u = 0, nd = 0;
       for (; u < n; ++u) {
         const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
-        const long long slot = qslot0 + (long long)(blk >> 1) * s.heads + g;
+        const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
         if (*abort_flag || !wait_bounded(&qempty[st], (uint32_t)(u / ST + 1) & 1u, s.err)) break;
-        jxd::mbar_arrive_expect_tx(&qfull[st], STAGE + 512);
-        load(smem + st * STAGE, bt.q + slot * tile_bytes(DP), blk & 1, &qfull[st]);
-        bulk_load(jxd::smem_u32(stats + st * 128), bt.lse2 + slot * TILE + (blk & 1) * BLK, 256, &qfull[st]);
-        bulk_load(jxd::smem_u32(stats + st * 128 + 64), bt.delta + slot * TILE + (blk & 1) * BLK, 256, &qfull[st]);
+        jxd::mbar_arrive_expect_tx(&qfull[st], STAGE + 2 * BLK * 4);
+        load(smem + st * STAGE, bt.q + slot * tile_bytes(DP), blk % PER_TILE, &qfull[st]);
+        bulk_load(jxd::smem_u32(stats + st * 2 * BLK), bt.lse2 + slot * TILE + blk % PER_TILE * BLK, BLK * 4, &qfull[st]);
+        bulk_load(jxd::smem_u32(stats + st * 2 * BLK + BLK), bt.delta + slot * TILE + blk % PER_TILE * BLK, BLK * 4,
+                  &qfull[st]);
         if (*abort_flag || !wait_bounded(&dempty[st], (uint32_t)(u / ST + 1) & 1u, s.err)) { ++u; break; }
         jxd::mbar_arrive_expect_tx(&dfull[st], STAGE);
-        load(smem + (ST + st) * STAGE, bt.d + slot * tile_bytes(DP), blk & 1, &dfull[st]);
+        load(smem + (ST + st) * STAGE, bt.d + slot * tile_bytes(DP), blk % PER_TILE, &dfull[st]);
         ++nd;
       }
       if (nd < n) *abort_flag = 1;
@@ -517,7 +554,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       auto ready = [&](uint64_t* bar, int u) {
         return !*abort_flag && wait_bounded(bar, (uint32_t)u & 1u, s.err);
       };
-      // 128 x 64 scores
+      // 128 x BLK scores
       auto scores = [&](uint32_t d, uint32_t a0, uint32_t tile) {
         auto step = [&](int ks, uint32_t a, uint32_t p, uint32_t acc) {
           mma_f16_ts(d, a0 + a + ks * 8, jxd::smem_desc_k_sw128(tile + p + (ks >> 2) * HPANEL + (ks & 3) * 32), id_s,
@@ -531,45 +568,46 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
       };
-      // 128 x DP sums over the block's 64 rows; rows 0..31: hi at column 0, lo at 16, rows 32..63: 32 and 48
-      auto sums = [&](uint32_t a0, uint32_t tile) {
+      // 128 x DP sums over the block's rows; a0 holds 16 columns of hi, 16 of lo for every 32 rows
+      auto sums = [&](uint32_t d, uint32_t a0, uint32_t tile) {
         auto step = [&](int ks, uint32_t a, uint32_t p, uint32_t acc) {
-          mma_f16_ts(tmem + KV_Z, a0 + a + (ks >> 1) * 32 + (ks & 1) * 8,
-                     smem_desc_mn_sw128(tile + p + ks * 2048, HPANEL), id_o, acc);
+          mma_f16_ts(d, a0 + a + (ks >> 1) * 32 + (ks & 1) * 8, smem_desc_mn_sw128(tile + p + ks * 2048, HPANEL), id_o,
+                     acc);
         };
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
+        for (int ks = 0; ks < BLK / 16; ++ks) {
           step(ks, 16, 0, ks > 0);
           step(ks, 0, PART, 1);
         }
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) step(ks, 0, 0, 1);
+        for (int ks = 0; ks < BLK / 16; ++ks) step(ks, 0, 0, 1);
       };
       auto q_scores = [&](int u) {
         if (!ok || !(ok = ready(&qfull[u % ST], u / ST))) return;
         jxd::tc_fence_after();
-        scores(tmem + KV_X, tmem + KV_K, sbase + (u % ST) * STAGE);
+        scores(tmem + L::X, tmem + L::K, sbase + (u % ST) * STAGE);
         jxd::mma_commit(sfull);
       };
       auto d_scores = [&](int u) {
         if (!ok || !(ok = ready(&dfull[u % ST], u / ST))) return;
         jxd::tc_fence_after();
-        scores(tmem + KV_Y, tmem + KV_V, sbase + (ST + u % ST) * STAGE);
+        scores(tmem + L::Y, tmem + L::V, sbase + (ST + u % ST) * STAGE);
         jxd::mma_commit(dpfull);
       };
       q_scores(0);
       d_scores(0);
       for (int u = 0; ok && u < n; ++u) {
-        if (!(ok = ready(pfull, u) && ready(zfree, 2 * u + 1))) break;
+        // the sums' columns are drained: dV's of the step before, and dK's where they share them
+        if (!(ok = ready(pfull, u) && ready(L::APART ? zfree : wfree, u + 1))) break;
         jxd::tc_fence_after();
-        sums(tmem + KV_X, sbase + (ST + u % ST) * STAGE);
+        sums(tmem + L::Z, tmem + L::X, sbase + (ST + u % ST) * STAGE);
         jxd::mma_commit(zfull);
         jxd::mma_commit(&dempty[u % ST]);
         if (u + 1 < n) q_scores(u + 1);
-        if (!ok || !(ok = ready(dsfull, u) && ready(zfree, 2 * u))) break;
+        if (!ok || !(ok = ready(dsfull, u) && (L::APART ? ready(wfree, u + 1) : ready(zfree, u)))) break;
         jxd::tc_fence_after();
-        sums(tmem + KV_Y, sbase + (u % ST) * STAGE);
-        jxd::mma_commit(zfull);
+        sums(tmem + L::W, tmem + L::Y, sbase + (u % ST) * STAGE);
+        jxd::mma_commit(wfull);
         jxd::mma_commit(&qempty[u % ST]);
         if (u + 1 < n) d_scores(u + 1);
       }
@@ -582,9 +620,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const long long t = sq.k0 + j0 + row;
     float norm_v;
     const int e_k = stay_row<DP>(row < rows ? k + t * s.ldk + kd : nullptr, s.dim, half, row,
-                                 aligned16(k, s.dim, s.ldk), s.scale < 0.0f, tmem + lanes + KV_K, xch, bar, nullptr);
+                                 aligned16(k, s.dim, s.ldk), s.scale < 0.0f, tmem + lanes + L::K, xch, bar, nullptr);
     const int e_v = stay_row<DP>(row < rows ? v + t * s.ldv + kd : nullptr, s.dim, half, row,
-                                 aligned16(v, s.dim, s.ldv), false, tmem + lanes + KV_V, xch, bar, &norm_v);
+                                 aligned16(v, s.dim, s.ldv), false, tmem + lanes + L::V, xch, bar, &norm_v);
     tmem_st_wait();
     jxd::tc_fence_before();
     __syncwarp();
@@ -607,84 +645,91 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       __syncwarp();
       if (lane == 0) jxd::mbar_arrive(b8);
     };
+    constexpr int C = BLK / 2;  // columns of the scores that this thread has
     for (int u = 0; u < n; ++u) {
       const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
-      const long long slot = qslot0 + (long long)(blk >> 1) * s.heads + g;
+      const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
       const float inv_q = bt.inv_q[slot], inv_d = bt.inv_d[slot], norm_d = bt.norm_d[slot], top_d = bt.delta_top[slot];
-      const float* lse2 = stats + st * 128 + half * 32;
-      const float* delta = lse2 + 64;
+      const float* lse2 = stats + st * 2 * BLK + half * C;
+      const float* delta = lse2 + BLK;
       ready(&qfull[st], u / ST);  // landed before the scores were issued: its statistics are visible here too
       ready(sfull, u);
       const float f = f_row * inv_q;
-      float p[32];
-      float most = 0.0f;
-      {
+      const float2 f2 = make_float2(f, f);
+      const bool edge = blk * BLK < first_all || rows < TILE;  // some key is not seen by all of the block's rows
+      float2 p[C / 2];
+#pragma unroll
+      for (int c = 0; c < C; c += 32) {
         uint32_t r[32];
-        jxd::tmem_ld32(tmem + lanes + KV_X + half * 32, r);
+        jxd::tmem_ld32(tmem + lanes + L::X + half * C + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 l = *reinterpret_cast<const float4*>(lse2 + i);
-          p[i] = exp2_fast(fmaf(__uint_as_float(r[i]), f, -l.x));
-          p[i + 1] = exp2_fast(fmaf(__uint_as_float(r[i + 1]), f, -l.y));
-          p[i + 2] = exp2_fast(fmaf(__uint_as_float(r[i + 2]), f, -l.z));
-          p[i + 3] = exp2_fast(fmaf(__uint_as_float(r[i + 3]), f, -l.w));
+          const float4 l = *reinterpret_cast<const float4*>(lse2 + c + i);
+          const float2 z0 = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2,
+                                 make_float2(-l.x, -l.y));
+          const float2 z1 = fma2(make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), f2,
+                                 make_float2(-l.z, -l.w));
+          p[(c + i) / 2] = make_float2(exp2_fast(z0.x), exp2_fast(z0.y));
+          p[(c + i) / 2 + 1] = make_float2(exp2_fast(z1.x), exp2_fast(z1.y));
         }
       }
-      if (blk * BLK < first_all || rows < TILE) {
-        const int i0 = blk * BLK + half * 32;
+      if (edge) {
+        const int i0 = blk * BLK + half * C;
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i0 + i < first) p[i] = 0.0f;
+        for (int i = 0; i < C / 2; ++i) {
+          if (i0 + 2 * i < first) p[i].x = 0.0f;
+          if (i0 + 2 * i + 1 < first) p[i].y = 0.0f;
+        }
       }
-      {
+#pragma unroll
+      for (int c = 0; c < C; c += 32) {
         uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) split_half(p[2 * i], p[2 * i + 1], hi[i], lo[i]);
-        tmem_st16(tmem + lanes + KV_X + half * 32, hi);
-        tmem_st16(tmem + lanes + KV_X + half * 32 + 16, lo);
-        tmem_st_wait();
-        done(pfull);
+        for (int i = 0; i < 16; ++i) split_half(p[c / 2 + i].x, p[c / 2 + i].y, hi[i], lo[i]);
+        tmem_st16(tmem + lanes + L::X + half * C + c, hi);
+        tmem_st16(tmem + lanes + L::X + half * C + c + 16, lo);
       }
-#pragma unroll
-      for (int i = 0; i < 32; ++i) most = fmaxf(most, p[i]);
-      most = row_max(most, xch, half, row, bar);
+      tmem_st_wait();
+      done(pfull);
       if (u > 0) {
-        ready(zfull, 2 * u - 1);
-        drain<DP>(ak, tmem + lanes + KV_Z + half * (DP / 2), g_prev);
-        done(zfree);
+        ready(wfull, u - 1);
+        drain<DP>(ak, tmem + lanes + L::W + half * (DP / 2), g_prev);
+        done(wfree);
       }
-      const float fd = inv_v * inv_d;
-      const float sc = bound_scale(most * (norm_v * norm_d + top_d));
+      // P is at most 2^14
+      const float fd = inv_v * inv_d, sc = bound_scale(16384.0f * (norm_v * norm_d + top_d));
       const float pf = sc * fd, nf = -inverse_pow2(fd);
+      const float2 pf2 = make_float2(pf, pf), nf2 = make_float2(nf, nf);
       ready(dpfull, u);
-      {
+#pragma unroll
+      for (int c = 0; c < C; c += 32) {
         uint32_t r[32], hi[16], lo[16];
-        jxd::tmem_ld32(tmem + lanes + KV_Y + half * 32, r);
+        jxd::tmem_ld32(tmem + lanes + L::Y + half * C + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 d = *reinterpret_cast<const float4*>(delta + i);
-          const float a0 = (p[i] * pf) * fmaf(d.x, nf, __uint_as_float(r[i]));
-          const float a1 = (p[i + 1] * pf) * fmaf(d.y, nf, __uint_as_float(r[i + 1]));
-          const float a2 = (p[i + 2] * pf) * fmaf(d.z, nf, __uint_as_float(r[i + 2]));
-          const float a3 = (p[i + 3] * pf) * fmaf(d.w, nf, __uint_as_float(r[i + 3]));
-          split_half(a0, a1, hi[i / 2], lo[i / 2]);
-          split_half(a2, a3, hi[i / 2 + 1], lo[i / 2 + 1]);
+          const float4 d = *reinterpret_cast<const float4*>(delta + c + i);
+          const float2 e0 = fma2(make_float2(d.x, d.y), nf2, make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
+          const float2 e1 =
+              fma2(make_float2(d.z, d.w), nf2, make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])));
+          const float2 a0 = mul2(mul2(p[(c + i) / 2], pf2), e0), a1 = mul2(mul2(p[(c + i) / 2 + 1], pf2), e1);
+          split_half(a0.x, a0.y, hi[i / 2], lo[i / 2]);
+          split_half(a1.x, a1.y, hi[i / 2 + 1], lo[i / 2 + 1]);
         }
-        tmem_st16(tmem + lanes + KV_Y + half * 32, hi);
-        tmem_st16(tmem + lanes + KV_Y + half * 32 + 16, lo);
-        tmem_st_wait();
-        done(dsfull);
+        tmem_st16(tmem + lanes + L::Y + half * C + c, hi);
+        tmem_st16(tmem + lanes + L::Y + half * C + c + 16, lo);
       }
-      ready(zfull, 2 * u);
-      drain<DP>(av, tmem + lanes + KV_Z + half * (DP / 2), inv_d * 6.103515625e-05f);  // P's 2^14
+      tmem_st_wait();
+      done(dsfull);
+      ready(zfull, u);
+      drain<DP>(av, tmem + lanes + L::Z + half * (DP / 2), inv_d * 6.103515625e-05f);  // P's 2^14
       done(zfree);
       g_prev = inv_q * inverse_pow2(sc) * 6.103515625e-05f;
     }
     if (n > 0) {
-      ready(zfull, 2 * n - 1);
-      drain<DP>(ak, tmem + lanes + KV_Z + half * (DP / 2), g_prev);
+      ready(wfull, n - 1);
+      drain<DP>(ak, tmem + lanes + L::W + half * (DP / 2), g_prev);
     }
     if (row < rows) {
       const int left = s.dim - half * (DP / 2);

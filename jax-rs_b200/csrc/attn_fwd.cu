@@ -22,12 +22,33 @@ using namespace jxa;
 using jxg::wait_bounded;
 
 // ---- splitting -----------------------------------------------------------------
-// One block per (tile, head, tensor): 16 threads per row, 8 columns each (4 for DP = 64).
+// One block per (tile, head, tensor): 16 threads per row, 8 columns each (4 for
+// DP = 64), four rows per thread, all loads (o's too) before the first use.
+constexpr int SP_THREADS = 512, SP_ROWS = TILE * 16 / SP_THREADS;
+template <int CW>
+__device__ __forceinline__ void load_part(float (&x)[CW], const float* p, int left, bool vec) {
+#pragma unroll
+  for (int e = 0; e < CW; e += 4) {
+    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (vec && e + 4 <= left) {
+      f = *reinterpret_cast<const float4*>(p + e);
+    } else {
+      if (e < left) f.x = p[e];
+      if (e + 1 < left) f.y = p[e + 1];
+      if (e + 2 < left) f.z = p[e + 2];
+      if (e + 3 < left) f.w = p[e + 3];
+    }
+    x[e] = f.x;
+    x[e + 1] = f.y;
+    x[e + 2] = f.z;
+    x[e + 3] = f.w;
+  }
+}
 template <int DP>
-__global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant__ Shape s, int over_q,
-                                                         const __grid_constant__ TileSources src, int heads) {
+__global__ void __launch_bounds__(SP_THREADS) split_tiles_kernel(const __grid_constant__ Shape s, int over_q,
+                                                                const __grid_constant__ TileSources src, int heads) {
   constexpr int CW = DP / 16;  // columns per thread
-  __shared__ uint32_t sm_top[8], sm_low[8];
+  __shared__ uint32_t sm_top[SP_THREADS / 32], sm_low[SP_THREADS / 32];
   const TileSource& t = src.t[blockIdx.z];
   const int id = blockIdx.x, h = blockIdx.y;
   int j;
@@ -39,35 +60,32 @@ __global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant_
   const int rows = min(TILE, len - j * TILE);
   const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const int col = c * CW;
-  const float* base = t.x + row0 * t.ld + (long long)h * s.dim + col;
+  const long long hd = (long long)h * s.dim + col;
   const bool vec = (s.dim & 3) == 0 && (t.ld & 3) == 0 && (reinterpret_cast<uintptr_t>(t.x) & 15) == 0;
-  float x[8][CW];
-  uint32_t top = 0, low = 0x7fffffffu;  // the tile's largest row maximum, and the smallest one that is not zero
+  const bool vec_o = (s.dim & 3) == 0 && (s.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(t.o) & 15) == 0;
+  float x[SP_ROWS][CW], delta[SP_ROWS];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + 16 * i;
+  for (int i = 0; i < SP_ROWS; ++i) {
+    const int r = r0 + SP_THREADS / 16 * i;
+    load_part<CW>(x[i], t.x + (row0 + r) * t.ld + hd, r < rows ? s.dim - col : 0, vec);
+  }
+  if (t.o) {
+    float y[SP_ROWS][CW];
 #pragma unroll
-    for (int e = 0; e < CW; e += 4) {
-      float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < rows) {
-        const float* p = base + (long long)r * t.ld + e;
-        if (vec && col + e + 4 <= s.dim) {
-          f = *reinterpret_cast<const float4*>(p);
-        } else {
-          if (col + e < s.dim) f.x = p[0];
-          if (col + e + 1 < s.dim) f.y = p[1];
-          if (col + e + 2 < s.dim) f.z = p[2];
-          if (col + e + 3 < s.dim) f.w = p[3];
-        }
-      }
-      x[i][e] = f.x;
-      x[i][e + 1] = f.y;
-      x[i][e + 2] = f.z;
-      x[i][e + 3] = f.w;
+    for (int i = 0; i < SP_ROWS; ++i) {
+      const int r = r0 + SP_THREADS / 16 * i;
+      load_part<CW>(y[i], t.o + (row0 + r) * s.ldo + hd, r < rows ? s.dim - col : 0, vec_o);
+    }
+#pragma unroll
+    for (int i = 0; i < SP_ROWS; ++i) {
+      delta[i] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < CW; ++e) delta[i] = fmaf(x[i][e], y[i][e], delta[i]);
     }
   }
+  uint32_t top = 0, low = 0x7fffffffu;  // the tile's largest row maximum, and the smallest one that is not zero
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < SP_ROWS; ++i) {
     uint32_t m = 0;
 #pragma unroll
     for (int e = 0; e < CW; ++e) m = max(m, __float_as_uint(x[i][e]) & 0x7fffffffu);
@@ -84,7 +102,7 @@ __global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant_
   }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
+  for (int w = 0; w < SP_THREADS / 32; ++w) {
     top = max(top, sm_top[w]);
     low = min(low, sm_low[w]);
   }
@@ -95,19 +113,34 @@ __global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant_
     t.bad[slot] = unscaled(top) || (top && e_top - e_low > WIDE_BITS);
   }
   const float factor = scale_of(e_top);
+  uint8_t* out = t.tiles + slot * tile_bytes(DP);
+#pragma unroll
+  for (int i = 0; i < SP_ROWS; ++i) {
+    const int r = r0 + SP_THREADS / 16 * i;
+    uint32_t hi[CW / 2], lo[CW / 2];
+#pragma unroll
+    for (int e = 0; e < CW; ++e) x[i][e] *= factor;
+#pragma unroll
+    for (int e = 0; e < CW / 2; ++e) split_half(x[i][2 * e], x[i][2 * e + 1], hi[e], lo[e]);
+    const int at = col * 2;  // byte of the row
+    uint8_t* p = out + (at >> 7) * PANEL + r * 128 + ((((at & 127) >> 4) ^ (r & 7)) << 4) + (at & 15);
+    if constexpr (CW == 8) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(p + tile_part(DP)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    } else {
+      *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(p + tile_part(DP)) = make_uint2(lo[0], lo[1]);
+    }
+  }
   if (t.norm) {
     float most = 0.0f, most_delta = 0.0f;
     bool odd = false;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = r0 + 16 * i;
-      float n = 0.0f, d = 0.0f;
+    for (int i = 0; i < SP_ROWS; ++i) {
+      const int r = r0 + SP_THREADS / 16 * i;
+      float n = 0.0f, d = t.o ? delta[i] : 0.0f;
 #pragma unroll
-      for (int e = 0; e < CW; ++e) {
-        n += (x[i][e] * factor) * (x[i][e] * factor);
-        if (t.o && r < rows && col + e < s.dim)
-          d = fmaf(x[i][e], t.o[(row0 + r) * s.ldo + (long long)h * s.dim + col + e], d);
-      }
+      for (int e = 0; e < CW; ++e) n = fmaf(x[i][e], x[i][e], n);
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) {
         n += __shfl_xor_sync(0xffffffffu, n, o);
@@ -134,7 +167,7 @@ __global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant_
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < 8; ++w) {
+      for (int w = 1; w < SP_THREADS / 32; ++w) {
         most = fmaxf(most, __uint_as_float(sm_top[w]));
         most_delta = fmaxf(most_delta, __uint_as_float(sm_low[w]));
       }
@@ -143,23 +176,6 @@ __global__ void __launch_bounds__(256) split_tiles_kernel(const __grid_constant_
         t.delta_top[slot] = most_delta;
         if (odd) t.bad[slot] = 1;
       }
-    }
-  }
-  uint8_t* out = t.tiles + slot * tile_bytes(DP);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + 16 * i;
-    uint32_t hi[CW / 2], lo[CW / 2];
-#pragma unroll
-    for (int e = 0; e < CW / 2; ++e) split_half(x[i][2 * e] * factor, x[i][2 * e + 1] * factor, hi[e], lo[e]);
-    const int at = col * 2;  // byte of the row
-    uint8_t* p = out + (at >> 7) * PANEL + r * 128 + ((((at & 127) >> 4) ^ (r & 7)) << 4) + (at & 15);
-    if constexpr (CW == 8) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(p + tile_part(DP)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    } else {
-      *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[1]);
-      *reinterpret_cast<uint2*>(p + tile_part(DP)) = make_uint2(lo[0], lo[1]);
     }
   }
 }
@@ -501,8 +517,8 @@ namespace jxa {
 int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st) {
   const long long tiles = tile_count(over_q ? s.total_q : s.total_k, s.batch);
   const dim3 grid((unsigned)tiles, (unsigned)heads, (unsigned)count);
-  if (DP == 128) split_tiles_kernel<128><<<grid, 256, 0, st>>>(s, over_q, src, heads);
-  else split_tiles_kernel<64><<<grid, 256, 0, st>>>(s, over_q, src, heads);
+  if (DP == 128) split_tiles_kernel<128><<<grid, SP_THREADS, 0, st>>>(s, over_q, src, heads);
+  else split_tiles_kernel<64><<<grid, SP_THREADS, 0, st>>>(s, over_q, src, heads);
   JX_LAUNCH_CHECK("split_tiles_kernel");
   return JX_OK;
 }

@@ -71,17 +71,6 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {  // a in the l
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
-// hi and lo parts of two scaled values.
-__device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_half(a, b);
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  lo = pack_half(a - h.x, b - h.y);
-}
-__device__ __forceinline__ float exp2_fast(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
   asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
@@ -91,7 +80,27 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
-
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// hi and lo parts of two scaled values.
+__device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half(a, b);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  const float2 r = fma2(h, make_float2(-1.0f, -1.0f), make_float2(a, b));
+  lo = pack_half(r.x, r.y);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // ---- tcgen05 ------------------------------------------------------------------
 // D f32, A and B f16; N columns, M = 128 rows; B_MN: B is MN-major.
 __host__ __device__ constexpr uint32_t idesc_f16(int N, bool B_MN) {
