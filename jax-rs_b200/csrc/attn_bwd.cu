@@ -61,12 +61,12 @@ __device__ __forceinline__ float row_max(float v, float* xch, int half, int row,
   return v;
 }
 
-// A row's half into tensor memory; returns its scale's exponent and, with `norm`, the row's norm.
+// A row's half from an area into tensor memory; returns its scale's exponent and, with `norm`, the row's norm.
 template <int DP>
-__device__ __forceinline__ int stay_row(const float* src, int dim, int half, int row, bool vec, bool negate,
-                                        uint32_t taddr, float* xch, int id, float* norm) {
+__device__ __forceinline__ int stay_row(const uint8_t* area, int half, int row, bool negate, uint32_t taddr, float* xch,
+                                        int id, float* norm) {
   float x[DP / 2];
-  const float t = __uint_as_float(row_half_load<DP>(x, src, dim, half, vec));
+  const float t = __uint_as_float(half_from_area<DP>(x, area, row, half));
   const int e = (int)(__float_as_uint(row_max(t, xch, half, row, id)) >> 23);
   const float f = scale_of(e);
   if (norm) {
@@ -99,26 +99,6 @@ __device__ __forceinline__ void drain(float (&acc)[DP / 2], uint32_t taddr, floa
       acc[c + i + 1] = v.y;
     }
   }
-}
-
-// One row's half of a result.
-template <int DP>
-__device__ __forceinline__ void store_half(float* out, const float (&acc)[DP / 2], float factor, int n, bool vec) {
-  if (vec) {
-#pragma unroll
-    for (int c = 0; c < DP / 2; c += 4)
-      if (c < n)
-        *reinterpret_cast<float4*>(out + c) =
-            make_float4(acc[c] * factor, acc[c + 1] * factor, acc[c + 2] * factor, acc[c + 3] * factor);
-  } else {
-#pragma unroll
-    for (int c = 0; c < DP / 2; ++c)
-      if (c < n) out[c] = acc[c] * factor;
-  }
-}
-
-__device__ __forceinline__ bool aligned16(const void* p, int dim, long long ld) {
-  return (dim & 3) == 0 && (ld & 3) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
 // ---- dq ------------------------------------------------------------------------
@@ -175,19 +155,21 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const long long slot0 = (long long)first_tile(sq.k0, b) * s.kv_heads + hk;
   const long long qslot = ((long long)first_tile(sq.q0, b) + jt) * s.heads + h;
 
-  bool bad = threadIdx.x == 0 && (bt.bad_q[qslot] || bt.bad_d[qslot]);
-  for (int j = threadIdx.x; j < nb; j += BW_THREADS)
-    bad = bad || bt.bad_k[slot0 + (long long)j * s.kv_heads] || bt.bad_v[slot0 + (long long)j * s.kv_heads];
-  if (__syncthreads_or(bad)) {
-    for (int r = warp; r < rows; r += BW_THREADS / 32) {
-      const long long t = sq.q0 + i0 + r, hd = (long long)h * s.dim;
-      row_dq(q + t * s.ldq + hd, k + sq.k0 * s.ldk + (long long)hk * s.dim, v + sq.k0 * s.ldv + (long long)hk * s.dim,
-             o + t * s.ldo + hd, dout + t * s.ldo + hd, lse[(long long)h * s.total_q + t], dq + t * s.ldq + hd,
-             sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv, s.scale);
-    }
-    return;
-  }
-  if (threadIdx.x == 0) {
+  const long long hd = (long long)h * s.dim;
+  // Q passes through K's last stage, dout through V's last one; the copies for the first stages start at once
+  uint8_t *area_q = smem + (KS - 1) * STAGE, *area_d = smem + (KS + VS - 1) * STAGE;
+  auto copy_k = [&](int j) {
+    jxd::mbar_arrive_expect_tx(&kfull[j % KS], STAGE);
+    bulk_load(jxd::smem_u32(smem + j % KS * STAGE), bt.k + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
+              &kfull[j % KS]);
+  };
+  auto copy_v = [&](int j) {
+    jxd::mbar_arrive_expect_tx(&vfull[j % VS], STAGE);
+    bulk_load(jxd::smem_u32(smem + (KS + j % VS) * STAGE), bt.v + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
+              &vfull[j % VS]);
+  };
+  bool bad = false;
+  if (warp == 0 && lane == 0) {
     for (int i = 0; i < KS; ++i) {
       jxd::mbar_init(&kfull[i], 1);
       jxd::mbar_init(&kempty[i], 1);
@@ -205,31 +187,58 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     jxd::mbar_init(xfree, 8);
     *abort_flag = 0;
     jxd::fence_mbar_init();
-  }
-  if (warp == 1) {
+    jxd::fence_proxy_async_smem();
+    if (nb > 0) copy_k(0);
+  } else if (warp == 1) {
     jxd::tmem_alloc(tmem_slot, 512);
     jxd::tmem_relinquish();
+  } else if (warp >= BW_FIRST) {
+    const int tid = threadIdx.x - 32 * BW_FIRST;
+    float4 f[DP / 8], g[DP / 8];
+    rows_load<DP>(f, q + (sq.q0 + i0) * s.ldq + hd, s.ldq, rows, s.dim, aligned16(q, s.dim, s.ldq), tid);
+    rows_load<DP>(g, dout + (sq.q0 + i0) * s.ldo + hd, s.ldo, rows, s.dim, aligned16(dout, s.dim, s.ldo), tid);
+    rows_to_area<DP>(area_q, f, tid);
+    rows_to_area<DP>(area_d, g, tid);
+  } else if (warp >= 2) {
+    if (threadIdx.x == 64) bad = bt.bad_q[qslot] || bt.bad_d[qslot];
+    for (int j = (int)threadIdx.x - 64; j < nb; j += 64)
+      bad = bad || bt.bad_k[slot0 + (long long)j * s.kv_heads] || bt.bad_v[slot0 + (long long)j * s.kv_heads];
   }
   jxd::tc_fence_before();
-  __syncthreads();
+  bad = __syncthreads_or(bad);
   jxd::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (bad) {
+    // row by row, in plain f32
+    for (int r = warp; r < rows; r += BW_THREADS / 32) {
+      const long long t = sq.q0 + i0 + r;
+      row_dq(q + t * s.ldq + hd, k + sq.k0 * s.ldk + (long long)hk * s.dim, v + sq.k0 * s.ldv + (long long)hk * s.dim,
+             o + t * s.ldo + hd, dout + t * s.ldo + hd, lse[(long long)h * s.total_q + t], dq + t * s.ldq + hd,
+             sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv, s.scale);
+    }
+    if (warp == 0 && lane == 0 && nb > 0) wait_bounded(&kfull[0], 0, s.err);  // the copy has landed
+    if (warp == 1) {
+      __syncwarp();
+      jxd::tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
 
   if (warp < BW_FIRST) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
     if (warp == 0 && jxd::elect_one()) {
       int j = 0, nv = 0;
-      for (; j < nb; ++j) {
-        const long long at = (slot0 + (long long)j * s.kv_heads) * STAGE;
-        const int ks = j % KS, vs = j % VS;
-        if (*abort_flag || !wait_bounded(&kempty[ks], (uint32_t)(j / KS + 1) & 1u, s.err)) break;
-        jxd::mbar_arrive_expect_tx(&kfull[ks], STAGE);
-        bulk_load(jxd::smem_u32(smem + ks * STAGE), bt.k + at, STAGE, &kfull[ks]);
-        if (*abort_flag || !wait_bounded(&vempty[vs], (uint32_t)(j / VS + 1) & 1u, s.err)) { ++j; break; }
-        jxd::mbar_arrive_expect_tx(&vfull[vs], STAGE);
-        bulk_load(jxd::smem_u32(smem + (KS + vs) * STAGE), bt.v + at, STAGE, &vfull[vs]);
+      bool ok = wait_bounded(stayfull, 0, s.err);  // the areas are free again
+      for (; ok && j < nb; ++j) {
+        if (j > 0) {
+          if (!(ok = !*abort_flag && wait_bounded(&kempty[j % KS], (uint32_t)(j / KS + 1) & 1u, s.err))) break;
+          copy_k(j);
+        }
+        if (!(ok = !*abort_flag && wait_bounded(&vempty[j % VS], (uint32_t)(j / VS + 1) & 1u, s.err))) { ++j; break; }
+        copy_v(j);
         ++nv;
       }
+      if (!ok) j = max(j, min(nb, 1));  // the first K is under way in any case
       if (nv < nb) *abort_flag = 1;
       // every copy has landed before the CTA may end
       for (int u = max(0, j - KS); u < j; ++u) wait_bounded(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
@@ -296,13 +305,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_HIGH_REGS));
     const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane, bar = 1 + quarter;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const long long t = sq.q0 + i0 + row, hd = (long long)h * s.dim;
     float norm_d;
-    const int e_q = stay_row<DP>(row < rows ? q + t * s.ldq + hd : nullptr, s.dim, half, row,
-                                 aligned16(q, s.dim, s.ldq), s.scale < 0.0f, tmem + lanes + L::Q, xch, bar, nullptr);
-    const int e_d = stay_row<DP>(row < rows ? dout + t * s.ldo + hd : nullptr, s.dim, half, row,
-                                 aligned16(dout, s.dim, s.ldo), false, tmem + lanes + L::DO, xch, bar, &norm_d);
+    const int e_q = stay_row<DP>(area_q, half, row, s.scale < 0.0f, tmem + lanes + L::Q, xch, bar, nullptr);
+    const int e_d = stay_row<DP>(area_d, half, row, false, tmem + lanes + L::DO, xch, bar, &norm_d);
     tmem_st_wait();
+    jxd::fence_proxy_async_smem();  // the areas become copies' destinations
     jxd::tc_fence_before();
     __syncwarp();
     if (lane == 0) jxd::mbar_arrive(stayfull);
@@ -384,9 +391,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       g_prev = inv_k * inverse_pow2(sc) * 6.103515625e-05f;  // P's 2^14
     }
     if (nb > 0) add_part(nb - 1);
-    if (row < rows)
-      store_half<DP>(dq + t * s.ldq + hd + half * (DP / 2), acc, s.scale, s.dim - half * (DP / 2),
-                     aligned16(dq, s.dim, s.ldq));
+    // every MMA has retired: the stages are free
+    half_to_area<DP>(smem, acc, s.scale, row, half);
+    movers_sync();
+    rows_store<DP>(dq + (sq.q0 + i0) * s.ldq + hd, s.ldq, smem, rows, s.dim, aligned16(dq, s.dim, s.ldq),
+                   threadIdx.x - 32 * BW_FIRST);
   }
   jxd::tc_fence_before();
   __syncthreads();
@@ -470,27 +479,33 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const long long ld_k = bt.parts > 1 ? (long long)s.kv_heads * s.dim : s.ldk;
   const long long ld_v = bt.parts > 1 ? (long long)s.kv_heads * s.dim : s.ldv;
 
-  bool bad = threadIdx.x == 0 && (bt.bad_k[kslot] || bt.bad_v[kslot]);
-  {
-    const int t0 = blk0 / PER_TILE, nt = nblk > 0 ? (sq.lq + TILE - 1) / TILE - t0 : 0;
-    for (long long e = threadIdx.x; e < (long long)nt * s.group; e += BW_THREADS) {
-      const long long slot = qslot0 + (t0 + e / s.group) * s.heads + e % s.group;
-      bad = bad || bt.bad_q[slot] || bt.bad_d[slot];
-    }
-  }
-  if (__syncthreads_or(bad)) {
-    // the first part computes every row whole, the others add zeros
-    for (int r = warp; r < rows; r += BW_THREADS / 32) {
-      const long long t = sq.k0 + j0 + r;
-      row_dkv(q + sq.q0 * s.ldq + (long long)h0 * s.dim, o + sq.q0 * s.ldo + (long long)h0 * s.dim,
-              dout + sq.q0 * s.ldo + (long long)h0 * s.dim, lse + (long long)h0 * s.total_q + sq.q0,
-              k + t * s.ldk + kd, v + t * s.ldv + kd, out_k + t * ld_k + kd, out_v + t * ld_v + kd,
-              part == 0 ? sq.first_row(j0 + r, s.causal) : sq.lq, sq.lq, s.group, s.dim, s.ldq, s.ldo, s.total_q,
-              s.scale);
-    }
-    return;
-  }
-  if (threadIdx.x == 0) {
+  const int n = it1 - it0;
+  // K passes through the last stages of Q's ring, V through those of dout's; the first stages' copies start at once
+  constexpr int AREA_STAGES = area_bytes(DP) / STAGE;
+  uint8_t *area_k = smem + (ST - AREA_STAGES) * STAGE, *area_v = smem + (2 * ST - AREA_STAGES) * STAGE;
+  // a block: its rows of each part's panels
+  auto load = [&](uint8_t* dst, const uint8_t* tile, int hb, uint64_t* bar) {
+#pragma unroll
+    for (int e = 0; e < 2 * (DP / 64); ++e)
+      bulk_load(jxd::smem_u32(dst + e * HPANEL), tile + (long long)e * PANEL + hb * HPANEL, HPANEL, bar);
+  };
+  auto copy_q = [&](int u) {
+    const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
+    const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
+    jxd::mbar_arrive_expect_tx(&qfull[st], STAGE + 2 * BLK * 4);
+    load(smem + st * STAGE, bt.q + slot * tile_bytes(DP), blk % PER_TILE, &qfull[st]);
+    bulk_load(jxd::smem_u32(stats + st * 2 * BLK), bt.lse2 + slot * TILE + blk % PER_TILE * BLK, BLK * 4, &qfull[st]);
+    bulk_load(jxd::smem_u32(stats + st * 2 * BLK + BLK), bt.delta + slot * TILE + blk % PER_TILE * BLK, BLK * 4,
+              &qfull[st]);
+  };
+  auto copy_d = [&](int u) {
+    const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
+    const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
+    jxd::mbar_arrive_expect_tx(&dfull[st], STAGE);
+    load(smem + (ST + st) * STAGE, bt.d + slot * tile_bytes(DP), blk % PER_TILE, &dfull[st]);
+  };
+  bool bad = false;
+  if (warp == 0 && lane == 0) {
     for (int i = 0; i < ST; ++i) {
       jxd::mbar_init(&qfull[i], 1);
       jxd::mbar_init(&qempty[i], 1);
@@ -508,42 +523,68 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     jxd::mbar_init(wfree, 8);
     *abort_flag = 0;
     jxd::fence_mbar_init();
-  }
-  if (warp == 1) {
+    jxd::fence_proxy_async_smem();
+    if (n > 0) {
+      copy_q(0);
+      copy_d(0);
+    }
+  } else if (warp == 1) {
     jxd::tmem_alloc(tmem_slot, 512);
     jxd::tmem_relinquish();
+  } else if (warp >= BW_FIRST) {
+    const int tid = threadIdx.x - 32 * BW_FIRST;
+    float4 f[DP / 8], g[DP / 8];
+    rows_load<DP>(f, k + (sq.k0 + j0) * s.ldk + kd, s.ldk, rows, s.dim, aligned16(k, s.dim, s.ldk), tid);
+    rows_load<DP>(g, v + (sq.k0 + j0) * s.ldv + kd, s.ldv, rows, s.dim, aligned16(v, s.dim, s.ldv), tid);
+    rows_to_area<DP>(area_k, f, tid);
+    rows_to_area<DP>(area_v, g, tid);
+  } else if (warp >= 2) {
+    if (threadIdx.x == 64) bad = bt.bad_k[kslot] || bt.bad_v[kslot];
+    const int t0 = blk0 / PER_TILE, nt = nblk > 0 ? (sq.lq + TILE - 1) / TILE - t0 : 0;
+    for (long long e = (int)threadIdx.x - 64; e < (long long)nt * s.group; e += 64) {
+      const long long slot = qslot0 + (t0 + e / s.group) * s.heads + e % s.group;
+      bad = bad || bt.bad_q[slot] || bt.bad_d[slot];
+    }
   }
   jxd::tc_fence_before();
-  __syncthreads();
+  bad = __syncthreads_or(bad);
   jxd::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n = it1 - it0;
+  if (bad) {
+    // row by row, in plain f32: the first part computes every row whole, the others add zeros
+    for (int r = warp; r < rows; r += BW_THREADS / 32) {
+      const long long t = sq.k0 + j0 + r;
+      row_dkv(q + sq.q0 * s.ldq + (long long)h0 * s.dim, o + sq.q0 * s.ldo + (long long)h0 * s.dim,
+              dout + sq.q0 * s.ldo + (long long)h0 * s.dim, lse + (long long)h0 * s.total_q + sq.q0,
+              k + t * s.ldk + kd, v + t * s.ldv + kd, out_k + t * ld_k + kd, out_v + t * ld_v + kd,
+              part == 0 ? sq.first_row(j0 + r, s.causal) : sq.lq, sq.lq, s.group, s.dim, s.ldq, s.ldo, s.total_q,
+              s.scale);
+    }
+    if (warp == 0 && lane == 0 && n > 0) {  // the copies have landed
+      wait_bounded(&qfull[0], 0, s.err);
+      wait_bounded(&dfull[0], 0, s.err);
+    }
+    if (warp == 1) {
+      __syncwarp();
+      jxd::tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
 
   if (warp < BW_FIRST) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
     if (warp == 0 && jxd::elect_one()) {
-      // a block: its rows of each part's panels
-      auto load = [&](uint8_t* dst, const uint8_t* tile, int hb, uint64_t* bar) {
-#pragma unroll
-        for (int e = 0; e < 2 * (DP / 64); ++e)
-          bulk_load(jxd::smem_u32(dst + e * HPANEL), tile + (long long)e * PANEL + hb * HPANEL, HPANEL, bar);
-      };
-      int u = 0, nd = 0;
-      for (; u < n; ++u) {
-        const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
-        const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
-        if (*abort_flag || !wait_bounded(&qempty[st], (uint32_t)(u / ST + 1) & 1u, s.err)) break;
-        jxd::mbar_arrive_expect_tx(&qfull[st], STAGE + 2 * BLK * 4);
-        load(smem + st * STAGE, bt.q + slot * tile_bytes(DP), blk % PER_TILE, &qfull[st]);
-        bulk_load(jxd::smem_u32(stats + st * 2 * BLK), bt.lse2 + slot * TILE + blk % PER_TILE * BLK, BLK * 4, &qfull[st]);
-        bulk_load(jxd::smem_u32(stats + st * 2 * BLK + BLK), bt.delta + slot * TILE + blk % PER_TILE * BLK, BLK * 4,
-                  &qfull[st]);
-        if (*abort_flag || !wait_bounded(&dempty[st], (uint32_t)(u / ST + 1) & 1u, s.err)) { ++u; break; }
-        jxd::mbar_arrive_expect_tx(&dfull[st], STAGE);
-        load(smem + (ST + st) * STAGE, bt.d + slot * tile_bytes(DP), blk % PER_TILE, &dfull[st]);
+      int u = min(n, 1), nd = u;
+      bool ok = wait_bounded(stayfull, 0, s.err);  // the areas are free again
+      for (; ok && u < n; ++u) {
+        if (!(ok = !*abort_flag && wait_bounded(&qempty[u % ST], (uint32_t)(u / ST + 1) & 1u, s.err))) break;
+        copy_q(u);
+        if (!(ok = !*abort_flag && wait_bounded(&dempty[u % ST], (uint32_t)(u / ST + 1) & 1u, s.err))) { ++u; break; }
+        copy_d(u);
         ++nd;
       }
-      if (nd < n) *abort_flag = 1;
+      if (!ok) *abort_flag = 1;
+      // every copy has landed before the CTA may end
       for (int e = max(0, u - ST); e < u; ++e) wait_bounded(&qfull[e % ST], (uint32_t)(e / ST) & 1u, s.err);
       for (int e = max(0, nd - ST); e < nd; ++e) wait_bounded(&dfull[e % ST], (uint32_t)(e / ST) & 1u, s.err);
     }
@@ -617,13 +658,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_HIGH_REGS));
     const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane, bar = 1 + quarter;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const long long t = sq.k0 + j0 + row;
     float norm_v;
-    const int e_k = stay_row<DP>(row < rows ? k + t * s.ldk + kd : nullptr, s.dim, half, row,
-                                 aligned16(k, s.dim, s.ldk), s.scale < 0.0f, tmem + lanes + L::K, xch, bar, nullptr);
-    const int e_v = stay_row<DP>(row < rows ? v + t * s.ldv + kd : nullptr, s.dim, half, row,
-                                 aligned16(v, s.dim, s.ldv), false, tmem + lanes + L::V, xch, bar, &norm_v);
+    const int e_k = stay_row<DP>(area_k, half, row, s.scale < 0.0f, tmem + lanes + L::K, xch, bar, nullptr);
+    const int e_v = stay_row<DP>(area_v, half, row, false, tmem + lanes + L::V, xch, bar, &norm_v);
     tmem_st_wait();
+    jxd::fence_proxy_async_smem();  // the areas become copies' destinations
     jxd::tc_fence_before();
     __syncwarp();
     if (lane == 0) jxd::mbar_arrive(stayfull);
@@ -731,11 +770,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       ready(wfull, n - 1);
       drain<DP>(ak, tmem + lanes + L::W + half * (DP / 2), g_prev);
     }
-    if (row < rows) {
-      const int left = s.dim - half * (DP / 2);
-      store_half<DP>(out_k + t * ld_k + kd + half * (DP / 2), ak, s.scale, left, aligned16(out_k, s.dim, ld_k));
-      store_half<DP>(out_v + t * ld_v + kd + half * (DP / 2), av, 1.0f, left, aligned16(out_v, s.dim, ld_v));
-    }
+    // every MMA has retired: the stages are free
+    const int tid = threadIdx.x - 32 * BW_FIRST;
+    half_to_area<DP>(smem, ak, s.scale, row, half);
+    half_to_area<DP>(smem + ST * STAGE, av, 1.0f, row, half);
+    movers_sync();
+    rows_store<DP>(out_k + (sq.k0 + j0) * ld_k + kd, ld_k, smem, rows, s.dim, aligned16(out_k, s.dim, ld_k), tid);
+    rows_store<DP>(out_v + (sq.k0 + j0) * ld_v + kd, ld_v, smem + ST * STAGE, rows, s.dim,
+                   aligned16(out_v, s.dim, ld_v), tid);
   }
   jxd::tc_fence_before();
   __syncthreads();

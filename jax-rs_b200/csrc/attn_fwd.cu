@@ -239,34 +239,25 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
   const int nb = (nk + TILE - 1) / TILE;
   const long long slot0 = (long long)first_tile(sq.k0, b) * s.kv_heads + hk;
 
-  // Q's rows, and whether the tile has to be computed row by row
-  const int quarter = warp & 3, half = (warp - FW_FIRST) >> 2;
+  const int quarter = warp & 3, half = (warp - FW_FIRST) >> 2, tid = threadIdx.x - 32 * FW_FIRST;
   const int row = quarter * 32 + lane;
   const bool soft = warp >= FW_FIRST;
-  float x[DP / 2];
-  uint32_t top = 0;
-  if (soft) {
-    const bool vec = (s.dim & 3) == 0 && (s.ldq & 3) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
-    top = row_half_load<DP>(
-        x, row < rows ? q + (sq.q0 + i0 + row) * s.ldq + (long long)h * s.dim : nullptr, s.dim, half, vec);
-    reinterpret_cast<uint32_t*>(xch)[half * 128 + row] = top;
-  }
-  __syncthreads();
-  if (soft) top = max(top, reinterpret_cast<uint32_t*>(xch)[(half ^ 1) * 128 + row]);
-  bool bad = unscaled(top);
-  for (int j = threadIdx.x; j < nb; j += FW_THREADS)
-    bad = bad || ft.bad_k[slot0 + (long long)j * s.kv_heads] || ft.bad_v[slot0 + (long long)j * s.kv_heads];
-  if (__syncthreads_or(bad)) {
-    for (int r = warp; r < rows; r += FW_THREADS / 32) {
-      const long long t = sq.q0 + i0 + r;
-      row_fwd(q + t * s.ldq + (long long)h * s.dim, k + sq.k0 * s.ldk + (long long)hk * s.dim,
-              v + sq.k0 * s.ldv + (long long)hk * s.dim, o + t * s.ldo + (long long)h * s.dim,
-              lse ? lse + (long long)h * s.total_q + t : nullptr, sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv,
-              s.scale);
-    }
-    return;
-  }
-  if (threadIdx.x == 0) {
+  // Q passes through the last two stages; the copies for the others start at once
+  uint8_t* area = smem + (STAGES - 2) * STAGE;
+  const long long hd = (long long)h * s.dim;
+  // copies, in the order of use: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1), of each its lo part, then hi
+  auto copy = [&](int u, int stage) {
+    const int w = u >> 1;
+    const bool is_v = w == 2 * nb - 1 || (w >= 2 && (w & 1) == 0);
+    const int j = w == 0 ? 0 : w == 2 * nb - 1 ? nb - 1 : is_v ? w / 2 - 1 : (w + 1) / 2;
+    jxd::mbar_arrive_expect_tx(&full[stage], STAGE);
+    bulk_load(jxd::smem_u32(smem + stage * STAGE),
+              (is_v ? ft.v : ft.k) + (slot0 + (long long)j * s.kv_heads) * tile_bytes(DP) + (u & 1 ? 0 : STAGE), STAGE,
+              &full[stage]);
+  };
+  const int first = min(4 * nb, STAGES - 2);
+  bool bad = false;
+  if (warp == 0 && lane == 0) {
     for (int i = 0; i < STAGES; ++i) {
       jxd::mbar_init(&full[i], 1);
       jxd::mbar_init(&empty[i], 1);
@@ -280,31 +271,59 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     jxd::mbar_init(qfull, 8);
     *abort_flag = 0;
     jxd::fence_mbar_init();
-  }
-  if (warp == 1) {
+    jxd::fence_proxy_async_smem();
+    for (int u = 0; u < first; ++u) copy(u, u);
+  } else if (warp == 1) {
     jxd::tmem_alloc(tmem_slot, 512);
     jxd::tmem_relinquish();
+  } else if (soft) {
+    float4 f[DP / 8];
+    rows_load<DP>(f, q + (sq.q0 + i0) * s.ldq + hd, s.ldq, rows, s.dim, aligned16(q, s.dim, s.ldq), tid);
+    rows_to_area<DP>(area, f, tid);
+  } else if (warp >= 2) {
+    for (int j = (int)threadIdx.x - 64; j < nb; j += 64)
+      bad = bad || ft.bad_k[slot0 + (long long)j * s.kv_heads] || ft.bad_v[slot0 + (long long)j * s.kv_heads];
   }
   jxd::tc_fence_before();
   __syncthreads();
   jxd::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  float x[DP / 2];
+  uint32_t top = 0;
+  if (soft) {
+    top = half_from_area<DP>(x, area, row, half);
+    reinterpret_cast<uint32_t*>(xch)[half * 128 + row] = top;
+    pair_sync(1 + quarter);
+    top = max(top, reinterpret_cast<uint32_t*>(xch)[(half ^ 1) * 128 + row]);
+    bad = unscaled(top);
+  }
+  if (__syncthreads_or(bad)) {
+    // row by row, in plain f32
+    for (int r = warp; r < rows; r += FW_THREADS / 32) {
+      const long long t = sq.q0 + i0 + r;
+      row_fwd(q + t * s.ldq + hd, k + sq.k0 * s.ldk + (long long)hk * s.dim, v + sq.k0 * s.ldv + (long long)hk * s.dim,
+              o + t * s.ldo + hd, lse ? lse + (long long)h * s.total_q + t : nullptr, sq.visible(i0 + r, s.causal),
+              s.dim, s.ldk, s.ldv, s.scale);
+    }
+    if (warp == 0 && lane == 0)  // every copy has landed before the CTA may end
+      for (int u = 0; u < first; ++u) wait_bounded(&full[u], 0, s.err);
+    if (warp == 1) {
+      __syncwarp();
+      jxd::tmem_dealloc(tmem, 512);
+    }
+    return;
+  }
 
   if (!soft) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FW_LOW_REGS));
     if (warp == 0 && jxd::elect_one()) {
-      // ---- copies, in the order of use: K0 K1 V0 K2 V1 ... K(n-1) V(n-2) V(n-1)
-      int stage = 0, issued = 0;
+      // ---- the remaining copies
+      int stage = first % STAGES, issued = first;
       uint32_t phase = 0;
-      for (int u = 0; u < 4 * nb && !*abort_flag; ++u) {
-        const int w = u >> 1;  // tile in this order; its lo part, then hi
-        const bool is_v = w == 2 * nb - 1 || (w >= 2 && (w & 1) == 0);
-        const int j = w == 0 ? 0 : w == 2 * nb - 1 ? nb - 1 : is_v ? w / 2 - 1 : (w + 1) / 2;
+      if (4 * nb > first && !wait_bounded(qfull, 0, s.err)) *abort_flag = 1;  // the last stages are free of Q
+      for (int u = first; u < 4 * nb && !*abort_flag; ++u) {
         if (!wait_bounded(&empty[stage], phase ^ 1u, s.err)) { *abort_flag = 1; break; }
-        jxd::mbar_arrive_expect_tx(&full[stage], STAGE);
-        bulk_load(jxd::smem_u32(smem + stage * STAGE),
-                  (is_v ? ft.v : ft.k) + (slot0 + (long long)j * s.kv_heads) * tile_bytes(DP) + (u & 1 ? 0 : PART), STAGE,
-                  &full[stage]);
+        copy(u, stage);
         ++issued;
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
@@ -383,6 +402,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     const int e_row = (int)(top >> 23);
     row_half_store<DP>(x, s.scale < 0.0f ? -scale_of(e_row) : scale_of(e_row), tmem + lanes + T_Q, half);
     tmem_st_wait();
+    jxd::fence_proxy_async_smem();  // the area becomes a copy's destination
     jxd::tc_fence_before();
     __syncwarp();
     if (lane == 0) jxd::mbar_arrive(qfull);
@@ -481,25 +501,13 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     xch[half * 128 + row] = sum;
     pair_sync(1 + quarter);
     sum += xch[(half ^ 1) * 128 + row];
-    if (row < rows) {
-      const long long t = sq.q0 + i0 + row;
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      float* out = o + t * s.ldo + (long long)h * s.dim + half * (DP / 2);
-      const int n = s.dim - half * (DP / 2);
-      if ((s.dim & 3) == 0 && (s.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
-#pragma unroll
-        for (int c = 0; c < DP / 2; c += 4)
-          if (c < n)
-            *reinterpret_cast<float4*>(out + c) =
-                make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
-      } else {
-#pragma unroll
-        for (int c = 0; c < DP / 2; ++c)
-          if (c < n) out[c] = acc[c] * inv;
-      }
-      if (lse && half == 0)
-        lse[(long long)h * s.total_q + t] = sum == 0.0f ? -INFINITY : (m + (log2f(sum) - P_SHIFT)) * LN2;
-    }
+    // every MMA has retired: the stages are free
+    half_to_area<DP>(smem, acc, sum == 0.0f ? 0.0f : 1.0f / sum, row, half);
+    if (lse && half == 0 && row < rows)
+      lse[(long long)h * s.total_q + sq.q0 + i0 + row] =
+          sum == 0.0f ? -INFINITY : (m + (log2f(sum) - P_SHIFT)) * LN2;
+    movers_sync();
+    rows_store<DP>(o + (sq.q0 + i0) * s.ldo + hd, s.ldo, smem, rows, s.dim, aligned16(o, s.dim, s.ldo), tid);
   }
   jxd::tc_fence_before();
   __syncthreads();

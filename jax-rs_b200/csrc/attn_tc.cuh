@@ -189,35 +189,98 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 }
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
-// ---- the operand that stays: rows of a [rows, heads, dim] tensor into tensor memory ----
-// Two warps share 32 rows (TMEM lanes); this thread's row is `src` (NULL: zeros)
-// and its columns are half * DP/2 ..+DP/2.  Returns the largest magnitude's bits.
+// ---- rows of a [rows, heads, dim] tensor through shared memory ----
+// 256 threads move a tile of 128 rows between global memory, whole rows at a time,
+// and a thread-per-row layout: an area of 128 x DP floats, the 16-byte chunk c
+// of row r at r * 4 DP + ((c ^ (r & 7)) << 4), without conflicts either way.
+// (Thread-per-row accesses to global memory took 5500 cycles a tile, this 1500.)
+constexpr int MOVERS = 256;
+__host__ __device__ constexpr int area_bytes(int DP) { return TILE * DP * 4; }  // a tile's hi and lo parts' size, too
+
+__device__ __forceinline__ void movers_sync() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+__device__ __forceinline__ bool aligned16(const void* p, int dim, long long ld) {
+  return (dim & 3) == 0 && (ld & 3) == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
 template <int DP>
-__device__ __forceinline__ uint32_t row_half_load(float (&x)[DP / 2], const float* src, int dim, int half, bool vec) {
-  uint32_t top = 0;
+__device__ __forceinline__ uint32_t area_at(uint32_t row, uint32_t chunk) {
+  return row * (DP * 4) + ((chunk ^ (row & 7)) << 4);
+}
+// `src`: the tile's first row; zeros behind `rows` and `dim`.
+template <int DP>
+__device__ __forceinline__ void rows_load(float4 (&x)[DP / 8], const float* src, long long ld, int rows, int dim,
+                                          bool vec, int tid) {
 #pragma unroll
-  for (int c = 0; c < DP / 2; c += 4) {
-    const int col = half * (DP / 2) + c;
-    float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (src) {
-      if (vec && col + 4 <= dim) {
-        f = *reinterpret_cast<const float4*>(src + col);
+  for (int i = 0; i < DP / 8; ++i) {
+    const int f = i * MOVERS + tid, r = f / (DP / 4), c = f % (DP / 4) * 4;
+    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < rows) {
+      const float* p = src + r * ld + c;
+      if (vec) {
+        if (c < dim) x[i] = *reinterpret_cast<const float4*>(p);
       } else {
-        if (col < dim) f.x = src[col];
-        if (col + 1 < dim) f.y = src[col + 1];
-        if (col + 2 < dim) f.z = src[col + 2];
-        if (col + 3 < dim) f.w = src[col + 3];
+        if (c < dim) x[i].x = p[0];
+        if (c + 1 < dim) x[i].y = p[1];
+        if (c + 2 < dim) x[i].z = p[2];
+        if (c + 3 < dim) x[i].w = p[3];
       }
     }
-    x[c] = f.x;
-    x[c + 1] = f.y;
-    x[c + 2] = f.z;
-    x[c + 3] = f.w;
+  }
+}
+template <int DP>
+__device__ __forceinline__ void rows_to_area(uint8_t* area, const float4 (&x)[DP / 8], int tid) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[c + i]) & 0x7fffffffu);
+  for (int i = 0; i < DP / 8; ++i) {
+    const int f = i * MOVERS + tid;
+    *reinterpret_cast<float4*>(area + area_at<DP>(f / (DP / 4), f % (DP / 4))) = x[i];
+  }
+}
+// This thread's half of row `row`; returns the largest magnitude's bits.
+template <int DP>
+__device__ __forceinline__ uint32_t half_from_area(float (&x)[DP / 2], const uint8_t* area, int row, int half) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c) {
+    const float4 f = *reinterpret_cast<const float4*>(area + area_at<DP>(row, half * (DP / 8) + c));
+    x[4 * c] = f.x;
+    x[4 * c + 1] = f.y;
+    x[4 * c + 2] = f.z;
+    x[4 * c + 3] = f.w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[4 * c + i]) & 0x7fffffffu);
   }
   return top;
 }
+// The halves, times `factor`, and out again: dst is the tile's first row.
+template <int DP>
+__device__ __forceinline__ void half_to_area(uint8_t* area, const float (&x)[DP / 2], float factor, int row, int half) {
+#pragma unroll
+  for (int c = 0; c < DP / 8; ++c)
+    *reinterpret_cast<float4*>(area + area_at<DP>(row, half * (DP / 8) + c)) =
+        make_float4(x[4 * c] * factor, x[4 * c + 1] * factor, x[4 * c + 2] * factor, x[4 * c + 3] * factor);
+}
+template <int DP>
+__device__ __forceinline__ void rows_store(float* dst, long long ld, const uint8_t* area, int rows, int dim, bool vec,
+                                           int tid) {
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i) {
+    const int f = i * MOVERS + tid, r = f / (DP / 4), c = f % (DP / 4) * 4;
+    if (r < rows) {
+      const float4 x = *reinterpret_cast<const float4*>(area + area_at<DP>(r, c / 4));
+      float* p = dst + r * ld + c;
+      if (vec) {
+        if (c < dim) *reinterpret_cast<float4*>(p) = x;
+      } else {
+        if (c < dim) p[0] = x.x;
+        if (c + 1 < dim) p[1] = x.y;
+        if (c + 2 < dim) p[2] = x.z;
+        if (c + 3 < dim) p[3] = x.w;
+      }
+    }
+  }
+}
+
+// ---- the operand that stays: rows into tensor memory ----
+// Two warps share 32 rows (TMEM lanes), each thread half a row.
 // Stores the scaled halves' parts: hi at column `col` of tensor memory, lo DP/2 columns behind it.
 template <int DP>
 __device__ __forceinline__ void row_half_store(const float (&x)[DP / 2], float factor, uint32_t taddr, int half) {
