@@ -40,6 +40,7 @@ struct BwdTiles {
   const int *bad_q, *bad_k, *bad_v, *bad_d;
   const float *norm_v, *norm_d, *lse2, *delta, *delta_top;
   int q_tiles, k_tiles, parts;
+  const int *order_q, *order_k;
   float *part_k, *part_v;  // [parts][total_k * kv_heads * dim], used where parts > 1
 };
 
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int id = bt.q_tiles - 1 - (int)(blockIdx.x / (unsigned)s.heads), h = (int)(blockIdx.x % (unsigned)s.heads);
+  const int id = bt.order_q[blockIdx.x / (unsigned)s.heads], h = (int)(blockIdx.x % (unsigned)s.heads);
   int jt;
   const int b = seq_of_tile(s.cu_q, s.batch, id, &jt);
   const Seq sq = seq_bounds(s, b);
@@ -455,11 +456,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the first keys of a sequence, which the most rows see, start first
+  // the keys that the most rows see start first
   unsigned w = blockIdx.x;
   const int part = (int)(w % (unsigned)bt.parts);
   w /= (unsigned)bt.parts;
-  const int hk = (int)(w % (unsigned)s.kv_heads), id = (int)(w / (unsigned)s.kv_heads);
+  const int hk = (int)(w % (unsigned)s.kv_heads), id = bt.order_k[w / (unsigned)s.kv_heads];
   int jt;
   const int b = seq_of_tile(s.cu_k, s.batch, id, &jt);
   const Seq sq = seq_bounds(s, b);
@@ -866,7 +867,7 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
   const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
   // tiles first, then arrays whose pieces the copies read 16-byte aligned, then the rest
-  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (5 * ks + 6 * qs) * 4 + 2 * part_floats * 4;
+  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (5 * ks + 6 * qs + qt + kt) * 4 + 2 * part_floats * 4;
   void* p = nullptr;
   if (int rc = jx::scratch_get(bytes + 64, &p, st)) return rc;
   uint8_t* at = static_cast<uint8_t*>(p);
@@ -884,13 +885,16 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   float *inv_q = (float*)take(qs * 4), *inv_d = (float*)take(qs * 4), *norm_d = (float*)take(qs * 4);
   float* delta_top = (float*)take(qs * 4);
   int *bad_k = (int*)take(ks * 4), *bad_v = (int*)take(ks * 4), *bad_q = (int*)take(qs * 4), *bad_d = (int*)take(qs * 4);
+  int *order_q = (int*)take(qt * 4), *order_k = (int*)take(kt * 4);
   TileSources kv = {}, qd = {};
   kv.t[0] = {k, s.ldk, tk, inv_k, bad_k};
   kv.t[1] = {v, s.ldv, tv, inv_v, bad_v, norm_v};
   qd.t[0] = {q, s.ldq, tq, inv_q, bad_q};
   qd.t[1] = {dout, s.ldo, td, inv_d, bad_d, norm_d, o, lse, lse2, delta, delta_top};
   const BwdTiles bt = {tq,     tk,     tv,    td,    inv_q, inv_k,     inv_v,   inv_d,   bad_q, bad_k,  bad_v,
-                       bad_d,  norm_v, norm_d, lse2, delta, delta_top, (int)qt, (int)kt, parts, part_k, part_v};
+                       bad_d,  norm_v, norm_d, lse2, delta, delta_top, (int)qt, (int)kt, parts, order_q, order_k, part_k, part_v};
+  kv.order = order_k;
+  kv.order_other = order_q;
   int rc = split_tiles(s, false, kv, 2, s.kv_heads, DP, st);
   if (!rc) rc = split_tiles(s, true, qd, 2, s.heads, DP, st);
   if (!rc)

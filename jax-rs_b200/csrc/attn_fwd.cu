@@ -22,13 +22,11 @@ using namespace jxa;
 using jxg::wait_bounded;
 
 // ---- splitting -----------------------------------------------------------------
-// One block per (tile, head, tensor): 16 threads per row, 8 columns each (4 for
-// DP = 64), four rows per thread, all loads (o's too) before the first use.
-constexpr int SP_THREADS = 512, SP_ROWS = TILE * 16 / SP_THREADS;
-template <int CW>
-__device__ __forceinline__ void load_part(float (&x)[CW], const float* p, int left, bool vec) {
+// One block per (tile, head, tensor): eight columns of two or four rows per thread.
+constexpr int SP_THREADS = 512;
+__device__ __forceinline__ void load_part(float (&x)[8], const float* p, int left, bool vec) {
 #pragma unroll
-  for (int e = 0; e < CW; e += 4) {
+  for (int e = 0; e < 8; e += 4) {
     float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
     if (vec && e + 4 <= left) {
       f = *reinterpret_cast<const float4*>(p + e);
@@ -44,13 +42,66 @@ __device__ __forceinline__ void load_part(float (&x)[CW], const float* p, int le
     x[e + 3] = f.w;
   }
 }
+
+// Tiles that the tile's CTA works through: key tiles that a query tile's last row
+// sees, or query tiles that see a key tile's first key.
+__device__ __forceinline__ int tile_work(const Shape& s, bool over_q, int id) {
+  const int32_t* cu = over_q ? s.cu_q : s.cu_k;
+  int lo = 0, hi = s.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((cu[mid] >> 7) + mid <= id) lo = mid;
+    else hi = mid;
+  }
+  const int j = id - ((cu[lo] >> 7) + lo);
+  const Seq sq = seq_bounds(s, lo);
+  const int len = over_q ? sq.lq : sq.lk;
+  if (j < 0 || (long long)j * TILE >= len) return 0;
+  if (over_q) return (sq.visible(min(j * TILE + TILE, sq.lq) - 1, s.causal) + TILE - 1) / TILE + 1;
+  return max(0, (sq.lq - sq.first_row(j * TILE, s.causal) + TILE - 1) / TILE) + 1;
+}
+// One block: a counting sort by falling work.  Ids of equal work come in any order,
+// which changes when they are computed and nothing else.
+__device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, int* order) {
+  __shared__ int count[ORDER_KEYS], sums[SP_THREADS / 32];
+  static_assert(ORDER_KEYS == 2 * SP_THREADS, "two keys per thread");
+  const int tid = threadIdx.x;
+  count[tid] = count[tid + SP_THREADS] = 0;
+  __syncthreads();
+  auto key = [&](int id) { return ORDER_KEYS - 1 - min(tile_work(s, over_q, id) >> shift, ORDER_KEYS - 1); };
+  for (int id = tid; id < tiles; id += SP_THREADS) atomicAdd(&count[key(id)], 1);
+  __syncthreads();
+  // exclusive prefix sums
+  const int a = count[2 * tid], b = count[2 * tid + 1];
+  int x = a + b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if ((tid & 31) >= o) x += y;
+  }
+  if ((tid & 31) == 31) sums[tid >> 5] = x;
+  __syncthreads();
+  for (int w = 0; w < (tid >> 5); ++w) x += sums[w];
+  count[2 * tid] = x - a - b;
+  count[2 * tid + 1] = x - b;
+  __syncthreads();
+  for (int id = tid; id < tiles; id += SP_THREADS) order[atomicAdd(&count[key(id)], 1)] = id;
+}
+
 template <int DP>
-__global__ void __launch_bounds__(SP_THREADS) split_tiles_kernel(const __grid_constant__ Shape s, int over_q,
-                                                                const __grid_constant__ TileSources src, int heads) {
-  constexpr int CW = DP / 16;  // columns per thread
+__global__ void __launch_bounds__(SP_THREADS, 2) split_tiles_kernel(const __grid_constant__ Shape s, int over_q,
+                                                                   const __grid_constant__ TileSources src, int heads,
+                                                                   int tiles, int tiles_other) {
+  constexpr int PER_ROW = DP / 8, STEP = SP_THREADS / PER_ROW, ROWS = TILE / STEP;  // threads; rows at a time; rows each
   __shared__ uint32_t sm_top[SP_THREADS / 32], sm_low[SP_THREADS / 32];
+  if (blockIdx.x == 0) {  // one block per order that is asked for
+    if (blockIdx.y == 0 && blockIdx.z == 0 && src.order) order_tiles(s, over_q, tiles, src.shift, src.order);
+    if (blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1 && src.order_other)
+      order_tiles(s, !over_q, tiles_other, src.shift, src.order_other);
+    return;
+  }
   const TileSource& t = src.t[blockIdx.z];
-  const int id = blockIdx.x, h = blockIdx.y;
+  const int id = blockIdx.x - 1, h = blockIdx.y;
   int j;
   const int b = seq_of_tile(over_q ? s.cu_q : s.cu_k, s.batch, id, &j);
   const Seq sq = seq_bounds(s, b);
@@ -58,44 +109,32 @@ __global__ void __launch_bounds__(SP_THREADS) split_tiles_kernel(const __grid_co
   if (j < 0 || (long long)j * TILE >= len) return;
   const long long row0 = (over_q ? sq.q0 : sq.k0) + (long long)j * TILE;
   const int rows = min(TILE, len - j * TILE);
-  const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4;
-  const int col = c * CW;
+  const int c = threadIdx.x % PER_ROW, r0 = threadIdx.x / PER_ROW;
+  const int col = c * 8, left = s.dim - col;
   const long long hd = (long long)h * s.dim + col;
   const bool vec = (s.dim & 3) == 0 && (t.ld & 3) == 0 && (reinterpret_cast<uintptr_t>(t.x) & 15) == 0;
-  const bool vec_o = (s.dim & 3) == 0 && (s.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(t.o) & 15) == 0;
-  float x[SP_ROWS][CW], delta[SP_ROWS];
+  float x[ROWS][8];
+  {
+    const float* p = t.x + (row0 + r0) * t.ld + hd;
 #pragma unroll
-  for (int i = 0; i < SP_ROWS; ++i) {
-    const int r = r0 + SP_THREADS / 16 * i;
-    load_part<CW>(x[i], t.x + (row0 + r) * t.ld + hd, r < rows ? s.dim - col : 0, vec);
-  }
-  if (t.o) {
-    float y[SP_ROWS][CW];
-#pragma unroll
-    for (int i = 0; i < SP_ROWS; ++i) {
-      const int r = r0 + SP_THREADS / 16 * i;
-      load_part<CW>(y[i], t.o + (row0 + r) * s.ldo + hd, r < rows ? s.dim - col : 0, vec_o);
-    }
-#pragma unroll
-    for (int i = 0; i < SP_ROWS; ++i) {
-      delta[i] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < CW; ++e) delta[i] = fmaf(x[i][e], y[i][e], delta[i]);
-    }
+    for (int i = 0; i < ROWS; ++i, p += STEP * t.ld) load_part(x[i], p, r0 + STEP * i < rows ? left : 0, vec);
   }
   uint32_t top = 0, low = 0x7fffffffu;  // the tile's largest row maximum, and the smallest one that is not zero
 #pragma unroll
-  for (int i = 0; i < SP_ROWS; ++i) {
+  for (int i = 0; i < ROWS; ++i) {
     uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < CW; ++e) m = max(m, __float_as_uint(x[i][e]) & 0x7fffffffu);
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[i][e]) & 0x7fffffffu);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = PER_ROW / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     top = max(top, m);
     if (m) low = min(low, m);
   }
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 16));
-  low = min(low, __shfl_xor_sync(0xffffffffu, low, 16));
+#pragma unroll
+  for (int o = PER_ROW; o < 32; o <<= 1) {
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
   if ((threadIdx.x & 31) == 0) {
     sm_top[threadIdx.x >> 5] = top;
     sm_low[threadIdx.x >> 5] = low;
@@ -113,36 +152,36 @@ __global__ void __launch_bounds__(SP_THREADS) split_tiles_kernel(const __grid_co
     t.bad[slot] = unscaled(top) || (top && e_top - e_low > WIDE_BITS);
   }
   const float factor = scale_of(e_top);
-  uint8_t* out = t.tiles + slot * tile_bytes(DP);
+  const int at = col * 2;  // byte of the row; r0 + STEP * i has the same low three bits for every i
+  uint8_t* out = t.tiles + slot * tile_bytes(DP) + (at >> 7) * PANEL + r0 * 128 + ((((at & 127) >> 4) ^ (r0 & 7)) << 4);
+  static_assert(STEP % 8 == 0, "rows of a thread share their swizzle");
 #pragma unroll
-  for (int i = 0; i < SP_ROWS; ++i) {
-    const int r = r0 + SP_THREADS / 16 * i;
-    uint32_t hi[CW / 2], lo[CW / 2];
+  for (int i = 0; i < ROWS; ++i) {
+    uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int e = 0; e < CW; ++e) x[i][e] *= factor;
-#pragma unroll
-    for (int e = 0; e < CW / 2; ++e) split_half(x[i][2 * e], x[i][2 * e + 1], hi[e], lo[e]);
-    const int at = col * 2;  // byte of the row
-    uint8_t* p = out + (at >> 7) * PANEL + r * 128 + ((((at & 127) >> 4) ^ (r & 7)) << 4) + (at & 15);
-    if constexpr (CW == 8) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(p + tile_part(DP)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    } else {
-      *reinterpret_cast<uint2*>(p) = make_uint2(hi[0], hi[1]);
-      *reinterpret_cast<uint2*>(p + tile_part(DP)) = make_uint2(lo[0], lo[1]);
-    }
+    for (int e = 0; e < 4; ++e) split_half(x[i][2 * e] * factor, x[i][2 * e + 1] * factor, hi[e], lo[e]);
+    *reinterpret_cast<uint4*>(out + i * STEP * 128) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(out + i * STEP * 128 + tile_part(DP)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
   if (t.norm) {
+    const bool vec_o = (s.dim & 3) == 0 && (s.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(t.o) & 15) == 0;
     float most = 0.0f, most_delta = 0.0f;
     bool odd = false;
+    const float* p = t.o + (row0 + r0) * s.ldo + hd;
 #pragma unroll
-    for (int i = 0; i < SP_ROWS; ++i) {
-      const int r = r0 + SP_THREADS / 16 * i;
-      float n = 0.0f, d = t.o ? delta[i] : 0.0f;
+    for (int i = 0; i < ROWS; ++i, p += STEP * s.ldo) {
+      const int r = r0 + STEP * i;
+      float n = 0.0f, d = 0.0f;
 #pragma unroll
-      for (int e = 0; e < CW; ++e) n = fmaf(x[i][e], x[i][e], n);
+      for (int e = 0; e < 8; ++e) n = fmaf(x[i][e] * factor, x[i][e] * factor, n);
+      if (t.o) {
+        float y[8];
+        load_part(y, p, r < rows ? left : 0, vec_o);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) {
+        for (int e = 0; e < 8; ++e) d = fmaf(x[i][e], y[e], d);
+      }
+#pragma unroll
+      for (int o = PER_ROW / 2; o > 0; o >>= 1) {
         n += __shfl_xor_sync(0xffffffffu, n, o);
         d += __shfl_xor_sync(0xffffffffu, d, o);
       }
@@ -204,7 +243,7 @@ struct FwdTiles {
   const float* inv_v;
   const int* bad_k;
   const int* bad_v;
-  int q_tiles;
+  const int* order;  // of the query tiles
 };
 
 template <int DP>
@@ -227,8 +266,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // the last tiles of a sequence, which see the most keys, start first
-  const int id = ft.q_tiles - 1 - (int)(blockIdx.x / (unsigned)s.heads), h = (int)(blockIdx.x % (unsigned)s.heads);
+  // the tiles that see the most keys start first
+  const int id = ft.order[blockIdx.x / (unsigned)s.heads], h = (int)(blockIdx.x % (unsigned)s.heads);
   int jt;
   const int b = seq_of_tile(s.cu_q, s.batch, id, &jt);
   const Seq sq = seq_bounds(s, b);
@@ -523,10 +562,13 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 namespace jxa {
 
 int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st) {
-  const long long tiles = tile_count(over_q ? s.total_q : s.total_k, s.batch);
-  const dim3 grid((unsigned)tiles, (unsigned)heads, (unsigned)count);
-  if (DP == 128) split_tiles_kernel<128><<<grid, SP_THREADS, 0, st>>>(s, over_q, src, heads);
-  else split_tiles_kernel<64><<<grid, SP_THREADS, 0, st>>>(s, over_q, src, heads);
+  const int tiles = (int)tile_count(over_q ? s.total_q : s.total_k, s.batch);
+  const int other = (int)tile_count(over_q ? s.total_k : s.total_q, s.batch);
+  TileSources ts = src;
+  for (ts.shift = 0; (std::max(tiles, other) >> ts.shift) >= ORDER_KEYS - 1; ++ts.shift) {}
+  const dim3 grid((unsigned)tiles + 1, (unsigned)heads, (unsigned)count);
+  if (DP == 128) split_tiles_kernel<128><<<grid, SP_THREADS, 0, st>>>(s, over_q, ts, heads, tiles, other);
+  else split_tiles_kernel<64><<<grid, SP_THREADS, 0, st>>>(s, over_q, ts, heads, tiles, other);
   JX_LAUNCH_CHECK("split_tiles_kernel");
   return JX_OK;
 }
@@ -558,14 +600,15 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
   JX_REQUIRE(qt * s.heads < (1LL << 31) && kt < (1LL << 31), "attention: too many rows");
   const size_t slots = (size_t)kt * s.kv_heads, bytes = slots * tile_bytes(DP);
   void* p = nullptr;
-  if (int rc = jx::scratch_get(2 * bytes + 4 * slots * sizeof(float), &p, st)) return rc;
+  if (int rc = jx::scratch_get(2 * bytes + 4 * slots * sizeof(float) + qt * sizeof(int), &p, st)) return rc;
   uint8_t* base = static_cast<uint8_t*>(p);
   float* inv = reinterpret_cast<float*>(base + 2 * bytes);
   int* bad = reinterpret_cast<int*>(inv + 2 * slots);
   TileSources src = {};
   src.t[0] = {k, s.ldk, base, inv, bad};
   src.t[1] = {v, s.ldv, base + bytes, inv + slots, bad + slots};
-  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, (int)qt};
+  src.order_other = bad + 2 * slots;
+  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, src.order_other};
   int rc = split_tiles(s, false, src, 2, s.kv_heads, DP, st);
   if (!rc) {
     const unsigned grid = (unsigned)(qt * s.heads);

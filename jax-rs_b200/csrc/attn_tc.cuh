@@ -316,7 +316,14 @@ struct TileSource {
 };
 struct TileSources {
   TileSource t[2];
+  // Order of work over the same launch's tiles (over_q: query tiles by their key
+  // tiles, else key tiles by their query rows): ids by falling work, those
+  // behind a sequence's end last.  May be NULL.  work >> shift is below ORDER_KEYS.
+  int* order;
+  int* order_other;  // of the other side's tiles
+  int shift;
 };
+constexpr int ORDER_KEYS = 1024;
 
 // Implemented in attn_fwd.cu: splits 1 or 2 tensors of `heads` heads over the same packed sequences.
 int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st);
