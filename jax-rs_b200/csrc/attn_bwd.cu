@@ -3,18 +3,22 @@
 //
 // Two kernels, each with its sums in registers, so that every sum has a fixed
 // order and nothing is added atomically; the price is that the scores and
-// dout v^T are computed in both (seven products a tile instead of five).
+// dout v^T are computed in both (seven products a tile instead of five).  All
+// four operands are split into tiles once, and each kernel streams two of them.
 //
 // dq: one CTA per (128 query rows, head), streaming K and V tiles.
-//   S = Q K^T, dP = dO V^T        Q and dO in tensor memory
-//   dS = P (dP - delta)           P = exp2(S f - lse2)
-//   dQ += dS K                    dS in tensor memory, over S's columns
+//   S = Q K^T, dP = dO V^T,  dS = P (dP - delta),  dQ += dS K
 // dk, dv: one CTA per (128 keys, key head, part of the query rows), streaming
-// blocks of 64 rows of Q and dO of every head of the group.
-//   S^T = K Q^T, dP^T = V dO^T    K and V in tensor memory
-//   dV += P^T dO, dK += dS^T Q    P^T over S^T's columns, dS^T over dP^T's
-// An operand computed here needs its scale before its largest value is known:
-// P <= 1 and |dP - delta| <= |dout row| |v row| + |delta| (norms) bound dS; it
+// blocks of Q and dO of every head of the group.
+//   S^T = K Q^T, dP^T = V dO^T,  dV += P^T dO, dK += dS^T Q
+// with P = exp2(S f - lse2), computed operands in tensor memory.
+//
+// The products of a step wait for each other through the registers (S -> P -> dV,
+// dP -> dS -> dK), 1000 to 1800 cycles each way, so scores are issued a step
+// ahead where tensor memory has the room; the layouts below say where that is.
+//
+// A computed operand needs its scale before its largest value is known: P <= 1
+// and |dP - delta| <= |dout row| |v row| + |delta| (norms) bound dS; it
 // overestimates by some bits of the 39 there are (a row of 2^14 keys with equal
 // weights keeps 21 bits of each dS).
 #include <algorithm>
@@ -53,47 +57,18 @@ __device__ __forceinline__ float bound_scale(float bound) {
   return __uint_as_float((uint32_t)(268 - min(max(e, 41), 254)) << 23);
 }
 
-// The largest of a row's two halves; `xch` is [2][128].
-__device__ __forceinline__ float row_max(float v, float* xch, int half, int row, int id) {
-  xch[half * 128 + row] = v;
-  pair_sync(id);
-  v = fmaxf(v, xch[(half ^ 1) * 128 + row]);
-  pair_sync(id);
-  return v;
-}
-
-// A row's half from an area into tensor memory; returns its scale's exponent and, with `norm`, the row's norm.
-template <int DP>
-__device__ __forceinline__ int stay_row(const uint8_t* area, int half, int row, bool negate, uint32_t taddr, float* xch,
-                                        int id, float* norm) {
-  float x[DP / 2];
-  const float t = __uint_as_float(half_from_area<DP>(x, area, row, half));
-  const int e = (int)(__float_as_uint(row_max(t, xch, half, row, id)) >> 23);
-  const float f = scale_of(e);
-  if (norm) {
-    float n = 0.0f;
-#pragma unroll
-    for (int c = 0; c < DP / 2; ++c) n = fmaf(x[c] * f, x[c] * f, n);
-    xch[half * 128 + row] = n;
-    pair_sync(id);
-    *norm = sqrtf(n + xch[(half ^ 1) * 128 + row]) * inverse_of(e);
-    pair_sync(id);
-  }
-  row_half_store<DP>(x, negate ? -f : f, taddr, half);
-  return e;
-}
 
 // acc += part * factor for this thread's DP/2 columns of a tensor-memory sum.
 template <int DP>
 __device__ __forceinline__ void drain(float (&acc)[DP / 2], uint32_t taddr, float factor) {
   const float2 f2 = make_float2(factor, factor);
 #pragma unroll
-  for (int c = 0; c < DP / 2; c += 16) {
-    uint32_t r[16];
-    jxd::tmem_ld16(taddr + c, r);
+  for (int c = 0; c < DP / 2; c += 32) {
+    uint32_t r[32];
+    jxd::tmem_ld32(taddr + c, r);
     jxd::tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < 16; i += 2) {
+    for (int i = 0; i < 32; i += 2) {
       const float2 v = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2,
                             make_float2(acc[c + i], acc[c + i + 1]));
       acc[c + i] = v.x;
@@ -102,22 +77,82 @@ __device__ __forceinline__ void drain(float (&acc)[DP / 2], uint32_t taddr, floa
   }
 }
 
+// A tile of 128 columns from shared memory into tensor memory: hi in 64 columns,
+// lo in the next 64; this thread has half of row `row`.
+__device__ __forceinline__ void tile_to_tmem(const uint8_t* tile, int row, int half, uint32_t taddr) {
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const uint8_t* p = tile + part * tile_part(128) + half * PANEL + row * 128;
+    uint32_t r[32];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + ((c ^ (row & 7)) << 4));
+      r[4 * c] = x.x;
+      r[4 * c + 1] = x.y;
+      r[4 * c + 2] = x.z;
+      r[4 * c + 3] = x.w;
+    }
+    tmem_st32(taddr + part * 64 + half * 32, r);
+  }
+}
+
+// Scores: D[128 x N] = A B^T over DP columns, small parts first.  A's tile lies in
+// tensor memory at `a` (TS), or in shared memory at `a`; B's has `panel` bytes a
+// panel and `part` a part.
+template <int DP, int N, bool TS>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, uint32_t panel, uint32_t part) {
+  constexpr uint32_t id = idesc_f16(N, false);
+  auto step = [&](int ks, bool a_lo, bool b_lo, uint32_t acc) {
+    const uint64_t bd = jxd::smem_desc_k_sw128(b + (b_lo ? part : 0) + (ks >> 2) * panel + (ks & 3) * 32);
+    if constexpr (TS) {
+      mma_f16_ts(d, a + (a_lo ? DP / 2 : 0) + ks * 8, bd, id, acc);
+    } else {
+      mma_f16_ss(d, jxd::smem_desc_k_sw128(a + (a_lo ? tile_part(DP) : 0) + (ks >> 2) * PANEL + (ks & 3) * 32), bd, id,
+                 acc);
+    }
+  };
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    step(ks, true, false, ks > 0);
+    step(ks, false, true, 1);
+  }
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) step(ks, false, false, 1);
+}
+
+// Sums: D[128 x DP] = A B over ROWS rows of B; A in tensor memory, 16 columns of
+// hi and 16 of lo for every 32 rows.
+template <int DP, int ROWS>
+__device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b, uint32_t panel, uint32_t part) {
+  constexpr uint32_t id = idesc_f16(DP, true);
+  auto step = [&](int ks, bool a_lo, bool b_lo, uint32_t acc) {
+    mma_f16_ts(d, a + (ks >> 1) * 32 + (ks & 1) * 8 + (a_lo ? 16 : 0),
+               smem_desc_mn_sw128(b + (b_lo ? part : 0) + ks * 2048, panel), id, acc);
+  };
+#pragma unroll
+  for (int ks = 0; ks < ROWS / 16; ++ks) {
+    step(ks, true, false, ks > 0);
+    step(ks, false, true, 1);
+  }
+#pragma unroll
+  for (int ks = 0; ks < ROWS / 16; ++ks) step(ks, false, false, 1);
+}
+
 // ---- dq ------------------------------------------------------------------------
-// Tensor memory: Q, dO, X (scores), Y (dP) and the sum's part D.  At DP = 128 the
-// first four fill it: dS goes over X and D over Y, and S(j+1) has to wait for
-// dS(j) K.  At DP = 64 D has its own columns: dS goes over Y, and S(j+1) runs
-// while dS(j) is computed.
+// Tensor memory at DP = 128: Q and dO (from shared memory they would not leave room
+// for K and V), X for S, then dS, and Y for dP, then the sum's part D: S(j+1)
+// follows dS(j) K.  At DP = 64 Q and dO stay in shared memory, S alternates
+// between two X, dS goes over its S and D has its own columns: S runs two tiles
+// ahead and dP one.
 template <int DP>
 struct DqLayout {
   static constexpr bool AHEAD = DP == 64;
-  static constexpr uint32_t Q = 0, DO = AHEAD ? 64 : 128, X = AHEAD ? 128 : 256, Y = AHEAD ? 256 : 384;
-  static constexpr uint32_t DS = AHEAD ? Y : X, D = AHEAD ? 384 : Y;
+  static constexpr int KS = AHEAD ? 3 : 2, VS = AHEAD ? 2 : 1;  // stages
+  static constexpr uint32_t Q = 0, DO = 128;                    // DP = 128
+  static constexpr uint32_t X = AHEAD ? 0 : 256, X_STEP = AHEAD ? 128 : 0, Y = AHEAD ? 256 : 384, D = 384;
+  static constexpr int STAY = AHEAD ? 2 * tile_bytes(DP) : 0;   // shared memory for Q and dO
+  static constexpr size_t SMEM = STAY + (size_t)(KS + VS) * tile_bytes(DP) + 1024 + 256;
 };
-__host__ __device__ constexpr int dq_k_stages(int DP) { return DP == 128 ? 2 : 3; }
-__host__ __device__ constexpr int dq_v_stages(int DP) { return DP == 128 ? 1 : 2; }
-__host__ __device__ constexpr size_t dq_smem(int DP) {
-  return (size_t)(dq_k_stages(DP) + dq_v_stages(DP)) * tile_bytes(DP) + 1024 + 2 * 128 * 4 + 256;
-}
 
 template <int DP>
 __global__ void __launch_bounds__(BW_THREADS, 1)
@@ -125,23 +160,23 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                    const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
                    const float* __restrict__ lse, const float* __restrict__ dout, float* dq) {
   using L = DqLayout<DP>;
-  constexpr int KS = dq_k_stages(DP), VS = dq_v_stages(DP), STAGE = tile_bytes(DP), PART = tile_part(DP);
+  constexpr int KS = L::KS, VS = L::VS, STAGE = tile_bytes(DP), PART = tile_part(DP);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  float* xch = reinterpret_cast<float*>(smem + (KS + VS) * STAGE);
-  uint64_t* kfull = reinterpret_cast<uint64_t*>(xch + 2 * 128);
+  uint8_t* ring = smem + L::STAY;  // K's stages, then V's
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(ring + (KS + VS) * STAGE);
   uint64_t* kempty = kfull + KS;
   uint64_t* vfull = kempty + KS;
   uint64_t* vempty = vfull + VS;
-  uint64_t* stayfull = vempty + VS;
-  uint64_t* sfull = stayfull + 1;
-  uint64_t* dpfull = sfull + 1;
+  uint64_t* stayfull = vempty + VS;  // Q's and dO's tiles have landed
+  uint64_t* moved = stayfull + 1;    // and are in tensor memory (DP = 128)
+  uint64_t* sfull = moved + 1;       // [2]
+  uint64_t* dpfull = sfull + 2;
   uint64_t* dsfull = dpfull + 1;
   uint64_t* dqfull = dsfull + 1;
   uint64_t* dfree = dqfull + 1;  // D is drained
-  uint64_t* xfree = dfree + 1;   // X is read
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(xfree + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dfree + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -155,18 +190,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const int nb = (sq.visible(i0 + rows - 1, s.causal) + TILE - 1) / TILE;
   const long long slot0 = (long long)first_tile(sq.k0, b) * s.kv_heads + hk;
   const long long qslot = ((long long)first_tile(sq.q0, b) + jt) * s.heads + h;
-
   const long long hd = (long long)h * s.dim;
-  // Q passes through K's last stage, dout through V's last one; the copies for the first stages start at once
-  uint8_t *area_q = smem + (KS - 1) * STAGE, *area_d = smem + (KS + VS - 1) * STAGE;
+
+  // at DP = 128 Q passes through K's last stage, dO through V's
+  uint8_t* at_q = L::AHEAD ? smem : ring + (KS - 1) * STAGE;
+  uint8_t* at_d = L::AHEAD ? smem + STAGE : ring + (KS + VS - 1) * STAGE;
+  constexpr int K_FIRST = L::AHEAD ? KS : KS - 1, V_FIRST = L::AHEAD ? VS : VS - 1;  // stages that are free at once
   auto copy_k = [&](int j) {
     jxd::mbar_arrive_expect_tx(&kfull[j % KS], STAGE);
-    bulk_load(jxd::smem_u32(smem + j % KS * STAGE), bt.k + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
+    bulk_load(jxd::smem_u32(ring + j % KS * STAGE), bt.k + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
               &kfull[j % KS]);
   };
   auto copy_v = [&](int j) {
     jxd::mbar_arrive_expect_tx(&vfull[j % VS], STAGE);
-    bulk_load(jxd::smem_u32(smem + (KS + j % VS) * STAGE), bt.v + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
+    bulk_load(jxd::smem_u32(ring + (KS + j % VS) * STAGE), bt.v + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
               &vfull[j % VS]);
   };
   bool bad = false;
@@ -179,30 +216,31 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       jxd::mbar_init(&vfull[i], 1);
       jxd::mbar_init(&vempty[i], 1);
     }
-    jxd::mbar_init(stayfull, 8);
-    jxd::mbar_init(sfull, 1);
+    jxd::mbar_init(stayfull, 1);
+    jxd::mbar_init(moved, 8);
+    jxd::mbar_init(&sfull[0], 1);
+    jxd::mbar_init(&sfull[1], 1);
     jxd::mbar_init(dpfull, 1);
     jxd::mbar_init(dsfull, 8);
     jxd::mbar_init(dqfull, 1);
     jxd::mbar_init(dfree, 8);
-    jxd::mbar_init(xfree, 8);
     *abort_flag = 0;
     jxd::fence_mbar_init();
     jxd::fence_proxy_async_smem();
-    if (nb > 0) copy_k(0);
+    if (nb > 0) {
+      jxd::mbar_arrive_expect_tx(stayfull, 2 * STAGE);
+      bulk_load(jxd::smem_u32(at_q), bt.q + qslot * STAGE, STAGE, stayfull);
+      copy_k(0);
+      bulk_load(jxd::smem_u32(at_d), bt.d + qslot * STAGE, STAGE, stayfull);
+      for (int j = 1; j < min(nb, K_FIRST); ++j) copy_k(j);
+      for (int j = 0; j < min(nb, V_FIRST); ++j) copy_v(j);
+    }
   } else if (warp == 1) {
     jxd::tmem_alloc(tmem_slot, 512);
     jxd::tmem_relinquish();
-  } else if (warp >= BW_FIRST) {
-    const int tid = threadIdx.x - 32 * BW_FIRST;
-    float4 f[DP / 8], g[DP / 8];
-    rows_load<DP>(f, q + (sq.q0 + i0) * s.ldq + hd, s.ldq, rows, s.dim, aligned16(q, s.dim, s.ldq), tid);
-    rows_load<DP>(g, dout + (sq.q0 + i0) * s.ldo + hd, s.ldo, rows, s.dim, aligned16(dout, s.dim, s.ldo), tid);
-    rows_to_area<DP>(area_q, f, tid);
-    rows_to_area<DP>(area_d, g, tid);
   } else if (warp >= 2) {
     if (threadIdx.x == 64) bad = bt.bad_q[qslot] || bt.bad_d[qslot];
-    for (int j = (int)threadIdx.x - 64; j < nb; j += 64)
+    for (int j = (int)threadIdx.x - 64; j < nb; j += BW_THREADS - 64)
       bad = bad || bt.bad_k[slot0 + (long long)j * s.kv_heads] || bt.bad_v[slot0 + (long long)j * s.kv_heads];
   }
   jxd::tc_fence_before();
@@ -217,7 +255,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
              o + t * s.ldo + hd, dout + t * s.ldo + hd, lse[(long long)h * s.total_q + t], dq + t * s.ldq + hd,
              sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv, s.scale);
     }
-    if (warp == 0 && lane == 0 && nb > 0) wait_bounded(&kfull[0], 0, s.err);  // the copy has landed
+    if (warp == 0 && lane == 0 && nb > 0) {  // the copies have landed
+      wait_bounded(stayfull, 0, s.err);
+      for (int j = 0; j < min(nb, K_FIRST); ++j) wait_bounded(&kfull[j], 0, s.err);
+      for (int j = 0; j < min(nb, V_FIRST); ++j) wait_bounded(&vfull[j], 0, s.err);
+    }
     if (warp == 1) {
       __syncwarp();
       jxd::tmem_dealloc(tmem, 512);
@@ -227,42 +269,32 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 
   if (warp < BW_FIRST) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
-    if (warp == 0 && jxd::elect_one()) {
-      int j = 0, nv = 0;
-      bool ok = wait_bounded(stayfull, 0, s.err);  // the areas are free again
-      for (; ok && j < nb; ++j) {
-        if (j > 0) {
-          if (!(ok = !*abort_flag && wait_bounded(&kempty[j % KS], (uint32_t)(j / KS + 1) & 1u, s.err))) break;
-          copy_k(j);
+    if (warp == 0 && nb > 0 && jxd::elect_one()) {
+      // ---- the remaining copies
+      int nk = min(nb, K_FIRST), nv = min(nb, V_FIRST);
+      bool ok = L::AHEAD || wait_bounded(moved, 0, s.err);  // the stages that Q and dO passed through are free
+      auto free_stage = [&](uint64_t* bar, int use) {
+        return ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)(use + 1) & 1u, s.err);
+      };
+      while (ok && (nk < nb || nv < nb)) {
+        if (nv < nb && nv < nk) {
+          if (!free_stage(&vempty[nv % VS], nv / VS)) break;
+          copy_v(nv++);
+        } else {
+          if (!free_stage(&kempty[nk % KS], nk / KS)) break;
+          copy_k(nk++);
         }
-        if (!(ok = !*abort_flag && wait_bounded(&vempty[j % VS], (uint32_t)(j / VS + 1) & 1u, s.err))) { ++j; break; }
-        copy_v(j);
-        ++nv;
       }
-      if (!ok) j = max(j, min(nb, 1));  // the first K is under way in any case
-      if (nv < nb) *abort_flag = 1;
+      if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may end
-      for (int u = max(0, j - KS); u < j; ++u) wait_bounded(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
+      wait_bounded(stayfull, 0, s.err);
+      for (int u = max(0, nk - KS); u < nk; ++u) wait_bounded(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
       for (int u = max(0, nv - VS); u < nv; ++u) wait_bounded(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err);
     }
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
-      constexpr uint32_t id_s = idesc_f16(128, false), id_o = idesc_f16(DP, true);
-      const uint32_t sbase = jxd::smem_u32(smem);
-      bool ok = wait_bounded(stayfull, 0, s.err);
-      // 128 x 128 scores of a row operand in tensor memory and a streamed tile
-      auto scores = [&](uint32_t d, uint32_t a0, uint32_t tile) {
-        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
-          mma_f16_ts(d, a0 + a + ks * 8, jxd::smem_desc_k_sw128(tile + part + (ks >> 2) * PANEL + (ks & 3) * 32), id_s,
-                     acc);
-        };
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          step(ks, DP / 2, 0, ks > 0);
-          step(ks, 0, PART, 1);
-        }
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
-      };
+      // ---- MMA
+      const uint32_t kbase = jxd::smem_u32(ring), vbase = kbase + KS * STAGE;
+      bool ok = wait_bounded(L::AHEAD ? stayfull : moved, 0, s.err);
       auto ready = [&](uint64_t* bar, int n) {
         ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)n & 1u, s.err);
         jxd::tc_fence_after();
@@ -270,51 +302,61 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       };
       auto q_scores = [&](int j) {
         if (!ready(&kfull[j % KS], j / KS)) return;
-        if (L::AHEAD && j > 0 && !ready(xfree, j - 1)) return;
-        scores(tmem + L::X, tmem + L::Q, sbase + (j % KS) * STAGE);
-        jxd::mma_commit(sfull);
+        mma_scores<DP, 128, !L::AHEAD>(tmem + L::X + (j & 1) * L::X_STEP, L::AHEAD ? jxd::smem_u32(at_q) : tmem + L::Q,
+                                       kbase + (j % KS) * STAGE, PANEL, PART);
+        jxd::mma_commit(&sfull[j & 1]);
       };
-      q_scores(0);
-      for (int j = 0; ok && j < nb; ++j) {
-        if (!ready(&vfull[j % VS], j / VS)) break;
-        if (!L::AHEAD && !ready(dfree, j + 1)) break;  // D is Y
-        scores(tmem + L::Y, tmem + L::DO, sbase + (KS + j % VS) * STAGE);
+      auto d_scores = [&](int j) {
+        if (!ready(&vfull[j % VS], j / VS)) return;
+        mma_scores<DP, 128, !L::AHEAD>(tmem + L::Y, L::AHEAD ? jxd::smem_u32(at_d) : tmem + L::DO,
+                                       vbase + (j % VS) * STAGE, PANEL, PART);
         jxd::mma_commit(dpfull);
         jxd::mma_commit(&vempty[j % VS]);
-        if (L::AHEAD && j + 1 < nb) q_scores(j + 1);
+      };
+      q_scores(0);
+      if (L::AHEAD && nb > 1) q_scores(1);
+      d_scores(0);
+      for (int j = 0; ok && j < nb; ++j) {
         if (!ready(dsfull, j)) break;
+        if (L::AHEAD && j + 1 < nb) d_scores(j + 1);    // Y is read
         if (L::AHEAD && !ready(dfree, j + 1)) break;
-        const uint32_t kt = sbase + (j % KS) * STAGE;
-        auto step = [&](int ks, uint32_t a, uint32_t part, uint32_t acc) {
-          mma_f16_ts(tmem + L::D, tmem + L::DS + a + (ks >> 1) * 32 + (ks & 1) * 8,
-                     smem_desc_mn_sw128(kt + part + ks * 2048, PANEL), id_o, acc);
-        };
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          step(ks, 16, 0, ks > 0);
-          step(ks, 0, PART, 1);
-        }
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) step(ks, 0, 0, 1);
+        mma_sums<DP, 128>(tmem + L::D, tmem + L::X + (j & 1) * L::X_STEP, kbase + (j % KS) * STAGE, PANEL, PART);
         jxd::mma_commit(dqfull);
         jxd::mma_commit(&kempty[j % KS]);
-        if (!L::AHEAD && j + 1 < nb) q_scores(j + 1);
+        if (L::AHEAD) {
+          if (j + 2 < nb) q_scores(j + 2);
+        } else if (j + 1 < nb) {
+          q_scores(j + 1);
+          if (!ready(dfree, j)) break;  // D is Y
+          d_scores(j + 1);
+        }
       }
       if (!ok) *abort_flag = 1;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_HIGH_REGS));
-    const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane, bar = 1 + quarter;
+    const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    float norm_d;
-    const int e_q = stay_row<DP>(area_q, half, row, s.scale < 0.0f, tmem + lanes + L::Q, xch, bar, nullptr);
-    const int e_d = stay_row<DP>(area_d, half, row, false, tmem + lanes + L::DO, xch, bar, &norm_d);
-    tmem_st_wait();
-    jxd::fence_proxy_async_smem();  // the areas become copies' destinations
-    jxd::tc_fence_before();
-    __syncwarp();
-    if (lane == 0) jxd::mbar_arrive(stayfull);
-    const float f_row = inverse_of(e_q) * (fabsf(s.scale) * LOG2E), inv_d = inverse_of(e_d);
+    bool ok = true;
+    auto ready = [&](uint64_t* bar, int n) {
+      ok = ok && warp_wait(bar, (uint32_t)n & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+    };
+    auto done = [&](uint64_t* bar) {
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(bar);
+    };
+    if (!L::AHEAD && nb > 0) {
+      ready(stayfull, 0);
+      if constexpr (!L::AHEAD) {
+        tile_to_tmem(at_q, row, half, tmem + lanes + L::Q);
+        tile_to_tmem(at_d, row, half, tmem + lanes + L::DO);
+      }
+      tmem_st_wait();
+      done(moved);
+    }
+    const float f_tile = bt.inv_q[qslot] * (s.scale * LOG2E), inv_d = bt.inv_d[qslot], norm_d = bt.norm_d[qslot];
     const float lse2 = bt.lse2[qslot * TILE + row], delta = bt.delta[qslot * TILE + row];
     const int vis = row < rows ? sq.visible(i0 + row, s.causal) : 0;
     const int vis_all = sq.visible(i0, s.causal);
@@ -323,31 +365,23 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
     for (int c = 0; c < DP / 2; ++c) acc[c] = 0.0f;
     float g_prev = 0.0f;
-    bool ok = true;
-    auto done = [&](uint64_t* b8) {
-      jxd::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) jxd::mbar_arrive(b8);
-    };
-    auto add_part = [&](int j) {
-      ok = ok && warp_wait(dqfull, (uint32_t)j & 1u, abort_flag, s.err);
-      jxd::tc_fence_after();
-      drain<DP>(acc, tmem + lanes + L::D + half * (DP / 2), g_prev);
-      done(dfree);
-    };
-    for (int j = 0; j < nb; ++j) {
+    float2 p[32];
+    // P of tile j, scaled for dS, and what undoes dS's scale
+    float dl = 0.0f, g = 0.0f;
+    auto weights = [&](int j) {
       const long long slot = slot0 + (long long)j * s.kv_heads;
       const float inv_k = bt.inv_k[slot], inv_v = bt.inv_v[slot], norm_v = bt.norm_v[slot];
-      if (!L::AHEAD && j > 0) add_part(j - 1);
-      ok = ok && warp_wait(sfull, (uint32_t)j & 1u, abort_flag, s.err);
-      jxd::tc_fence_after();
-      const float f = f_row * inv_k;
-      const float2 f2 = make_float2(f, f), l2 = make_float2(-lse2, -lse2);
-      float2 p[32];
+      // P is at most 2^14
+      const float fd = inv_d * inv_v, sc = bound_scale(16384.0f * (norm_d * norm_v + fabsf(delta)));
+      const float f = f_tile * inv_k, pf = sc * fd;
+      dl = -delta * inverse_pow2(fd);
+      g = inv_k * inverse_pow2(sc) * 6.103515625e-05f;  // P's 2^14
+      const float2 f2 = make_float2(f, f), l2 = make_float2(-lse2, -lse2), pf2 = make_float2(pf, pf);
+      ready(&sfull[j & 1], j >> 1);
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t r[32];
-        jxd::tmem_ld32(tmem + lanes + L::X + half * 64 + c, r);
+        jxd::tmem_ld32(tmem + lanes + L::X + (j & 1) * L::X_STEP + half * 64 + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -355,7 +389,6 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           p[(c + i) / 2] = make_float2(exp2_fast(z.x), exp2_fast(z.y));
         }
       }
-      if (L::AHEAD) done(xfree);
       if (j * TILE + TILE > vis_all) {  // some row does not see all of the tile's keys
         const int key0 = j * TILE + half * 64;
 #pragma unroll
@@ -364,15 +397,23 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           if (key0 + 2 * i + 1 >= vis) p[i].y = 0.0f;
         }
       }
-      // P is at most 2^14
-      const float fd = inv_d * inv_v, sc = bound_scale(16384.0f * (norm_d * norm_v + fabsf(delta)));
-      const float pf = sc * fd, dl = -delta * inverse_pow2(fd);
-      const float2 pf2 = make_float2(pf, pf), one2 = make_float2(1.0f, 1.0f), dl2 = make_float2(dl, dl);
 #pragma unroll
       for (int i = 0; i < 32; ++i) p[i] = mul2(p[i], pf2);
-      if (L::AHEAD && j > 0) add_part(j - 1);
-      ok = ok && warp_wait(dpfull, (uint32_t)j & 1u, abort_flag, s.err);
-      jxd::tc_fence_after();
+    };
+    auto add_part = [&](int j) {
+      ready(dqfull, j);
+      drain<DP>(acc, tmem + lanes + L::D + half * (DP / 2), g_prev);
+      done(dfree);
+    };
+    if (L::AHEAD && nb > 0) weights(0);
+    for (int j = 0; j < nb; ++j) {
+      if (!L::AHEAD) {
+        if (j > 0) add_part(j - 1);
+        weights(j);
+      }
+      ready(dpfull, j);
+      const float2 one2 = make_float2(1.0f, 1.0f), dl2 = make_float2(dl, dl);
+      const uint32_t ds = tmem + lanes + L::X + (j & 1) * L::X_STEP + half * 64;
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         uint32_t r[32], hi[16], lo[16];
@@ -381,15 +422,21 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float2 e = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), one2, dl2);
-          const float2 ds = mul2(p[c / 2 + i], e);
-          split_half(ds.x, ds.y, hi[i], lo[i]);
+          const float2 x = mul2(p[c / 2 + i], e);
+          split_half(x.x, x.y, hi[i], lo[i]);
         }
-        tmem_st16(tmem + lanes + L::DS + half * 64 + c, hi);
-        tmem_st16(tmem + lanes + L::DS + half * 64 + c + 16, lo);
+        tmem_st16(ds + c, hi);
+        tmem_st16(ds + c + 16, lo);
       }
       tmem_st_wait();
       done(dsfull);
-      g_prev = inv_k * inverse_pow2(sc) * 6.103515625e-05f;  // P's 2^14
+      if (L::AHEAD) {
+        if (j > 0) add_part(j - 1);
+        g_prev = g;
+        if (j + 1 < nb) weights(j + 1);
+      } else {
+        g_prev = g;
+      }
     }
     if (nb > 0) add_part(nb - 1);
     // every MMA has retired: the stages are free
@@ -408,23 +455,27 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 }
 
 // ---- dk, dv --------------------------------------------------------------------
-// Query rows per step: 128 at DP = 64, where the parts of dV and dK have columns of
-// their own (Z and W); 64 at DP = 128, where they share Z.  (An MMA of 64 columns
-// takes 45 cycles where half of one of 128 would be 32.)
+// DP = 64: blocks of 128 query rows, K and V in shared memory; two X for S^T, Y
+// for dP^T (dS^T over it), the parts of dV and dK in Z and W:
+//   S(u+1), dV(u), dK(u), dP(u+1)
+// DP = 128: blocks of 64 rows, K in shared memory, V in tensor memory; two X, two
+// Y, and Z for both sums' parts, each drained while the scores after it run:
+//   dV(u), dP(u+1), dK(u), S(u+2)
+// (An MMA of 64 columns takes 45 cycles where half of one of 128 would be 32, which
+// is what the block of 64 rows costs.)
 template <int DP>
 struct KvLayout {
   static constexpr bool APART = DP == 64;
   static constexpr int BLK = APART ? 128 : 64;
-  static constexpr uint32_t K = 0, V = APART ? 64 : 128, X = APART ? 128 : 256, Y = APART ? 256 : 320, Z = 384,
-                            W = APART ? 448 : 384;
-  static constexpr int PANEL_BYTES = BLK * 128;             // of a block
-  static constexpr int STAGE = DP / 64 * 2 * PANEL_BYTES;   // one block of Q or of dout: 32 KB
+  static constexpr int QS = 3, DS = 2;  // stages of Q and of dout
+  static constexpr uint32_t V = 0;      // DP = 128
+  static constexpr uint32_t X = APART ? 0 : 128, X_STEP = BLK, Y = 256, Y_STEP = APART ? 0 : BLK;
+  static constexpr uint32_t Z = 384, W = APART ? 448 : 384;
+  static constexpr int PANEL_BYTES = BLK * 128;                                    // of a block
+  static constexpr int STAGE = DP / 64 * 2 * PANEL_BYTES;                          // one block: 32 KB
+  static constexpr int STAY = APART ? 2 * tile_bytes(DP) : tile_bytes(DP);         // shared memory for K (and V)
+  static constexpr size_t SMEM = STAY + (size_t)(QS + DS) * STAGE + 1024 + 256;
 };
-constexpr int KV_STAGES = 3;  // of Q and of dout each
-__host__ __device__ constexpr size_t kv_smem(int DP) {
-  return (size_t)2 * KV_STAGES * (DP == 64 ? KvLayout<64>::STAGE : KvLayout<128>::STAGE) + 1024 +
-         KV_STAGES * 1024 /*lse2, delta*/ + 2 * 128 * 4 + 256;
-}
 
 template <int DP>
 __global__ void __launch_bounds__(BW_THREADS, 1)
@@ -432,22 +483,22 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
                     const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
                     const float* __restrict__ lse, const float* __restrict__ dout, float* dk, float* dv) {
   using L = KvLayout<DP>;
-  constexpr int ST = KV_STAGES, BLK = L::BLK, STAGE = L::STAGE, PART = STAGE / 2, HPANEL = L::PANEL_BYTES;
+  constexpr int QS = L::QS, DS = L::DS, BLK = L::BLK, STAGE = L::STAGE, PART = STAGE / 2, HPANEL = L::PANEL_BYTES;
   constexpr int PER_TILE = TILE / BLK;  // blocks of a tile
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  float* stats = reinterpret_cast<float*>(smem + 2 * ST * STAGE);  // [ST][lse2 BLK, delta BLK]
-  float* xch = stats + ST * 2 * BLK;
-  uint64_t* qfull = reinterpret_cast<uint64_t*>(xch + 2 * 128);
-  uint64_t* qempty = qfull + ST;
-  uint64_t* dfull = qempty + ST;
-  uint64_t* dempty = dfull + ST;
-  uint64_t* stayfull = dempty + ST;
-  uint64_t* sfull = stayfull + 1;
-  uint64_t* pfull = sfull + 1;
-  uint64_t* dpfull = pfull + 1;
-  uint64_t* dsfull = dpfull + 1;
+  uint8_t* ring = smem + L::STAY;  // Q's stages, then dout's
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(ring + (QS + DS) * STAGE);
+  uint64_t* qempty = qfull + QS;
+  uint64_t* dfull = qempty + QS;
+  uint64_t* dempty = dfull + DS;
+  uint64_t* stayfull = dempty + DS;  // K's and V's tiles have landed
+  uint64_t* moved = stayfull + 1;    // V's is in tensor memory (DP = 128)
+  uint64_t* sfull = moved + 1;       // [2]
+  uint64_t* dpfull = sfull + 2;      // [2]
+  uint64_t* pfull = dpfull + 2;
+  uint64_t* dsfull = pfull + 1;
   uint64_t* zfull = dsfull + 1;
   uint64_t* zfree = zfull + 1;  // dV's part
   uint64_t* wfull = zfree + 1;  // dK's
@@ -469,7 +520,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const int blk0 = sq.first_row(j0, s.causal) / BLK;
   const int nblk = max(0, (sq.lq + BLK - 1) / BLK - blk0);
   const long long steps = (long long)s.group * nblk;
-  const int it0 = (int)(steps * part / bt.parts), it1 = (int)(steps * (part + 1) / bt.parts);
+  const int it0 = (int)(steps * part / bt.parts), n = (int)(steps * (part + 1) / bt.parts) - it0;
   const long long qslot0 = (long long)first_tile(sq.q0, b) * s.heads + (long long)hk * s.group;
   const long long kslot = ((long long)first_tile(sq.k0, b) + jt) * s.kv_heads + hk;
   const int h0 = hk * s.group;
@@ -480,43 +531,49 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const long long ld_k = bt.parts > 1 ? (long long)s.kv_heads * s.dim : s.ldk;
   const long long ld_v = bt.parts > 1 ? (long long)s.kv_heads * s.dim : s.ldv;
 
-  const int n = it1 - it0;
-  // K passes through the last stages of Q's ring, V through those of dout's; the first stages' copies start at once
-  constexpr int AREA_STAGES = area_bytes(DP) / STAGE;
-  uint8_t *area_k = smem + (ST - AREA_STAGES) * STAGE, *area_v = smem + (2 * ST - AREA_STAGES) * STAGE;
+  // at DP = 128 V passes through Q's last two stages
+  uint8_t* at_v = L::APART ? smem + tile_bytes(DP) : ring + (QS - 2) * STAGE;
+  constexpr int Q_FIRST = L::APART ? QS : QS - 2;  // stages that are free at once
+  // step u's block, as its tile's slot and its place in the tile
+  auto slot_of = [&](int u, int* place) {
+    const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk;
+    *place = blk % PER_TILE;
+    return qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
+  };
   // a block: its rows of each part's panels
-  auto load = [&](uint8_t* dst, const uint8_t* tile, int hb, uint64_t* bar) {
+  auto load = [&](uint8_t* dst, const uint8_t* tile, int place, uint64_t* bar) {
+    jxd::mbar_arrive_expect_tx(bar, STAGE);
 #pragma unroll
     for (int e = 0; e < 2 * (DP / 64); ++e)
-      bulk_load(jxd::smem_u32(dst + e * HPANEL), tile + (long long)e * PANEL + hb * HPANEL, HPANEL, bar);
+      bulk_load(jxd::smem_u32(dst + e * HPANEL), tile + (long long)e * PANEL + place * HPANEL, HPANEL, bar);
   };
   auto copy_q = [&](int u) {
-    const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
-    const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
-    jxd::mbar_arrive_expect_tx(&qfull[st], STAGE + 2 * BLK * 4);
-    load(smem + st * STAGE, bt.q + slot * tile_bytes(DP), blk % PER_TILE, &qfull[st]);
-    bulk_load(jxd::smem_u32(stats + st * 2 * BLK), bt.lse2 + slot * TILE + blk % PER_TILE * BLK, BLK * 4, &qfull[st]);
-    bulk_load(jxd::smem_u32(stats + st * 2 * BLK + BLK), bt.delta + slot * TILE + blk % PER_TILE * BLK, BLK * 4,
-              &qfull[st]);
+    int place;
+    const long long slot = slot_of(u, &place);
+    load(ring + u % QS * STAGE, bt.q + slot * tile_bytes(DP), place, &qfull[u % QS]);
   };
   auto copy_d = [&](int u) {
-    const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
-    const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
-    jxd::mbar_arrive_expect_tx(&dfull[st], STAGE);
-    load(smem + (ST + st) * STAGE, bt.d + slot * tile_bytes(DP), blk % PER_TILE, &dfull[st]);
+    int place;
+    const long long slot = slot_of(u, &place);
+    load(ring + (QS + u % DS) * STAGE, bt.d + slot * tile_bytes(DP), place, &dfull[u % DS]);
   };
   bool bad = false;
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < QS; ++i) {
       jxd::mbar_init(&qfull[i], 1);
       jxd::mbar_init(&qempty[i], 1);
+    }
+    for (int i = 0; i < DS; ++i) {
       jxd::mbar_init(&dfull[i], 1);
       jxd::mbar_init(&dempty[i], 1);
     }
-    jxd::mbar_init(stayfull, 8);
-    jxd::mbar_init(sfull, 1);
+    jxd::mbar_init(stayfull, 1);
+    jxd::mbar_init(moved, 8);
+    for (int i = 0; i < 2; ++i) {
+      jxd::mbar_init(&sfull[i], 1);
+      jxd::mbar_init(&dpfull[i], 1);
+    }
     jxd::mbar_init(pfull, 8);
-    jxd::mbar_init(dpfull, 1);
     jxd::mbar_init(dsfull, 8);
     jxd::mbar_init(zfull, 1);
     jxd::mbar_init(zfree, 8);
@@ -526,23 +583,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     jxd::fence_mbar_init();
     jxd::fence_proxy_async_smem();
     if (n > 0) {
-      copy_q(0);
-      copy_d(0);
+      jxd::mbar_arrive_expect_tx(stayfull, 2 * tile_bytes(DP));
+      bulk_load(jxd::smem_u32(smem), bt.k + kslot * tile_bytes(DP), tile_bytes(DP), stayfull);
+      bulk_load(jxd::smem_u32(at_v), bt.v + kslot * tile_bytes(DP), tile_bytes(DP), stayfull);
+      for (int u = 0; u < min(n, Q_FIRST); ++u) copy_q(u);
+      for (int u = 0; u < min(n, DS); ++u) copy_d(u);
     }
   } else if (warp == 1) {
     jxd::tmem_alloc(tmem_slot, 512);
     jxd::tmem_relinquish();
-  } else if (warp >= BW_FIRST) {
-    const int tid = threadIdx.x - 32 * BW_FIRST;
-    float4 f[DP / 8], g[DP / 8];
-    rows_load<DP>(f, k + (sq.k0 + j0) * s.ldk + kd, s.ldk, rows, s.dim, aligned16(k, s.dim, s.ldk), tid);
-    rows_load<DP>(g, v + (sq.k0 + j0) * s.ldv + kd, s.ldv, rows, s.dim, aligned16(v, s.dim, s.ldv), tid);
-    rows_to_area<DP>(area_k, f, tid);
-    rows_to_area<DP>(area_v, g, tid);
   } else if (warp >= 2) {
     if (threadIdx.x == 64) bad = bt.bad_k[kslot] || bt.bad_v[kslot];
     const int t0 = blk0 / PER_TILE, nt = nblk > 0 ? (sq.lq + TILE - 1) / TILE - t0 : 0;
-    for (long long e = (int)threadIdx.x - 64; e < (long long)nt * s.group; e += 64) {
+    for (long long e = (int)threadIdx.x - 64; e < (long long)nt * s.group; e += BW_THREADS - 64) {
       const long long slot = qslot0 + (t0 + e / s.group) * s.heads + e % s.group;
       bad = bad || bt.bad_q[slot] || bt.bad_d[slot];
     }
@@ -562,8 +615,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
               s.scale);
     }
     if (warp == 0 && lane == 0 && n > 0) {  // the copies have landed
-      wait_bounded(&qfull[0], 0, s.err);
-      wait_bounded(&dfull[0], 0, s.err);
+      wait_bounded(stayfull, 0, s.err);
+      for (int u = 0; u < min(n, Q_FIRST); ++u) wait_bounded(&qfull[u], 0, s.err);
+      for (int u = 0; u < min(n, DS); ++u) wait_bounded(&dfull[u], 0, s.err);
     }
     if (warp == 1) {
       __syncwarp();
@@ -574,100 +628,104 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 
   if (warp < BW_FIRST) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
-    if (warp == 0 && jxd::elect_one()) {
-      int u = min(n, 1), nd = u;
-      bool ok = wait_bounded(stayfull, 0, s.err);  // the areas are free again
-      for (; ok && u < n; ++u) {
-        if (!(ok = !*abort_flag && wait_bounded(&qempty[u % ST], (uint32_t)(u / ST + 1) & 1u, s.err))) break;
-        copy_q(u);
-        if (!(ok = !*abort_flag && wait_bounded(&dempty[u % ST], (uint32_t)(u / ST + 1) & 1u, s.err))) { ++u; break; }
-        copy_d(u);
-        ++nd;
+    if (warp == 0 && n > 0 && jxd::elect_one()) {
+      // ---- the remaining copies
+      int nq = min(n, Q_FIRST), nd = min(n, DS);
+      bool ok = L::APART || wait_bounded(moved, 0, s.err);  // the stages that V passed through are free
+      auto free_stage = [&](uint64_t* bar, int use) {
+        return ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)(use + 1) & 1u, s.err);
+      };
+      while (ok && (nq < n || nd < n)) {
+        // Q is wanted up to one block earlier than dout
+        if (nd < n && (nq == n || nd + 1 < nq)) {
+          if (!free_stage(&dempty[nd % DS], nd / DS)) break;
+          copy_d(nd++);
+        } else {
+          if (!free_stage(&qempty[nq % QS], nq / QS)) break;
+          copy_q(nq++);
+        }
       }
       if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may end
-      for (int e = max(0, u - ST); e < u; ++e) wait_bounded(&qfull[e % ST], (uint32_t)(e / ST) & 1u, s.err);
-      for (int e = max(0, nd - ST); e < nd; ++e) wait_bounded(&dfull[e % ST], (uint32_t)(e / ST) & 1u, s.err);
+      wait_bounded(stayfull, 0, s.err);
+      for (int e = max(0, nq - QS); e < nq; ++e) wait_bounded(&qfull[e % QS], (uint32_t)(e / QS) & 1u, s.err);
+      for (int e = max(0, nd - DS); e < nd; ++e) wait_bounded(&dfull[e % DS], (uint32_t)(e / DS) & 1u, s.err);
     }
     if (warp == 1 && n > 0 && jxd::elect_one()) {
-      constexpr uint32_t id_s = idesc_f16(BLK, false), id_o = idesc_f16(DP, true);
-      const uint32_t sbase = jxd::smem_u32(smem);
-      bool ok = wait_bounded(stayfull, 0, s.err);
-      auto ready = [&](uint64_t* bar, int u) {
-        return !*abort_flag && wait_bounded(bar, (uint32_t)u & 1u, s.err);
-      };
-      // 128 x BLK scores
-      auto scores = [&](uint32_t d, uint32_t a0, uint32_t tile) {
-        auto step = [&](int ks, uint32_t a, uint32_t p, uint32_t acc) {
-          mma_f16_ts(d, a0 + a + ks * 8, jxd::smem_desc_k_sw128(tile + p + (ks >> 2) * HPANEL + (ks & 3) * 32), id_s,
-                     acc);
-        };
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          step(ks, DP / 2, 0, ks > 0);
-          step(ks, 0, PART, 1);
-        }
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) step(ks, 0, 0, 1);
-      };
-      // 128 x DP sums over the block's rows; a0 holds 16 columns of hi, 16 of lo for every 32 rows
-      auto sums = [&](uint32_t d, uint32_t a0, uint32_t tile) {
-        auto step = [&](int ks, uint32_t a, uint32_t p, uint32_t acc) {
-          mma_f16_ts(d, a0 + a + (ks >> 1) * 32 + (ks & 1) * 8, smem_desc_mn_sw128(tile + p + ks * 2048, HPANEL), id_o,
-                     acc);
-        };
-#pragma unroll
-        for (int ks = 0; ks < BLK / 16; ++ks) {
-          step(ks, 16, 0, ks > 0);
-          step(ks, 0, PART, 1);
-        }
-#pragma unroll
-        for (int ks = 0; ks < BLK / 16; ++ks) step(ks, 0, 0, 1);
+      // ---- MMA
+      const uint32_t qbase = jxd::smem_u32(ring), dbase = qbase + QS * STAGE;
+      bool ok = wait_bounded(stayfull, 0, s.err) && (L::APART || wait_bounded(moved, 0, s.err));
+      auto ready = [&](uint64_t* bar, int i) {
+        ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)i & 1u, s.err);
+        jxd::tc_fence_after();
+        return ok;
       };
       auto q_scores = [&](int u) {
-        if (!ok || !(ok = ready(&qfull[u % ST], u / ST))) return;
-        jxd::tc_fence_after();
-        scores(tmem + L::X, tmem + L::K, sbase + (u % ST) * STAGE);
-        jxd::mma_commit(sfull);
+        if (u >= n || !ready(&qfull[u % QS], u / QS)) return;
+        mma_scores<DP, BLK, false>(tmem + L::X + (u & 1) * L::X_STEP, jxd::smem_u32(smem), qbase + (u % QS) * STAGE,
+                                   HPANEL, PART);
+        jxd::mma_commit(&sfull[u & 1]);
       };
       auto d_scores = [&](int u) {
-        if (!ok || !(ok = ready(&dfull[u % ST], u / ST))) return;
-        jxd::tc_fence_after();
-        scores(tmem + L::Y, tmem + L::V, sbase + (ST + u % ST) * STAGE);
-        jxd::mma_commit(dpfull);
+        if (u >= n || !ready(&dfull[u % DS], u / DS)) return;
+        mma_scores<DP, BLK, !L::APART>(tmem + L::Y + (u & 1) * L::Y_STEP,
+                                       L::APART ? jxd::smem_u32(at_v) : tmem + L::V, dbase + (u % DS) * STAGE, HPANEL,
+                                       PART);
+        jxd::mma_commit(&dpfull[u & 1]);
+      };
+      auto v_sums = [&](int u) {
+        mma_sums<DP, BLK>(tmem + L::Z, tmem + L::X + (u & 1) * L::X_STEP, dbase + (u % DS) * STAGE, HPANEL, PART);
+        jxd::mma_commit(zfull);
+        jxd::mma_commit(&dempty[u % DS]);
+      };
+      auto k_sums = [&](int u) {
+        mma_sums<DP, BLK>(tmem + L::W, tmem + L::Y + (u & 1) * L::Y_STEP, qbase + (u % QS) * STAGE, HPANEL, PART);
+        jxd::mma_commit(wfull);
+        jxd::mma_commit(&qempty[u % QS]);
       };
       q_scores(0);
       d_scores(0);
+      if (!L::APART) q_scores(1);
       for (int u = 0; ok && u < n; ++u) {
-        // the sums' columns are drained: dV's of the step before, and dK's where they share them
-        if (!(ok = ready(pfull, u) && ready(L::APART ? zfree : wfree, u + 1))) break;
-        jxd::tc_fence_after();
-        sums(tmem + L::Z, tmem + L::X, sbase + (ST + u % ST) * STAGE);
-        jxd::mma_commit(zfull);
-        jxd::mma_commit(&dempty[u % ST]);
-        if (u + 1 < n) q_scores(u + 1);
-        if (!ok || !(ok = ready(dsfull, u) && (L::APART ? ready(wfree, u + 1) : ready(zfree, u)))) break;
-        jxd::tc_fence_after();
-        sums(tmem + L::W, tmem + L::Y, sbase + (u % ST) * STAGE);
-        jxd::mma_commit(wfull);
-        jxd::mma_commit(&qempty[u % ST]);
-        if (u + 1 < n) d_scores(u + 1);
+        if constexpr (L::APART) {
+          q_scores(u + 1);  // over P of u-1, which dV(u-1) has read
+          if (!ready(pfull, u) || !ready(zfree, u + 1)) break;
+          v_sums(u);
+          if (!ready(dsfull, u) || !ready(wfree, u + 1)) break;
+          k_sums(u);
+          d_scores(u + 1);
+        } else {
+          if (!ready(pfull, u) || !ready(wfree, u + 1)) break;
+          v_sums(u);
+          d_scores(u + 1);
+          if (!ready(dsfull, u) || !ready(zfree, u)) break;
+          k_sums(u);
+          q_scores(u + 2);
+        }
       }
       if (!ok) *abort_flag = 1;
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BW_HIGH_REGS));
-    const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane, bar = 1 + quarter;
+    const int quarter = warp & 3, half = (warp - BW_FIRST) >> 2, row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    float norm_v;
-    const int e_k = stay_row<DP>(area_k, half, row, s.scale < 0.0f, tmem + lanes + L::K, xch, bar, nullptr);
-    const int e_v = stay_row<DP>(area_v, half, row, false, tmem + lanes + L::V, xch, bar, &norm_v);
-    tmem_st_wait();
-    jxd::fence_proxy_async_smem();  // the areas become copies' destinations
-    jxd::tc_fence_before();
-    __syncwarp();
-    if (lane == 0) jxd::mbar_arrive(stayfull);
-    const float f_row = inverse_of(e_k) * (fabsf(s.scale) * LOG2E), inv_v = inverse_of(e_v);
+    bool ok = true;
+    auto ready = [&](uint64_t* bar, int i) {
+      ok = ok && warp_wait(bar, (uint32_t)i & 1u, abort_flag, s.err);
+      jxd::tc_fence_after();
+    };
+    auto done = [&](uint64_t* bar) {
+      jxd::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) jxd::mbar_arrive(bar);
+    };
+    if (!L::APART && n > 0) {
+      ready(stayfull, 0);
+      if constexpr (!L::APART) tile_to_tmem(at_v, row, half, tmem + lanes + L::V);
+      tmem_st_wait();
+      done(moved);
+    }
+    const float f_tile = bt.inv_k[kslot] * (s.scale * LOG2E), inv_v = bt.inv_v[kslot], norm_v = bt.norm_v[kslot];
     const int first = row < rows ? sq.first_row(j0 + row, s.causal) : 0x7fffffff;  // first query row that sees this key
     const int first_all = sq.first_row(j0 + rows - 1, s.causal);
 
@@ -675,37 +733,29 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 #pragma unroll
     for (int c = 0; c < DP / 2; ++c) ak[c] = av[c] = 0.0f;
     float g_prev = 0.0f;
-    bool ok = true;
-    auto ready = [&](uint64_t* b8, int u) {
-      ok = ok && warp_wait(b8, (uint32_t)u & 1u, abort_flag, s.err);
-      jxd::tc_fence_after();
-    };
-    auto done = [&](uint64_t* b8) {
-      jxd::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) jxd::mbar_arrive(b8);
-    };
     constexpr int C = BLK / 2;  // columns of the scores that this thread has
     for (int u = 0; u < n; ++u) {
-      const int g = (it0 + u) / nblk, blk = blk0 + (it0 + u) % nblk, st = u % ST;
-      const long long slot = qslot0 + (long long)(blk / PER_TILE) * s.heads + g;
+      int place;
+      const long long slot = slot_of(u, &place);
+      const int i0 = (blk0 + (it0 + u) % nblk) * BLK;  // the block's first row
       const float inv_q = bt.inv_q[slot], inv_d = bt.inv_d[slot], norm_d = bt.norm_d[slot], top_d = bt.delta_top[slot];
-      const float* lse2 = stats + st * 2 * BLK + half * C;
-      const float* delta = lse2 + BLK;
-      ready(&qfull[st], u / ST);  // landed before the scores were issued: its statistics are visible here too
-      ready(sfull, u);
-      const float f = f_row * inv_q;
+      const float* lse2 = bt.lse2 + slot * TILE + place * BLK + half * C;
+      const float* delta = bt.delta + slot * TILE + place * BLK + half * C;
+      const uint32_t xa = tmem + lanes + L::X + (u & 1) * L::X_STEP + half * C;
+      const uint32_t ya = tmem + lanes + L::Y + (u & 1) * L::Y_STEP + half * C;
+      const float f = f_tile * inv_q;
       const float2 f2 = make_float2(f, f);
-      const bool edge = blk * BLK < first_all || rows < TILE;  // some key is not seen by all of the block's rows
+      const bool edge = i0 < first_all || rows < TILE;  // some key is not seen by all of the block's rows
       float2 p[C / 2];
+      ready(&sfull[u & 1], u >> 1);
 #pragma unroll
       for (int c = 0; c < C; c += 32) {
         uint32_t r[32];
-        jxd::tmem_ld32(tmem + lanes + L::X + half * C + c, r);
+        jxd::tmem_ld32(xa + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 l = *reinterpret_cast<const float4*>(lse2 + c + i);
+          const float4 l = __ldg(reinterpret_cast<const float4*>(lse2 + c + i));
           const float2 z0 = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2,
                                  make_float2(-l.x, -l.y));
           const float2 z1 = fma2(make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), f2,
@@ -715,11 +765,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         }
       }
       if (edge) {
-        const int i0 = blk * BLK + half * C;
 #pragma unroll
         for (int i = 0; i < C / 2; ++i) {
-          if (i0 + 2 * i < first) p[i].x = 0.0f;
-          if (i0 + 2 * i + 1 < first) p[i].y = 0.0f;
+          if (i0 + half * C + 2 * i < first) p[i].x = 0.0f;
+          if (i0 + half * C + 2 * i + 1 < first) p[i].y = 0.0f;
         }
       }
 #pragma unroll
@@ -727,8 +776,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) split_half(p[c / 2 + i].x, p[c / 2 + i].y, hi[i], lo[i]);
-        tmem_st16(tmem + lanes + L::X + half * C + c, hi);
-        tmem_st16(tmem + lanes + L::X + half * C + c + 16, lo);
+        tmem_st16(xa + c, hi);
+        tmem_st16(xa + c + 16, lo);
       }
       tmem_st_wait();
       done(pfull);
@@ -741,15 +790,15 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const float fd = inv_v * inv_d, sc = bound_scale(16384.0f * (norm_v * norm_d + top_d));
       const float pf = sc * fd, nf = -inverse_pow2(fd);
       const float2 pf2 = make_float2(pf, pf), nf2 = make_float2(nf, nf);
-      ready(dpfull, u);
+      ready(&dpfull[u & 1], u >> 1);
 #pragma unroll
       for (int c = 0; c < C; c += 32) {
         uint32_t r[32], hi[16], lo[16];
-        jxd::tmem_ld32(tmem + lanes + L::Y + half * C + c, r);
+        jxd::tmem_ld32(ya + c, r);
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 d = *reinterpret_cast<const float4*>(delta + c + i);
+          const float4 d = __ldg(reinterpret_cast<const float4*>(delta + c + i));
           const float2 e0 = fma2(make_float2(d.x, d.y), nf2, make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
           const float2 e1 =
               fma2(make_float2(d.z, d.w), nf2, make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])));
@@ -757,8 +806,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
           split_half(a0.x, a0.y, hi[i / 2], lo[i / 2]);
           split_half(a1.x, a1.y, hi[i / 2 + 1], lo[i / 2 + 1]);
         }
-        tmem_st16(tmem + lanes + L::Y + half * C + c, hi);
-        tmem_st16(tmem + lanes + L::Y + half * C + c + 16, lo);
+        tmem_st16(ya + c, hi);
+        tmem_st16(ya + c + 16, lo);
       }
       tmem_st_wait();
       done(dsfull);
@@ -771,14 +820,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       ready(wfull, n - 1);
       drain<DP>(ak, tmem + lanes + L::W + half * (DP / 2), g_prev);
     }
-    // every MMA has retired: the stages are free
+    // every MMA has retired: the tiles' and the stages' memory is free
     const int tid = threadIdx.x - 32 * BW_FIRST;
+    uint8_t* area_v = smem + area_bytes(DP);
     half_to_area<DP>(smem, ak, s.scale, row, half);
-    half_to_area<DP>(smem + ST * STAGE, av, 1.0f, row, half);
+    half_to_area<DP>(area_v, av, 1.0f, row, half);
     movers_sync();
     rows_store<DP>(out_k + (sq.k0 + j0) * ld_k + kd, ld_k, smem, rows, s.dim, aligned16(out_k, s.dim, ld_k), tid);
-    rows_store<DP>(out_v + (sq.k0 + j0) * ld_v + kd, ld_v, smem + ST * STAGE, rows, s.dim,
-                   aligned16(out_v, s.dim, ld_v), tid);
+    rows_store<DP>(out_v + (sq.k0 + j0) * ld_v + kd, ld_v, area_v, rows, s.dim, aligned16(out_v, s.dim, ld_v), tid);
   }
   jxd::tc_fence_before();
   __syncthreads();
@@ -832,13 +881,13 @@ __global__ void __launch_bounds__(256) attn_dkv_join_kernel(const __grid_constan
 template <int DP>
 int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, const float* v, const float* o,
            const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st) {
-  if (int rc = prepare_kernel((const void*)attn_dq_kernel<DP>, DP == 128 ? 2 : 3, dq_smem(DP), BW_LAUNCH_REGS))
+  if (int rc = prepare_kernel((const void*)attn_dq_kernel<DP>, DP == 128 ? 2 : 3, DqLayout<DP>::SMEM, BW_LAUNCH_REGS))
     return rc;
-  if (int rc = prepare_kernel((const void*)attn_dkv_kernel<DP>, DP == 128 ? 4 : 5, kv_smem(DP), BW_LAUNCH_REGS))
+  if (int rc = prepare_kernel((const void*)attn_dkv_kernel<DP>, DP == 128 ? 4 : 5, KvLayout<DP>::SMEM, BW_LAUNCH_REGS))
     return rc;
-  attn_dq_kernel<DP><<<(unsigned)((long long)bt.q_tiles * s.heads), BW_THREADS, dq_smem(DP), st>>>(
+  attn_dq_kernel<DP><<<(unsigned)((long long)bt.q_tiles * s.heads), BW_THREADS, DqLayout<DP>::SMEM, st>>>(
       s, bt, q, k, v, o, lse, dout, dq);
-  attn_dkv_kernel<DP><<<(unsigned)((long long)bt.k_tiles * s.kv_heads * bt.parts), BW_THREADS, kv_smem(DP), st>>>(
+  attn_dkv_kernel<DP><<<(unsigned)((long long)bt.k_tiles * s.kv_heads * bt.parts), BW_THREADS, KvLayout<DP>::SMEM, st>>>(
       s, bt, q, k, v, o, lse, dout, dk, dv);
   if (bt.parts > 1) {
     const dim3 grid((unsigned)(bt.k_tiles * (TILE / JOIN_ROWS)), (unsigned)s.kv_heads);
