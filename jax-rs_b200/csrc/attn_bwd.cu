@@ -77,22 +77,27 @@ __device__ __forceinline__ void drain(float (&acc)[DP / 2], uint32_t taddr, floa
   }
 }
 
-// A tile of 128 columns from shared memory into tensor memory: hi in 64 columns,
-// lo in the next 64; this thread has half of row `row`.
+// A tile from shared memory into tensor memory: hi in DP/2 columns, lo in the next
+// DP/2; this thread has half of row `row`.
+template <int DP>
 __device__ __forceinline__ void tile_to_tmem(const uint8_t* tile, int row, int half, uint32_t taddr) {
+  constexpr int CHUNKS = DP / 16;  // of 16 bytes, per half row
 #pragma unroll
   for (int part = 0; part < 2; ++part) {
-    const uint8_t* p = tile + part * tile_part(128) + half * PANEL + row * 128;
-    uint32_t r[32];
+    const uint8_t* p = tile + part * tile_part(DP) + (DP == 128 ? half * PANEL : 0) + row * 128;
+    uint32_t r[4 * CHUNKS];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
+    for (int i = 0; i < CHUNKS; ++i) {
+      const int c = DP == 128 ? i : half * CHUNKS + i;
       const uint4 x = *reinterpret_cast<const uint4*>(p + ((c ^ (row & 7)) << 4));
-      r[4 * c] = x.x;
-      r[4 * c + 1] = x.y;
-      r[4 * c + 2] = x.z;
-      r[4 * c + 3] = x.w;
+      r[4 * i] = x.x;
+      r[4 * i + 1] = x.y;
+      r[4 * i + 2] = x.z;
+      r[4 * i + 3] = x.w;
     }
-    tmem_st32(taddr + part * 64 + half * 32, r);
+    const uint32_t to = taddr + part * (DP / 2) + half * (DP / 4);
+    if constexpr (DP == 128) tmem_st32(to, r);
+    else tmem_st16(to, r);
   }
 }
 
@@ -141,16 +146,16 @@ __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b, uin
 // ---- dq ------------------------------------------------------------------------
 // Tensor memory at DP = 128: Q and dO (from shared memory they would not leave room
 // for K and V), X for S, then dS, and Y for dP, then the sum's part D: S(j+1)
-// follows dS(j) K.  At DP = 64 Q and dO stay in shared memory, S alternates
-// between two X, dS goes over its S and D has its own columns: S runs two tiles
-// ahead and dP one.
+// follows dS(j) K.  At DP = 64 Q stays in shared memory, S alternates between two
+// X, dS goes over its S and D has its own columns: S runs two tiles ahead and dP
+// one.
 template <int DP>
 struct DqLayout {
   static constexpr bool AHEAD = DP == 64;
-  static constexpr int KS = AHEAD ? 3 : 2, VS = AHEAD ? 2 : 1;  // stages
-  static constexpr uint32_t Q = 0, DO = 128;                    // DP = 128
+  static constexpr int KS = AHEAD ? 4 : 2, VS = AHEAD ? 2 : 1;  // stages
+  static constexpr uint32_t Q = 0, DO = AHEAD ? 448 : 128;      // (Q: DP = 128)
   static constexpr uint32_t X = AHEAD ? 0 : 256, X_STEP = AHEAD ? 128 : 0, Y = AHEAD ? 256 : 384, D = 384;
-  static constexpr int STAY = AHEAD ? 2 * tile_bytes(DP) : 0;   // shared memory for Q and dO
+  static constexpr int STAY = AHEAD ? tile_bytes(DP) : 0;       // shared memory for Q
   static constexpr size_t SMEM = STAY + (size_t)(KS + VS) * tile_bytes(DP) + 1024 + 256;
 };
 
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   uint64_t* vfull = kempty + KS;
   uint64_t* vempty = vfull + VS;
   uint64_t* stayfull = vempty + VS;  // Q's and dO's tiles have landed
-  uint64_t* moved = stayfull + 1;    // and are in tensor memory (DP = 128)
+  uint64_t* moved = stayfull + 1;    // and those that go there are in tensor memory
   uint64_t* sfull = moved + 1;       // [2]
   uint64_t* dpfull = sfull + 2;
   uint64_t* dsfull = dpfull + 1;
@@ -192,10 +197,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const long long qslot = ((long long)first_tile(sq.q0, b) + jt) * s.heads + h;
   const long long hd = (long long)h * s.dim;
 
-  // at DP = 128 Q passes through K's last stage, dO through V's
+  // dO passes through V's last stage, Q (at DP = 128) through K's
   uint8_t* at_q = L::AHEAD ? smem : ring + (KS - 1) * STAGE;
-  uint8_t* at_d = L::AHEAD ? smem + STAGE : ring + (KS + VS - 1) * STAGE;
-  constexpr int K_FIRST = L::AHEAD ? KS : KS - 1, V_FIRST = L::AHEAD ? VS : VS - 1;  // stages that are free at once
+  uint8_t* at_d = ring + (KS + VS - 1) * STAGE;
+  constexpr int K_FIRST = L::AHEAD ? KS : KS - 1, V_FIRST = VS - 1;  // stages that are free at once
   auto copy_k = [&](int j) {
     jxd::mbar_arrive_expect_tx(&kfull[j % KS], STAGE);
     bulk_load(jxd::smem_u32(ring + j % KS * STAGE), bt.k + (slot0 + (long long)j * s.kv_heads) * STAGE, STAGE,
@@ -272,7 +277,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     if (warp == 0 && nb > 0 && jxd::elect_one()) {
       // ---- the remaining copies
       int nk = min(nb, K_FIRST), nv = min(nb, V_FIRST);
-      bool ok = L::AHEAD || wait_bounded(moved, 0, s.err);  // the stages that Q and dO passed through are free
+      bool ok = wait_bounded(moved, 0, s.err);  // the stages that Q and dO passed through are free
       auto free_stage = [&](uint64_t* bar, int use) {
         return ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)(use + 1) & 1u, s.err);
       };
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
       // ---- MMA
       const uint32_t kbase = jxd::smem_u32(ring), vbase = kbase + KS * STAGE;
-      bool ok = wait_bounded(L::AHEAD ? stayfull : moved, 0, s.err);
+      bool ok = wait_bounded(stayfull, 0, s.err) && wait_bounded(moved, 0, s.err);
       auto ready = [&](uint64_t* bar, int n) {
         ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)n & 1u, s.err);
         jxd::tc_fence_after();
@@ -308,8 +313,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       };
       auto d_scores = [&](int j) {
         if (!ready(&vfull[j % VS], j / VS)) return;
-        mma_scores<DP, 128, !L::AHEAD>(tmem + L::Y, L::AHEAD ? jxd::smem_u32(at_d) : tmem + L::DO,
-                                       vbase + (j % VS) * STAGE, PANEL, PART);
+        mma_scores<DP, 128, true>(tmem + L::Y, tmem + L::DO, vbase + (j % VS) * STAGE, PANEL, PART);
         jxd::mma_commit(dpfull);
         jxd::mma_commit(&vempty[j % VS]);
       };
@@ -347,12 +351,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       __syncwarp();
       if (lane == 0) jxd::mbar_arrive(bar);
     };
-    if (!L::AHEAD && nb > 0) {
+    if (nb > 0) {
       ready(stayfull, 0);
-      if constexpr (!L::AHEAD) {
-        tile_to_tmem(at_q, row, half, tmem + lanes + L::Q);
-        tile_to_tmem(at_d, row, half, tmem + lanes + L::DO);
-      }
+      if constexpr (!L::AHEAD) tile_to_tmem<DP>(at_q, row, half, tmem + lanes + L::Q);
+      tile_to_tmem<DP>(at_d, row, half, tmem + lanes + L::DO);
       tmem_st_wait();
       done(moved);
     }
@@ -474,8 +476,13 @@ struct KvLayout {
   static constexpr int PANEL_BYTES = BLK * 128;                                    // of a block
   static constexpr int STAGE = DP / 64 * 2 * PANEL_BYTES;                          // one block: 32 KB
   static constexpr int STAY = APART ? 2 * tile_bytes(DP) : tile_bytes(DP);         // shared memory for K (and V)
-  static constexpr size_t SMEM = STAY + (size_t)(QS + DS) * STAGE + 1024 + 256;
+  static constexpr int STATS = 2 * 2 * BLK * 4;  // lse2 and delta of two blocks
+  // What is left of an SM's 227 KB for aligning the tiles to 1024 bytes.  The array is
+  // declared so aligned; a base that were not would be refused.
+  static constexpr int SPARE = 768;
+  static constexpr size_t SMEM = STAY + (size_t)(QS + DS) * STAGE + STATS + 256 + SPARE;
 };
+static_assert(KvLayout<64>::SMEM <= 232448 && KvLayout<128>::SMEM <= 232448, "shared memory of an SM");
 
 template <int DP>
 __global__ void __launch_bounds__(BW_THREADS, 1)
@@ -485,11 +492,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   using L = KvLayout<DP>;
   constexpr int QS = L::QS, DS = L::DS, BLK = L::BLK, STAGE = L::STAGE, PART = STAGE / 2, HPANEL = L::PANEL_BYTES;
   constexpr int PER_TILE = TILE / BLK;  // blocks of a tile
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw_addr = jxd::smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t raw_addr = jxd::smem_u32(smem_raw), shift = ((raw_addr + 1023u) & ~1023u) - raw_addr;
+  if (shift > (uint32_t)L::SPARE) {
+    if (threadIdx.x == 0) atomicOr(s.err, JX_DEVERR_TIMEOUT);
+    return;
+  }
+  uint8_t* smem = smem_raw + shift;
   uint8_t* ring = smem + L::STAY;  // Q's stages, then dout's
-  uint64_t* qfull = reinterpret_cast<uint64_t*>(ring + (QS + DS) * STAGE);
+  float* stats = reinterpret_cast<float*>(ring + (QS + DS) * STAGE);  // [2][lse2 BLK, delta BLK]
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(stats + 4 * BLK);
   uint64_t* qempty = qfull + QS;
   uint64_t* dfull = qempty + QS;
   uint64_t* dempty = dfull + DS;
@@ -503,7 +515,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   uint64_t* zfree = zfull + 1;  // dV's part
   uint64_t* wfull = zfree + 1;  // dK's
   uint64_t* wfree = wfull + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(wfree + 1);
+  uint64_t* tfull = wfree + 1;  // [2] statistics
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfull + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -557,6 +570,14 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const long long slot = slot_of(u, &place);
     load(ring + (QS + u % DS) * STAGE, bt.d + slot * tile_bytes(DP), place, &dfull[u % DS]);
   };
+  auto copy_stats = [&](int u) {
+    int place;
+    const long long slot = slot_of(u, &place);
+    float* dst = stats + (u & 1) * 2 * BLK;
+    jxd::mbar_arrive_expect_tx(&tfull[u & 1], 2 * BLK * 4);
+    bulk_load(jxd::smem_u32(dst), bt.lse2 + slot * TILE + place * BLK, BLK * 4, &tfull[u & 1]);
+    bulk_load(jxd::smem_u32(dst + BLK), bt.delta + slot * TILE + place * BLK, BLK * 4, &tfull[u & 1]);
+  };
   bool bad = false;
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < QS; ++i) {
@@ -572,6 +593,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     for (int i = 0; i < 2; ++i) {
       jxd::mbar_init(&sfull[i], 1);
       jxd::mbar_init(&dpfull[i], 1);
+      jxd::mbar_init(&tfull[i], 1);
     }
     jxd::mbar_init(pfull, 8);
     jxd::mbar_init(dsfull, 8);
@@ -587,6 +609,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       bulk_load(jxd::smem_u32(smem), bt.k + kslot * tile_bytes(DP), tile_bytes(DP), stayfull);
       bulk_load(jxd::smem_u32(at_v), bt.v + kslot * tile_bytes(DP), tile_bytes(DP), stayfull);
       for (int u = 0; u < min(n, Q_FIRST); ++u) copy_q(u);
+      for (int u = 0; u < min(n, 2); ++u) copy_stats(u);
       for (int u = 0; u < min(n, DS); ++u) copy_d(u);
     }
   } else if (warp == 1) {
@@ -618,6 +641,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       wait_bounded(stayfull, 0, s.err);
       for (int u = 0; u < min(n, Q_FIRST); ++u) wait_bounded(&qfull[u], 0, s.err);
       for (int u = 0; u < min(n, DS); ++u) wait_bounded(&dfull[u], 0, s.err);
+      for (int u = 0; u < min(n, 2); ++u) wait_bounded(&tfull[u], 0, s.err);
     }
     if (warp == 1) {
       __syncwarp();
@@ -630,19 +654,29 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BW_LOW_REGS));
     if (warp == 0 && n > 0 && jxd::elect_one()) {
       // ---- the remaining copies
-      int nq = min(n, Q_FIRST), nd = min(n, DS);
+      // Q(0) Q(1) dout(0) statistics(0) Q(2) dout(1) statistics(1) ...: dK(u), which the copies of
+      // block u+3 of Q and u+2 of the statistics wait for, needs nothing behind dout(u+1) in this order
+      int nq = min(n, Q_FIRST), nd = min(n, DS), nt = min(n, 2);
       bool ok = L::APART || wait_bounded(moved, 0, s.err);  // the stages that V passed through are free
       auto free_stage = [&](uint64_t* bar, int use) {
         return ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)(use + 1) & 1u, s.err);
       };
-      while (ok && (nq < n || nd < n)) {
-        // Q is wanted up to one block earlier than dout
-        if (nd < n && (nq == n || nd + 1 < nq)) {
+      for (int i = 0; ok && i <= n; ++i) {
+        if (i == nq && i < n) {
+          if (!free_stage(&qempty[i % QS], i / QS)) break;
+          copy_q(i);
+          ++nq;
+        }
+        if (i - 1 == nd) {
           if (!free_stage(&dempty[nd % DS], nd / DS)) break;
-          copy_d(nd++);
-        } else {
-          if (!free_stage(&qempty[nq % QS], nq / QS)) break;
-          copy_q(nq++);
+          copy_d(nd);
+          ++nd;
+        }
+        if (i - 1 == nt) {
+          // block nt - 2's statistics were last read for its dS, before dK(nt-2), which freed its stage of Q
+          if (!free_stage(&qempty[(nt - 2) % QS], (nt - 2) / QS + 1)) break;
+          copy_stats(nt);
+          ++nt;
         }
       }
       if (!ok) *abort_flag = 1;
@@ -650,6 +684,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       wait_bounded(stayfull, 0, s.err);
       for (int e = max(0, nq - QS); e < nq; ++e) wait_bounded(&qfull[e % QS], (uint32_t)(e / QS) & 1u, s.err);
       for (int e = max(0, nd - DS); e < nd; ++e) wait_bounded(&dfull[e % DS], (uint32_t)(e / DS) & 1u, s.err);
+      for (int e = max(0, nt - 2); e < nt; ++e) wait_bounded(&tfull[e & 1], (uint32_t)(e >> 1) & 1u, s.err);
     }
     if (warp == 1 && n > 0 && jxd::elect_one()) {
       // ---- MMA
@@ -721,7 +756,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     };
     if (!L::APART && n > 0) {
       ready(stayfull, 0);
-      if constexpr (!L::APART) tile_to_tmem(at_v, row, half, tmem + lanes + L::V);
+      if constexpr (!L::APART) tile_to_tmem<DP>(at_v, row, half, tmem + lanes + L::V);
       tmem_st_wait();
       done(moved);
     }
@@ -739,14 +774,15 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const long long slot = slot_of(u, &place);
       const int i0 = (blk0 + (it0 + u) % nblk) * BLK;  // the block's first row
       const float inv_q = bt.inv_q[slot], inv_d = bt.inv_d[slot], norm_d = bt.norm_d[slot], top_d = bt.delta_top[slot];
-      const float* lse2 = bt.lse2 + slot * TILE + place * BLK + half * C;
-      const float* delta = bt.delta + slot * TILE + place * BLK + half * C;
+      const float* lse2 = stats + (u & 1) * 2 * BLK + half * C;
+      const float* delta = lse2 + BLK;
       const uint32_t xa = tmem + lanes + L::X + (u & 1) * L::X_STEP + half * C;
       const uint32_t ya = tmem + lanes + L::Y + (u & 1) * L::Y_STEP + half * C;
       const float f = f_tile * inv_q;
       const float2 f2 = make_float2(f, f);
       const bool edge = i0 < first_all || rows < TILE;  // some key is not seen by all of the block's rows
       float2 p[C / 2];
+      ready(&tfull[u & 1], u >> 1);
       ready(&sfull[u & 1], u >> 1);
 #pragma unroll
       for (int c = 0; c < C; c += 32) {
@@ -755,7 +791,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 l = __ldg(reinterpret_cast<const float4*>(lse2 + c + i));
+          const float4 l = *reinterpret_cast<const float4*>(lse2 + c + i);
           const float2 z0 = fma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2,
                                  make_float2(-l.x, -l.y));
           const float2 z1 = fma2(make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])), f2,
@@ -798,7 +834,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         jxd::tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
-          const float4 d = __ldg(reinterpret_cast<const float4*>(delta + c + i));
+          const float4 d = *reinterpret_cast<const float4*>(delta + c + i);
           const float2 e0 = fma2(make_float2(d.x, d.y), nf2, make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])));
           const float2 e1 =
               fma2(make_float2(d.z, d.w), nf2, make_float2(__uint_as_float(r[i + 2]), __uint_as_float(r[i + 3])));
