@@ -61,6 +61,25 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dkv_kernel(const __g
           s.total_q, s.scale);
 }
 
+// Whether the tensor-core kernels or the plain-f32 rings take a forward call, from
+// the hints, in microseconds as measured at dim 128: the rings read K and V once
+// for every 32 query rows of a key head, 18 us and about 1 ns a key and head each
+// time (0.25 ns at 4 rows: HBM's rate); the tiles cost 2.3 us per 128 keys for each wave of
+// (query tile, head) CTAs, and the split of K and V 0.4 ns a key and head.
+// (4 sequences of 8192 keys, 64 heads on 1: rings 93, tiles 278; 1000 keys x 8, 20
+// rows, 16 heads: 140 and 101; 2048 keys x 4, 64 rows a head: 91 and 68.)
+bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
+  const double rows = (double)max_q * s.group;
+  if (rows <= 16) return false;
+  if (rows > 128) return true;
+  const double keys = (double)s.total_k * s.kv_heads;
+  const double ctas = (double)s.batch * s.heads * ((max_q + 127) / 128);
+  const double waves = ceil(ctas / jx::num_sms());
+  const double rings = ceil(rows / 32) * (18 + keys * 1e-3);
+  const double tiles = 20 + 2.3 * waves * (double)((max_k + 127) / 128) + keys * 0.4e-3;
+  return tiles < rings;
+}
+
 int check_shape(const char* what, Shape& s, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q,
                 int64_t total_k, int64_t max_q, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
                 int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int causal) {
@@ -111,7 +130,7 @@ int jx_attention_f32(const float* q, const float* k, const float* v, float* o, f
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
   JX_REQUIRE(total_q * heads < (1LL << 31), "attention: too many rows");
-  if (total_k > 0 && max_q * s.group > 16) return attention_fwd_tiles(s, q, k, v, o, lse, st);
+  if (total_k > 0 && tiles_are_faster(s, max_q, max_k)) return attention_fwd_tiles(s, q, k, v, o, lse, st);
   return attention_decode(s, q, k, v, o, lse, max_q * s.group, st);
 }
 
@@ -131,8 +150,9 @@ int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const f
   JX_REQUIRE(total_k == 0 || (k && v && dk && dv), "attention_bwd: NULL pointer");
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
-  if (total_q > 0 && total_k > 0 && max_q * s.group > 16)
-    return attention_bwd_tiles(s, q, k, v, o, lse, dout, dq, dk, dv, st);
+  // row by row only where five launches would be the whole time (16 rows, 16 keys: 21 us against 44; 100 keys: equal)
+  if (total_q > 0 && total_k > 0 && (max_q * s.group > 16 || max_k > 96))
+    return attention_bwd_tiles(s, q, k, v, o, lse, dout, dq, dk, dv, max_q, st);
   const long long bq = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
   const long long bk = (total_k * kv_heads + ROW_WARPS - 1) / ROW_WARPS;
   JX_REQUIRE(bq < (1LL << 31) && bk < (1LL << 31), "attention_bwd: too many rows");

@@ -941,12 +941,14 @@ int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, c
 namespace jxa {
 
 int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
-                        const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st) {
+                        const float* lse, const float* dout, float* dq, float* dk, float* dv, long long max_q,
+                        cudaStream_t st) {
   const int DP = s.dim <= 64 ? 64 : 128;
   const long long kt = tile_count(s.total_k, s.batch), qt = tile_count(s.total_q, s.batch);
-  // key tiles are few where heads are shared: enough parts of the query rows for four CTAs per SM
-  const long long ctas = kt * s.kv_heads;
-  const int parts = (int)std::max<long long>(1, std::min<long long>(8, 4LL * jx::num_sms() / std::max(1LL, ctas)));
+  // key tiles are few where heads are shared: enough parts of the query rows for four CTAs per SM, of four blocks at least
+  const long long ctas = kt * s.kv_heads, blocks = s.group * ((max_q + 63) / 64);
+  const int parts =
+      (int)std::max<long long>(1, std::min(std::min<long long>(8, blocks / 4), 4LL * jx::num_sms() / std::max(1LL, ctas)));
   JX_REQUIRE(qt * s.heads < (1LL << 31) && kt * s.kv_heads * parts < (1LL << 31) && kt < (1LL << 27),
              "attention_bwd: too many rows");
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
@@ -971,17 +973,17 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   float* delta_top = (float*)take(qs * 4);
   int *bad_k = (int*)take(ks * 4), *bad_v = (int*)take(ks * 4), *bad_q = (int*)take(qs * 4), *bad_d = (int*)take(qs * 4);
   int *order_q = (int*)take(qt * 4), *order_k = (int*)take(kt * 4);
-  TileSources kv = {}, qd = {};
-  kv.t[0] = {k, s.ldk, tk, inv_k, bad_k};
-  kv.t[1] = {v, s.ldv, tv, inv_v, bad_v, norm_v};
-  qd.t[0] = {q, s.ldq, tq, inv_q, bad_q};
-  qd.t[1] = {dout, s.ldo, td, inv_d, bad_d, norm_d, o, lse, lse2, delta, delta_top};
+  TileSources src = {};
+  src.keys = src.queries = 2;
+  src.order_q = order_q;
+  src.order_k = order_k;
+  src.t[0] = {k, s.ldk, tk, inv_k, bad_k};
+  src.t[1] = {v, s.ldv, tv, inv_v, bad_v, norm_v};
+  src.t[2] = {q, s.ldq, tq, inv_q, bad_q};
+  src.t[3] = {dout, s.ldo, td, inv_d, bad_d, norm_d, o, lse, lse2, delta, delta_top};
   const BwdTiles bt = {tq,     tk,     tv,    td,    inv_q, inv_k,     inv_v,   inv_d,   bad_q, bad_k,  bad_v,
                        bad_d,  norm_v, norm_d, lse2, delta, delta_top, (int)qt, (int)kt, parts, order_q, order_k, part_k, part_v};
-  kv.order = order_k;
-  kv.order_other = order_q;
-  int rc = split_tiles(s, false, kv, 2, s.kv_heads, DP, st);
-  if (!rc) rc = split_tiles(s, true, qd, 2, s.heads, DP, st);
+  int rc = split_tiles(s, src, DP, st);
   if (!rc)
     rc = DP == 128 ? launch<128>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st)
                    : launch<64>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st);

@@ -58,10 +58,10 @@ struct Cursor {
   bool on;
 
   // To the first key at or behind `pos`, in a sequence from b on.
-  __device__ __forceinline__ void settle(const Shape& s, long long end) {
+  __device__ __forceinline__ void settle(const Shape& s, long long end, int row_base) {
     for (on = false; b < s.batch; ++b) {
       sq = seq_bounds(s, b);
-      if (sq.lq == 0 || sq.lk == 0) continue;
+      if ((long long)sq.lq * s.group <= row_base || sq.lk == 0) continue;
       const long long base = (sq.k0 + (long long)b * VOID) * s.kv_heads, in = max(0LL, pos - base);
       const int len = sq.lk + VOID;
       if (in >= (long long)s.kv_heads * len) continue;
@@ -79,7 +79,7 @@ struct Cursor {
   __device__ __forceinline__ int keys(long long end) const {  // of the next stage
     return (int)min((long long)min(DC_KEYS, sq.lk - key), end - pos);
   }
-  __device__ __forceinline__ void step(const Shape& s, int n, long long end) {
+  __device__ __forceinline__ void step(const Shape& s, int n, long long end, int row_base) {
     pos += n;
     key += n;
     on = pos < end;
@@ -89,7 +89,7 @@ struct Cursor {
       on = pos < end;
       if (++hk == s.kv_heads && on) {
         ++b;
-        settle(s, end);
+        settle(s, end, row_base);
       }
     }
   }
@@ -158,13 +158,13 @@ __device__ __forceinline__ float4 sum_groups(const float (&x)[E], int g) {
 }
 
 // Ring w of `rings` takes the positions w * per .. +per.  warps_per_ring = WR in
-// {1, 2, 4, 8}; warp i of a ring has the rows i * R .. +R of a sequence.
+// {1, 2, 4, 8}; warp i of a ring has the rows row_base + i * R .. +R of a sequence.
 template <int R, int DP, bool VEC>
 __global__ void __launch_bounds__(32 * DC_WARPS, 1)
     attn_decode_kernel(const __grid_constant__ Shape s, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const float* __restrict__ q, const float* __restrict__ k,
                        const float* __restrict__ v, float* o, float* lse, float* __restrict__ part, long long per,
-                       int WR) {
+                       int WR, int row_base) {
   constexpr int E = DP / DC_LPK, STEPS = DC_KEYS / DC_GROUPS, STAGE = dc_stage(DP);
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / DC_LPK, l = lane % DC_LPK;
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
   Cursor c;
   c.pos = begin;
   c.b = seq_of_position(s, begin);
-  c.settle(s, end);
+  c.settle(s, end, row_base);
   Cursor pc = c;  // the copies' place, up to nst stages ahead
   int in_st = 0, out_st = 0, issued = 0;
   uint32_t in_ph = 0, out_ph = 0;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
       in_st = 0;
       in_ph ^= 1u;
     }
-    pc.step(s, n, end);
+    pc.step(s, n, end, row_base);
   };
   if (wr == 0)
     for (int i = 0; i < nst; ++i) produce();
@@ -244,11 +244,12 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
     // one piece of a (sequence, key head)
     const int b = c.b, hk = c.hk, first_key = c.key;
     const Seq sq = c.sq;
-    const int all_rows = (int)min((long long)sq.lq * s.group, (long long)R * WR), row0 = wr * R;
+    // rows row_base + row0 .. of the sequence
+    const int all_rows = (int)min((long long)sq.lq * s.group - row_base, (long long)R * WR), row0 = wr * R;
     float qr[R][E], acc[R][E], m[R], sum[R];
     int vis[R], vis_least = sq.lk;
     {
-      int i = row0 / s.group, hg = row0 - i * s.group;
+      int i = (row_base + row0) / s.group, hg = row_base + row0 - i * s.group;
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const bool on = row0 + r < all_rows;
@@ -362,7 +363,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
         out_st = 0;
         out_ph ^= 1u;
       }
-      c.step(s, n, end);
+      c.step(s, n, end, row_base);
       if (wr == 0) produce();
     }
     if (!ok) break;
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
     // the head's first position
     const long long seg = (sq.k0 + (long long)b * VOID) * s.kv_heads + (long long)hk * (sq.lk + VOID);
     const bool last = seg >= begin && seg + sq.lk <= end;
-    int i = row0 / s.group, hg = row0 - i * s.group;
+    int i = (row_base + row0) / s.group, hg = row_base + row0 - i * s.group;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float t = m[r];
@@ -427,7 +428,7 @@ constexpr int JN_AHEAD = 8;
 __global__ void __launch_bounds__(32 * JN_WARPS)
     attn_join_kernel(const __grid_constant__ Shape s, const float* __restrict__ q, const float* __restrict__ k,
                      const float* __restrict__ v, const float* part, float* o, float* lse, long long per,
-                     int ring_rows, int DP) {
+                     int ring_rows, int DP, int row_base, int last_pass) {
   __shared__ float red[2 * JN_WARPS];
   __shared__ float4 acc[JN_WARPS][32];
   const long long tok = blockIdx.x / (unsigned)s.heads;
@@ -438,7 +439,8 @@ __global__ void __launch_bounds__(32 * JN_WARPS)
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the rings' results are complete and visible behind it
   if (tok < sq.q0 || tok >= sq.q0 + sq.lq) return;
   const int i = (int)(tok - sq.q0);
-  const long long row = (long long)i * s.group + h % s.group;
+  const long long row = (long long)i * s.group + h % s.group - row_base;
+  if (row < 0 || (row >= ring_rows && !last_pass)) return;  // another pass's
   float* out = o + tok * s.ldo + (long long)h * s.dim;
   if (row >= ring_rows || sq.lk == 0) {
     if (warp == 0)
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(32 * JN_WARPS)
   }
 }
 
-using DecodeKernel = void (*)(Shape, CUtensorMap, CUtensorMap, const float*, const float*, const float*, float*, float*, float*, long long, int);
+using DecodeKernel = void (*)(Shape, CUtensorMap, CUtensorMap, const float*, const float*, const float*, float*, float*, float*, long long, int, int);
 
 template <int R>
 DecodeKernel kernel_of(int DP, bool vec) {
@@ -535,6 +537,7 @@ int attention_decode(const Shape& s, const float* q, const float* k, const float
                    s.ldk < (1LL << 37) && s.ldv < (1LL << 37);  // what a tensor map takes
   const int R = rows <= 1 ? 1 : rows <= 2 ? 2 : 4;
   const int WR = rows <= 4 ? 1 : rows <= 8 ? 2 : rows <= 16 ? 4 : 8;
+  const int passes = (int)std::max<long long>(1, (rows + R * WR - 1) / (R * WR));  // K and V are read once a pass
   const DecodeKernel kernel = R == 1 ? kernel_of<1>(DP, vec) : R == 2 ? kernel_of<2>(DP, vec) : kernel_of<4>(DP, vec);
   if (int rc = prepare_kernel((const void*)kernel, 8 + (R >> 1) * 4 + (DP == 128) * 2 + vec, dc_smem(DP), 0)) return rc;
   CUtensorMap map_k = {}, map_v = {};
@@ -554,21 +557,26 @@ int attention_decode(const Shape& s, const float* q, const float* k, const float
   void* part = nullptr;
   if (int rc = jx::scratch_get(sizeof(float) * (size_t)grid * (DC_WARPS / WR) * 2 * R * WR * (DP + 4), &part, st))
     return rc;
-  if (rings > 0)
-    kernel<<<grid, 32 * DC_WARPS, dc_smem(DP), st>>>(s, map_k, map_v, q, k, v, o, lse, static_cast<float*>(part), per, WR);
-  // the join's blocks may start while the last rings finish; they wait for them before they read
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(s.total_q * s.heads));
-  cfg.blockDim = dim3(32 * JN_WARPS);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess)
-    e = cudaLaunchKernelEx(&cfg, attn_join_kernel, s, q, k, v, static_cast<const float*>(part), o, lse, per, R * WR, DP);
+  cudaError_t e = cudaSuccess;
+  for (int p = 0; p < passes && e == cudaSuccess; ++p) {
+    const int row_base = p * R * WR;
+    kernel<<<grid, 32 * DC_WARPS, dc_smem(DP), st>>>(s, map_k, map_v, q, k, v, o, lse, static_cast<float*>(part), per,
+                                                     WR, row_base);
+    // the join's blocks may start while the last rings finish; they wait for them before they read
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(s.total_q * s.heads));
+    cfg.blockDim = dim3(32 * JN_WARPS);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaGetLastError();
+    if (e == cudaSuccess)
+      e = cudaLaunchKernelEx(&cfg, attn_join_kernel, s, q, k, v, static_cast<const float*>(part), o, lse, per, R * WR,
+                             DP, row_base, (int)(p == passes - 1));
+  }
   jx::scratch_release(part, st);
   return e == cudaSuccess ? JX_OK : jx::check_cuda(e, "attn_decode_kernel");
 }

@@ -89,19 +89,25 @@ __device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, i
 }
 
 template <int DP>
-__global__ void __launch_bounds__(SP_THREADS, 2) split_tiles_kernel(const __grid_constant__ Shape s, int over_q,
-                                                                   const __grid_constant__ TileSources src, int heads,
-                                                                   int tiles, int tiles_other) {
+__global__ void __launch_bounds__(SP_THREADS, 2) split_tiles_kernel(const __grid_constant__ Shape s,
+                                                                   const __grid_constant__ TileSources src) {
   constexpr int PER_ROW = DP / 8, STEP = SP_THREADS / PER_ROW, ROWS = TILE / STEP;  // threads; rows at a time; rows each
   __shared__ uint32_t sm_top[SP_THREADS / 32], sm_low[SP_THREADS / 32];
-  if (blockIdx.x == 0) {  // one block per order that is asked for
-    if (blockIdx.y == 0 && blockIdx.z == 0 && src.order) order_tiles(s, over_q, tiles, src.shift, src.order);
-    if (blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1 && src.order_other)
-      order_tiles(s, !over_q, tiles_other, src.shift, src.order_other);
+  if (blockIdx.x < 2) {  // the orders
+    if (blockIdx.x == 0 && src.order_q) order_tiles(s, true, src.q_tiles, src.shift, src.order_q);
+    if (blockIdx.x == 1 && src.order_k) order_tiles(s, false, src.k_tiles, src.shift, src.order_k);
     return;
   }
-  const TileSource& t = src.t[blockIdx.z];
-  const int id = blockIdx.x - 1, h = blockIdx.y;
+  // the tensor, tile and head
+  long long at_block = blockIdx.x - 2;
+  const long long per_k = (long long)src.k_tiles * s.kv_heads, per_q = (long long)src.q_tiles * s.heads;
+  const bool over_q = at_block >= src.keys * per_k;
+  if (over_q) at_block -= src.keys * per_k;
+  const int which = (int)(at_block / (over_q ? per_q : per_k)) + (over_q ? src.keys : 0);
+  at_block %= over_q ? per_q : per_k;
+  const int heads = over_q ? s.heads : s.kv_heads;
+  const TileSource& t = src.t[which];
+  const int id = (int)(at_block / heads), h = (int)(at_block - (long long)id * heads);
   int j;
   const int b = seq_of_tile(over_q ? s.cu_q : s.cu_k, s.batch, id, &j);
   const Seq sq = seq_bounds(s, b);
@@ -561,14 +567,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 
 namespace jxa {
 
-int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st) {
-  const int tiles = (int)tile_count(over_q ? s.total_q : s.total_k, s.batch);
-  const int other = (int)tile_count(over_q ? s.total_k : s.total_q, s.batch);
+int split_tiles(const Shape& s, const TileSources& src, int DP, cudaStream_t st) {
   TileSources ts = src;
-  for (ts.shift = 0; (std::max(tiles, other) >> ts.shift) >= ORDER_KEYS - 1; ++ts.shift) {}
-  const dim3 grid((unsigned)tiles + 1, (unsigned)heads, (unsigned)count);
-  if (DP == 128) split_tiles_kernel<128><<<grid, SP_THREADS, 0, st>>>(s, over_q, ts, heads, tiles, other);
-  else split_tiles_kernel<64><<<grid, SP_THREADS, 0, st>>>(s, over_q, ts, heads, tiles, other);
+  ts.q_tiles = (int)tile_count(s.total_q, s.batch);
+  ts.k_tiles = (int)tile_count(s.total_k, s.batch);
+  for (ts.shift = 0; (std::max(ts.q_tiles, ts.k_tiles) >> ts.shift) >= ORDER_KEYS - 1; ++ts.shift) {}
+  const long long blocks =
+      2 + (long long)src.keys * ts.k_tiles * s.kv_heads + (long long)src.queries * ts.q_tiles * s.heads;
+  JX_REQUIRE(blocks < (1LL << 31), "attention: too many rows");
+  if (DP == 128) split_tiles_kernel<128><<<(unsigned)blocks, SP_THREADS, 0, st>>>(s, ts);
+  else split_tiles_kernel<64><<<(unsigned)blocks, SP_THREADS, 0, st>>>(s, ts);
   JX_LAUNCH_CHECK("split_tiles_kernel");
   return JX_OK;
 }
@@ -607,9 +615,10 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
   TileSources src = {};
   src.t[0] = {k, s.ldk, base, inv, bad};
   src.t[1] = {v, s.ldv, base + bytes, inv + slots, bad + slots};
-  src.order_other = bad + 2 * slots;
-  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, src.order_other};
-  int rc = split_tiles(s, false, src, 2, s.kv_heads, DP, st);
+  src.keys = 2;
+  src.order_q = bad + 2 * slots;
+  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, src.order_q};
+  int rc = split_tiles(s, src, DP, st);
   if (!rc) {
     const unsigned grid = (unsigned)(qt * s.heads);
     if (DP == 128) {

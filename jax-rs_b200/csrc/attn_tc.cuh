@@ -306,7 +306,7 @@ __device__ __forceinline__ void row_half_store(const float (&x)[DP / 2], float f
   }
 }
 
-// Streams that are split into tiles, for one launch of split_tiles_kernel.
+// A tensor that is split into tiles.
 struct TileSource {
   const float* x;
   long long ld;
@@ -323,25 +323,28 @@ struct TileSource {
   float* delta;
   float* delta_top;
 };
+// One launch of split_tiles_kernel: tensors over the keys' tiles, then over the
+// query rows'.
 struct TileSources {
-  TileSource t[2];
-  // Order of work over the same launch's tiles (over_q: query tiles by their key
-  // tiles, else key tiles by their query rows): ids by falling work, those
-  // behind a sequence's end last.  May be NULL.  work >> shift is below ORDER_KEYS.
-  int* order;
-  int* order_other;  // of the other side's tiles
-  int shift;
+  TileSource t[4];
+  int keys, queries;  // tensors of each kind
+  // Order of work: ids by falling work (query tiles by their key tiles, key tiles
+  // by their query rows), those behind a sequence's end last.  May be NULL.  work
+  // >> shift is below ORDER_KEYS.
+  int *order_q, *order_k;
+  int shift, q_tiles, k_tiles;
 };
 constexpr int ORDER_KEYS = 1024;
 
-// Implemented in attn_fwd.cu: splits 1 or 2 tensors of `heads` heads over the same packed sequences.
-int split_tiles(const Shape& s, bool over_q, const TileSources& src, int count, int heads, int DP, cudaStream_t st);
+// Implemented in attn_fwd.cu: one launch that splits all tensors of `src`.
+int split_tiles(const Shape& s, const TileSources& src, int DP, cudaStream_t st);
 int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs);
 int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
                         cudaStream_t st);
 int attention_decode(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
                      long long rows, cudaStream_t st);
 int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
-                        const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st);
+                        const float* lse, const float* dout, float* dq, float* dk, float* dv, long long max_q,
+                        cudaStream_t st);
 
 }  // namespace jxa
