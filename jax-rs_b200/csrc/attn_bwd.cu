@@ -368,11 +368,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     for (int c = 0; c < DP / 2; ++c) acc[c] = 0.0f;
     float g_prev = 0.0f;
     float2 p[32];
-    // P of tile j, scaled for dS, and what undoes dS's scale
-    float dl = 0.0f, g = 0.0f;
+    // P of tile j, scaled for dS, and what undoes dS's scale; the next tile's numbers are loaded a tile ahead
+    float dl = 0.0f, g = 0.0f, inv_k = 0.0f, inv_v = 0.0f, norm_v = 0.0f, next_k = 0.0f, next_v = 0.0f, next_n = 0.0f;
+    auto look_ahead = [&](int j) {
+      const long long slot = slot0 + (long long)min(j, nb - 1) * s.kv_heads;
+      next_k = bt.inv_k[slot];
+      next_v = bt.inv_v[slot];
+      next_n = bt.norm_v[slot];
+    };
+    if (nb > 0) look_ahead(0);
     auto weights = [&](int j) {
-      const long long slot = slot0 + (long long)j * s.kv_heads;
-      const float inv_k = bt.inv_k[slot], inv_v = bt.inv_v[slot], norm_v = bt.norm_v[slot];
+      inv_k = next_k;
+      inv_v = next_v;
+      norm_v = next_n;
+      look_ahead(j + 1);
       // P is at most 2^14
       const float fd = inv_d * inv_v, sc = bound_scale(16384.0f * (norm_d * norm_v + fabsf(delta)));
       const float f = f_tile * inv_k, pf = sc * fd;
@@ -769,11 +778,22 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     for (int c = 0; c < DP / 2; ++c) ak[c] = av[c] = 0.0f;
     float g_prev = 0.0f;
     constexpr int C = BLK / 2;  // columns of the scores that this thread has
-    for (int u = 0; u < n; ++u) {
+    // a block's numbers are loaded a block ahead
+    float next_q = 0.0f, next_d = 0.0f, next_n = 0.0f, next_t = 0.0f;
+    auto look_ahead = [&](int u) {
       int place;
-      const long long slot = slot_of(u, &place);
-      const int i0 = (blk0 + (it0 + u) % nblk) * BLK;  // the block's first row
-      const float inv_q = bt.inv_q[slot], inv_d = bt.inv_d[slot], norm_d = bt.norm_d[slot], top_d = bt.delta_top[slot];
+      const long long slot = slot_of(min(u, n - 1), &place);
+      next_q = bt.inv_q[slot];
+      next_d = bt.inv_d[slot];
+      next_n = bt.norm_d[slot];
+      next_t = bt.delta_top[slot];
+    };
+    if (n > 0) look_ahead(0);
+    int i0 = (blk0 + (n > 0 ? it0 % nblk : 0) - 1) * BLK;  // the block's first row
+    for (int u = 0; u < n; ++u) {
+      i0 = i0 + BLK >= sq.lq ? blk0 * BLK : i0 + BLK;  // the next block, or the next head's first
+      const float inv_q = next_q, inv_d = next_d, norm_d = next_n, top_d = next_t;
+      look_ahead(u + 1);
       const float* lse2 = stats + (u & 1) * 2 * BLK + half * C;
       const float* delta = lse2 + BLK;
       const uint32_t xa = tmem + lanes + L::X + (u & 1) * L::X_STEP + half * C;
