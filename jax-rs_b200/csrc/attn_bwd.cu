@@ -44,7 +44,7 @@ struct BwdTiles {
   const int *bad_q, *bad_k, *bad_v, *bad_d;
   const float *norm_v, *norm_d, *lse2, *delta, *delta_top;
   int q_tiles, k_tiles, parts;
-  const int *order_q, *order_k;
+  const TileRef *order_q, *order_k;
   float *part_k, *part_v;  // [parts][total_k * kv_heads * dim], used where parts > 1
 };
 
@@ -185,11 +185,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int id = bt.order_q[blockIdx.x / (unsigned)s.heads], h = (int)(blockIdx.x % (unsigned)s.heads);
-  int jt;
-  const int b = seq_of_tile(s.cu_q, s.batch, id, &jt);
-  const Seq sq = seq_bounds(s, b);
-  if (jt < 0 || (long long)jt * TILE >= sq.lq) return;
+  const TileRef ref = load_ref(bt.order_q + blockIdx.x / (unsigned)s.heads);
+  const int h = (int)(blockIdx.x % (unsigned)s.heads), b = ref.b, jt = ref.jt;
+  const Seq sq = seq_of(ref);
+  if (jt < 0) return;
   const int i0 = jt * TILE, rows = min(TILE, sq.lq - i0);
   const int hk = h / s.group;
   const int nb = (sq.visible(i0 + rows - 1, s.causal) + TILE - 1) / TILE;
@@ -533,11 +532,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   unsigned w = blockIdx.x;
   const int part = (int)(w % (unsigned)bt.parts);
   w /= (unsigned)bt.parts;
-  const int hk = (int)(w % (unsigned)s.kv_heads), id = bt.order_k[w / (unsigned)s.kv_heads];
-  int jt;
-  const int b = seq_of_tile(s.cu_k, s.batch, id, &jt);
-  const Seq sq = seq_bounds(s, b);
-  if (jt < 0 || (long long)jt * TILE >= sq.lk) return;
+  const TileRef ref = load_ref(bt.order_k + w / (unsigned)s.kv_heads);
+  const int hk = (int)(w % (unsigned)s.kv_heads), b = ref.b, jt = ref.jt;
+  const Seq sq = seq_of(ref);
+  if (jt < 0) return;
   const int j0 = jt * TILE, rows = min(TILE, sq.lk - j0);
   const int blk0 = sq.first_row(j0, s.causal) / BLK;
   const int nblk = max(0, (sq.lq + BLK - 1) / BLK - blk0);
@@ -974,7 +972,8 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
   const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
   // tiles first, then arrays whose pieces the copies read 16-byte aligned, then the rest
-  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (5 * ks + 6 * qs + qt + kt) * 4 + 2 * part_floats * 4;
+  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (5 * ks + 6 * qs) * 4 + (qt + kt) * sizeof(TileRef) +
+                       2 * part_floats * 4;
   void* p = nullptr;
   if (int rc = jx::scratch_get(bytes + 64, &p, st)) return rc;
   uint8_t* at = static_cast<uint8_t*>(p);
@@ -984,6 +983,7 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
     return r;
   };
   uint8_t *tk = take(ks * tb), *tv = take(ks * tb), *tq = take(qs * tb), *td = take(qs * tb);
+  TileRef *order_q = (TileRef*)take(qt * sizeof(TileRef)), *order_k = (TileRef*)take(kt * sizeof(TileRef));
   float* lse2 = (float*)take(qs * TILE * 4);
   float* delta = (float*)take(qs * TILE * 4);
   float* part_k = (float*)take(part_floats * 4);
@@ -992,7 +992,6 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   float *inv_q = (float*)take(qs * 4), *inv_d = (float*)take(qs * 4), *norm_d = (float*)take(qs * 4);
   float* delta_top = (float*)take(qs * 4);
   int *bad_k = (int*)take(ks * 4), *bad_v = (int*)take(ks * 4), *bad_q = (int*)take(qs * 4), *bad_d = (int*)take(qs * 4);
-  int *order_q = (int*)take(qt * 4), *order_k = (int*)take(kt * 4);
   TileSources src = {};
   src.keys = src.queries = 2;
   src.order_q = order_q;

@@ -45,7 +45,7 @@ __device__ __forceinline__ void load_part(float (&x)[8], const float* p, int lef
 
 // Tiles that the tile's CTA works through: key tiles that a query tile's last row
 // sees, or query tiles that see a key tile's first key.
-__device__ __forceinline__ int tile_work(const Shape& s, bool over_q, int id) {
+__device__ __forceinline__ int tile_work(const Shape& s, bool over_q, int id, TileRef* ref) {
   const int32_t* cu = over_q ? s.cu_q : s.cu_k;
   int lo = 0, hi = s.batch;
   while (hi - lo > 1) {
@@ -55,20 +55,22 @@ __device__ __forceinline__ int tile_work(const Shape& s, bool over_q, int id) {
   }
   const int j = id - ((cu[lo] >> 7) + lo);
   const Seq sq = seq_bounds(s, lo);
-  const int len = over_q ? sq.lq : sq.lk;
-  if (j < 0 || (long long)j * TILE >= len) return 0;
+  const bool in = j >= 0 && (long long)j * TILE < (over_q ? sq.lq : sq.lk);
+  *ref = {sq.q0, sq.k0, sq.lq, sq.lk, lo, in ? j : -1};
+  if (!in) return 0;
   if (over_q) return (sq.visible(min(j * TILE + TILE, sq.lq) - 1, s.causal) + TILE - 1) / TILE + 1;
   return max(0, (sq.lq - sq.first_row(j * TILE, s.causal) + TILE - 1) / TILE) + 1;
 }
 // One block: a counting sort by falling work.  Ids of equal work come in any order,
 // which changes when they are computed and nothing else.
-__device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, int* order) {
+__device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, TileRef* order) {
   __shared__ int count[ORDER_KEYS], sums[SP_THREADS / 32];
   static_assert(ORDER_KEYS == 2 * SP_THREADS, "two keys per thread");
   const int tid = threadIdx.x;
   count[tid] = count[tid + SP_THREADS] = 0;
   __syncthreads();
-  auto key = [&](int id) { return ORDER_KEYS - 1 - min(tile_work(s, over_q, id) >> shift, ORDER_KEYS - 1); };
+  TileRef ref;
+  auto key = [&](int id) { return ORDER_KEYS - 1 - min(tile_work(s, over_q, id, &ref) >> shift, ORDER_KEYS - 1); };
   for (int id = tid; id < tiles; id += SP_THREADS) atomicAdd(&count[key(id)], 1);
   __syncthreads();
   // exclusive prefix sums
@@ -85,7 +87,10 @@ __device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, i
   count[2 * tid] = x - a - b;
   count[2 * tid + 1] = x - b;
   __syncthreads();
-  for (int id = tid; id < tiles; id += SP_THREADS) order[atomicAdd(&count[key(id)], 1)] = id;
+  for (int id = tid; id < tiles; id += SP_THREADS) {
+    const int at = atomicAdd(&count[key(id)], 1);
+    order[at] = ref;
+  }
 }
 
 template <int DP>
@@ -249,7 +254,7 @@ struct FwdTiles {
   const float* inv_v;
   const int* bad_k;
   const int* bad_v;
-  const int* order;  // of the query tiles
+  const TileRef* order;  // of the query tiles
 };
 
 template <int DP>
@@ -273,11 +278,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the tiles that see the most keys start first
-  const int id = ft.order[blockIdx.x / (unsigned)s.heads], h = (int)(blockIdx.x % (unsigned)s.heads);
-  int jt;
-  const int b = seq_of_tile(s.cu_q, s.batch, id, &jt);
-  const Seq sq = seq_bounds(s, b);
-  if (jt < 0 || (long long)jt * TILE >= sq.lq) return;
+  const TileRef ref = load_ref(ft.order + blockIdx.x / (unsigned)s.heads);
+  const int h = (int)(blockIdx.x % (unsigned)s.heads), b = ref.b, jt = ref.jt;
+  const Seq sq = seq_of(ref);
+  if (jt < 0) return;
   const int i0 = jt * TILE, rows = min(TILE, sq.lq - i0);
   const int hk = h / s.group;
   const int nk = sq.visible(i0 + rows - 1, s.causal);  // keys that the tile's last row sees
@@ -608,16 +612,17 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
   JX_REQUIRE(qt * s.heads < (1LL << 31) && kt < (1LL << 31), "attention: too many rows");
   const size_t slots = (size_t)kt * s.kv_heads, bytes = slots * tile_bytes(DP);
   void* p = nullptr;
-  if (int rc = jx::scratch_get(2 * bytes + 4 * slots * sizeof(float) + qt * sizeof(int), &p, st)) return rc;
+  if (int rc = jx::scratch_get(2 * bytes + qt * sizeof(TileRef) + 4 * slots * sizeof(float), &p, st)) return rc;
   uint8_t* base = static_cast<uint8_t*>(p);
-  float* inv = reinterpret_cast<float*>(base + 2 * bytes);
+  TileRef* order = reinterpret_cast<TileRef*>(base + 2 * bytes);
+  float* inv = reinterpret_cast<float*>(order + qt);
   int* bad = reinterpret_cast<int*>(inv + 2 * slots);
   TileSources src = {};
   src.t[0] = {k, s.ldk, base, inv, bad};
   src.t[1] = {v, s.ldv, base + bytes, inv + slots, bad + slots};
   src.keys = 2;
-  src.order_q = bad + 2 * slots;
-  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, src.order_q};
+  src.order_q = order;
+  FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, order};
   int rc = split_tiles(s, src, DP, st);
   if (!rc) {
     const unsigned grid = (unsigned)(qt * s.heads);

@@ -323,15 +323,41 @@ struct TileSource {
   float* delta;
   float* delta_top;
 };
+// A tile of a packed sequence, as a CTA finds it with one load: everything that the
+// offsets say about it.
+struct __align__(16) TileRef {
+  long long q0, k0;  // of its sequence
+  int lq, lk, b, jt;  // jt: the tile's index within it, or -1: no tile
+};
+__device__ __forceinline__ TileRef load_ref(const TileRef* p) {
+  const int4 a = reinterpret_cast<const int4*>(p)[0], b = reinterpret_cast<const int4*>(p)[1];
+  TileRef r;
+  r.q0 = (long long)(uint32_t)a.x | ((long long)a.y << 32);
+  r.k0 = (long long)(uint32_t)a.z | ((long long)a.w << 32);
+  r.lq = b.x;
+  r.lk = b.y;
+  r.b = b.z;
+  r.jt = b.w;
+  return r;
+}
+__device__ __forceinline__ Seq seq_of(const TileRef& r) {
+  Seq s;
+  s.q0 = r.q0;
+  s.k0 = r.k0;
+  s.lq = r.lq;
+  s.lk = r.lk;
+  return s;
+}
+
 // One launch of split_tiles_kernel: tensors over the keys' tiles, then over the
 // query rows'.
 struct TileSources {
   TileSource t[4];
   int keys, queries;  // tensors of each kind
-  // Order of work: ids by falling work (query tiles by their key tiles, key tiles
-  // by their query rows), those behind a sequence's end last.  May be NULL.  work
+  // Order of work: tiles by falling work (query tiles by their key tiles, key tiles
+  // by their query rows), the ids behind a sequence's end last.  May be NULL.  work
   // >> shift is below ORDER_KEYS.
-  int *order_q, *order_k;
+  TileRef *order_q, *order_k;
   int shift, q_tiles, k_tiles;
 };
 constexpr int ORDER_KEYS = 1024;
