@@ -513,10 +513,12 @@ JX_API int jx_layernorm_bwd_f32(const float *dy, const float *x, const float *ga
  * that sees no key gets o = 0 and lse = -inf.  A key that a row does not see has
  * no effect on it, whatever its values.  lse [heads, total_q] may be NULL.
  * max_q / max_k: the longest sequences, a hint for the choice of kernel; any
- * value >= 0 gives right results.  The products run on the tensor cores with
- * each f32 operand split in two f16 parts under a power-of-two scale (22 bits),
- * f32 sums; a batch of at most 16 query rows per key head runs in plain f32,
- * split along the keys. */
+ * value >= 0 gives right results.  Prompts run on the tensor cores, each f32
+ * operand split in two f16 parts under a power-of-two scale (22 bits), f32 sums;
+ * few query rows per key head (decoding) run in plain f32.  128 rows of one head
+ * that hold a non-finite value, or largest magnitudes more than 2^20 apart, are
+ * computed row by row: as right, but slowly.  Make a first call of each kind
+ * before any stream capture, as for the library's other tensor-core kernels. */
 JX_API int jx_attention_f32(const float *q, const float *k, const float *v, float *o, float *lse,
                             const int32_t *cu_q, const int32_t *cu_k, int64_t batch, int64_t total_q, int64_t total_k,
                             int64_t max_q, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -526,8 +528,8 @@ JX_API int jx_attention_f32(const float *q, const float *k, const float *v, floa
  * lse of the forward pass.  dout has o's row stride, dq / dk / dv those of q / k
  * / v.  With p = exp(x - lse): dv = p^T dout, ds = p * (dout v^T -
  * rowsum(dout * o)), dq = scale * ds k, dk = scale * ds^T q, dk and dv summed
- * over the query heads that share a key head.  Every sum has a fixed order:
- * the same inputs give the same bits. */
+ * over the query heads that share a key head.  lse must be the forward pass's
+ * (p <= 1).  Every sum has a fixed order: the same inputs give the same bits. */
 JX_API int jx_attention_bwd_f32(const float *q, const float *k, const float *v, const float *o, const float *lse,
                                 const float *dout, float *dq, float *dk, float *dv, const int32_t *cu_q,
                                 const int32_t *cu_k, int64_t batch, int64_t total_q, int64_t total_k, int64_t max_q,
