@@ -185,6 +185,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiles are complete behind it
+  asm volatile("griddepcontrol.launch_dependents;");
   const TileRef ref = load_ref(bt.order_q + blockIdx.x / (unsigned)s.heads);
   const int h = (int)(blockIdx.x % (unsigned)s.heads), b = ref.b, jt = ref.jt;
   const Seq sq = seq_of(ref);
@@ -492,6 +494,12 @@ struct KvLayout {
 };
 static_assert(KvLayout<64>::SMEM <= 232448 && KvLayout<128>::SMEM <= 232448, "shared memory of an SM");
 
+// dk's and dv's CTAs start as dq's last ones run: they read nothing of dq's, and all
+// of dq's CTAs have seen the split complete before the first of these starts.
+// What follows in the stream waits for this kernel alone, so that it must not end
+// before dq's.
+__device__ __forceinline__ void after_dq() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 template <int DP>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_dkv_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
@@ -504,6 +512,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const uint32_t raw_addr = jxd::smem_u32(smem_raw), shift = ((raw_addr + 1023u) & ~1023u) - raw_addr;
   if (shift > (uint32_t)L::SPARE) {
     if (threadIdx.x == 0) atomicOr(s.err, JX_DEVERR_TIMEOUT);
+    after_dq();
     return;
   }
   uint8_t* smem = smem_raw + shift;
@@ -535,7 +544,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   const TileRef ref = load_ref(bt.order_k + w / (unsigned)s.kv_heads);
   const int hk = (int)(w % (unsigned)s.kv_heads), b = ref.b, jt = ref.jt;
   const Seq sq = seq_of(ref);
-  if (jt < 0) return;
+  if (jt < 0) {
+    after_dq();
+    return;
+  }
   const int j0 = jt * TILE, rows = min(TILE, sq.lk - j0);
   const int blk0 = sq.first_row(j0, s.causal) / BLK;
   const int nblk = max(0, (sq.lq + BLK - 1) / BLK - blk0);
@@ -654,6 +666,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       __syncwarp();
       jxd::tmem_dealloc(tmem, 512);
     }
+    after_dq();
     return;
   }
 
@@ -890,6 +903,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     __syncwarp();
     jxd::tmem_dealloc(tmem, 512);
   }
+  after_dq();
 }
 
 // The parts' sums in order, 16 key rows of one key head per block.
@@ -939,10 +953,10 @@ int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, c
     return rc;
   if (int rc = prepare_kernel((const void*)attn_dkv_kernel<DP>, DP == 128 ? 4 : 5, KvLayout<DP>::SMEM, BW_LAUNCH_REGS))
     return rc;
-  attn_dq_kernel<DP><<<(unsigned)((long long)bt.q_tiles * s.heads), BW_THREADS, DqLayout<DP>::SMEM, st>>>(
-      s, bt, q, k, v, o, lse, dout, dq);
-  attn_dkv_kernel<DP><<<(unsigned)((long long)bt.k_tiles * s.kv_heads * bt.parts), BW_THREADS, KvLayout<DP>::SMEM, st>>>(
-      s, bt, q, k, v, o, lse, dout, dk, dv);
+  JX_CUDA(launch_overlapped(attn_dq_kernel<DP>, (long long)bt.q_tiles * s.heads, BW_THREADS, DqLayout<DP>::SMEM, st, s,
+                            bt, q, k, v, o, lse, dout, dq));
+  JX_CUDA(launch_overlapped(attn_dkv_kernel<DP>, (long long)bt.k_tiles * s.kv_heads * bt.parts, BW_THREADS,
+                            KvLayout<DP>::SMEM, st, s, bt, q, k, v, o, lse, dout, dk, dv));
   if (bt.parts > 1) {
     const dim3 grid((unsigned)(bt.k_tiles * (TILE / JOIN_ROWS)), (unsigned)s.kv_heads);
     const bool vec = !(s.dim & 3) && !(s.ldk & 3) && !(s.ldv & 3) &&

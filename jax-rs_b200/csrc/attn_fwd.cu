@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) split_tiles_kernel(const __grid
                                                                    const __grid_constant__ TileSources src) {
   constexpr int PER_ROW = DP / 8, STEP = SP_THREADS / PER_ROW, ROWS = TILE / STEP;  // threads; rows at a time; rows each
   __shared__ uint32_t sm_top[SP_THREADS / 32], sm_low[SP_THREADS / 32];
+  asm volatile("griddepcontrol.launch_dependents;");
   if (blockIdx.x < 2) {  // the orders
     if (blockIdx.x == 0 && src.order_q) order_tiles(s, true, src.q_tiles, src.shift, src.order_q);
     if (blockIdx.x == 1 && src.order_k) order_tiles(s, false, src.k_tiles, src.shift, src.order_k);
@@ -277,6 +278,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the split is complete behind it
   // the tiles that see the most keys start first
   const TileRef ref = load_ref(ft.order + blockIdx.x / (unsigned)s.heads);
   const int h = (int)(blockIdx.x % (unsigned)s.heads), b = ref.b, jt = ref.jt;
@@ -628,13 +630,13 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
     const unsigned grid = (unsigned)(qt * s.heads);
     if (DP == 128) {
       if (!(rc = prepare_kernel((const void*)attn_fwd_kernel<128>, 0, fw_smem(128), FW_LAUNCH_REGS)))
-        attn_fwd_kernel<128><<<grid, FW_THREADS, fw_smem(128), st>>>(s, ft, q, k, v, o, lse);
+        rc = jx::check_cuda(launch_overlapped(attn_fwd_kernel<128>, grid, FW_THREADS, fw_smem(128), st, s, ft, q, k, v, o, lse),
+                            "attn_fwd_kernel");
     } else {
       if (!(rc = prepare_kernel((const void*)attn_fwd_kernel<64>, 1, fw_smem(64), FW_LAUNCH_REGS)))
-        attn_fwd_kernel<64><<<grid, FW_THREADS, fw_smem(64), st>>>(s, ft, q, k, v, o, lse);
+        rc = jx::check_cuda(launch_overlapped(attn_fwd_kernel<64>, grid, FW_THREADS, fw_smem(64), st, s, ft, q, k, v, o, lse),
+                            "attn_fwd_kernel");
     }
-    const cudaError_t e = cudaGetLastError();
-    if (!rc && e != cudaSuccess) rc = jx::check_cuda(e, "attn_fwd_kernel");
   }
   jx::scratch_release(p, st);
   return rc;

@@ -362,6 +362,23 @@ struct TileSources {
 };
 constexpr int ORDER_KEYS = 1024;
 
+// A launch whose CTAs may start while the last ones of the launch before it run.
+template <typename... Params, typename... Args>
+cudaError_t launch_overlapped(void (*kernel)(Params...), long long grid, int threads, size_t smem, cudaStream_t st,
+                              const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Implemented in attn_fwd.cu: one launch that splits all tensors of `src`.
 int split_tiles(const Shape& s, const TileSources& src, int DP, cudaStream_t st);
 int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs);
