@@ -22,8 +22,11 @@ using namespace jxa;
 using jxg::wait_bounded;
 
 // ---- splitting -----------------------------------------------------------------
-// One block per (tile, head, tensor): eight columns of two or four rows per thread.
-constexpr int SP_THREADS = 512;
+// One block per (tile, head, tensor): eight columns of four rows per thread.  (Of 64
+// columns with 512 threads, two rows each, the packed gradient's call takes 6 us
+// longer: the fewer blocks of an SM load and store in step.)
+__host__ __device__ constexpr int sp_threads(int DP) { return 4 * DP; }
+
 __device__ __forceinline__ void load_part(float (&x)[8], const float* p, int left, bool vec) {
 #pragma unroll
   for (int e = 0; e < 8; e += 4) {
@@ -63,19 +66,21 @@ __device__ __forceinline__ int tile_work(const Shape& s, bool over_q, int id, Ti
 }
 // One block: a counting sort by falling work.  Ids of equal work come in any order,
 // which changes when they are computed and nothing else.
+template <int THREADS>
 __device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, TileRef* order) {
-  __shared__ int count[ORDER_KEYS], sums[SP_THREADS / 32];
-  static_assert(ORDER_KEYS == 2 * SP_THREADS, "two keys per thread");
+  constexpr int EACH = ORDER_KEYS / THREADS;  // keys of a thread
+  __shared__ int count[ORDER_KEYS], sums[THREADS / 32];
   const int tid = threadIdx.x;
-  count[tid] = count[tid + SP_THREADS] = 0;
+  for (int i = tid; i < ORDER_KEYS; i += THREADS) count[i] = 0;
   __syncthreads();
   TileRef ref;
   auto key = [&](int id) { return ORDER_KEYS - 1 - min(tile_work(s, over_q, id, &ref) >> shift, ORDER_KEYS - 1); };
-  for (int id = tid; id < tiles; id += SP_THREADS) atomicAdd(&count[key(id)], 1);
+  for (int id = tid; id < tiles; id += THREADS) atomicAdd(&count[key(id)], 1);
   __syncthreads();
   // exclusive prefix sums
-  const int a = count[2 * tid], b = count[2 * tid + 1];
-  int x = a + b;
+  int own[EACH], x = 0;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) x += own[i] = count[EACH * tid + i];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -84,24 +89,25 @@ __device__ void order_tiles(const Shape& s, bool over_q, int tiles, int shift, T
   if ((tid & 31) == 31) sums[tid >> 5] = x;
   __syncthreads();
   for (int w = 0; w < (tid >> 5); ++w) x += sums[w];
-  count[2 * tid] = x - a - b;
-  count[2 * tid + 1] = x - b;
+#pragma unroll
+  for (int i = EACH - 1; i >= 0; --i) count[EACH * tid + i] = x -= own[i];
   __syncthreads();
-  for (int id = tid; id < tiles; id += SP_THREADS) {
+  for (int id = tid; id < tiles; id += THREADS) {
     const int at = atomicAdd(&count[key(id)], 1);
     order[at] = ref;
   }
 }
 
 template <int DP>
-__global__ void __launch_bounds__(SP_THREADS, 2) split_tiles_kernel(const __grid_constant__ Shape s,
-                                                                   const __grid_constant__ TileSources src) {
+__global__ void __launch_bounds__(sp_threads(DP), 1024 / sp_threads(DP))
+    split_tiles_kernel(const __grid_constant__ Shape s, const __grid_constant__ TileSources src) {
+  constexpr int SP_THREADS = sp_threads(DP);
   constexpr int PER_ROW = DP / 8, STEP = SP_THREADS / PER_ROW, ROWS = TILE / STEP;  // threads; rows at a time; rows each
   __shared__ uint32_t sm_top[SP_THREADS / 32], sm_low[SP_THREADS / 32];
   asm volatile("griddepcontrol.launch_dependents;");
   if (blockIdx.x < 2) {  // the orders
-    if (blockIdx.x == 0 && src.order_q) order_tiles(s, true, src.q_tiles, src.shift, src.order_q);
-    if (blockIdx.x == 1 && src.order_k) order_tiles(s, false, src.k_tiles, src.shift, src.order_k);
+    if (blockIdx.x == 0 && src.order_q) order_tiles<SP_THREADS>(s, true, src.q_tiles, src.shift, src.order_q);
+    if (blockIdx.x == 1 && src.order_k) order_tiles<SP_THREADS>(s, false, src.k_tiles, src.shift, src.order_k);
     return;
   }
   // the tensor, tile and head
@@ -581,8 +587,8 @@ int split_tiles(const Shape& s, const TileSources& src, int DP, cudaStream_t st)
   const long long blocks =
       2 + (long long)src.keys * ts.k_tiles * s.kv_heads + (long long)src.queries * ts.q_tiles * s.heads;
   JX_REQUIRE(blocks < (1LL << 31), "attention: too many rows");
-  if (DP == 128) split_tiles_kernel<128><<<(unsigned)blocks, SP_THREADS, 0, st>>>(s, ts);
-  else split_tiles_kernel<64><<<(unsigned)blocks, SP_THREADS, 0, st>>>(s, ts);
+  if (DP == 128) split_tiles_kernel<128><<<(unsigned)blocks, sp_threads(DP), 0, st>>>(s, ts);
+  else split_tiles_kernel<64><<<(unsigned)blocks, sp_threads(DP), 0, st>>>(s, ts);
   JX_LAUNCH_CHECK("split_tiles_kernel");
   return JX_OK;
 }
