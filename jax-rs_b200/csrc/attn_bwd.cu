@@ -28,7 +28,6 @@
 namespace {
 
 using namespace jxa;
-using jxg::wait_bounded;
 
 constexpr int BW_THREADS = 384;  // warp 0 copies, warp 1 MMA, warps 4..11 the rest
 constexpr int BW_FIRST = 4;
@@ -262,9 +261,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
              sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv, s.scale);
     }
     if (warp == 0 && lane == 0 && nb > 0) {  // the copies have landed
-      wait_bounded(stayfull, 0, s.err);
-      for (int j = 0; j < min(nb, K_FIRST); ++j) wait_bounded(&kfull[j], 0, s.err);
-      for (int j = 0; j < min(nb, V_FIRST); ++j) wait_bounded(&vfull[j], 0, s.err);
+      wait_suspended(stayfull, 0, s.err);
+      for (int j = 0; j < min(nb, K_FIRST); ++j) wait_suspended(&kfull[j], 0, s.err);
+      for (int j = 0; j < min(nb, V_FIRST); ++j) wait_suspended(&vfull[j], 0, s.err);
     }
     if (warp == 1) {
       __syncwarp();
@@ -278,9 +277,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     if (warp == 0 && nb > 0 && jxd::elect_one()) {
       // ---- the remaining copies
       int nk = min(nb, K_FIRST), nv = min(nb, V_FIRST);
-      bool ok = wait_bounded(moved, 0, s.err);  // the stages that Q and dO passed through are free
+      bool ok = wait_suspended(moved, 0, s.err);  // the stages that Q and dO passed through are free
       auto free_stage = [&](uint64_t* bar, int use) {
-        return ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)(use + 1) & 1u, s.err);
+        return ok = ok && !*abort_flag && wait_suspended(bar, (uint32_t)(use + 1) & 1u, s.err);
       };
       while (ok && (nk < nb || nv < nb)) {
         if (nv < nb && nv < nk) {
@@ -293,16 +292,16 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       }
       if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may end
-      wait_bounded(stayfull, 0, s.err);
-      for (int u = max(0, nk - KS); u < nk; ++u) wait_bounded(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
-      for (int u = max(0, nv - VS); u < nv; ++u) wait_bounded(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err);
+      wait_suspended(stayfull, 0, s.err);
+      for (int u = max(0, nk - KS); u < nk; ++u) wait_suspended(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
+      for (int u = max(0, nv - VS); u < nv; ++u) wait_suspended(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err);
     }
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
       // ---- MMA
       const uint32_t kbase = jxd::smem_u32(ring), vbase = kbase + KS * STAGE;
-      bool ok = wait_bounded(stayfull, 0, s.err) && wait_bounded(moved, 0, s.err);
+      bool ok = wait_suspended(stayfull, 0, s.err) && wait_suspended(moved, 0, s.err);
       auto ready = [&](uint64_t* bar, int n) {
-        ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)n & 1u, s.err);
+        ok = ok && !*abort_flag && wait_suspended(bar, (uint32_t)n & 1u, s.err);
         jxd::tc_fence_after();
         return ok;
       };
@@ -657,10 +656,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
               s.scale);
     }
     if (warp == 0 && lane == 0 && n > 0) {  // the copies have landed
-      wait_bounded(stayfull, 0, s.err);
-      for (int u = 0; u < min(n, Q_FIRST); ++u) wait_bounded(&qfull[u], 0, s.err);
-      for (int u = 0; u < min(n, DS); ++u) wait_bounded(&dfull[u], 0, s.err);
-      for (int u = 0; u < min(n, 2); ++u) wait_bounded(&tfull[u], 0, s.err);
+      wait_suspended(stayfull, 0, s.err);
+      for (int u = 0; u < min(n, Q_FIRST); ++u) wait_suspended(&qfull[u], 0, s.err);
+      for (int u = 0; u < min(n, DS); ++u) wait_suspended(&dfull[u], 0, s.err);
+      for (int u = 0; u < min(n, 2); ++u) wait_suspended(&tfull[u], 0, s.err);
     }
     if (warp == 1) {
       __syncwarp();
@@ -677,9 +676,9 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       // Q(0) Q(1) dout(0) statistics(0) Q(2) dout(1) statistics(1) ...: dK(u), which the copies of
       // block u+3 of Q and u+2 of the statistics wait for, needs nothing behind dout(u+1) in this order
       int nq = min(n, Q_FIRST), nd = min(n, DS), nt = min(n, 2);
-      bool ok = L::APART || wait_bounded(moved, 0, s.err);  // the stages that V passed through are free
+      bool ok = L::APART || wait_suspended(moved, 0, s.err);  // the stages that V passed through are free
       auto free_stage = [&](uint64_t* bar, int use) {
-        return ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)(use + 1) & 1u, s.err);
+        return ok = ok && !*abort_flag && wait_suspended(bar, (uint32_t)(use + 1) & 1u, s.err);
       };
       for (int i = 0; ok && i <= n; ++i) {
         if (i == nq && i < n) {
@@ -701,17 +700,17 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       }
       if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may end
-      wait_bounded(stayfull, 0, s.err);
-      for (int e = max(0, nq - QS); e < nq; ++e) wait_bounded(&qfull[e % QS], (uint32_t)(e / QS) & 1u, s.err);
-      for (int e = max(0, nd - DS); e < nd; ++e) wait_bounded(&dfull[e % DS], (uint32_t)(e / DS) & 1u, s.err);
-      for (int e = max(0, nt - 2); e < nt; ++e) wait_bounded(&tfull[e & 1], (uint32_t)(e >> 1) & 1u, s.err);
+      wait_suspended(stayfull, 0, s.err);
+      for (int e = max(0, nq - QS); e < nq; ++e) wait_suspended(&qfull[e % QS], (uint32_t)(e / QS) & 1u, s.err);
+      for (int e = max(0, nd - DS); e < nd; ++e) wait_suspended(&dfull[e % DS], (uint32_t)(e / DS) & 1u, s.err);
+      for (int e = max(0, nt - 2); e < nt; ++e) wait_suspended(&tfull[e & 1], (uint32_t)(e >> 1) & 1u, s.err);
     }
     if (warp == 1 && n > 0 && jxd::elect_one()) {
       // ---- MMA
       const uint32_t qbase = jxd::smem_u32(ring), dbase = qbase + QS * STAGE;
-      bool ok = wait_bounded(stayfull, 0, s.err) && (L::APART || wait_bounded(moved, 0, s.err));
+      bool ok = wait_suspended(stayfull, 0, s.err) && (L::APART || wait_suspended(moved, 0, s.err));
       auto ready = [&](uint64_t* bar, int i) {
-        ok = ok && !*abort_flag && wait_bounded(bar, (uint32_t)i & 1u, s.err);
+        ok = ok && !*abort_flag && wait_suspended(bar, (uint32_t)i & 1u, s.err);
         jxd::tc_fence_after();
         return ok;
       };

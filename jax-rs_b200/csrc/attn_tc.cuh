@@ -163,8 +163,7 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
       "l"(src), "r"(bytes), "r"(jxd::smem_u32(bar))
       : "memory");
 }
-// jxg::wait_bounded that polls without suspending the thread: the steps that wait
-// here are a few hundred cycles apart.
+// Whether a phase is complete.
 __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -176,22 +175,31 @@ __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool spin_bounded(uint64_t* bar, uint32_t parity, unsigned int* err) {
-  if (poll(bar, parity)) return true;
-  const uint64_t t0 = jxg::global_ns();
-  while (true) {
-    for (int i = 0; i < 1024; ++i)
-      if (poll(bar, parity)) return true;
-    if (jxg::global_ns() - t0 > 4000000000ull) {
+// Bounded waits in a few instructions (2^26 of them are seconds): where jxg::wait_bounded
+// with its clock stood at every wait, the gradients' loops were so long that fetching
+// instructions cost packed sequences 7% of their time.
+__device__ __forceinline__ bool wait_polling(uint64_t* bar, uint32_t parity, unsigned int* err) {
+  for (uint32_t i = 0; !poll(bar, parity); ++i) {
+    if (i == 1u << 26) {
       atomicOr(err, JX_DEVERR_TIMEOUT);
       return false;
     }
   }
+  return true;
+}
+__device__ __forceinline__ bool wait_suspended(uint64_t* bar, uint32_t parity, unsigned int* err) {
+  for (uint32_t i = 0; !jxd::mbar_try_wait(bar, parity); ++i) {
+    if (i == 1u << 26) {
+      atomicOr(err, JX_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
 }
 // One lane polls for its warp.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
   int got = 1;
-  if ((threadIdx.x & 31) == 0) got = spin_bounded(bar, parity, err) ? 1 : 0;
+  if ((threadIdx.x & 31) == 0) got = wait_polling(bar, parity, err) ? 1 : 0;
   got = __shfl_sync(0xffffffffu, got, 0);
   if (!got) *abort_flag = 1;
   return got != 0;
