@@ -297,11 +297,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       for (int u = max(0, nv - VS); u < nv; ++u) wait_suspended(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err);
     }
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
-      // ---- MMA
+      // ---- MMA (its waits stand between products: nothing is looked at there but the barrier)
       const uint32_t kbase = jxd::smem_u32(ring), vbase = kbase + KS * STAGE;
       bool ok = wait_suspended(stayfull, 0, s.err) && wait_suspended(moved, 0, s.err);
       auto ready = [&](uint64_t* bar, int n) {
-        ok = ok && !*abort_flag && wait_suspended(bar, (uint32_t)n & 1u, s.err);
+        ok = ok && wait_polling(bar, (uint32_t)n & 1u, s.err);
         jxd::tc_fence_after();
         return ok;
       };
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
     auto ready = [&](uint64_t* bar, int n) {
-      ok = ok && warp_wait(bar, (uint32_t)n & 1u, abort_flag, s.err);
+      warp_wait(bar, (uint32_t)n & 1u, ok, abort_flag, s.err);
       jxd::tc_fence_after();
     };
     auto done = [&](uint64_t* bar) {
@@ -710,7 +710,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const uint32_t qbase = jxd::smem_u32(ring), dbase = qbase + QS * STAGE;
       bool ok = wait_suspended(stayfull, 0, s.err) && (L::APART || wait_suspended(moved, 0, s.err));
       auto ready = [&](uint64_t* bar, int i) {
-        ok = ok && !*abort_flag && wait_suspended(bar, (uint32_t)i & 1u, s.err);
+        ok = ok && wait_polling(bar, (uint32_t)i & 1u, s.err);
         jxd::tc_fence_after();
         return ok;
       };
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
     auto ready = [&](uint64_t* bar, int i) {
-      ok = ok && warp_wait(bar, (uint32_t)i & 1u, abort_flag, s.err);
+      warp_wait(bar, (uint32_t)i & 1u, ok, abort_flag, s.err);
       jxd::tc_fence_after();
     };
     auto done = [&](uint64_t* bar) {
@@ -790,20 +790,24 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     constexpr int C = BLK / 2;  // columns of the scores that this thread has
     // a block's numbers are loaded a block ahead
     float next_q = 0.0f, next_d = 0.0f, next_n = 0.0f, next_t = 0.0f;
-    auto look_ahead = [&](int u) {
-      int place;
-      const long long slot = slot_of(min(u, n - 1), &place);
+    int ahead_g = n > 0 ? it0 / nblk : 0, ahead_b = n > 0 ? it0 % nblk : 0;  // its head and place among the head's blocks
+    auto look_ahead = [&](bool more) {
+      const long long slot = qslot0 + (long long)((blk0 + ahead_b) / PER_TILE) * s.heads + ahead_g;
+      if (more && ++ahead_b == nblk) {
+        ahead_b = 0;
+        ++ahead_g;
+      }
       next_q = bt.inv_q[slot];
       next_d = bt.inv_d[slot];
       next_n = bt.norm_d[slot];
       next_t = bt.delta_top[slot];
     };
-    if (n > 0) look_ahead(0);
+    if (n > 0) look_ahead(n > 1);
     int i0 = (blk0 + (n > 0 ? it0 % nblk : 0) - 1) * BLK;  // the block's first row
     for (int u = 0; u < n; ++u) {
       i0 = i0 + BLK >= sq.lq ? blk0 * BLK : i0 + BLK;  // the next block, or the next head's first
       const float inv_q = next_q, inv_d = next_d, norm_d = next_n, top_d = next_t;
-      look_ahead(u + 1);
+      look_ahead(u + 2 < n);
       const float* lse2 = stats + (u & 1) * 2 * BLK + half * C;
       const float* delta = lse2 + BLK;
       const uint32_t xa = tmem + lanes + L::X + (u & 1) * L::X_STEP + half * C;
@@ -812,7 +816,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       const float2 f2 = make_float2(f, f);
       const bool edge = i0 < first_all || rows < TILE;  // some key is not seen by all of the block's rows
       float2 p[C / 2];
-      ready(&tfull[u & 1], u >> 1);
+      warp_wait(&tfull[u & 1], (uint32_t)(u >> 1) & 1u, ok, abort_flag, s.err);
       ready(&sfull[u & 1], u >> 1);
 #pragma unroll
       for (int c = 0; c < C; c += 32) {

@@ -251,7 +251,7 @@ constexpr uint32_t T_Q = 256, T_O = 384;  // columns of tensor memory; S0 at 0, 
 // before the hi part is.
 __host__ __device__ constexpr int fw_stages(int DP) { return DP == 128 ? 6 : 12; }
 __host__ __device__ constexpr size_t fw_smem(int DP) {
-  return (size_t)fw_stages(DP) * tile_part(DP) + 1024 /*align*/ + 2 * 128 * 4 /*exchange*/ + 512 /*barriers*/;
+  return (size_t)fw_stages(DP) * tile_part(DP) + 1024 /*align*/ + 4 * 128 * 4 /*exchange*/ + 512 /*barriers*/;
 }
 
 struct FwdTiles {
@@ -272,8 +272,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
-  float* xch = reinterpret_cast<float*>(smem + STAGES * STAGE);  // [2][128]
-  uint64_t* full = reinterpret_cast<uint64_t*>(xch + 2 * 128);   // [STAGES]
+  float* xch = reinterpret_cast<float*>(smem + STAGES * STAGE);  // [2][2][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(xch + 4 * 128);   // [STAGES]
   uint64_t* empty = full + STAGES;                               // [STAGES]
   uint64_t* sfull = empty + STAGES;                              // [2]
   uint64_t* pfull = sfull + 2;                                   // [2]
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       bool ok = wait_bounded(qfull, 0, s.err);
       // the next stage's shared-memory address once its copy has landed
       auto next = [&]() {
-        ok = ok && !*abort_flag && wait_bounded(&full[stage], phase, s.err);
+        ok = ok && wait_polling(&full[stage], phase, s.err);
         jxd::tc_fence_after();
         return sbase + stage * STAGE;
       };
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       scores(0);
       for (int j = 0; j < nb && ok; ++j) {
         if (j + 1 < nb) scores(j + 1);
-        if (!ok || !(ok = !*abort_flag && wait_bounded(&pfull[j & 1], (uint32_t)(j >> 1) & 1u, s.err) &&
-                          wait_bounded(ofree, (uint32_t)(j + 1) & 1u, s.err)))
+        if (!ok || !(ok = wait_polling(&pfull[j & 1], (uint32_t)(j >> 1) & 1u, s.err) &&
+                          wait_polling(ofree, (uint32_t)(j + 1) & 1u, s.err)))
           break;
         const uint32_t p = tmem + (j & 1) * 128u, d = tmem + T_O;
         // P's keys 0..63: hi at column 0, lo at 32; keys 64..127: hi at 64, lo at 96
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     bool ok = true;
 
     auto add_part = [&](int j, float alpha, float inv_v) {
-      ok = ok && warp_wait(ofull, (uint32_t)j & 1u, abort_flag, s.err);
+      warp_wait(ofull, (uint32_t)j & 1u, ok, abort_flag, s.err);
       jxd::tc_fence_after();
 #pragma unroll
       for (int c = 0; c < DP / 2; c += 32) {
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       const float inv_k = ft.inv_k[slot0 + (long long)j * s.kv_heads];
       const float inv_v = ft.inv_v[slot0 + (long long)j * s.kv_heads];
       const float f = fmaxf(f_row * inv_k, 1.17549435e-38f);  // above zero, so that a masked score stays -inf
-      ok = ok && warp_wait(&sfull[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag, s.err);
+      warp_wait(&sfull[j & 1], (uint32_t)(j >> 1) & 1u, ok, abort_flag, s.err);
       jxd::tc_fence_after();
       const uint32_t s_addr = tmem + lanes + (j & 1) * 128u + half * 64u;
       float sc[64];
@@ -522,11 +522,11 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       float mx = sc[0];
 #pragma unroll
       for (int i = 1; i < 64; ++i) mx = fmaxf(mx, sc[i]);
-      // the row's other half
-      xch[half * 128 + row] = mx;
+      // the row's other half (two turns: who writes a place again has seen the other at the turn between)
+      float* turn = xch + (j & 1) * 256;
+      turn[half * 128 + row] = mx;
       pair_sync(1 + quarter);
-      mx = fmaxf(mx, xch[(half ^ 1) * 128 + row]);
-      pair_sync(1 + quarter);
+      mx = fmaxf(mx, turn[(half ^ 1) * 128 + row]);
       const float m_new = mx == -INFINITY ? m : fmaxf(m, mx * f);
       const float base = m_new == -INFINITY ? 0.0f : m_new;
       const float alpha = exp2_fast(m - base);
@@ -555,6 +555,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     }
     if (nb > 0) add_part(nb - 1, alpha_prev, inv_v_prev);
 
+    xch += (nb & 1) * 256;
     xch[half * 128 + row] = sum;
     pair_sync(1 + quarter);
     sum += xch[(half ^ 1) * 128 + row];

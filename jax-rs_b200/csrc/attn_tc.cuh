@@ -196,13 +196,20 @@ __device__ __forceinline__ bool wait_suspended(uint64_t* bar, uint32_t parity, u
   }
   return true;
 }
-// One lane polls for its warp.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, unsigned int* err) {
-  int got = 1;
-  if ((threadIdx.x & 31) == 0) got = wait_polling(bar, parity, err) ? 1 : 0;
-  got = __shfl_sync(0xffffffffu, got, 0);
-  if (!got) *abort_flag = 1;
-  return got != 0;
+// A warp waits, every lane for itself: polling by one lane and telling the others
+// cost 100 cycles more at each of the three to five waits of a step.
+__device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, bool& ok, volatile int* abort_flag,
+                                          unsigned int* err) {
+  uint32_t i = ok ? 0 : 1u << 26;
+  while (!poll(bar, parity)) {
+    if (i++ >= 1u << 26) {
+      if (ok) atomicOr(err, JX_DEVERR_TIMEOUT);
+      ok = false;
+      *abort_flag = 1;
+      break;
+    }
+  }
+  __syncwarp();
 }
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
