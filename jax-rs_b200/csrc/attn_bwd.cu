@@ -39,9 +39,10 @@ static_assert(128 * BW_LOW_REGS + 256 * BW_HIGH_REGS <= BW_THREADS * BW_LAUNCH_R
 
 struct BwdTiles {
   const uint8_t *q, *k, *v, *d;  // tiles; d is dout
-  const float *inv_q, *inv_k, *inv_v, *inv_d;
+  const float4* num_q;  // of a tile of query rows: what undoes Q's scale and dout's, dout's largest row norm, delta's largest magnitude
+  const float4* num_k;  // of a tile of keys: what undoes K's scale and V's, V's largest row norm
   const int *bad_q, *bad_k, *bad_v, *bad_d;
-  const float *norm_v, *norm_d, *lse2, *delta, *delta_top;
+  const float *lse2, *delta;
   int q_tiles, k_tiles, parts;
   const TileRef *order_q, *order_k;
   float *part_k, *part_v;  // [parts][total_k * kv_heads * dim], used where parts > 1
@@ -358,7 +359,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       tmem_st_wait();
       done(moved);
     }
-    const float f_tile = bt.inv_q[qslot] * (s.scale * LOG2E), inv_d = bt.inv_d[qslot], norm_d = bt.norm_d[qslot];
+    const float4 num = bt.num_q[qslot];
+    const float f_tile = num.x * (s.scale * LOG2E), inv_d = num.y, norm_d = num.z;
     const float lse2 = bt.lse2[qslot * TILE + row], delta = bt.delta[qslot * TILE + row];
     const int vis = row < rows ? sq.visible(i0 + row, s.causal) : 0;
     const int vis_all = sq.visible(i0, s.causal);
@@ -369,19 +371,13 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     float g_prev = 0.0f;
     float2 p[32];
     // P of tile j, scaled for dS, and what undoes dS's scale; the next tile's numbers are loaded a tile ahead
-    float dl = 0.0f, g = 0.0f, inv_k = 0.0f, inv_v = 0.0f, norm_v = 0.0f, next_k = 0.0f, next_v = 0.0f, next_n = 0.0f;
-    auto look_ahead = [&](int j) {
-      const long long slot = slot0 + (long long)min(j, nb - 1) * s.kv_heads;
-      next_k = bt.inv_k[slot];
-      next_v = bt.inv_v[slot];
-      next_n = bt.norm_v[slot];
-    };
-    if (nb > 0) look_ahead(0);
+    float dl = 0.0f, g = 0.0f;
+    const float4* num_k = bt.num_k + slot0;
+    float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (nb > 0) next = *num_k;
     auto weights = [&](int j) {
-      inv_k = next_k;
-      inv_v = next_v;
-      norm_v = next_n;
-      look_ahead(j + 1);
+      const float inv_k = next.x, inv_v = next.y, norm_v = next.z;
+      if (j + 1 < nb) next = *(num_k += s.kv_heads);
       // P is at most 2^14
       const float fd = inv_d * inv_v, sc = bound_scale(16384.0f * (norm_d * norm_v + fabsf(delta)));
       const float f = f_tile * inv_k, pf = sc * fd;
@@ -485,11 +481,11 @@ struct KvLayout {
   static constexpr int PANEL_BYTES = BLK * 128;                                    // of a block
   static constexpr int STAGE = DP / 64 * 2 * PANEL_BYTES;                          // one block: 32 KB
   static constexpr int STAY = APART ? 2 * tile_bytes(DP) : tile_bytes(DP);         // shared memory for K (and V)
-  static constexpr int STATS = 2 * 2 * BLK * 4;  // lse2 and delta of two blocks
+  static constexpr int STATS = 2 * BLK + 4;  // floats of a block's lse2, delta and its tile's numbers; two blocks
   // What is left of an SM's 227 KB for aligning the tiles to 1024 bytes.  The array is
   // declared so aligned; a base that were not would be refused.
   static constexpr int SPARE = 768;
-  static constexpr size_t SMEM = STAY + (size_t)(QS + DS) * STAGE + STATS + 256 + SPARE;
+  static constexpr size_t SMEM = STAY + (size_t)(QS + DS) * STAGE + 2 * STATS * 4 + 208 + SPARE;
 };
 static_assert(KvLayout<64>::SMEM <= 232448 && KvLayout<128>::SMEM <= 232448, "shared memory of an SM");
 
@@ -516,8 +512,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   }
   uint8_t* smem = smem_raw + shift;
   uint8_t* ring = smem + L::STAY;  // Q's stages, then dout's
-  float* stats = reinterpret_cast<float*>(ring + (QS + DS) * STAGE);  // [2][lse2 BLK, delta BLK]
-  uint64_t* qfull = reinterpret_cast<uint64_t*>(stats + 4 * BLK);
+  float* stats = reinterpret_cast<float*>(ring + (QS + DS) * STAGE);  // [2][lse2 BLK, delta BLK, numbers 4]
+  uint64_t* qfull = reinterpret_cast<uint64_t*>(stats + 2 * L::STATS);
   uint64_t* qempty = qfull + QS;
   uint64_t* dfull = qempty + QS;
   uint64_t* dempty = dfull + DS;
@@ -591,10 +587,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   auto copy_stats = [&](int u) {
     int place;
     const long long slot = slot_of(u, &place);
-    float* dst = stats + (u & 1) * 2 * BLK;
-    jxd::mbar_arrive_expect_tx(&tfull[u & 1], 2 * BLK * 4);
+    float* dst = stats + (u & 1) * L::STATS;
+    jxd::mbar_arrive_expect_tx(&tfull[u & 1], L::STATS * 4);
     bulk_load(jxd::smem_u32(dst), bt.lse2 + slot * TILE + place * BLK, BLK * 4, &tfull[u & 1]);
     bulk_load(jxd::smem_u32(dst + BLK), bt.delta + slot * TILE + place * BLK, BLK * 4, &tfull[u & 1]);
+    bulk_load(jxd::smem_u32(dst + 2 * BLK), bt.num_q + slot, 16, &tfull[u & 1]);
   };
   bool bad = false;
   if (warp == 0 && lane == 0) {
@@ -779,7 +776,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       tmem_st_wait();
       done(moved);
     }
-    const float f_tile = bt.inv_k[kslot] * (s.scale * LOG2E), inv_v = bt.inv_v[kslot], norm_v = bt.norm_v[kslot];
+    const float4 num_k = bt.num_k[kslot];
+    const float f_tile = num_k.x * (s.scale * LOG2E), inv_v = num_k.y, norm_v = num_k.z;
     const int first = row < rows ? sq.first_row(j0 + row, s.causal) : 0x7fffffff;  // first query row that sees this key
     const int first_all = sq.first_row(j0 + rows - 1, s.causal);
 
@@ -788,35 +786,19 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     for (int c = 0; c < DP / 2; ++c) ak[c] = av[c] = 0.0f;
     float g_prev = 0.0f;
     constexpr int C = BLK / 2;  // columns of the scores that this thread has
-    // a block's numbers are loaded a block ahead
-    float next_q = 0.0f, next_d = 0.0f, next_n = 0.0f, next_t = 0.0f;
-    int ahead_g = n > 0 ? it0 / nblk : 0, ahead_b = n > 0 ? it0 % nblk : 0;  // its head and place among the head's blocks
-    auto look_ahead = [&](bool more) {
-      const long long slot = qslot0 + (long long)((blk0 + ahead_b) / PER_TILE) * s.heads + ahead_g;
-      if (more && ++ahead_b == nblk) {
-        ahead_b = 0;
-        ++ahead_g;
-      }
-      next_q = bt.inv_q[slot];
-      next_d = bt.inv_d[slot];
-      next_n = bt.norm_d[slot];
-      next_t = bt.delta_top[slot];
-    };
-    if (n > 0) look_ahead(n > 1);
     int i0 = (blk0 + (n > 0 ? it0 % nblk : 0) - 1) * BLK;  // the block's first row
     for (int u = 0; u < n; ++u) {
       i0 = i0 + BLK >= sq.lq ? blk0 * BLK : i0 + BLK;  // the next block, or the next head's first
-      const float inv_q = next_q, inv_d = next_d, norm_d = next_n, top_d = next_t;
-      look_ahead(u + 2 < n);
-      const float* lse2 = stats + (u & 1) * 2 * BLK + half * C;
+      const float* lse2 = stats + (u & 1) * L::STATS + half * C;
       const float* delta = lse2 + BLK;
       const uint32_t xa = tmem + lanes + L::X + (u & 1) * L::X_STEP + half * C;
       const uint32_t ya = tmem + lanes + L::Y + (u & 1) * L::Y_STEP + half * C;
-      const float f = f_tile * inv_q;
-      const float2 f2 = make_float2(f, f);
       const bool edge = i0 < first_all || rows < TILE;  // some key is not seen by all of the block's rows
       float2 p[C / 2];
       warp_wait(&tfull[u & 1], (uint32_t)(u >> 1) & 1u, ok, abort_flag, s.err);
+      const float4 num = *reinterpret_cast<const float4*>(stats + (u & 1) * L::STATS + 2 * BLK);
+      const float inv_q = num.x, inv_d = num.y, norm_d = num.z, top_d = num.w, f = f_tile * inv_q;
+      const float2 f2 = make_float2(f, f);
       ready(&sfull[u & 1], u >> 1);
 #pragma unroll
       for (int c = 0; c < C; c += 32) {
@@ -989,7 +971,7 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
   const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
   // tiles first, then arrays whose pieces the copies read 16-byte aligned, then the rest
-  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (5 * ks + 6 * qs) * 4 + (qt + kt) * sizeof(TileRef) +
+  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (6 * ks + 6 * qs) * 4 + (qt + kt) * sizeof(TileRef) +
                        2 * part_floats * 4;
   void* p = nullptr;
   if (int rc = jx::scratch_get(bytes + 64, &p, st)) return rc;
@@ -1003,22 +985,21 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   TileRef *order_q = (TileRef*)take(qt * sizeof(TileRef)), *order_k = (TileRef*)take(kt * sizeof(TileRef));
   float* lse2 = (float*)take(qs * TILE * 4);
   float* delta = (float*)take(qs * TILE * 4);
+  float *num_q = (float*)take(qs * 16), *num_k = (float*)take(ks * 16);
   float* part_k = (float*)take(part_floats * 4);
   float* part_v = (float*)take(part_floats * 4);
-  float *inv_k = (float*)take(ks * 4), *inv_v = (float*)take(ks * 4), *norm_v = (float*)take(ks * 4);
-  float *inv_q = (float*)take(qs * 4), *inv_d = (float*)take(qs * 4), *norm_d = (float*)take(qs * 4);
-  float* delta_top = (float*)take(qs * 4);
   int *bad_k = (int*)take(ks * 4), *bad_v = (int*)take(ks * 4), *bad_q = (int*)take(qs * 4), *bad_d = (int*)take(qs * 4);
   TileSources src = {};
   src.keys = src.queries = 2;
   src.order_q = order_q;
   src.order_k = order_k;
-  src.t[0] = {k, s.ldk, tk, inv_k, bad_k};
-  src.t[1] = {v, s.ldv, tv, inv_v, bad_v, norm_v};
-  src.t[2] = {q, s.ldq, tq, inv_q, bad_q};
-  src.t[3] = {dout, s.ldo, td, inv_d, bad_d, norm_d, o, lse, lse2, delta, delta_top};
-  const BwdTiles bt = {tq,     tk,     tv,    td,    inv_q, inv_k,     inv_v,   inv_d,   bad_q, bad_k,  bad_v,
-                       bad_d,  norm_v, norm_d, lse2, delta, delta_top, (int)qt, (int)kt, parts, order_q, order_k, part_k, part_v};
+  src.t[0] = {k, s.ldk, tk, num_k, bad_k, 4};
+  src.t[1] = {v, s.ldv, tv, num_k + 1, bad_v, 4, num_k + 2};
+  src.t[2] = {q, s.ldq, tq, num_q, bad_q, 4};
+  src.t[3] = {dout, s.ldo, td, num_q + 1, bad_d, 4, num_q + 2, o, lse, lse2, delta, num_q + 3};
+  const BwdTiles bt = {tq,    tk,    tv,    td,    (const float4*)num_q, (const float4*)num_k, bad_q, bad_k,
+                       bad_v, bad_d, lse2,  delta, (int)qt,              (int)kt,              parts, order_q,
+                       order_k, part_k, part_v};
   int rc = split_tiles(s, src, DP, st);
   if (!rc)
     rc = DP == 128 ? launch<128>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st)

@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(sp_threads(DP), 1024 / sp_threads(DP))
   const int e_top = (int)(top >> 23), e_low = (int)(low >> 23);
   const long long slot = (long long)id * heads + h;
   if (threadIdx.x == 0) {
-    t.inverse[slot] = inverse_of(e_top);
+    t.inverse[slot * t.step] = inverse_of(e_top);
     t.bad[slot] = unscaled(top) || (top && e_top - e_low > WIDE_BITS);
   }
   const float factor = scale_of(e_top);
@@ -228,9 +228,9 @@ __global__ void __launch_bounds__(sp_threads(DP), 1024 / sp_threads(DP))
         most = fmaxf(most, __uint_as_float(sm_top[w]));
         most_delta = fmaxf(most_delta, __uint_as_float(sm_low[w]));
       }
-      t.norm[slot] = sqrtf(most) * inverse_of(e_top);
+      t.norm[slot * t.step] = sqrtf(most) * inverse_of(e_top);
       if (t.o) {
-        t.delta_top[slot] = most_delta;
+        t.delta_top[slot * t.step] = most_delta;
         if (odd) t.bad[slot] = 1;
       }
     }
@@ -627,8 +627,8 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
   float* inv = reinterpret_cast<float*>(order + qt);
   int* bad = reinterpret_cast<int*>(inv + 2 * slots);
   TileSources src = {};
-  src.t[0] = {k, s.ldk, base, inv, bad};
-  src.t[1] = {v, s.ldv, base + bytes, inv + slots, bad + slots};
+  src.t[0] = {k, s.ldk, base, inv, bad, 1};
+  src.t[1] = {v, s.ldv, base + bytes, inv + slots, bad + slots, 1};
   src.keys = 2;
   src.order_q = order;
   FwdTiles ft = {base, base + bytes, inv, inv + slots, bad, bad + slots, order};

@@ -326,12 +326,13 @@ struct TileSource {
   const float* x;
   long long ld;
   uint8_t* tiles;
-  float* inverse;  // of the tile's scale, [id][head]
+  float* inverse;  // of the tile's scale, [id][head], `step` floats apart, as are norm and delta_top
   int* bad;        // the tile is marked, [id][head]
-  float* norm;     // largest Euclidean norm of the tile's rows, [id][head]; may be NULL
+  int step;
+  float* norm;     // largest Euclidean norm of the tile's rows; may be NULL
   // for dout alone (NULL otherwise): o and lse; the rows' lse in base 2 less
   // P_SHIFT (+inf for rows without keys or behind the end) and rowsum(dout o), [id][head][TILE]; the
-  // largest magnitude of the latter, [id][head]
+  // largest magnitude of the latter
   const float* o;
   const float* lse;
   float* lse2;
