@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
       // ---- MMA (its waits stand between products: nothing is looked at there but the barrier)
       const uint32_t kbase = jxd::smem_u32(ring), vbase = kbase + KS * STAGE;
-      bool ok = wait_suspended(stayfull, 0, s.err) && wait_suspended(moved, 0, s.err);
+      bool ok = wait_polling(stayfull, 0, s.err);
       auto ready = [&](uint64_t* bar, int n) {
         ok = ok && wait_polling(bar, (uint32_t)n & 1u, s.err);
         jxd::tc_fence_after();
@@ -318,9 +318,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         jxd::mma_commit(dpfull);
         jxd::mma_commit(&vempty[j % VS]);
       };
-      q_scores(0);
-      if (L::AHEAD && nb > 1) q_scores(1);
-      d_scores(0);
+      if (!L::AHEAD) ready(moved, 0);
+      if (ok) q_scores(0);
+      if (L::AHEAD && ok && nb > 1) q_scores(1);
+      if (L::AHEAD) ready(moved, 0);
+      if (ok) d_scores(0);
       for (int j = 0; ok && j < nb; ++j) {
         if (!ready(dsfull, j)) break;
         if (L::AHEAD && j + 1 < nb) d_scores(j + 1);    // Y is read
