@@ -175,9 +175,9 @@ __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded waits in a few instructions (2^26 of them are seconds): where jxg::wait_bounded
-// with its clock stood at every wait, the gradients' loops were so long that fetching
-// instructions cost packed sequences 7% of their time.
+// Bounded waits in a few instructions (2^26 of them are seconds).  With
+// jxg::wait_bounded and its clock at every wait the gradient of packed sequences took 7%
+// longer.  The copies' thread may be suspended; the others poll.
 __device__ __forceinline__ bool wait_polling(uint64_t* bar, uint32_t parity, unsigned int* err) {
   for (uint32_t i = 0; !poll(bar, parity); ++i) {
     if (i == 1u << 26) {
