@@ -528,7 +528,8 @@ JX_API int jx_attention_f32(const float *q, const float *k, const float *v, floa
  * lse of the forward pass.  dout has o's row stride, dq / dk / dv those of q / k
  * / v.  With p = exp(x - lse): dv = p^T dout, ds = p * (dout v^T -
  * rowsum(dout * o)), dq = scale * ds k, dk = scale * ds^T q, dk and dv summed
- * over the query heads that share a key head.  lse must be the forward pass's
+ * over the query heads that share a key head.  No gradient may overlap an input or
+ * another gradient (interleaved rows of one buffer are fine).  lse must be the forward pass's
  * (p <= 1).  Every sum has a fixed order: the same inputs give the same bits. */
 JX_API int jx_attention_bwd_f32(const float *q, const float *k, const float *v, const float *o, const float *lse,
                                 const float *dout, float *dq, float *dk, float *dv, const int32_t *cu_q,

@@ -1,6 +1,8 @@
 """Attention at the edges of its kernels: every kernel at every length, values that the scaled operands do not
 serve, unusual scales, offsets beyond 32 bits, and how far non-finite values reach.  Tolerances as in
 test_gpu_attention.py."""
+import math
+
 import pytest
 
 from test_gpu_attention import Case
@@ -161,3 +163,32 @@ def test_many_sequences(jx, dev):
     c.check_forward()
     c.backward(jx)
     c.check_backward()
+
+
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim,causal", [
+    ([4096], [64], 8, 8, 64, False),     # dq has far more to do than dk and dv
+    ([64], [4096], 8, 2, 128, False),    # and far less
+    ([3000, 0, 500], [0, 700, 1], 4, 1, 64, False),
+    ([2048], [0], 8, 8, 128, True),
+    ([1500, 700], [1500, 700], 8, 2, 128, True),
+])
+def test_what_follows_in_the_stream_sees_everything(jx, dev, q_lens, k_lens, heads, kv_heads, dim, causal):
+    """Launches overlap; copies behind a call, without a wait on the host, must still find it complete."""
+    t = dev.torch
+    c = Case(dev, q_lens, k_lens, heads, kv_heads, dim, causal)
+    c.forward(jx)
+    outs = (c.o, c.lse, c.dq, c.dk, c.dv)
+    c.backward(jx)
+    t.cuda.synchronize()
+    want = [x.clone() for x in outs]
+    for _ in range(5):
+        for x in outs:
+            x.fill_(math.nan)
+        c.forward(jx)
+        after = [x.clone() for x in (c.o, c.lse)]
+        c.backward(jx)
+        after += [x.clone() for x in (c.dq, c.dk, c.dv)]
+        t.cuda.synchronize()
+        for x, y in zip(after, want):
+            assert t.equal(x, y)
+    assert jx.device_status() == 0

@@ -86,3 +86,22 @@ def test_clip_refusals(jx):
         jx.grad_norm(p, n, 2, None)
     with pytest.raises(jx.JaxRsError, match="too many tensors"):
         jx.grad_norm(p, n, (1 << 20) + 1, 16)
+
+
+def test_attention_outputs_apart_from_inputs(jx):
+    size = [*_GOOD.values(), None]
+    good = [16 * (i + 1) for i in range(7)]  # q, k, v, o, lse, cu_q, cu_k
+    for i in (0, 1, 2):
+        p = list(good)
+        p[3] = p[i]
+        _refused(jx, "must not be an input", "jx_attention_f32", *p, *size)
+    good = [16 * (i + 1) for i in range(11)]  # q, k, v, o, lse, dout, dq, dk, dv, cu_q, cu_k
+    for i in range(6):
+        for j in (6, 7, 8):
+            p = list(good)
+            p[j] = p[i]
+            _refused(jx, "must not be an input", "jx_attention_bwd_f32", *p, *size)
+    for i, j in ((6, 7), (7, 8), (6, 8)):
+        p = list(good)
+        p[j] = p[i]
+        _refused(jx, "different tensors", "jx_attention_bwd_f32", *p, *size)
