@@ -108,7 +108,7 @@ def test_non_finite_rows_stay_apart(jx, dev):
     assert bool(t.isnan(y[[2, 4]]).all())
 
 
-@pytest.mark.parametrize("rows,cols", SIZES + [(5000, 64), (2500, 333)])
+@pytest.mark.parametrize("rows,cols", SIZES + [(5000, 64), (2500, 333), (300, 8500), (250, 16384), (400, 9001)])
 @pytest.mark.parametrize("pad,shift,affine,wanted", [(0, 0, True, "all"), (3, 1, True, "all"), (4, 0, False, "all"),
                                                      (0, 0, True, "dx"), (0, 0, True, "weights"),
                                                      (0, 0, True, "gamma"), (0, 0, True, "beta")])
