@@ -423,8 +423,9 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
 
 // One block per (query row, head): the pieces in order; rows without keys; rows
 // behind the ones that the rings took (where the caller's hint was too small).
-constexpr int JN_WARPS = 4;
-constexpr int JN_AHEAD = 8;
+// JN_WARPS warps load JN_AHEAD pieces each at a time: 4 and 8, or 32 and 4 where the
+// pieces are many (4 rows, 4 heads, 14400 keys, 257 pieces a head: both kernels 22 us against 39).
+template <int JN_WARPS, int JN_AHEAD>
 __global__ void __launch_bounds__(32 * JN_WARPS)
     attn_join_kernel(const __grid_constant__ Shape s, const float* __restrict__ q, const float* __restrict__ k,
                      const float* __restrict__ v, const float* part, float* o, float* lse, long long per,
@@ -557,25 +558,19 @@ int attention_decode(const Shape& s, const float* q, const float* k, const float
   void* part = nullptr;
   if (int rc = jx::scratch_get(sizeof(float) * (size_t)grid * (DC_WARPS / WR) * 2 * R * WR * (DP + 4), &part, st))
     return rc;
+  const bool wide = rings > 32LL * s.batch * s.kv_heads;  // more pieces a head, on average, than four warps load at once
   cudaError_t e = cudaSuccess;
   for (int p = 0; p < passes && e == cudaSuccess; ++p) {
     const int row_base = p * R * WR;
     kernel<<<grid, 32 * DC_WARPS, dc_smem(DP), st>>>(s, map_k, map_v, q, k, v, o, lse, static_cast<float*>(part), per,
                                                      WR, row_base);
     // the join's blocks may start while the last rings finish; they wait for them before they read
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(s.total_q * s.heads));
-    cfg.blockDim = dim3(32 * JN_WARPS);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
     e = cudaGetLastError();
-    if (e == cudaSuccess)
-      e = cudaLaunchKernelEx(&cfg, attn_join_kernel, s, q, k, v, static_cast<const float*>(part), o, lse, per, R * WR,
-                             DP, row_base, (int)(p == passes - 1));
+    if (e == cudaSuccess) {
+      const auto join = wide ? attn_join_kernel<32, 4> : attn_join_kernel<4, 8>;
+      e = launch_overlapped(join, s.total_q * s.heads, wide ? 1024 : 128, 0, st, s, q, k, v,
+                            static_cast<const float*>(part), o, lse, per, R * WR, DP, row_base, (int)(p == passes - 1));
+    }
   }
   jx::scratch_release(part, st);
   return e == cudaSuccess ? JX_OK : jx::check_cuda(e, "attn_decode_kernel");

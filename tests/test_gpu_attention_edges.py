@@ -36,6 +36,16 @@ def test_many_rows_per_key_head(jx, dev, heads, kv_heads, lens, dim):
     c.check_forward()
 
 
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv_heads,dim", [
+    ([1], [16384], 1, 1, 128), ([1], [4100], 1, 1, 33), ([2, 4, 4, 1], [10194, 17, 30, 4], 2, 1, 127),
+    ([4], [14400], 4, 4, 128), ([1, 3], [5, 6000], 3, 1, 64)])
+def test_many_pieces_of_a_head(jx, dev, q_lens, k_lens, heads, kv_heads, dim):
+    """Long histories of few heads: hundreds of rings share a head, and one block joins their pieces."""
+    c = Case(dev, q_lens, k_lens, heads, kv_heads, dim)
+    c.forward(jx)
+    c.check_forward()
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("heads,kv_heads,n", [(1, 1, 3000), (4, 1, 1500), (6, 3, 700)])
