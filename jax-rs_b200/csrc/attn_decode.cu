@@ -40,11 +40,10 @@ __host__ __device__ constexpr int dc_stage(int DP) { return DC_KEYS * 2 * DP * 4
 __host__ __device__ constexpr int dc_stages(int DP) { return DC_RING / dc_stage(DP); }  // of all rings
 __host__ __device__ constexpr size_t dc_smem(int DP) { return DC_RING + 2 * 8 * dc_stages(DP) + 128; }
 
-// One lane polls for its warp.
+// Every lane for itself: one lane that asks and tells the others takes 150 cycles more.
 __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsigned int* err) {
-  int got = 1;
-  if ((threadIdx.x & 31) == 0) got = wait_bounded(bar, parity, err) ? 1 : 0;
-  return __shfl_sync(0xffffffffu, got, 0) != 0;
+  const bool ok = wait_suspended(bar, parity, err);
+  return __all_sync(0xffffffffu, ok);
 }
 
 // A place in the line of positions.  A head takes lk + VOID of them: starting and
@@ -52,14 +51,21 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsign
 // weigh what they cost.
 constexpr int VOID = 32;
 struct Cursor {
-  long long pos;  // line_start(k0, b) + hk * (lk + VOID) + key
-  int b, hk, key;
+  long long pos;  // line_start(k0, b) + hk * (lk + VOID) + key, as this head was entered
+  int b, hk, key, left, entered;  // keys of the head that are left in the range; the key that it was entered at
   Seq sq;
   bool on;
 
+  __device__ __forceinline__ void enter(long long end) {
+    on = pos < end;
+    entered = key;
+    left = on ? (int)min((long long)(sq.lk - key), end - pos) : 0;
+  }
   // To the first key at or behind `pos`, in a sequence from b on.
   __device__ __forceinline__ void settle(const Shape& s, long long end, int row_base) {
-    for (on = false; b < s.batch; ++b) {
+    on = false;
+    left = 0;
+    for (; b < s.batch; ++b) {
       sq = seq_bounds(s, b);
       if ((long long)sq.lq * s.group <= row_base || sq.lk == 0) continue;
       const long long base = (sq.k0 + (long long)b * VOID) * s.kv_heads, in = max(0LL, pos - base);
@@ -72,25 +78,23 @@ struct Cursor {
         if (++hk == s.kv_heads) continue;
       }
       pos = base + (long long)hk * len + key;
-      on = pos < end;
+      enter(end);
       return;
     }
   }
-  __device__ __forceinline__ int keys(long long end) const {  // of the next stage
-    return (int)min((long long)min(DC_KEYS, sq.lk - key), end - pos);
-  }
-  __device__ __forceinline__ void step(const Shape& s, int n, long long end, int row_base) {
-    pos += n;
-    key += n;
-    on = pos < end;
-    if (key == sq.lk) {
-      key = 0;
-      pos += VOID;
-      on = pos < end;
-      if (++hk == s.kv_heads && on) {
-        ++b;
-        settle(s, end, row_base);
-      }
+  // Behind the last of the head's keys in the range.
+  __device__ __forceinline__ void advance(const Shape& s, long long end, int row_base) {
+    pos += key - entered;
+    on = false;
+    if (key < sq.lk) return;  // the range ends here
+    key = 0;
+    pos += VOID;
+    if (pos >= end) return;
+    if (++hk < s.kv_heads) {
+      enter(end);
+    } else {
+      ++b;
+      settle(s, end, row_base);
     }
   }
 };
@@ -201,23 +205,28 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
   c.settle(s, end, row_base);
   Cursor pc = c;  // the copies' place, up to nst stages ahead
   int in_st = 0, out_st = 0, issued = 0;
+  bool sends = true;  // lane 0's: if it gives up, the warp finds out when the stage does not come
   uint32_t in_ph = 0, out_ph = 0;
   bool ok = true;
   auto produce = [&]() {  // the ring's first warp: the next stage's rows
     if (!pc.on || !ok) return;
-    const int st = in_st, n = pc.keys(end);
-    ok = ring_wait(&empty[st], in_ph ^ 1u, s.err);
-    if (!ok) return;
+    const int st = in_st, n = min(DC_KEYS, pc.left);
     const long long t = pc.sq.k0 + pc.key;
     float* dst = stages + (size_t)st * (STAGE / 4);
     if constexpr (VEC) {
       // eight rows each, whatever n is: the rest is other sequences' or zeros, and masked
       if (lane == 0) {
-        jxd::mbar_arrive_expect_tx(&full[st], (uint32_t)STAGE);
-        jxd::tma_load_3d(dst, &map_k, &full[st], 0, (int)t, pc.hk);
-        jxd::tma_load_3d(dst + DC_KEYS * DP, &map_v, &full[st], 0, (int)t, pc.hk);
+        sends = sends && wait_suspended(&empty[st], in_ph ^ 1u, s.err);
+        if (sends) {
+          jxd::mbar_arrive_expect_tx(&full[st], (uint32_t)STAGE);
+          jxd::tma_load_3d(dst, &map_k, &full[st], 0, (int)t, pc.hk);
+          jxd::tma_load_3d(dst + DC_KEYS * DP, &map_v, &full[st], 0, (int)t, pc.hk);
+          ++issued;
+        }
       }
     } else {
+      ok = ring_wait(&empty[st], in_ph ^ 1u, s.err);
+      if (!ok) return;
       const long long hd = (long long)pc.hk * s.dim;
       for (int r = 0; r < n; ++r)
         for (int col = lane; col < s.dim; col += 32) {
@@ -229,13 +238,14 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
                        : "memory");
         }
       asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(jxd::smem_u32(&full[st])) : "memory");
+      ++issued;
     }
-    ++issued;
     if (++in_st == nst) {
       in_st = 0;
       in_ph ^= 1u;
     }
-    pc.step(s, n, end, row_base);
+    pc.key += n;
+    if ((pc.left -= n) == 0) pc.advance(s, end, row_base);
   };
   if (wr == 0)
     for (int i = 0; i < nst; ++i) produce();
@@ -272,8 +282,8 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
         }
       }
     }
-    while (c.on && c.b == b && c.hk == hk) {
-      const int n = c.keys(end), st = out_st, j0 = c.key;
+    while (c.left > 0) {
+      const int n = min(DC_KEYS, c.left), st = out_st, j0 = c.key;
       ok = ok && ring_wait(&full[st], out_ph, s.err);
       if (!ok) break;
       const float* base = stages + (size_t)st * (STAGE / 4);
@@ -363,10 +373,12 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
         out_st = 0;
         out_ph ^= 1u;
       }
-      c.step(s, n, end, row_base);
+      c.key += n;
+      c.left -= n;
       if (wr == 0) produce();
     }
     if (!ok) break;
+    c.advance(s, end, row_base);
     // join the warp's groups, store
     // the head's first position
     const long long seg = (sq.k0 + (long long)b * VOID) * s.kv_heads + (long long)hk * (sq.lk + VOID);
@@ -417,7 +429,7 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
   }
   // not before: the join's blocks would wait where rings still stream (37.0 us against 33.2 at the start of the kernel)
   asm volatile("griddepcontrol.launch_dependents;");
-  if (!ok && wr == 0)  // every copy has landed before the CTA may end
+  if (!ok && wr == 0 && (!VEC || lane == 0))  // every copy has landed before the CTA may end
     for (int u = max(0, issued - nst); u < issued; ++u) wait_bounded(&full[u % nst], (uint32_t)(u / nst) & 1u, s.err);
 }
 
