@@ -131,7 +131,10 @@ int jx_attention_f32(const float* q, const float* k, const float* v, float* o, f
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
   JX_REQUIRE(total_q * heads < (1LL << 31), "attention: too many rows");
-  if (total_k > 0 && tiles_are_faster(s, max_q, max_k)) return attention_fwd_tiles(s, q, k, v, o, lse, st);
+  max_q = std::min(max_q, total_q);
+  max_k = std::min(max_k, total_k);
+  if (total_k == 0) return attention_decode(s, q, k, v, o, lse, 1, st);  // its last launch writes rows without keys
+  if (tiles_are_faster(s, max_q, max_k)) return attention_fwd_tiles(s, q, k, v, o, lse, st);
   return attention_decode(s, q, k, v, o, lse, max_q * s.group, st);
 }
 
@@ -158,6 +161,8 @@ int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const f
   }
   cudaStream_t st = jx::as_stream(stream);
   s.err = jx::device_error_word();
+  max_q = std::min(max_q, total_q);
+  max_k = std::min(max_k, total_k);
   // row by row only where five launches would be the whole time (16 rows, 16 keys: 21 us against 44; 100 keys: equal)
   if (total_q > 0 && total_k > 0 && (max_q * s.group > 16 || max_k > 96))
     return attention_bwd_tiles(s, q, k, v, o, lse, dout, dq, dk, dv, max_q, st);

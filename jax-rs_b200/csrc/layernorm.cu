@@ -18,8 +18,8 @@
 //
 // Forward, 16384 x 4096: 86 us, 6.2 TB/s, with four vectors in each of 256 threads; two
 // in 512 take 122, one in 1024 142, eight in 128 88 (a block waits for its row's
-// sums twice, so several blocks per SM must be in different places; few rows turn
-// this round).  Backward, 16384 x 2048: 60 us, 6.7 TB/s, and 4 for the join behind it; two blocks
+// sums twice, so several blocks per SM must be in different places; where rows are
+// few it is the other way).  Backward, 16384 x 2048: 60 us, 6.7 TB/s, and 4 for the join behind it; two blocks
 // per SM instead of three take 66.  Beyond 8192 columns a cluster shares a row.
 #include <math.h>
 

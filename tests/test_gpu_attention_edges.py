@@ -46,6 +46,17 @@ def test_many_pieces_of_a_head(jx, dev, q_lens, k_lens, heads, kv_heads, dim):
     c.check_forward()
 
 
+@pytest.mark.parametrize("q_lens,k_lens", [([40000], [0]), ([5], [7]), ([300, 2], [0, 400])])
+def test_hints_beyond_the_tensors(jx, dev, q_lens, k_lens):
+    """A hint costs no launches for rows that are not there, and rows without keys none of their own."""
+    c = Case(dev, q_lens, k_lens, 8, 2, 64)
+    c.forward(jx, max_q=1 << 62, max_k=1 << 62)
+    c.check_forward()
+    c.backward(jx, max_q=1 << 62, max_k=1 << 62)
+    c.check_backward()
+    assert jx.device_status() == 0
+
+
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("heads,kv_heads,n", [(1, 1, 3000), (4, 1, 1500), (6, 3, 700)])
