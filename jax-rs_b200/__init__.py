@@ -206,7 +206,8 @@ def check(status: int, what: str = ""):
 
 
 def call(name, *args):
-    return check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    return status if status == JX_OK else check(status, name)
 
 
 def init(device: int = 0):

@@ -13,7 +13,7 @@
 // attn_join_kernel joins the pieces.
 //
 // One token behind eight histories, 14.7k keys of 8 heads of 128 (118 MB): 33 us for
-// both kernels, 3.6 TB/s, against 18 us of reading at the copy rate.  The
+// both kernels (30 in a captured graph), 3.6 TB/s, against 18 us of reading at the copy rate.  The
 // kernel itself takes 25 us; the rest is the join, which waits for the slowest
 // ring.  Copying row by row (one bulk copy of 512 B each) took 37 us, the rate of
 // copy instructions being the bound.
@@ -48,8 +48,8 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsign
 
 // A place in the line of positions.  A head takes lk + VOID of them: starting and
 // storing a head costs a ring about as much as VOID keys, so that short heads
-// weigh what they cost.
-constexpr int VOID = 32;
+// weigh what they cost (8 histories, 3 of them short: 16, 24, 32, 40 and 72 take 40.3, 36.8, 30.2, 30.1 and 30.4 us).
+constexpr int VOID = 40;
 struct Cursor {
   long long pos;  // line_start(k0, b) + hk * (lk + VOID) + key, as this head was entered
   int b, hk, key, left, entered;  // keys of the head that are left in the range; the key that it was entered at
