@@ -80,6 +80,20 @@ bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
   return tiles < rings;
 }
 
+// Whether the gradients are computed row by row (two launches, a warp per row and head)
+// or by tiles (four, or five where heads are shared), from the hints, in
+// microseconds as measured: a row's warp takes 0.3 us a key, a key's 0.72 us a row of its
+// heads, each besides what all of them together cost; the tiles' cost is their
+// launches and 0.14 us a CTA.  (8 heads, 8 rows and keys: 13 and 15; 16 of
+// each: 19 and 16; 16 sequences, 32 heads on 8, 8 of each: 39 and 99; 1 row behind
+// 128 keys: 172 and 101.)
+bool rows_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
+  const double rows = (double)max_q * s.group, keys = (double)max_k, heads = (double)s.batch * s.heads;
+  const double by_row =
+      6 + 0.72 * rows + 0.3 * keys + 0.3e-3 * heads * (double)max_q * keys + 6e-3 * (double)s.total_k * s.kv_heads;
+  return by_row < 15 + (s.group > 1 ? 8 : 0) + 0.14 * heads;
+}
+
 int check_shape(const char* what, Shape& s, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q,
                 int64_t total_k, int64_t max_q, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
                 int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int causal) {
@@ -163,8 +177,7 @@ int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const f
   s.err = jx::device_error_word();
   max_q = std::min(max_q, total_q);
   max_k = std::min(max_k, total_k);
-  // row by row only where five launches would be the whole time (16 rows, 16 keys: 21 us against 44; 100 keys: equal)
-  if (total_q > 0 && total_k > 0 && (max_q * s.group > 16 || max_k > 96))
+  if (total_q > 0 && total_k > 0 && !rows_are_faster(s, max_q, max_k))
     return attention_bwd_tiles(s, q, k, v, o, lse, dout, dq, dk, dv, max_q, st);
   const long long bq = (total_q * heads + ROW_WARPS - 1) / ROW_WARPS;
   const long long bk = (total_k * kv_heads + ROW_WARPS - 1) / ROW_WARPS;
