@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     float acc[DP / 2];
 #pragma unroll
     for (int c = 0; c < DP / 2; ++c) acc[c] = 0.0f;
-    float m = -INFINITY, sum = 0.0f, alpha_prev = 0.0f, inv_v_prev = 0.0f;
+    float m = -INFINITY, shift = INFINITY, sum = 0.0f, alpha_prev = 0.0f, inv_v_prev = 0.0f;
     bool ok = true;
 
     auto add_part = [&](int j, float alpha, float inv_v) {
@@ -533,10 +533,12 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       pair_sync(1 + quarter);
       mx = fmaxf(mx, turn[(half ^ 1) * 128 + row]);
       const float m_new = mx == -INFINITY ? m : fmaxf(m, mx * f);
-      const float base = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = exp2_fast(m - base);
+      // the shift as it is rounded: everything else is computed with it, so that its error cancels
+      const float up = m_new == -INFINITY ? P_SHIFT : P_SHIFT - m_new;
+      const float alpha = exp2_fast(up - shift);
       m = m_new;
-      const float2 f2 = make_float2(f, f), b2 = make_float2(P_SHIFT - base, P_SHIFT - base);
+      if (m_new != -INFINITY) shift = up;
+      const float2 f2 = make_float2(f, f), b2 = make_float2(up, up);
       float2 add = make_float2(0.0f, 0.0f);
       uint32_t hi[32], lo[32];
 #pragma unroll
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     half_to_area<DP>(smem, acc, sum == 0.0f ? 0.0f : 1.0f / sum, row, half);
     if (lse && half == 0 && row < rows)
       lse[(long long)h * s.total_q + sq.q0 + i0 + row] =
-          sum == 0.0f ? -INFINITY : (m + (log2f(sum) - P_SHIFT)) * LN2;
+          sum == 0.0f ? -INFINITY : fmaf(P_SHIFT - shift, LN2, log2f(sum * 6.103515625e-05f) * LN2);  // 2^-14
     movers_sync();
     rows_store<DP>(o + (sq.q0 + i0) * s.ldo + hd, s.ldo, smem, rows, s.dim, aligned16(o, s.dim, s.ldo), tid);
   }
