@@ -514,8 +514,9 @@ JX_API int jx_layernorm_bwd_f32(const float *dy, const float *x, const float *ga
  * no effect on it, whatever its values.  lse [heads, total_q] may be NULL.
  * max_q / max_k: the longest sequences, a hint for the choice of kernel; any
  * value >= 0 gives right results.  Prompts run on the tensor cores, each f32
- * operand split in two f16 parts under a power-of-two scale (22 bits), f32 sums;
- * few query rows per key head (decoding) run in plain f32.  128 rows of one head
+ * operand split in two f16 parts under a power-of-two scale, f32 sums: 22 bits of
+ * every value down to 2^-28 of the largest among 128 rows of its head, an absolute
+ * 2^-50 of that one below.  Few query rows per key head (decoding) run in plain f32.  128 rows of one head
  * that hold a non-finite value, or largest magnitudes more than 2^20 apart, are
  * computed row by row: as right, but slowly.  Make a first call of each kind
  * before any stream capture, as for the library's other tensor-core kernels. */

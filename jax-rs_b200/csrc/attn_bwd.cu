@@ -119,11 +119,15 @@ __device__ __forceinline__ void mma_scores(uint32_t d, uint32_t a, uint32_t b, u
   constexpr uint32_t id = idesc_f16(N, false);
   auto step = [&](int ks, bool a_lo, bool b_lo, uint32_t acc) {
     const uint64_t bd = jxd::smem_desc_k_sw128(b + (b_lo ? part : 0) + (ks >> 2) * panel + (ks & 3) * 32);
+    const bool shrink = !a_lo && !b_lo && ks == 0;
     if constexpr (TS) {
-      mma_f16_ts(d, a + (a_lo ? DP / 2 : 0) + ks * 8, bd, id, acc);
+      const uint32_t ad = a + (a_lo ? DP / 2 : 0) + ks * 8;
+      if (shrink) mma_f16_ts_shrink(d, ad, bd, id);
+      else mma_f16_ts(d, ad, bd, id, acc);
     } else {
-      mma_f16_ss(d, jxd::smem_desc_k_sw128(a + (a_lo ? tile_part(DP) : 0) + (ks >> 2) * PANEL + (ks & 3) * 32), bd, id,
-                 acc);
+      const uint64_t ad = jxd::smem_desc_k_sw128(a + (a_lo ? tile_part(DP) : 0) + (ks >> 2) * PANEL + (ks & 3) * 32);
+      if (shrink) mma_f16_ss_shrink(d, ad, bd, id);
+      else mma_f16_ss(d, ad, bd, id, acc);
     }
   };
 #pragma unroll
@@ -141,8 +145,10 @@ template <int DP, int ROWS>
 __device__ __forceinline__ void mma_sums(uint32_t d, uint32_t a, uint32_t b, uint32_t panel, uint32_t part) {
   constexpr uint32_t id = idesc_f16(DP, true);
   auto step = [&](int ks, bool a_lo, bool b_lo, uint32_t acc) {
-    mma_f16_ts(d, a + (ks >> 1) * 32 + (ks & 1) * 8 + (a_lo ? 16 : 0),
-               smem_desc_mn_sw128(b + (b_lo ? part : 0) + ks * 2048, panel), id, acc);
+    const uint32_t ad = a + (ks >> 1) * 32 + (ks & 1) * 8 + (a_lo ? 16 : 0);
+    const uint64_t bd = smem_desc_mn_sw128(b + (b_lo ? part : 0) + ks * 2048, panel);
+    if (!a_lo && !b_lo && ks == 0) mma_f16_ts_shrink(d, ad, bd, id);
+    else mma_f16_ts(d, ad, bd, id, acc);
   };
 #pragma unroll
   for (int ks = 0; ks < ROWS / 16; ++ks) {

@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
       // ---- MMA
       constexpr uint32_t id_s = idesc_f16(128, false), id_o = idesc_f16(DP, true);
+      constexpr uint32_t SHRINK = 2;  // acc: 0 from zero, 1 onto the sum, SHRINK onto the sum times 2^-LO_BITS
       const uint32_t sbase = jxd::smem_u32(smem);
       int stage = 0;
       uint32_t phase = 0;
@@ -413,8 +414,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
       auto scores = [&](int j) {
         const uint32_t d = tmem + (j & 1) * 128u;
         auto step = [&](uint32_t kt, int ks, uint32_t a, uint32_t acc) {
-          mma_f16_ts(d, tmem + T_Q + a + ks * 8, jxd::smem_desc_k_sw128(kt + (ks >> 2) * PANEL + (ks & 3) * 32), id_s,
-                     acc);
+          const uint64_t bd = jxd::smem_desc_k_sw128(kt + (ks >> 2) * PANEL + (ks & 3) * 32);
+          if (acc == SHRINK) mma_f16_ts_shrink(d, tmem + T_Q + a + ks * 8, bd, id_s);
+          else mma_f16_ts(d, tmem + T_Q + a + ks * 8, bd, id_s, acc);
         };
         uint32_t kt = next();
         if (!ok) return;
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) step(kt, ks, DP / 2, 1);  // lo.hi
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) step(kt, ks, 0, 1);
+        for (int ks = 0; ks < DP / 16; ++ks) step(kt, ks, 0, ks > 0 ? 1 : SHRINK);
         jxd::mma_commit(&sfull[j & 1]);
         release();
       };
@@ -439,7 +441,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         const uint32_t p = tmem + (j & 1) * 128u, d = tmem + T_O;
         // P's keys 0..63: hi at column 0, lo at 32; keys 64..127: hi at 64, lo at 96
         auto step = [&](uint32_t vt, int ks, uint32_t a, uint32_t acc) {
-          mma_f16_ts(d, p + a + (ks >> 2) * 64 + (ks & 3) * 8, smem_desc_mn_sw128(vt + ks * 2048, PANEL), id_o, acc);
+          const uint32_t at = p + a + (ks >> 2) * 64 + (ks & 3) * 8;
+          const uint64_t bd = smem_desc_mn_sw128(vt + ks * 2048, PANEL);
+          if (acc == SHRINK) mma_f16_ts_shrink(d, at, bd, id_o);
+          else mma_f16_ts(d, at, bd, id_o, acc);
         };
         uint32_t vt = next();
         if (!ok) break;
@@ -451,7 +456,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) step(vt, ks, 32, 1);
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) step(vt, ks, 0, 1);
+        for (int ks = 0; ks < 8; ++ks) step(vt, ks, 0, ks > 0 ? 1 : SHRINK);
         jxd::mma_commit(ofull);
         release();
       }

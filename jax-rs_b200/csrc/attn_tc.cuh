@@ -2,15 +2,17 @@
 // tiles split into two f16 parts, their layout in scratch and shared memory,
 // and the tcgen05 wrappers for operands in tensor memory.
 //
-// Numbers.  An f32 operand x is held as hi + lo, hi = f16(x s), lo = f16(x s -
-// hi), with s a power of two that brings the largest magnitude of its scaling
-// group (a row of the operand that stays, a tile of 128 rows of the one that
-// streams) into [2^14, 2^15).  hi + lo keeps 22 bits of every value within 2^-17
-// of the largest and an absolute 2^-39 of the largest below that.  A product is
-// lo.hi + hi.lo + hi.hi, three f16 products with f32 sums: twice the rate of
-// the same with tf32 parts, whose 22 bits are the same.  A tile that holds a
-// non-finite value, or rows whose largest values differ by more than 2^20, is
-// marked; the tiles of output that need it are computed row by row in plain f32.
+// Numbers.  An f32 operand x is held as hi + 2^-11 lo, hi = f16(x s), lo =
+// f16((x s - hi) 2^11), with s a power of two that brings the largest magnitude of
+// its scaling group (a row of forward's Q, 128 rows of one head otherwise) into
+// [2^14, 2^15).  hi + 2^-11 lo keeps 22 bits of every value within 2^-28 of the
+// largest and an absolute 2^-50 of the largest below that (without the 2^11, lo
+// would run out of f16's exponents at 2^-17).  A product is 2^-11 (lo.hi + hi.lo) +
+// hi.hi, three f16 products with f32 sums: twice the rate of the same with tf32
+// parts, whose 22 bits are the same; the first hi.hi product shrinks the sum so far
+// by 2^-11 as it adds.  A tile that holds a non-finite value, or rows whose largest
+// values differ by more than 2^20, is marked; the tiles of output that need it are
+// computed row by row in plain f32.
 //
 // Sums.  The tensor core truncates as it accumulates, so a sum in tensor memory
 // spans at most 128 terms, small parts first; spans are added in f32 registers.
@@ -37,6 +39,7 @@ namespace jxa {
 constexpr int TILE = 128;
 constexpr int PANEL = TILE * 128;  // bytes of 128 rows x 64 f16 columns
 constexpr int WIDE_BITS = 20;
+constexpr int LO_BITS = 11;  // lo parts are held times 2^LO_BITS
 constexpr float P_SHIFT = 14.0f;  // softmax weights are scaled by 2^14 for their f16 parts
 
 __host__ __device__ constexpr int tile_part(int DP) { return DP / 64 * PANEL; }      // one part of a tile
@@ -89,11 +92,12 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
-// hi and lo parts of two scaled values.
+// hi and lo parts of two scaled values; both steps of the remainder are exact.
 __device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pack_half(a, b);
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  const float2 r = fma2(h, make_float2(-1.0f, -1.0f), make_float2(a, b));
+  constexpr float UP = 1 << LO_BITS;
+  const float2 r = fma2(h, make_float2(-UP, -UP), mul2(make_float2(a, b), make_float2(UP, UP)));
   lo = pack_half(r.x, r.y);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -105,6 +109,24 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // D f32, A and B f16; N columns, M = 128 rows; B_MN: B is MN-major.
 __host__ __device__ constexpr uint32_t idesc_f16(int N, bool B_MN) {
   return (1u << 4) | (B_MN ? (1u << 16) : 0u) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// D[tmem] = A[tmem] * B[smem] + D * 2^-LO_BITS: the step from the sum of the small products to hi.hi
+__device__ __forceinline__ void mma_f16_ts_shrink(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p, %4;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "n"(LO_BITS)
+      : "memory");
+}
+// D[tmem] = A[smem] * B[smem] + D * 2^-LO_BITS
+__device__ __forceinline__ void mma_f16_ss_shrink(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p, %4;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "n"(LO_BITS)
+      : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem]
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {

@@ -1,0 +1,34 @@
+"""Attention where an operand's rows or columns differ widely in size: each column, and each row, against its own
+magnitude.  Tolerances as in test_gpu_attention.py: the forward pass element by element, the gradients' norms by column
+or by row (64 values at least, as independent as those of a whole tensor) with ||error|| <= 2e-6 ||mag|| + 1e-5 ||want||."""
+import pytest
+
+from test_gpu_attention import Case
+
+pytestmark = pytest.mark.gpu
+
+
+def check(c, dims, rows=slice(None), keys=slice(None)):
+    """Norms over `dims` of the gradients of [tokens, heads, dim]."""
+    _, _, _, g, m = c.reference(True)
+    for name, got, want, mag in zip(("dq", "dk", "dv"), (c.dq, c.dk, c.dv), g, m):
+        at = rows if name == "dq" else keys
+        n = lambda x: x[at].double().norm(dim=dims)
+        share = n(got.double() - want) / (2e-6 * n(mag) + 1e-5 * n(want) + 1e-300)
+        assert float(share.max()) <= 1, (name, float(share.max()), int(share.argmax()))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("power", [12, 20, 25])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+def test_one_large_column(jx, dev, dim, power, which):
+    """A column 2^power times the others, which no row's largest value shows; scores stay as they were."""
+    c = Case(dev, [300], [300], 2, 1, dim)
+    getattr(c, which)[:, :, 0] *= 2.0 ** power
+    if which in ("q", "k"):
+        (c.k if which == "q" else c.q)[:, :, 0] *= 2.0 ** -power
+    c.forward(jx)
+    c.check_forward()
+    c.backward(jx)
+    check(c, 0)
+    assert jx.device_status() == 0
