@@ -28,9 +28,12 @@
 // to 700 us with the power limit's clock.
 //
 // A computed operand needs its scale before its largest value is known: P <= 1
-// and |dP - delta| <= |dout row| |v row| + |delta| (norms) bound dS; it
-// overestimates by some bits of the 39 there are (a row of 2^14 keys with equal
-// weights keeps 21 bits of each dS).
+// and |dP - delta| <= |dout row| |v row| + |delta| (norms) bound dS.  The norms
+// are the row's own for dq, and for dk and dv the largest among the block's rows
+// that see the key: rows of dout may differ in size, and one scale for all would
+// leave small ones few bits.  The bound overestimates by log2 of the keys that
+// share a row's weight and some bits more, of the 28 that there are above the
+// last value with 22 bits.
 #include <algorithm>
 
 #include "attn_tc.cuh"
@@ -49,10 +52,11 @@ static_assert(128 * BW_LOW_REGS + 256 * BW_HIGH_REGS <= BW_THREADS * BW_LAUNCH_R
 
 struct BwdTiles {
   const uint8_t *q, *k, *v, *d;  // tiles; d is dout
-  const float4* num_q;  // of a tile of query rows: what undoes Q's scale and dout's, dout's largest row norm, delta's largest magnitude
+  const float4* num_q;  // of a tile of query rows: what undoes Q's scale and dout's, dout's largest row norm
   const float4* num_k;  // of a tile of keys: what undoes K's scale and V's, V's largest row norm
   const int *bad_q, *bad_k, *bad_v, *bad_d;
-  const float *lse2, *delta;
+  const float *lse2, *delta, *row_norm;
+  const float2* later;
   int q_tiles, k_tiles, parts;
   const TileRef *order_q, *order_k;
   float *part_k, *part_v;  // [parts][total_k * kv_heads * dim], used where parts > 1
@@ -66,7 +70,9 @@ __device__ __forceinline__ float bound_scale(float bound) {
   const int e = (int)(__float_as_uint(bound) >> 23);
   return __uint_as_float((uint32_t)(268 - min(max(e, 41), 254)) << 23);
 }
-
+// A row's norm is taken as this part of its tile's at least, so that the scale of an
+// all but empty row stays finite: rows of less than 2^-20 are zeros (or the tile is marked).
+constexpr float LEAST_NORM = 1.4901161e-08f;  // 2^-26
 
 // acc += part * factor for this thread's DP/2 columns of a tensor-memory sum.
 template <int DP>
@@ -378,7 +384,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       done(moved);
     }
     const float4 num = bt.num_q[qslot];
-    const float f_tile = num.x * (s.scale * LOG2E), inv_d = num.y, norm_d = num.z;
+    const float f_tile = num.x * (s.scale * LOG2E), inv_d = num.y;
+    const float norm_d = fmaxf(bt.row_norm[qslot * TILE + row], num.z * LEAST_NORM);
     const float lse2 = bt.lse2[qslot * TILE + row], delta = bt.delta[qslot * TILE + row];
     const int vis = row < rows ? sq.visible(i0 + row, s.causal) : 0;
     const int vis_all = sq.visible(i0, s.causal);
@@ -491,7 +498,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 template <int DP>
 struct KvLayout {
   static constexpr bool APART = DP == 64;
-  static constexpr int BLK = APART ? 128 : 64;
+  static constexpr int BLK = kv_block(DP);
   static constexpr int QS = 3, DS = 2;  // stages of Q and of dout
   static constexpr uint32_t V = 0;      // DP = 128
   static constexpr uint32_t X = APART ? 0 : 128, X_STEP = BLK, Y = 256, Y_STEP = APART ? 0 : BLK;
@@ -805,8 +812,15 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     float g_prev = 0.0f;
     constexpr int C = BLK / 2;  // columns of the scores that this thread has
     int i0 = (blk0 + (n > 0 ? it0 % nblk : 0) - 1) * BLK;  // the block's first row
+    const float2* later = bt.later + (qslot0 + (n > 0 ? it0 / nblk : 0)) * TILE;  // of the head's first tile
     for (int u = 0; u < n; ++u) {
-      i0 = i0 + BLK >= sq.lq ? blk0 * BLK : i0 + BLK;  // the next block, or the next head's first
+      i0 += BLK;  // the next block, or the next head's first
+      if (i0 >= sq.lq) {
+        i0 = blk0 * BLK;
+        later += TILE;
+      }
+      // the block's rows from the first that sees this key on
+      const float2 tops = later[(long long)(i0 / TILE) * s.heads * TILE + i0 % TILE + min(max(first - i0, 0), BLK - 1)];
       const float* lse2 = stats + (u & 1) * L::STATS + half * C;
       const float* delta = lse2 + BLK;
       const uint32_t xa = tmem + lanes + L::X + (u & 1) * L::X_STEP + half * C;
@@ -815,7 +829,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       float2 p[C / 2];
       warp_wait(&tfull[u & 1], (uint32_t)(u >> 1) & 1u, ok, abort_flag, s.err);
       const float4 num = *reinterpret_cast<const float4*>(stats + (u & 1) * L::STATS + 2 * BLK);
-      const float inv_q = num.x, inv_d = num.y, norm_d = num.z, top_d = num.w, f = f_tile * inv_q;
+      const float inv_q = num.x, inv_d = num.y, norm_d = fmaxf(tops.x, num.z * LEAST_NORM), f = f_tile * inv_q;
       const float2 f2 = make_float2(f, f);
       ready(&sfull[u & 1], u >> 1);
 #pragma unroll
@@ -857,7 +871,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
         done(wfree);
       }
       // P is at most 2^14
-      const float fd = inv_v * inv_d, sc = bound_scale(16384.0f * (norm_v * norm_d + top_d));
+      const float fd = inv_v * inv_d, sc = bound_scale(16384.0f * (norm_v * norm_d + tops.y));
       const float pf = sc * fd, nf = -inverse_pow2(fd);
       const float2 pf2 = make_float2(pf, pf), nf2 = make_float2(nf, nf);
       ready(&dpfull[u & 1], u >> 1);
@@ -989,7 +1003,7 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
   const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
   // tiles first, then arrays whose pieces the copies read 16-byte aligned, then the rest
-  const size_t bytes = (2 * ks + 2 * qs) * tb + 2 * qs * TILE * 4 + (6 * ks + 6 * qs) * 4 + (qt + kt) * sizeof(TileRef) +
+  const size_t bytes = (2 * ks + 2 * qs) * tb + 5 * qs * TILE * 4 + (6 * ks + 6 * qs) * 4 + (qt + kt) * sizeof(TileRef) +
                        2 * part_floats * 4;
   void* p = nullptr;
   if (int rc = jx::scratch_get(bytes + 64, &p, st)) return rc;
@@ -1003,6 +1017,8 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   TileRef *order_q = (TileRef*)take(qt * sizeof(TileRef)), *order_k = (TileRef*)take(kt * sizeof(TileRef));
   float* lse2 = (float*)take(qs * TILE * 4);
   float* delta = (float*)take(qs * TILE * 4);
+  float* row_norm = (float*)take(qs * TILE * 4);
+  float2* later = (float2*)take(qs * TILE * 8);
   float *num_q = (float*)take(qs * 16), *num_k = (float*)take(ks * 16);
   float* part_k = (float*)take(part_floats * 4);
   float* part_v = (float*)take(part_floats * 4);
@@ -1014,10 +1030,9 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
   src.t[0] = {k, s.ldk, tk, num_k, bad_k, 4};
   src.t[1] = {v, s.ldv, tv, num_k + 1, bad_v, 4, num_k + 2};
   src.t[2] = {q, s.ldq, tq, num_q, bad_q, 4};
-  src.t[3] = {dout, s.ldo, td, num_q + 1, bad_d, 4, num_q + 2, o, lse, lse2, delta, num_q + 3};
+  src.t[3] = {dout, s.ldo, td, num_q + 1, bad_d, 4, num_q + 2, o, lse, lse2, delta, row_norm, later};
   const BwdTiles bt = {tq,    tk,    tv,    td,    (const float4*)num_q, (const float4*)num_k, bad_q, bad_k,
-                       bad_v, bad_d, lse2,  delta, (int)qt,              (int)kt,              parts, order_q,
-                       order_k, part_k, part_v};
+                       bad_v, bad_d, lse2,  delta, row_norm, later, (int)qt, (int)kt, parts, order_q, order_k, part_k, part_v};
   int rc = split_tiles(s, src, DP, st);
   if (!rc)
     rc = DP == 128 ? launch<128>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st)

@@ -187,8 +187,9 @@ __global__ void __launch_bounds__(sp_threads(DP), 1024 / sp_threads(DP))
     *reinterpret_cast<uint4*>(out + i * STEP * 128 + tile_part(DP)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
   if (t.norm) {
+    __shared__ float sm_norm[TILE], sm_delta[TILE];  // of the rows: the scaled norm's square, |rowsum(dout o)|
     const bool vec_o = (s.dim & 3) == 0 && (s.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(t.o) & 15) == 0;
-    float most = 0.0f, most_delta = 0.0f;
+    float most = 0.0f;
     bool odd = false;
     const float* p = t.o + (row0 + r0) * s.ldo + hd;
 #pragma unroll
@@ -214,30 +215,40 @@ __global__ void __launch_bounds__(sp_threads(DP), 1024 / sp_threads(DP))
         odd = odd || !isfinite(d) || isnan(z) || z == INFINITY;
         t.lse2[slot * TILE + r] = z == -INFINITY ? INFINITY : z * LOG2E - P_SHIFT;
         t.delta[slot * TILE + r] = d;
-        most_delta = fmaxf(most_delta, fabsf(d));
+        t.row_norm[slot * TILE + r] = sqrtf(n) * inverse_of(e_top);
+        sm_norm[r] = n;
+        sm_delta[r] = fabsf(d);
       }
     }
     odd = __syncthreads_or(odd);
+    if (t.o && threadIdx.x < TILE) {  // from the back, over the rows of each block
+      const int r = threadIdx.x, end = (r | (kv_block(DP) - 1)) + 1;
+      float n = sm_norm[r], d = sm_delta[r];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-      most_delta = fmaxf(most_delta, __shfl_xor_sync(0xffffffffu, most_delta, o));
+      for (int o = 1; o < 32; o <<= 1) {
+        n = fmaxf(n, __shfl_down_sync(0xffffffffu, n, o));
+        d = fmaxf(d, __shfl_down_sync(0xffffffffu, d, o));
+      }
+      for (int w = (r | 31) + 1; w < end; w += 32) {  // the block's later warps
+        float n1 = sm_norm[w + (r & 31)], d1 = sm_delta[w + (r & 31)];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+          d1 = fmaxf(d1, __shfl_xor_sync(0xffffffffu, d1, o));
+        }
+        n = fmaxf(n, n1);
+        d = fmaxf(d, d1);
+      }
+      t.later[slot * TILE + r] = make_float2(sqrtf(n) * inverse_of(e_top), d);
     }
-    if ((threadIdx.x & 31) == 0) {
-      sm_top[threadIdx.x >> 5] = __float_as_uint(most);
-      sm_low[threadIdx.x >> 5] = __float_as_uint(most_delta);
-    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((threadIdx.x & 31) == 0) sm_low[threadIdx.x >> 5] = __float_as_uint(most);
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < SP_THREADS / 32; ++w) {
-        most = fmaxf(most, __uint_as_float(sm_top[w]));
-        most_delta = fmaxf(most_delta, __uint_as_float(sm_low[w]));
-      }
+      for (int w = 1; w < SP_THREADS / 32; ++w) most = fmaxf(most, __uint_as_float(sm_low[w]));
       t.norm[slot * t.step] = sqrtf(most) * inverse_of(e_top);
-      if (t.o) {
-        t.delta_top[slot * t.step] = most_delta;
-        if (odd) t.bad[slot] = 1;
-      }
+      if (t.o && odd) t.bad[slot] = 1;
     }
   }
 }

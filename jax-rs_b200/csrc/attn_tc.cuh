@@ -39,6 +39,7 @@ namespace jxa {
 constexpr int TILE = 128;
 constexpr int PANEL = TILE * 128;  // bytes of 128 rows x 64 f16 columns
 constexpr int WIDE_BITS = 20;
+__host__ __device__ constexpr int kv_block(int DP) { return DP == 64 ? 128 : 64; }  // query rows of a step of dk and dv
 constexpr int LO_BITS = 11;  // lo parts are held times 2^LO_BITS
 constexpr float P_SHIFT = 14.0f;  // softmax weights are scaled by 2^14 for their f16 parts
 
@@ -353,13 +354,15 @@ struct TileSource {
   int step;
   float* norm;     // largest Euclidean norm of the tile's rows; may be NULL
   // for dout alone (NULL otherwise): o and lse; the rows' lse in base 2 less
-  // P_SHIFT (+inf for rows without keys or behind the end) and rowsum(dout o), [id][head][TILE]; the
-  // largest magnitude of the latter
+  // P_SHIFT (+inf for rows without keys or behind the end), rowsum(dout o), the rows'
+  // norms, and over each row and the later ones of its block the largest norm and
+  // the largest |rowsum(dout o)|: [id][head][TILE]
   const float* o;
   const float* lse;
   float* lse2;
   float* delta;
-  float* delta_top;
+  float* row_norm;
+  float2* later;
 };
 // A tile of a packed sequence, as a CTA finds it with one load: everything that the
 // offsets say about it.

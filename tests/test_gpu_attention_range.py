@@ -32,3 +32,31 @@ def test_one_large_column(jx, dev, dim, power, which):
     c.backward(jx)
     check(c, 0)
     assert jx.device_status() == 0
+
+
+ROWS = [(64, 256, True), (64, 2048, True), (64, 2048, False), (64, 8192, True), (128, 256, True), (128, 700, False),
+        (128, 2048, True), (128, 8192, True)]
+
+
+@pytest.mark.parametrize("dim,n,causal", ROWS)
+@pytest.mark.parametrize("power", [4, 7, 10, 14, 19])
+def test_few_large_rows_of_dout(jx, dev, dim, n, causal, power):
+    """One token in 128 with a gradient 2^power times the others': dq of the others, dk and dv of the keys that only
+    others see (the last ones of a causal sequence)."""
+    c = Case(dev, [n], [n], 2, 1, dim, causal)
+    c.dout[3::128] *= 2.0 ** power
+    c.forward(jx)
+    c.backward(jx)
+    check(c, (1, 2))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_lens,k_lens", [([1000], [1000]), ([130, 300, 77], [130, 500, 200]), ([400], [250])])
+def test_rows_of_dout_of_all_sizes(jx, dev, dim, q_lens, k_lens):
+    """Tokens that are predicted well and badly, in any order, heads sharing keys."""
+    c = Case(dev, q_lens, k_lens, 6, 2, dim)
+    t = dev.torch
+    c.dout *= 2.0 ** -t.randint(0, 20, (c.tq, 1, 1), device="cuda", generator=c.gen).float()
+    c.forward(jx)
+    c.backward(jx)
+    check(c, (1, 2))
