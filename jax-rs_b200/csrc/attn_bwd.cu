@@ -929,7 +929,7 @@ template <bool VEC>
 __global__ void __launch_bounds__(256) attn_dkv_join_kernel(const __grid_constant__ Shape s,
                                                            const __grid_constant__ BwdTiles bt, float* dk, float* dv) {
   int jt;
-  const int b = seq_of_tile(s.cu_k, s.batch, blockIdx.x / (TILE / JOIN_ROWS), &jt);
+  const int b = seq_of_tile(s.cu_k, s.batch, s.total_k, blockIdx.x / (TILE / JOIN_ROWS), &jt);
   const Seq sq = seq_bounds(s, b);
   const long long j0 = (long long)jt * TILE + blockIdx.x % (TILE / JOIN_ROWS) * JOIN_ROWS;
   if (jt < 0 || j0 >= sq.lk) return;

@@ -55,13 +55,14 @@ __device__ __forceinline__ void load_part(float (&x)[8], const float* p, int lef
 // sees, or query tiles that see a key tile's first key.
 __device__ __forceinline__ int tile_work(const Shape& s, bool over_q, int id, TileRef* ref) {
   const int32_t* cu = over_q ? s.cu_q : s.cu_k;
+  const long long total = over_q ? s.total_q : s.total_k;
   int lo = 0, hi = s.batch;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if ((cu[mid] >> 7) + mid <= id) lo = mid;
+    if (first_tile_of(cu, mid, total) <= id) lo = mid;
     else hi = mid;
   }
-  const int j = id - ((cu[lo] >> 7) + lo);
+  const int j = id - first_tile_of(cu, lo, total);
   const Seq sq = seq_bounds(s, lo);
   const bool in = j >= 0 && (long long)j * TILE < (over_q ? sq.lq : sq.lk);
   *ref = {sq.q0, sq.k0, sq.lq, sq.lk, lo, in ? j : -1};
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(sp_threads(DP), 1024 / sp_threads(DP))
   const TileSource& t = src.t[which];
   const int id = (int)(at_block / heads), h = (int)(at_block - (long long)id * heads);
   int j;
-  const int b = seq_of_tile(over_q ? s.cu_q : s.cu_k, s.batch, id, &j);
+  const int b = seq_of_tile(over_q ? s.cu_q : s.cu_k, s.batch, over_q ? s.total_q : s.total_k, id, &j);
   const Seq sq = seq_bounds(s, b);
   const int len = over_q ? sq.lq : sq.lk;
   if (j < 0 || (long long)j * TILE >= len) return;

@@ -48,13 +48,17 @@ __host__ __device__ constexpr int tile_bytes(int DP) { return 2 * tile_part(DP);
 
 inline long long tile_count(long long total, int batch) { return total / TILE + batch; }
 
+__device__ __forceinline__ int first_tile(long long start, int b) { return (int)(start >> 7) + b; }
+// The first tile of sequence b from its offset, taken into the tensor as seq_bounds takes it.
+__device__ __forceinline__ int first_tile_of(const int32_t* cu, int b, long long total) {
+  return first_tile(max(0LL, min((long long)cu[b], total)), b);
+}
 // Sequence and index within it of tile `id` (warp-uniform); the index may lie behind the sequence's end.
-__device__ __forceinline__ int seq_of_tile(const int32_t* cu, int batch, int id, int* j) {
-  const int b = last_at_most(batch, id, [&](int i) { return (long long)((cu[i] >> 7) + i); });
-  *j = id - ((cu[b] >> 7) + b);
+__device__ __forceinline__ int seq_of_tile(const int32_t* cu, int batch, long long total, int id, int* j) {
+  const int b = last_at_most(batch, id, [&](int i) { return (long long)first_tile_of(cu, i, total); });
+  *j = id - first_tile_of(cu, b, total);
   return b;
 }
-__device__ __forceinline__ int first_tile(long long start, int b) { return (int)(start >> 7) + b; }
 
 // Power of two that brings a magnitude with biased exponent e into [2^14, 2^15), and its inverse.
 // e below LEAST_E (zeros among them) takes LEAST_E's scale.
