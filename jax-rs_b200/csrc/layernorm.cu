@@ -208,9 +208,16 @@ __global__ void __launch_bounds__(block_of(T), PER_SM)
       mn = mean[r1];
       rn = rstd[r1];
     }
+    // Behind the end x is zero, and (0 - m) * rs may be infinite where no column's xhat is.
+    // (A select per element instead takes 75.5 us where this takes 71, 16384 x 2048.)
+    if (isinf(m * rs)) {
+#pragma unroll
+      for (int i = 0; i < N * V; ++i)
+        if (((i / V) * COL_T + t) * V >= cols) xv[i] = m;
+    }
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < N * V; ++i) {  // behind the end dy is zero
+    for (int i = 0; i < N * V; ++i) {  // behind the end dy is zero and xhat finite
       xv[i] = (xv[i] - m) * rs;
       dg[i] = fmaf(dv[i], xv[i], dg[i]);
       db[i] += dv[i];
