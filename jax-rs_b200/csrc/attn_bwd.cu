@@ -73,6 +73,8 @@ __device__ __forceinline__ float bound_scale(float bound) {
 // A row's norm is taken as this part of its tile's at least, so that the scale of an
 // all but empty row stays finite: rows of less than 2^-20 are zeros (or the tile is marked).
 constexpr float LEAST_NORM = 1.4901161e-08f;  // 2^-26
+// Scale of dS over that of dP: below 2^40 but for a bound of zero, whose dS is zero under any finite one.
+__device__ __forceinline__ float scale_ratio(float sc, float fd) { return fminf(sc * fd, 1.2676506e+30f); }  // 2^100
 
 // acc += part * factor for this thread's DP/2 columns of a tensor-memory sum.
 template <int DP>
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       if (j + 1 < nb) next = *(num_k += s.kv_heads);
       // P is at most 2^14
       const float fd = inv_d * inv_v, sc = bound_scale(16384.0f * (norm_d * norm_v + fabsf(delta)));
-      const float f = f_tile * inv_k, pf = sc * fd;
+      const float f = f_tile * inv_k, pf = scale_ratio(sc, fd);
       dl = -delta * inverse_pow2(fd);
       g = inv_k * inverse_pow2(sc) * 6.103515625e-05f;  // P's 2^14
       const float2 f2 = make_float2(f, f), l2 = make_float2(-lse2, -lse2), pf2 = make_float2(pf, pf);
@@ -872,7 +874,7 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       }
       // P is at most 2^14
       const float fd = inv_v * inv_d, sc = bound_scale(16384.0f * (norm_v * norm_d + tops.y));
-      const float pf = sc * fd, nf = -inverse_pow2(fd);
+      const float pf = scale_ratio(sc, fd), nf = -inverse_pow2(fd);
       const float2 pf2 = make_float2(pf, pf), nf2 = make_float2(nf, nf);
       ready(&dpfull[u & 1], u >> 1);
 #pragma unroll

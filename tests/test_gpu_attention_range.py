@@ -60,3 +60,17 @@ def test_rows_of_dout_of_all_sizes(jx, dev, dim, q_lens, k_lens):
     c.forward(jx)
     c.backward(jx)
     check(c, (1, 2))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("zero", [slice(0, 128), slice(0, 200), slice(130, 200)])
+def test_tiles_of_zero_gradient_and_large_values(jx, dev, dim, zero):
+    """dout of zero gives gradients of zero, however large v is."""
+    c = Case(dev, [200], [200], 2, 1, dim)
+    c.v *= 1e32
+    c.dout *= 1e-3
+    c.dout[zero] = 0.0
+    c.forward(jx)
+    c.backward(jx)
+    assert bool((c.dq[zero] == 0).all())
+    check(c, (1, 2))
