@@ -102,7 +102,7 @@ __device__ __forceinline__ void split_half(float a, float b, uint32_t& hi, uint3
   hi = pack_half(a, b);
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   constexpr float UP = 1 << LO_BITS;
-  const float2 r = fma2(h, make_float2(-UP, -UP), mul2(make_float2(a, b), make_float2(UP, UP)));
+  const float2 r = mul2(fma2(h, make_float2(-1.0f, -1.0f), make_float2(a, b)), make_float2(UP, UP));
   lo = pack_half(r.x, r.y);
 }
 __device__ __forceinline__ float exp2_fast(float x) {
