@@ -518,7 +518,11 @@ JX_API int jx_layernorm_bwd_f32(const float *dy, const float *x, const float *ga
  * every value down to 2^-28 of the largest among 128 rows of its head, an absolute
  * 2^-50 of that one below.  Few query rows per key head (decoding) run in plain f32.  128 rows of one head
  * that hold a non-finite value, or largest magnitudes more than 2^20 apart, are
- * computed row by row: as right, but slowly.  Make a first call of each kind
+ * computed row by row: as right, but slowly.  The tensor-core kernels keep their
+ * operands in scratch, in whole tiles of 128 rows per sequence and head; beyond
+ * 2 GB of it the key heads are taken in groups, and where one key head's tiles
+ * alone exceed that and would be mostly empty (many thousands of short sequences)
+ * the call runs in plain f32.  Make a first call of each kind
  * before any stream capture, as for the library's other tensor-core kernels. */
 JX_API int jx_attention_f32(const float *q, const float *k, const float *v, float *o, float *lse,
                             const int32_t *cu_q, const int32_t *cu_k, int64_t batch, int64_t total_q, int64_t total_k,

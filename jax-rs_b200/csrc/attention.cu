@@ -70,7 +70,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dkv_kernel(const __g
 // rows, 16 heads: 140 and 101; 2048 keys x 4, 64 rows a head: 91 and 68.)
 bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
   const double rows = (double)max_q * s.group;
-  if (rows <= 16) return false;
+  if (rows <= 16 || tiles_mostly_empty(s, false)) return false;
   if (rows > 128) return true;
   const double keys = (double)s.total_k * s.kv_heads;
   const double ctas = (double)s.batch * s.heads * ((max_q + 127) / 128);
@@ -87,7 +87,9 @@ bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
 // launches and 0.14 us a CTA.  (8 heads, 8 rows and keys: 13 and 15; 16 of
 // each: 19 and 16; 16 sequences, 32 heads on 8, 8 of each: 39 and 99; 1 row behind
 // 128 keys: 172 and 101.)
+// Tiles that would be mostly empty, and more than the scratch can hold, leave the call to the rows.
 bool rows_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
+  if (tiles_mostly_empty(s, true)) return true;
   const double rows = (double)max_q * s.group, keys = (double)max_k, heads = (double)s.batch * s.heads;
   const double by_row =
       6 + 0.72 * rows + 0.3 * keys + 0.3e-3 * heads * (double)max_q * keys + 6e-3 * (double)s.total_k * s.kv_heads;

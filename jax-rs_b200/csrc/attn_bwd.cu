@@ -991,9 +991,8 @@ int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, c
 
 namespace jxa {
 
-int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
-                        const float* lse, const float* dout, float* dq, float* dk, float* dv, long long max_q,
-                        cudaStream_t st) {
+static int bwd_heads(const Shape& s, const float* q, const float* k, const float* v, const float* o, const float* lse,
+              const float* dout, float* dq, float* dk, float* dv, long long max_q, cudaStream_t st) {
   const int DP = s.dim <= 64 ? 64 : 128;
   const long long kt = tile_count(s.total_k, s.batch), qt = tile_count(s.total_q, s.batch);
   // key tiles are few where heads are shared: enough parts of the query rows for four CTAs per SM, of four blocks at least
@@ -1041,6 +1040,21 @@ int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const fl
                    : launch<64>(s, bt, q, k, v, o, lse, dout, dq, dk, dv, st);
   jx::scratch_release(p, st);
   return rc;
+}
+
+int attention_bwd_tiles(const Shape& s, const float* q, const float* k, const float* v, const float* o,
+                        const float* lse, const float* dout, float* dq, float* dk, float* dv, long long max_q,
+                        cudaStream_t st) {
+  const int DP = s.dim <= 64 ? 64 : 128;
+  const long long tiles = 2 * tile_count(s.total_k, s.batch) + 2 * s.group * tile_count(s.total_q, s.batch);
+  const int each = group_of_heads(s.kv_heads, (size_t)tiles * tile_bytes(DP));
+  for (int hk = 0; hk < s.kv_heads; hk += each) {
+    const long long h = (long long)hk * s.group, hd = h * s.dim, kd = (long long)hk * s.dim;
+    if (int rc = bwd_heads(heads_of(s, std::min(each, s.kv_heads - hk)), q + hd, k + kd, v + kd, o + hd,
+                           lse + h * s.total_q, dout + hd, dq + hd, dk + kd, dv + kd, max_q, st))
+      return rc;
+  }
+  return JX_OK;
 }
 
 }  // namespace jxa

@@ -638,8 +638,7 @@ int prepare_kernel(const void* kernel, int variant, size_t smem, int launch_regs
   return JX_OK;
 }
 
-int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
-                        cudaStream_t st) {
+static int fwd_heads(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse, cudaStream_t st) {
   const int DP = s.dim <= 64 ? 64 : 128;
   const long long kt = tile_count(s.total_k, s.batch), qt = tile_count(s.total_q, s.batch);
   JX_REQUIRE(qt * s.heads < (1LL << 31) && kt < (1LL << 31), "attention: too many rows");
@@ -671,6 +670,19 @@ int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const fl
   }
   jx::scratch_release(p, st);
   return rc;
+}
+
+int attention_fwd_tiles(const Shape& s, const float* q, const float* k, const float* v, float* o, float* lse,
+                        cudaStream_t st) {
+  const int DP = s.dim <= 64 ? 64 : 128;
+  const int each = group_of_heads(s.kv_heads, 2 * (size_t)tile_count(s.total_k, s.batch) * tile_bytes(DP));
+  for (int hk = 0; hk < s.kv_heads; hk += each) {
+    const long long h = (long long)hk * s.group;
+    if (int rc = fwd_heads(heads_of(s, std::min(each, s.kv_heads - hk)), q + h * s.dim, k + (long long)hk * s.dim,
+                           v + (long long)hk * s.dim, o + h * s.dim, lse ? lse + h * s.total_q : nullptr, st))
+      return rc;
+  }
+  return JX_OK;
 }
 
 }  // namespace jxa

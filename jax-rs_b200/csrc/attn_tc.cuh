@@ -31,6 +31,8 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "attn_common.cuh"
 #include "tc_gemm.cuh"
 
@@ -47,6 +49,32 @@ __host__ __device__ constexpr int tile_part(int DP) { return DP / 64 * PANEL; } 
 __host__ __device__ constexpr int tile_bytes(int DP) { return 2 * tile_part(DP); }   // hi and lo
 
 inline long long tile_count(long long total, int batch) { return total / TILE + batch; }
+
+// Tiles are whole, so that sequences far shorter than 128 rows take scratch by
+// their number, not by their rows.  Beyond SCRATCH of it the key heads are taken in
+// groups, one group's launches behind the other's (SCRATCH is some ten thousand
+// CTAs' work, so that a group fills the GPU as all of them would).
+constexpr size_t SCRATCH = size_t{2} << 30;
+// Key heads of a group, for `bytes` of scratch a key head.
+inline int group_of_heads(int kv_heads, size_t bytes) {
+  const int most = (int)std::max<size_t>(1, std::min<size_t>(kv_heads, SCRATCH / std::max<size_t>(1, bytes)));
+  const int groups = (kv_heads + most - 1) / most;
+  return (kv_heads + groups - 1) / groups;
+}
+// Whether even one key head's tiles are beyond SCRATCH, and four times what its rows alone would fill.
+inline bool tiles_mostly_empty(const Shape& s, bool gradients) {
+  const long long per_q = gradients ? 2 * s.group : 0;
+  const long long tiles = 2 * tile_count(s.total_k, s.batch) + per_q * tile_count(s.total_q, s.batch);
+  const long long filled = 2 * tile_count(s.total_k, 1) + per_q * tile_count(s.total_q, 1);
+  return tiles > 4 * filled && (size_t)tiles * tile_bytes(s.dim <= 64 ? 64 : 128) > SCRATCH;
+}
+// The call's shape for `n` of its key heads.
+inline Shape heads_of(const Shape& s, int n) {
+  Shape r = s;
+  r.kv_heads = n;
+  r.heads = n * s.group;
+  return r;
+}
 
 __device__ __forceinline__ int first_tile(long long start, int b) { return (int)(start >> 7) + b; }
 // The first tile of sequence b from its offset, taken into the tensor as seq_bounds takes it.
