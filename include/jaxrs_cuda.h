@@ -607,6 +607,11 @@ JX_API int jx_mlp_step_times(jx_mlp *mlp, float *ms);
  * device error word and returns; *timed_out = 1 if the kernel reported it.
  * The context stays usable. */
 JX_API int jx_selftest_barrier_timeout(int timeout_ms, int *timed_out);
+/* Self-test of the attention kernels' waits (no reference counterpart): `waits`
+ * (1..64) waits in a row for a barrier that nothing completes, which share one
+ * limit of timeout_ms (1..1000).  *timed_out counts those that gave up, *waited_ms
+ * is the time that all of them took; JX_DEVERR_TIMEOUT is recorded. */
+JX_API int jx_selftest_wait_timeout(int timeout_ms, int waits, int *timed_out, float *waited_ms);
 /* Test hook (no reference counterpart): ORs flags into the current device's
  * jx_gemm_f32_noalloc error word, so a test can check that the word reaches
  * jx_device_status without making a wait run out. */

@@ -156,6 +156,7 @@ _SIGS = {
     "jx_mlp_set_dp_sharded": [vp, ci],
     "jx_mlp_step_times": [vp, C.POINTER(cf)],
     "jx_selftest_barrier_timeout": [ci, C.POINTER(ci)],
+    "jx_selftest_wait_timeout": [ci, ci, C.POINTER(ci), C.POINTER(cf)],
     "jx_selftest_noalloc_flag": [C.c_uint],
     "jx_mlp_destroy": [vp],
     "jx_nccl_unique_id_size": [],

@@ -96,6 +96,17 @@ bool rows_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
   return by_row < 15 + (s.group > 1 ? 8 : 0) + 0.14 * heads;
 }
 
+// Waits for a barrier that nothing completes, `waits` times with one time to give up.
+__global__ void wait_selftest_kernel(int waits, unsigned long long limit_ns, unsigned int* err, int* given_up,
+                                     unsigned long long* ns) {
+  __shared__ uint64_t bar;
+  jxd::mbar_init(&bar, 1);
+  const unsigned long long start = jxg::global_ns();
+  unsigned long long end = 0;
+  for (int i = 0; i < waits; ++i) *given_up += !wait_suspended(&bar, 0, err, end, limit_ns);
+  *ns = jxg::global_ns() - start;
+}
+
 int check_shape(const char* what, Shape& s, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t total_q,
                 int64_t total_k, int64_t max_q, int64_t max_k, int64_t heads, int64_t kv_heads, int64_t head_dim,
                 int64_t ldq, int64_t ldk, int64_t ldv, int64_t ldo, float scale, int causal) {
@@ -187,6 +198,33 @@ int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const f
   if (bq) attn_rows_dq_kernel<<<(unsigned)bq, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse, dout, dq);
   if (bk) attn_rows_dkv_kernel<<<(unsigned)bk, 32 * ROW_WARPS, 0, st>>>(s, q, k, v, o, lse, dout, dk, dv);
   JX_LAUNCH_CHECK("attention_bwd kernels");
+  return JX_OK;
+}
+
+int jx_selftest_wait_timeout(int timeout_ms, int waits, int* timed_out, float* waited_ms) {
+  JX_TRACE("jx_selftest_wait_timeout");
+  JX_REQUIRE(timed_out && waited_ms && timeout_ms >= 1 && timeout_ms <= 1000 && waits >= 1 && waits <= 64,
+             "jx_selftest_wait_timeout: 1..1000 ms, 1..64 waits");
+  unsigned int* err = jx::device_error_word();
+  if (!err) return jx::fail(JX_ENOMEM, "device error word unavailable");
+  void* buf = nullptr;
+  JX_CUDA(cudaMalloc(&buf, 16));
+  cudaError_t e = cudaMemset(buf, 0, 16);
+  if (e == cudaSuccess) {
+    wait_selftest_kernel<<<1, 1>>>(waits, timeout_ms * 1000000ull, err, reinterpret_cast<int*>(buf) + 2,
+                                   static_cast<unsigned long long*>(buf));
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  struct {
+    unsigned long long ns;
+    int given_up;
+  } h = {};
+  if (e == cudaSuccess) e = cudaMemcpy(&h, buf, 12, cudaMemcpyDeviceToHost);
+  cudaFree(buf);
+  if (e != cudaSuccess) return jx::check_cuda(e, "wait self-test");
+  *timed_out = h.given_up;
+  *waited_ms = (float)(h.ns * 1e-6);
   return JX_OK;
 }
 

@@ -286,9 +286,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
              sq.visible(i0 + r, s.causal), s.dim, s.ldk, s.ldv, s.scale);
     }
     if (warp == 0 && lane == 0 && nb > 0) {  // the copies have landed
-      wait_suspended(stayfull, 0, s.err);
-      for (int j = 0; j < min(nb, K_FIRST); ++j) wait_suspended(&kfull[j], 0, s.err);
-      for (int j = 0; j < min(nb, V_FIRST); ++j) wait_suspended(&vfull[j], 0, s.err);
+      unsigned long long end = 0;  // for all of them
+      wait_suspended(stayfull, 0, s.err, end);
+      for (int j = 0; j < min(nb, K_FIRST); ++j) wait_suspended(&kfull[j], 0, s.err, end);
+      for (int j = 0; j < min(nb, V_FIRST); ++j) wait_suspended(&vfull[j], 0, s.err, end);
     }
     if (warp == 1) {
       __syncwarp();
@@ -317,9 +318,10 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       }
       if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may end
-      wait_suspended(stayfull, 0, s.err);
-      for (int u = max(0, nk - KS); u < nk; ++u) wait_suspended(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err);
-      for (int u = max(0, nv - VS); u < nv; ++u) wait_suspended(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err);
+      unsigned long long end = 0;  // for all of them
+      wait_suspended(stayfull, 0, s.err, end);
+      for (int u = max(0, nk - KS); u < nk; ++u) wait_suspended(&kfull[u % KS], (uint32_t)(u / KS) & 1u, s.err, end);
+      for (int u = max(0, nv - VS); u < nv; ++u) wait_suspended(&vfull[u % VS], (uint32_t)(u / VS) & 1u, s.err, end);
     }
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
       // ---- MMA (its waits stand between products: nothing is looked at there but the barrier)
@@ -680,10 +682,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
               s.scale);
     }
     if (warp == 0 && lane == 0 && n > 0) {  // the copies have landed
-      wait_suspended(stayfull, 0, s.err);
-      for (int u = 0; u < min(n, Q_FIRST); ++u) wait_suspended(&qfull[u], 0, s.err);
-      for (int u = 0; u < min(n, DS); ++u) wait_suspended(&dfull[u], 0, s.err);
-      for (int u = 0; u < min(n, 2); ++u) wait_suspended(&tfull[u], 0, s.err);
+      unsigned long long end = 0;  // for all of them
+      wait_suspended(stayfull, 0, s.err, end);
+      for (int u = 0; u < min(n, Q_FIRST); ++u) wait_suspended(&qfull[u], 0, s.err, end);
+      for (int u = 0; u < min(n, DS); ++u) wait_suspended(&dfull[u], 0, s.err, end);
+      for (int u = 0; u < min(n, 2); ++u) wait_suspended(&tfull[u], 0, s.err, end);
     }
     if (warp == 1) {
       __syncwarp();
@@ -724,10 +727,11 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       }
       if (!ok) *abort_flag = 1;
       // every copy has landed before the CTA may end
-      wait_suspended(stayfull, 0, s.err);
-      for (int e = max(0, nq - QS); e < nq; ++e) wait_suspended(&qfull[e % QS], (uint32_t)(e / QS) & 1u, s.err);
-      for (int e = max(0, nd - DS); e < nd; ++e) wait_suspended(&dfull[e % DS], (uint32_t)(e / DS) & 1u, s.err);
-      for (int e = max(0, nt - 2); e < nt; ++e) wait_suspended(&tfull[e & 1], (uint32_t)(e >> 1) & 1u, s.err);
+      unsigned long long end = 0;  // for all of them
+      wait_suspended(stayfull, 0, s.err, end);
+      for (int e = max(0, nq - QS); e < nq; ++e) wait_suspended(&qfull[e % QS], (uint32_t)(e / QS) & 1u, s.err, end);
+      for (int e = max(0, nd - DS); e < nd; ++e) wait_suspended(&dfull[e % DS], (uint32_t)(e / DS) & 1u, s.err, end);
+      for (int e = max(0, nt - 2); e < nt; ++e) wait_suspended(&tfull[e & 1], (uint32_t)(e >> 1) & 1u, s.err, end);
     }
     if (warp == 1 && n > 0 && jxd::elect_one()) {
       // ---- MMA

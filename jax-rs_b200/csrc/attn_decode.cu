@@ -28,7 +28,6 @@
 namespace {
 
 using namespace jxa;
-using jxg::wait_bounded;
 
 constexpr int DC_WARPS = 8;
 constexpr int DC_KEYS = 8;  // keys per stage
@@ -429,8 +428,11 @@ __global__ void __launch_bounds__(32 * DC_WARPS, 1)
   }
   // not before: the join's blocks would wait where rings still stream (37.0 us against 33.2 at the start of the kernel)
   asm volatile("griddepcontrol.launch_dependents;");
-  if (!ok && wr == 0 && (!VEC || lane == 0))  // every copy has landed before the CTA may end
-    for (int u = max(0, issued - nst); u < issued; ++u) wait_bounded(&full[u % nst], (uint32_t)(u / nst) & 1u, s.err);
+  if (!ok && wr == 0 && (!VEC || lane == 0)) {  // every copy has landed before the CTA may end
+    unsigned long long end = 0;  // for all of them
+    for (int u = max(0, issued - nst); u < issued; ++u)
+      wait_suspended(&full[u % nst], (uint32_t)(u / nst) & 1u, s.err, end);
+  }
 }
 
 // One block per (query row, head): the pieces in order; rows without keys; rows

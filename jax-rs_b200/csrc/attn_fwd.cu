@@ -379,8 +379,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
               o + t * s.ldo + hd, lse ? lse + (long long)h * s.total_q + t : nullptr, sq.visible(i0 + r, s.causal),
               s.dim, s.ldk, s.ldv, s.scale);
     }
-    if (warp == 0 && lane == 0)  // every copy has landed before the CTA may end
-      for (int u = 0; u < first; ++u) wait_bounded(&full[u], 0, s.err);
+    if (warp == 0 && lane == 0) {  // every copy has landed before the CTA may end
+      unsigned long long end = 0;  // for all of them
+      for (int u = 0; u < first; ++u) wait_suspended(&full[u], 0, s.err, end);
+    }
     if (warp == 1) {
       __syncwarp();
       jxd::tmem_dealloc(tmem, 512);
@@ -402,8 +404,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1)
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
       // every copy has landed before the CTA may end
+      unsigned long long end = 0;  // for all of them
       for (int u = max(0, issued - STAGES); u < issued; ++u)
-        wait_bounded(&full[u % STAGES], (uint32_t)(u / STAGES) & 1u, s.err);
+        wait_suspended(&full[u % STAGES], (uint32_t)(u / STAGES) & 1u, s.err, end);
     }
     if (warp == 1 && nb > 0 && jxd::elect_one()) {
       // ---- MMA

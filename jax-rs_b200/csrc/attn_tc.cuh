@@ -230,9 +230,11 @@ __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded waits in a few instructions (2^26 of them are seconds).  With
-// jxg::wait_bounded and its clock at every wait the gradient of packed sequences took 7%
-// longer.  The copies' thread may be suspended; the others poll.
+// Bounded waits in a few instructions.  With jxg::wait_bounded and its clock at every
+// wait the gradient of packed sequences took 7% longer.  Polling takes some 20 to 50
+// cycles a time, so that 2^26 polls are one to two seconds.  The copies' thread may be
+// suspended, for as long as the hardware likes at each try, so that its limit is a
+// time: the clock is read from the 64th try on.
 __device__ __forceinline__ bool wait_polling(uint64_t* bar, uint32_t parity, unsigned int* err) {
   for (uint32_t i = 0; !poll(bar, parity); ++i) {
     if (i == 1u << 26) {
@@ -242,14 +244,24 @@ __device__ __forceinline__ bool wait_polling(uint64_t* bar, uint32_t parity, uns
   }
   return true;
 }
-__device__ __forceinline__ bool wait_suspended(uint64_t* bar, uint32_t parity, unsigned int* err) {
+constexpr unsigned long long WAIT_NS = 4000000000ull;
+// `end` (0 before the first late try) is the time at which waits that share it give up.
+__device__ __forceinline__ bool wait_suspended(uint64_t* bar, uint32_t parity, unsigned int* err,
+                                               unsigned long long& end, unsigned long long limit_ns = WAIT_NS) {
   for (uint32_t i = 0; !jxd::mbar_try_wait(bar, parity); ++i) {
-    if (i == 1u << 26) {
+    if (i < 64) continue;
+    const unsigned long long now = jxg::global_ns();
+    if (end == 0) end = now + limit_ns;
+    if (now >= end) {
       atomicOr(err, JX_DEVERR_TIMEOUT);
       return false;
     }
   }
   return true;
+}
+__device__ __forceinline__ bool wait_suspended(uint64_t* bar, uint32_t parity, unsigned int* err) {
+  unsigned long long end = 0;
+  return wait_suspended(bar, parity, err, end);
 }
 // A warp waits, every lane for itself: polling by one lane and telling the others
 // cost 100 cycles more at each of the three to five waits of a step.
