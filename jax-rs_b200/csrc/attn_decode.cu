@@ -66,8 +66,9 @@ struct Cursor {
     left = 0;
     for (; b < s.batch; ++b) {
       sq = seq_bounds(s, b);
-      if ((long long)sq.lq * s.group <= row_base || sq.lk == 0) continue;
       const long long base = (sq.k0 + (long long)b * VOID) * s.kv_heads, in = max(0LL, pos - base);
+      if (base >= end) return;  // this sequence and all behind it are other rings'
+      if ((long long)sq.lq * s.group <= row_base || sq.lk == 0) continue;
       const int len = sq.lk + VOID;
       if (in >= (long long)s.kv_heads * len) continue;
       hk = (int)(in / len);
