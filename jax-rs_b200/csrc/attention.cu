@@ -81,7 +81,7 @@ bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
 }
 
 // Whether the gradients are computed row by row (two launches, a warp per row and head)
-// or by tiles (four, or five where heads are shared), from the hints, in
+// or by tiles (two, or three where key tiles are few), from the hints, in
 // microseconds as measured: a row's warp takes 0.3 us a key, a key's 0.72 us a row of its
 // heads, each besides what all of them together cost; the tiles' cost is their
 // launches and 0.14 us a CTA.  (8 heads, 8 rows and keys: 13 and 15; 16 of

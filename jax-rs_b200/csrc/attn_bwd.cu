@@ -1,10 +1,10 @@
 // attn_bwd.cu -- attention's gradients on the tensor cores (operands and sums as
 // in attn_tc.cuh).
 //
-// Two kernels, each with its sums in registers, so that every sum has a fixed
+// Two kinds of CTAs, each with its sums in registers, so that every sum has a fixed
 // order and nothing is added atomically; the price is that the scores and
 // dout v^T are computed in both (seven products a tile instead of five).  All
-// four operands are split into tiles once, and each kernel streams two of them.
+// four operands are split into tiles once, and each kind streams two of them.
 //
 // dq: one CTA per (128 query rows, head), streaming K and V tiles.
 //   S = Q K^T, dP = dO V^T,  dS = P (dP - delta),  dQ += dS K
@@ -184,13 +184,12 @@ struct DqLayout {
 };
 
 template <int DP>
-__global__ void __launch_bounds__(BW_THREADS, 1)
-    attn_dq_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
-                   const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
-                   const float* __restrict__ lse, const float* __restrict__ dout, float* dq) {
+__device__ __forceinline__ void dq_tile(const Shape& s, const BwdTiles& bt, uint8_t* smem_raw, unsigned w,
+                                        const float* __restrict__ q, const float* __restrict__ k,
+                                        const float* __restrict__ v, const float* __restrict__ o,
+                                        const float* __restrict__ lse, const float* __restrict__ dout, float* dq) {
   using L = DqLayout<DP>;
   constexpr int KS = L::KS, VS = L::VS, STAGE = tile_bytes(DP), PART = tile_part(DP);
-  extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw_addr + 1023u) & ~1023u) - raw_addr);
   uint8_t* ring = smem + L::STAY;  // K's stages, then V's
@@ -209,10 +208,8 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiles are complete behind it
-  asm volatile("griddepcontrol.launch_dependents;");
-  const TileRef ref = load_ref(bt.order_q + blockIdx.x / (unsigned)s.heads);
-  const int h = (int)(blockIdx.x % (unsigned)s.heads), b = ref.b, jt = ref.jt;
+  const TileRef ref = load_ref(bt.order_q + w / (unsigned)s.heads);
+  const int h = (int)(w % (unsigned)s.heads), b = ref.b, jt = ref.jt;
   const Seq sq = seq_of(ref);
   if (jt < 0) return;
   const int i0 = jt * TILE, rows = min(TILE, sq.lq - i0);
@@ -518,25 +515,18 @@ struct KvLayout {
 };
 static_assert(KvLayout<64>::SMEM <= 232448 && KvLayout<128>::SMEM <= 232448, "shared memory of an SM");
 
-// dk's and dv's CTAs start as dq's last ones run: they read nothing of dq's, and all
-// of dq's CTAs have seen the split complete before the first of these starts.
-// What follows in the stream waits for this kernel alone, so that it must not end
-// before dq's.
-__device__ __forceinline__ void after_dq() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 template <int DP>
-__global__ void __launch_bounds__(BW_THREADS, 1)
-    attn_dkv_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
-                    const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
-                    const float* __restrict__ lse, const float* __restrict__ dout, float* dk, float* dv) {
+__device__ __forceinline__ void dkv_tile(const Shape& s, const BwdTiles& bt, uint8_t* smem_raw, unsigned w,
+                                         const float* __restrict__ q, const float* __restrict__ k,
+                                         const float* __restrict__ v, const float* __restrict__ o,
+                                         const float* __restrict__ lse, const float* __restrict__ dout, float* dk,
+                                         float* dv) {
   using L = KvLayout<DP>;
   constexpr int QS = L::QS, DS = L::DS, BLK = L::BLK, STAGE = L::STAGE, PART = STAGE / 2, HPANEL = L::PANEL_BYTES;
   constexpr int PER_TILE = TILE / BLK;  // blocks of a tile
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw_addr = jxd::smem_u32(smem_raw), shift = ((raw_addr + 1023u) & ~1023u) - raw_addr;
   if (shift > (uint32_t)L::SPARE) {
     if (threadIdx.x == 0) atomicOr(s.err, JX_DEVERR_TIMEOUT);
-    after_dq();
     return;
   }
   uint8_t* smem = smem_raw + shift;
@@ -562,16 +552,12 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the keys that the most rows see start first
-  unsigned w = blockIdx.x;
   const int part = (int)(w % (unsigned)bt.parts);
   w /= (unsigned)bt.parts;
   const TileRef ref = load_ref(bt.order_k + w / (unsigned)s.kv_heads);
   const int hk = (int)(w % (unsigned)s.kv_heads), b = ref.b, jt = ref.jt;
   const Seq sq = seq_of(ref);
-  if (jt < 0) {
-    after_dq();
-    return;
-  }
+  if (jt < 0) return;
   const int j0 = jt * TILE, rows = min(TILE, sq.lk - j0);
   const int blk0 = sq.first_row(j0, s.causal) / BLK;
   const int nblk = max(0, (sq.lq + BLK - 1) / BLK - blk0);
@@ -692,7 +678,6 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
       __syncwarp();
       jxd::tmem_dealloc(tmem, 512);
     }
-    after_dq();
     return;
   }
 
@@ -926,7 +911,20 @@ __global__ void __launch_bounds__(BW_THREADS, 1)
     __syncwarp();
     jxd::tmem_dealloc(tmem, 512);
   }
-  after_dq();
+}
+
+// Both in one launch, so that dk's and dv's CTAs start as dq's last ones run: the first
+// q_tiles * heads blocks are dq's.  Neither reads what the other writes.
+template <int DP>
+__global__ void __launch_bounds__(BW_THREADS, 1)
+    attn_bwd_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
+                    const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
+                    const float* __restrict__ lse, const float* __restrict__ dout, float* dq, float* dk, float* dv) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const unsigned dq_blocks = (unsigned)bt.q_tiles * (unsigned)s.heads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiles are complete behind it
+  if (blockIdx.x < dq_blocks) dq_tile<DP>(s, bt, smem_raw, blockIdx.x, q, k, v, o, lse, dout, dq);
+  else dkv_tile<DP>(s, bt, smem_raw, blockIdx.x - dq_blocks, q, k, v, o, lse, dout, dk, dv);
 }
 
 // The parts' sums in order, 16 key rows of one key head per block.
@@ -972,14 +970,10 @@ __global__ void __launch_bounds__(256) attn_dkv_join_kernel(const __grid_constan
 template <int DP>
 int launch(const Shape& s, const BwdTiles& bt, const float* q, const float* k, const float* v, const float* o,
            const float* lse, const float* dout, float* dq, float* dk, float* dv, cudaStream_t st) {
-  if (int rc = prepare_kernel((const void*)attn_dq_kernel<DP>, DP == 128 ? 2 : 3, DqLayout<DP>::SMEM, BW_LAUNCH_REGS))
-    return rc;
-  if (int rc = prepare_kernel((const void*)attn_dkv_kernel<DP>, DP == 128 ? 4 : 5, KvLayout<DP>::SMEM, BW_LAUNCH_REGS))
-    return rc;
-  JX_CUDA(launch_overlapped(attn_dq_kernel<DP>, (long long)bt.q_tiles * s.heads, BW_THREADS, DqLayout<DP>::SMEM, st, s,
-                            bt, q, k, v, o, lse, dout, dq));
-  JX_CUDA(launch_overlapped(attn_dkv_kernel<DP>, (long long)bt.k_tiles * s.kv_heads * bt.parts, BW_THREADS,
-                            KvLayout<DP>::SMEM, st, s, bt, q, k, v, o, lse, dout, dk, dv));
+  constexpr size_t smem = std::max(DqLayout<DP>::SMEM, KvLayout<DP>::SMEM);
+  if (int rc = prepare_kernel((const void*)attn_bwd_kernel<DP>, DP == 128 ? 2 : 3, smem, BW_LAUNCH_REGS)) return rc;
+  const long long blocks = (long long)bt.q_tiles * s.heads + (long long)bt.k_tiles * s.kv_heads * bt.parts;
+  JX_CUDA(launch_overlapped(attn_bwd_kernel<DP>, blocks, BW_THREADS, smem, st, s, bt, q, k, v, o, lse, dout, dq, dk, dv));
   if (bt.parts > 1) {
     const dim3 grid((unsigned)(bt.k_tiles * (TILE / JOIN_ROWS)), (unsigned)s.kv_heads);
     const bool vec = !(s.dim & 3) && !(s.ldk & 3) && !(s.ldv & 3) &&
@@ -1003,7 +997,7 @@ static int bwd_heads(const Shape& s, const float* q, const float* k, const float
   const long long ctas = kt * s.kv_heads, blocks = s.group * ((max_q + 63) / 64);
   const int parts =
       (int)std::max<long long>(1, std::min(std::min<long long>(8, blocks / 4), 4LL * jx::num_sms() / std::max(1LL, ctas)));
-  JX_REQUIRE(qt * s.heads < (1LL << 31) && kt * s.kv_heads * parts < (1LL << 31) && kt < (1LL << 27),
+  JX_REQUIRE(qt * s.heads + kt * s.kv_heads * parts < (1LL << 31) && kt < (1LL << 27),
              "attention_bwd: too many rows");
   const size_t ks = (size_t)kt * s.kv_heads, qs = (size_t)qt * s.heads, tb = tile_bytes(DP);
   const size_t part_floats = parts > 1 ? (size_t)parts * s.total_k * s.kv_heads * s.dim : 0;
