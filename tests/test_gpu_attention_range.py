@@ -74,3 +74,18 @@ def test_tiles_of_zero_gradient_and_large_values(jx, dev, dim, zero):
     c.backward(jx)
     assert bool((c.dq[zero] == 0).all())
     check(c, (1, 2))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_of_all_sizes(jx, dev, dim, which, causal):
+    """Rows of one operand over 2^19, large ones behind small ones and before them."""
+    c = Case(dev, [130, 700], [400, 700], 4, 2, dim, causal)
+    t, x = dev.torch, getattr(c, which)
+    x *= 2.0 ** -t.randint(0, 20, (x.shape[0], 1, 1), device="cuda", generator=c.gen).float()
+    x[3::128] *= 2.0 ** 4
+    c.forward(jx)
+    c.check_forward()
+    c.backward(jx)
+    check(c, (1, 2))
