@@ -156,7 +156,7 @@ int jx_attention_f32(const float* q, const float* k, const float* v, float* o, f
   JX_REQUIRE(q && o && cu_q && cu_k && (total_k == 0 || (k && v)), "attention: NULL pointer");
   JX_REQUIRE(o != q && o != k && o != v, "attention: o must not be an input");
   cudaStream_t st = jx::as_stream(stream);
-  s.err = jx::device_error_word();
+  if (!(s.err = jx::device_error_word())) return jx::fail(JX_ENOMEM, "device error word unavailable");
   JX_REQUIRE(total_q * heads < (1LL << 31), "attention: too many rows");
   max_q = std::min(max_q, total_q);
   max_k = std::min(max_k, total_k);
@@ -187,7 +187,7 @@ int jx_attention_bwd_f32(const float* q, const float* k, const float* v, const f
     }
   }
   cudaStream_t st = jx::as_stream(stream);
-  s.err = jx::device_error_word();
+  if (!(s.err = jx::device_error_word())) return jx::fail(JX_ENOMEM, "device error word unavailable");
   max_q = std::min(max_q, total_q);
   max_k = std::min(max_k, total_k);
   if (total_q > 0 && total_k > 0 && !rows_are_faster(s, max_q, max_k))
