@@ -913,18 +913,19 @@ __device__ __forceinline__ void dkv_tile(const Shape& s, const BwdTiles& bt, uin
   }
 }
 
-// Both in one launch, so that dk's and dv's CTAs start as dq's last ones run: the first
-// q_tiles * heads blocks are dq's.  Neither reads what the other writes.
+// Both in one launch, so that one kind's CTAs start as the other's last ones run.
+// Neither reads what the other writes.  dk's and dv's come first, being the longer
+// ones: 8 heads, 32 rows 15.6 us in a graph against 17.5 the other way round, 4096 packed tokens 184 against 186.
 template <int DP>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,
                     const float* __restrict__ k, const float* __restrict__ v, const float* __restrict__ o,
                     const float* __restrict__ lse, const float* __restrict__ dout, float* dq, float* dk, float* dv) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const unsigned dq_blocks = (unsigned)bt.q_tiles * (unsigned)s.heads;
+  const unsigned dkv_blocks = (unsigned)bt.k_tiles * (unsigned)s.kv_heads * (unsigned)bt.parts;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the tiles are complete behind it
-  if (blockIdx.x < dq_blocks) dq_tile<DP>(s, bt, smem_raw, blockIdx.x, q, k, v, o, lse, dout, dq);
-  else dkv_tile<DP>(s, bt, smem_raw, blockIdx.x - dq_blocks, q, k, v, o, lse, dout, dk, dv);
+  if (blockIdx.x < dkv_blocks) dkv_tile<DP>(s, bt, smem_raw, blockIdx.x, q, k, v, o, lse, dout, dk, dv);
+  else dq_tile<DP>(s, bt, smem_raw, blockIdx.x - dkv_blocks, q, k, v, o, lse, dout, dq);
 }
 
 // The parts' sums in order, 16 key rows of one key head per block.
