@@ -511,9 +511,13 @@ JX_API int jx_layernorm_bwd_f32(const float *dy, const float *x, const float *ga
  * causal != 0 aligns the sequence's ends: row i of lq sees the keys j <= i +
  * lk - lq, so that lq = 1 is a decoding step behind lk - 1 cached keys.  A row
  * that sees no key gets o = 0 and lse = -inf.  A key that a row does not see has
- * no effect on it, whatever its values.  lse [heads, total_q] may be NULL.
+ * no effect on it, whatever its values, but for the last bits' rounding of keys
+ * that share its 128 rows.  A cache with room to grow: the room behind a request's
+ * keys is a sequence without query rows (cu_q stands still there), and its values
+ * are no row's keys.  lse [heads, total_q] may be NULL.
  * max_q / max_k: the longest sequences, a hint for the choice of kernel; any
- * value >= 0 gives right results.  Prompts run on the tensor cores, each f32
+ * value >= 0 gives right results, but a decoding batch without its own (max_q =
+ * 1, say) is taken for prompts and is several times slower.  Prompts run on the tensor cores, each f32
  * operand split in two f16 parts under a power-of-two scale, f32 sums: 22 bits of
  * every value down to 2^-28 of the largest among 128 rows of its head, an absolute
  * 2^-50 of that one below.  Few query rows per key head (decoding) run in plain f32.  128 rows of one head

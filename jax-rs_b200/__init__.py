@@ -357,7 +357,9 @@ def _attention_sizes(batch, total_q, total_k, max_q, max_k, heads, kv_heads, hea
 def attention(q, k, v, o, lse, cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, head_dim, max_q=None,
               max_k=None, ldq=None, ldk=None, ldv=None, ldo=None, scale=None, causal=True, stream=None):
     """Attention over packed sequences with grouped heads; lse [heads, total_q] may be None.
-    Row strides default to dense rows, scale to 1 / sqrt(head_dim)."""
+    Row strides default to dense rows, scale to 1 / sqrt(head_dim).  max_q and max_k, the longest sequences, decide
+    which kernel runs: give them for a batch of several sequences (they default to all rows in one sequence, under
+    which a decoding batch takes the prompts' kernels, several times slower)."""
     call("jx_attention_f32", q, k, v, o, lse, cu_q, cu_k,
          *_attention_sizes(batch, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, ldq, ldk, ldv, ldo,
                            scale, causal), stream)
@@ -366,7 +368,7 @@ def attention(q, k, v, o, lse, cu_q, cu_k, batch, total_q, total_k, heads, kv_he
 def attention_bwd(q, k, v, o, lse, dout, dq, dk, dv, cu_q, cu_k, batch, total_q, total_k, heads, kv_heads, head_dim,
                   max_q=None, max_k=None, ldq=None, ldk=None, ldv=None, ldo=None, scale=None, causal=True,
                   stream=None):
-    """Gradients of attention; dout has o's row stride, dq, dk and dv those of q, k and v."""
+    """Gradients of attention; dout has o's row stride, dq, dk and dv those of q, k and v.  max_q and max_k as there."""
     call("jx_attention_bwd_f32", q, k, v, o, lse, dout, dq, dk, dv, cu_q, cu_k,
          *_attention_sizes(batch, total_q, total_k, max_q, max_k, heads, kv_heads, head_dim, ldq, ldk, ldv, ldo,
                            scale, causal), stream)

@@ -66,8 +66,10 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) attn_rows_dkv_kernel(const __g
 // for every 32 query rows of a key head, 18 us and about 1 ns a key and head each
 // time (0.25 ns at 4 rows: HBM's rate); the tiles cost 2.3 us per 128 keys for each wave of
 // (query tile, head) CTAs, and the split of K and V 0.4 ns a key and head.
-// (4 sequences of 8192 keys, 64 heads on 1: rings 93, tiles 278; 1000 keys x 8, 20
-// rows, 16 heads: 140 and 101; 2048 keys x 4, 64 rows a head: 91 and 68.)
+// (4 sequences of 8192 keys, 64 heads on 1: rings 83, tiles 248; 1000 keys x 8, 20
+// rows, 16 heads: 140 and 101; 2048 keys x 4, 64 rows a head: 91 and 68.  The figures
+// rest on few shapes; at dim 64 the first takes 73 and 181, and 700 and 1500 keys, 8 rows, 16
+// heads on 4 of dim 40 19 and 26.)
 bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
   const double rows = (double)max_q * s.group;
   if (rows <= 16 || tiles_mostly_empty(s, false)) return false;
@@ -84,9 +86,9 @@ bool tiles_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
 // or by tiles (two, or three where key tiles are few), from the hints, in
 // microseconds as measured: a row's warp takes 0.3 us a key, a key's 0.72 us a row of its
 // heads, each besides what all of them together cost; the tiles' cost is their
-// launches and 0.14 us a CTA.  (8 heads, 8 rows and keys: 13 and 15; 16 of
-// each: 19 and 16; 16 sequences, 32 heads on 8, 8 of each: 39 and 99; 1 row behind
-// 128 keys: 172 and 101.)
+// launches and 0.14 us a CTA.  (8 heads, 8 rows and keys: 12 and 16; 16 of
+// each: 19 and 16; 16 sequences, 32 heads on 8, 8 of each: 39 and 94; 1 row behind
+// 128 keys: 173 and 99.)
 // Tiles that would be mostly empty, and more than the scratch can hold, leave the call to the rows.
 bool rows_are_faster(const Shape& s, int64_t max_q, int64_t max_k) {
   if (tiles_mostly_empty(s, true)) return true;

@@ -18,14 +18,14 @@
 // ahead where tensor memory has the room; the layouts below say where that is.
 // An MMA of 64 columns takes 44 to 48 cycles, not the 32 that half of one of 128 is, so
 // that a tile's seven products of three parts each take 2600 (dq) and 3650 cycles (dk and dv) at dim 64;
-// the steps take 2740 and 4400.  What stands between two products on the MMA thread's
+// the steps take 3200 and 5000, the mean of 16 with the first one's latencies.  What stands between two products on the MMA thread's
 // way counts in full: its waits look at the barrier and at nothing else (an abort
 // flag read there cost 3% to 10% of the whole).
 //
-// 4096 packed tokens in 5 sequences, 16 heads, dim 64, causal: 175 us, of which the split
-// 36, dq 60, dk and dv 80; each of the four CTAs in a row on an SM spends 4.6 us on
-// its start, its first tiles' latency and its stores.  4096 tokens, 16 heads on 4, dim 128: 620
-// to 700 us with the power limit's clock.
+// 4096 packed tokens in 5 sequences, 16 heads, dim 64, causal: 195 us (178 to 185 in a
+// captured graph on a cool GPU), of which the split 31 and the products 159; each of the four
+// CTAs in a row on an SM spends 4.6 us on its start, its first tiles' latency and its
+// stores.  4096 tokens, 16 heads on 4, dim 128: 690 to 710 us with the power limit's clock.
 //
 // A computed operand needs its scale before its largest value is known: P <= 1
 // and |dP - delta| <= |dout row| |v row| + |delta| (norms) bound dS.  The norms
@@ -916,6 +916,8 @@ __device__ __forceinline__ void dkv_tile(const Shape& s, const BwdTiles& bt, uin
 // Both in one launch, so that one kind's CTAs start as the other's last ones run.
 // Neither reads what the other writes.  dk's and dv's come first, being the longer
 // ones: 8 heads, 32 rows 15.6 us in a graph against 17.5 the other way round, 4096 packed tokens 184 against 186.
+// (As launches of their own, where dk's has to wait for dq's end before it may read
+// the tiles, these take 23.3 and 180: dq's steps are 450 cycles shorter in a kernel of its own.)
 template <int DP>
 __global__ void __launch_bounds__(BW_THREADS, 1)
     attn_bwd_kernel(const __grid_constant__ Shape s, const __grid_constant__ BwdTiles bt, const float* __restrict__ q,

@@ -11,9 +11,9 @@
 // The MMA warp issues S(j+1) before part(j), so the softmax of tile j+1 has the
 // time of part(j) and S(j+2).  Tensor memory: S twice 128 columns, Q 128, part 128.
 //
-// A step takes 3280 cycles, 94% of the MMAs' rate, where the clock holds.  8192 tokens, 32
-// heads on 8, dim 128, causal: 1.30 to 1.36 ms, 1220 to 1270 TFLOP/s of f16 products, under
-// the power limit (1447 MHz).  Short sequences pay about 5 us per CTA besides: its
+// A step takes 3090 cycles (the mean of 64), 99% of the MMAs' rate.  8192 tokens, 32
+// heads on 8, dim 128, causal: 1.31 to 1.33 ms, 1240 to 1260 TFLOP/s of f16 products, under
+// the power limit (1372 MHz).  Short sequences pay about 5 us per CTA besides: its
 // start, Q on its way through shared memory, the first tiles' latency, O's store.
 // (Persistent CTAs, tried with the gradients, made the loops slower by what they saved.)
 #include <algorithm>

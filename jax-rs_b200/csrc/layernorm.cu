@@ -11,16 +11,23 @@
 //
 // Bound by HBM: 8 bytes an element forward, 12 backward.  A row is read once
 // and held in registers, by a warp (narrow rows) or by a block; the variance is
-// of the centred values, so a mean far from zero costs no digits.  Backward, a
+// of the centred values, so that a mean far from zero costs it no more than the
+// mean's own rounding in f32 does.  Backward, a
 // block keeps its columns' sums over all of its rows in registers and loads the
 // next row while it reduces the present one; the blocks' sums are added in
 // order by a second kernel.
 //
-// Forward, 16384 x 4096: 86 us, 6.2 TB/s, with four vectors in each of 256 threads; two
+// Forward, 16384 x 4096: 86 us alone, 6.2 TB/s, and 92 in a row of calls, with four vectors in each of 256 threads; two
 // in 512 take 122, one in 1024 142, eight in 128 88 (a block waits for its row's
 // sums twice, so several blocks per SM must be in different places; where rows are
-// few it is the other way).  Backward, 16384 x 2048: 60 us, 6.7 TB/s, and 4 for the join behind it; two blocks
-// per SM instead of three take 66.  Beyond 8192 columns a cluster shares a row.
+// few it is the other way).  Backward, 16384 x 2048: 60 us alone, 6.7 TB/s, the join behind it 8 alone,
+// and 71 for both in a row of calls (67 in a graph); two blocks
+// per SM instead of three take 6 more.  Beyond 8192 columns a cluster shares a row of the
+// gradient: 4096 x 16384 take 92 us forward and 172 backward, 4096 x 12000 76 and 152 (floors 82 and 123,
+// 60 and 90).  Beyond 16384 a row is read again from L2: 2000 x 20000 take 82 and 221 us (49 and 73).
+// Rows that are not aligned are read value by value, and 513 to 640 and 1025 to 1280 columns
+// take five of them a thread instead of eight: 30000 x 1111 59 us against 76 forward, 75 against 87 backward, 60000 x 637
+// 57 against 71 and 80 against 90.  (No other width has been tried so.)
 #include <math.h>
 
 #include <algorithm>
