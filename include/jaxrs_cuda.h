@@ -517,12 +517,13 @@ JX_API int jx_layernorm_bwd_f32(const float *dy, const float *x, const float *ga
  * are no row's keys.  lse [heads, total_q] may be NULL.
  * max_q / max_k: the longest sequences, a hint for the choice of kernel; any
  * value >= 0 gives right results, but a decoding batch without its own (max_q =
- * 1, say) is taken for prompts and is several times slower.  Prompts run on the tensor cores, each f32
- * operand split in two f16 parts under a power-of-two scale, f32 sums: 22 bits of
- * every value down to 2^-28 of the largest among 128 rows of its head, an absolute
- * 2^-50 of that one below.  Few query rows per key head (decoding) run in plain f32.  128 rows of one head
- * that hold a non-finite value, or largest magnitudes more than 2^20 apart, are
- * computed row by row: as right, but slowly.  The tensor-core kernels keep their
+ * 1, say) is taken for prompts and is several times slower.  Prompts run on the
+ * tensor cores, each f32 operand split in two f16 parts under a power-of-two scale,
+ * f32 sums: 22 bits of every value down to 2^-28 of the largest among 128 rows of
+ * its head, an absolute 2^-50 of that one below.  Few query rows per key head
+ * (decoding) run in plain f32.  128 rows of one head that hold a non-finite value,
+ * or largest magnitudes more than 2^20 apart, are computed row by row: as right, but
+ * slowly.  The tensor-core kernels keep their
  * operands in scratch, in whole tiles of 128 rows per sequence and head; beyond
  * 2 GB of it the key heads are taken in groups, and where one key head's tiles
  * alone exceed that and would be mostly empty (many thousands of short sequences)
@@ -539,7 +540,9 @@ JX_API int jx_attention_f32(const float *q, const float *k, const float *v, floa
  * rowsum(dout * o)), dq = scale * ds k, dk = scale * ds^T q, dk and dv summed
  * over the query heads that share a key head.  No gradient may overlap an input or
  * another gradient (interleaved rows of one buffer are fine).  lse must be the forward pass's
- * (p <= 1).  Every sum has a fixed order: the same inputs give the same bits. */
+ * (p <= 1).  The tensor-core kernels hold p and ds in two f16 parts too: p to
+ * 2^-50, ds to 2^-50 of |dout[i]| times the largest |v[j]| among 128 keys (norms).
+ * Every sum has a fixed order: the same inputs give the same bits. */
 JX_API int jx_attention_bwd_f32(const float *q, const float *k, const float *v, const float *o, const float *lse,
                                 const float *dout, float *dq, float *dk, float *dv, const int32_t *cu_q,
                                 const int32_t *cu_k, int64_t batch, int64_t total_q, int64_t total_k, int64_t max_q,
